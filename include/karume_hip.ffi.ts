@@ -228,6 +228,53 @@ export const KARUME_HIP_SYMBOLS = {
     result: "i32",
   },
   krm_argmax: { parameters: ["pointer", "u64", "u64", "u32", "u32", "i32"], result: "i32" },
+  krm_rope_tables: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u32", "u32", "u32", "u32", "f32"
+    ],
+    result: "i32",
+  },
+  krm_rope_rows: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u64", "u64", "u32", "u32", "u32", "u32", "i32", "u32",
+      "u32", "u64", "u64", "i32", "i32"
+    ],
+    result: "i32",
+  },
+  krm_kv4_page_bytes: {
+    parameters: [
+      "u32", "u32", "u32", "u32", "buffer"
+    ],
+    result: "i32",
+  },
+  krm_kv4_append: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u64",
+      "u64", "u32", "u32", "u32", "u32", "u32", "u32", "u32", "u32", "u32", "u32", "u64", "u64",
+      "u64", "u32", "i32", "u32", "u32", "i32"
+    ],
+    result: "i32",
+  },
+  krm_kv4_read: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u32", "u32", "u32", "u32",
+      "u32", "u32", "u32", "u32", "u32", "i32"
+    ],
+    result: "i32",
+  },
+  krm_kv4_attention_workspace: {
+    parameters: [
+      "u32", "u32", "u32", "u32", "u32", "u32", "u32", "u32", "i32", "buffer"
+    ],
+    result: "i32",
+  },
+  krm_kv4_attention: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u32", "u32", "u32", "u32",
+      "u32", "u32", "u32", "u32", "u32", "u32", "u32", "u32", "f32", "i32", "u64", "usize"
+    ],
+    result: "i32",
+  },
 } as const;
 
 export type KarumeHipLibrary = Deno.DynamicLibrary<typeof KARUME_HIP_SYMBOLS>;

@@ -538,6 +538,101 @@ int32_t krm_embedding(krm_ctx* ctx, krm_buf table, krm_buf index_i32, krm_buf ou
 int32_t krm_argmax(krm_ctx* ctx, krm_buf x, krm_buf out_i32, uint32_t rows, uint32_t dim,
                    int32_t io_dtype);
 
+/* ---- rotary positions, in general (no counterpart in the reference beyond krm_rope_half) --------
+ * krm_rope_tables: cos_table[p, j] = amplitude * cos((first_position + p) * inv_freq[j]) and the sine
+ * alike, for p < rows and j < pairs; `inv_freq` is f64 on the device, angle and reduction are in 64 bits,
+ * results f32 (off by 2^-23 of the amplitude at most while |angle| < 2^31).  Rows are `width` floats:
+ * `pairs`, or twice as many with the angles repeated (the tables of krm_rope_half, head_dim wide).
+ * Positions stay below 2^31.
+ * krm_rope_rows: the first rotary_dim (even, <= head_dim) elements of each head are turned by
+ * positions[row], the others are copied:
+ *   KRM_ROPE_HALF        pairs (j, j + rotary_dim/2)
+ *   KRM_ROPE_INTERLEAVED pairs (2 j, 2 j + 1)
+ *   a' = a cos - b sin,  b' = b cos + a sin    (products rounded, then joined; stored as io_dtype)
+ * with angle j of table row positions[row] (tables [table_rows, table_width] f32, table_width >=
+ * rotary_dim/2; entries past that are not read).  x rows are x_stride elements apart, [heads, head_dim]
+ * packed in each; out rows out_stride, or [heads, rows, head_dim] when to_head_major != 0.  A position
+ * outside the table gives NaN in the turned elements.  `out` is x itself (rows then keep their places)
+ * or does not overlap it. */
+#define KRM_ROPE_HALF 0
+#define KRM_ROPE_INTERLEAVED 1
+int32_t krm_rope_tables(krm_ctx* ctx, krm_buf inv_freq_f64, krm_buf cos_table_f32,
+                        krm_buf sin_table_f32, uint32_t first_position, uint32_t rows,
+                        uint32_t pairs, uint32_t width, float amplitude);
+int32_t krm_rope_rows(krm_ctx* ctx, krm_buf x, krm_buf positions_i32, krm_buf cos_table_f32,
+                      krm_buf sin_table_f32, krm_buf out, uint32_t rows, uint32_t heads,
+                      uint32_t head_dim, uint32_t rotary_dim, int32_t layout, uint32_t table_rows,
+                      uint32_t table_width, uint64_t x_stride, uint64_t out_stride,
+                      int32_t to_head_major, int32_t io_dtype);
+
+/* ---- paged 4-bit K/V cache (no counterpart in the reference, whose slots are contiguous f32 / fp16:
+ *      docs/decisions/0066-generation-context-state-slots.md:130-135) ------------------------------
+ * Sequences of a batch grow page by page: `cache` is `pages` pages of krm_kv4_page_bytes each (one such
+ * buffer a layer, 16-byte aligned), column c of sequence i lies in row c % page_rows of page
+ * page_table[i, c / page_rows] (int32 [nseq, table_stride] on the device; entries past a sequence's
+ * columns are not read).  Pages may be shared by sequences that only read them.
+ * Depth is 64, 128 or 256; a group of 32, 64 or 128 elements of a head's row (at most the depth) is held
+ * as 4-bit codes and an fp16 (step, minimum):
+ *   minimum = largest fp16 <= min(x) (+0 for a zero),
+ *   step = least fp16 >= (max(x) - minimum) / 15,
+ *   code = clamp(round-half-even((x - minimum) / step), 0, 15)      (f32 operations; step 0: code 0)
+ * and stands for step * code + minimum.  A group that holds a NaN or a magnitude above 32640 reads as
+ * NaN.  A page is, for each kv head in turn (P = page_rows, g = group):
+ *   key codes    [P, 4, D/32] u32: word (c, s) has elements 32 s + 8 c .. + 7, element 2 i in nibble i,
+ *                element 2 i + 1 in nibble 4 + i
+ *   key params   [P, D/g, 2] fp16 (step, minimum)
+ *   value codes  [P/4, D/8, 4] u32: word (b, w, t) has elements 8 w .. 8 w + 7 of row 4 b + t, in order
+ *   value params [P/4, D/g, 2, 4] fp16: the steps of rows 4 b .. 4 b + 3, then their minima
+ *
+ * A step's rows are packed: sequence i has rows cu_rows[i] .. cu_rows[i+1] - 1 (int32 [nseq+1]) and
+ * lens[i] columns with them (int32 [nseq]), so its rows stand at columns lens[i] - rows .. lens[i] - 1.
+ * All of these are read on the device, so that a recorded call replays while sequences grow within
+ * max_query rows a sequence, total_rows rows in all, table_stride pages (and max_columns columns, for
+ * the attention).  A sequence without rows is skipped.  One whose words break these limits, and a row
+ * that needs a page outside 0 .. pages - 1, raise *fault_u32 to 1 (0 = no such word; it is never
+ * cleared); nothing is read or written out of place.  Rows behind the last sequence are left as they were.
+ *
+ * krm_kv4_append: this step's keys and values (rows k_stride / v_stride elements apart, [Hkv, D] packed
+ * in each) are written to their columns, keys turned first by `positions` ([total_rows] int32; 0 = the
+ * column) as krm_rope_rows does with rotary_dim, layout and tables (rotary_dim 0: not turned), not
+ * rounded in between.  q != 0: query rows ([H, D], q_stride apart) are turned into q_out [total_rows, H,
+ * D] (q_out may be q where q_stride = H * D).  A refused sequence writes nothing, a row without its page
+ * no keys and values.  Two sequences of one call must not write to one page.
+ * krm_kv4_read: the same rows back, as values in out_dtype: k_out, v_out [total_rows, Hkv, D]; with
+ * cu_rows = the sums of lens, all columns.  Rows without their page are NaN.
+ * krm_kv4_attention: each row attends to columns max(0, p - window + 1) .. p of its sequence (p its own
+ * column; window 0 = all), which krm_kv4_append must have written, with scores half_scale^2 q . k:
+ *   q, out [total_rows, H, D] io_dtype (out is not q); H a multiple of Hkv.
+ * fp16 rows: keys, values and weights are rounded to fp16, sums are f32; f32 rows: f32 class throughout.
+ * A refused sequence's rows, and rows that see a page outside the cache, are NaN.  `workspace`
+ * (krm_kv4_attention_workspace bytes, 16-byte aligned; 0 bytes: may be 0) belongs to one call at a
+ * time; its contents need no preparation. */
+int32_t krm_kv4_page_bytes(uint32_t kv_heads, uint32_t depth, uint32_t group, uint32_t page_rows,
+                           size_t* bytes);
+int32_t krm_kv4_append(krm_ctx* ctx, krm_buf q, krm_buf k, krm_buf v, krm_buf q_out,
+                       krm_buf positions_i32, krm_buf cos_table_f32, krm_buf sin_table_f32,
+                       krm_buf cache, krm_buf page_table_i32, krm_buf cu_rows_i32, krm_buf lens_i32,
+                       krm_buf fault_u32, uint32_t nseq, uint32_t max_query, uint32_t total_rows,
+                       uint32_t heads, uint32_t kv_heads, uint32_t depth, uint32_t group,
+                       uint32_t page_rows, uint32_t pages, uint32_t table_stride, uint64_t q_stride,
+                       uint64_t k_stride, uint64_t v_stride, uint32_t rotary_dim, int32_t layout,
+                       uint32_t table_rows, uint32_t table_width, int32_t io_dtype);
+int32_t krm_kv4_read(krm_ctx* ctx, krm_buf cache, krm_buf page_table_i32, krm_buf cu_rows_i32,
+                     krm_buf lens_i32, krm_buf k_out, krm_buf v_out, krm_buf fault_u32, uint32_t nseq,
+                     uint32_t max_query, uint32_t total_rows, uint32_t kv_heads, uint32_t depth,
+                     uint32_t group, uint32_t page_rows, uint32_t pages, uint32_t table_stride,
+                     int32_t out_dtype);
+int32_t krm_kv4_attention_workspace(uint32_t nseq, uint32_t max_query, uint32_t max_columns,
+                                    uint32_t total_rows, uint32_t heads, uint32_t kv_heads,
+                                    uint32_t depth, uint32_t window, int32_t io_dtype, size_t* bytes);
+int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_table_i32,
+                          krm_buf cu_rows_i32, krm_buf lens_i32, krm_buf out, krm_buf fault_u32,
+                          uint32_t nseq, uint32_t max_query, uint32_t max_columns,
+                          uint32_t total_rows, uint32_t heads, uint32_t kv_heads, uint32_t depth,
+                          uint32_t group, uint32_t page_rows, uint32_t pages, uint32_t table_stride,
+                          uint32_t window, float half_scale, int32_t io_dtype, krm_buf workspace,
+                          size_t workspace_bytes);
+
 /* ==== DIAGNOSTICS ============================================================================
  * Not ops of the runtime: measurement probes that bench.py uses to state what a launch and a
  * read of a given size cost on this machine.  A host binds them only if it wants those floors

@@ -10,13 +10,14 @@ from .format_model import (ContainerError, IrError, KarumeModel, PackedInt4, Saf
                            i4_resident_initializers, open_model, packed_int4,
                            parse_safetensors, tensor_bytes)
 from .runtime import (COMPUTE_F16, COMPUTE_F32, EPILOGUE_NONE, EPILOGUE_SILU_PAIRS, F16, F32,
-                      PROBE_EMPTY, PROBE_READ, DeviceBuffer, ExecutionError,
-                      GpuContext, GpuDeviceLostError, GpuEvent, GpuGraph, GpuOutOfMemoryError,
+                      PROBE_EMPTY, PROBE_READ, ROPE_HALF, ROPE_INTERLEAVED, DeviceBuffer,
+                      ExecutionError, GpuContext, GpuDeviceLostError, GpuEvent, GpuGraph, GpuOutOfMemoryError,
                       GpuValidationError, KarumeError, acquire_gpu, dtype_code, version)
 
 from .decoder_loader import GraphShapeError, decoder_weights_from_model
 from .generation import (GenerationContext, GenerationContextError, PrefillChunk,
                          generate_greedy, plan_prefill_chunks)
+from .rotary import rope_frequencies
 
 __all__ = [
     "GenerationContext", "GenerationContextError", "PrefillChunk", "generate_greedy",
@@ -26,7 +27,7 @@ __all__ = [
     "ContainerError", "IrError", "KarumeModel", "PackedInt4", "SafetensorsError",
     "i4_resident_initializers", "open_model", "packed_int4", "parse_safetensors", "tensor_bytes",
     "COMPUTE_F16", "COMPUTE_F32", "EPILOGUE_NONE", "EPILOGUE_SILU_PAIRS", "F16", "F32",
-    "PROBE_EMPTY", "PROBE_READ", "DeviceBuffer", "ExecutionError", "GpuContext",
+    "PROBE_EMPTY", "PROBE_READ", "ROPE_HALF", "ROPE_INTERLEAVED", "rope_frequencies", "DeviceBuffer", "ExecutionError", "GpuContext",
     "GpuDeviceLostError", "GpuEvent", "GpuGraph", "GpuOutOfMemoryError", "GpuValidationError", "KarumeError",
     "acquire_gpu", "dtype_code", "version",
 ]

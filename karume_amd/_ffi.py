@@ -109,6 +109,20 @@ PROTOTYPES = {
     "krm_add": (i32, [c_ctx, c_buf, c_buf, c_buf, u64, i32]),
     "krm_embedding": (i32, [c_ctx, c_buf, c_buf, c_buf, u32, u32, u32, i32, i32]),
     "krm_argmax": (i32, [c_ctx, c_buf, c_buf, u32, u32, i32]),
+    "krm_rope_tables": (i32, [c_ctx, c_buf, c_buf, c_buf, u32, u32, u32, u32, C.c_float]),
+    "krm_rope_rows": (i32, [c_ctx, c_buf, c_buf, c_buf, c_buf, c_buf, u32, u32, u32, u32, i32,
+                            u32, u32, u64, u64, i32, i32]),
+    "krm_kv4_page_bytes": (i32, [u32, u32, u32, u32, C.POINTER(size_t)]),
+    "krm_kv4_append": (i32, [c_ctx, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf,
+                             c_buf, c_buf, c_buf, u32, u32, u32, u32, u32, u32, u32, u32, u32,
+                             u32, u64, u64, u64, u32, i32, u32, u32, i32]),
+    "krm_kv4_read": (i32, [c_ctx, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, u32, u32, u32,
+                           u32, u32, u32, u32, u32, u32, i32]),
+    "krm_kv4_attention_workspace": (i32, [u32, u32, u32, u32, u32, u32, u32, u32, i32,
+                                          C.POINTER(size_t)]),
+    "krm_kv4_attention": (i32, [c_ctx, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, u32, u32,
+                                u32, u32, u32, u32, u32, u32, u32, u32, u32, u32, C.c_float, i32,
+                                c_buf, size_t]),
 }
 
 _lib = None

@@ -24,6 +24,7 @@ PROBE_READ = 1
 EPILOGUE_NONE = 0
 CHUNK_OUT_ROW_MAJOR, CHUNK_APPEND, CHUNK_OUT_F16 = 1, 2, 4
 EPILOGUE_SILU_PAIRS = 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 
 _NP_DTYPE_CODE = {np.dtype(np.float32): F32, np.dtype(np.float16): F16}
 
@@ -220,6 +221,12 @@ class GpuContext:
     def _check(self, status: int) -> None:
         if status != 0:
             message = self._lib.krm_last_error(self._handle).decode("utf-8", "replace")
+            raise _ERRORS.get(status, KarumeError)(message)
+
+    def _check_free(self, status: int) -> None:
+        """The status of a call that has no context."""
+        if status != 0:
+            message = self._lib.krm_last_error(None).decode("utf-8", "replace")
             raise _ERRORS.get(status, KarumeError)(message)
 
     def sync(self) -> None:
@@ -620,6 +627,99 @@ class GpuContext:
                io_dtype: int = F32) -> None:
         self._check(self._lib.krm_argmax(self._handle, _addr(x), _addr(out_i32), rows, dim,
                                          io_dtype))
+
+    # -- rotary positions in general ---------------------------------------------------------------
+    def rope_tables(self, inv_freq_f64: BufferLike, cos_table: BufferLike, sin_table: BufferLike,
+                    *, rows: int, pairs: int, width: Optional[int] = None, first: int = 0,
+                    amplitude: float = 1.0) -> None:
+        """cos / sin of positions first .. first + rows - 1 (rope_frequencies() gives the f64
+        frequencies); width = 2 * pairs repeats the angles, as rope_half reads them."""
+        self._check(self._lib.krm_rope_tables(
+            self._handle, _addr(inv_freq_f64), _addr(cos_table), _addr(sin_table), first, rows,
+            pairs, pairs if width is None else width, float(amplitude)))
+
+    def rope_rows(self, x: BufferLike, positions: BufferLike, cos_table: BufferLike,
+                  sin_table: BufferLike, out: BufferLike, *, rows: int, heads: int, head_dim: int,
+                  rotary_dim: int, table_rows: int, table_width: Optional[int] = None,
+                  layout: int = ROPE_HALF, x_stride: Optional[int] = None,
+                  out_stride: Optional[int] = None, to_head_major: bool = False,
+                  io_dtype: int = F32) -> None:
+        """Turn the first rotary_dim elements of every head by positions[row]; strides are elements
+        between rows (default: packed)."""
+        packed = heads * head_dim
+        self._check(self._lib.krm_rope_rows(
+            self._handle, _addr(x), _addr(positions), _addr(cos_table), _addr(sin_table),
+            _addr(out), rows, heads, head_dim, rotary_dim, layout, table_rows,
+            rotary_dim // 2 if table_width is None else table_width,
+            packed if x_stride is None else x_stride, packed if out_stride is None else out_stride,
+            int(to_head_major), io_dtype))
+
+    # -- paged 4-bit K/V cache -----------------------------------------------------------------------
+    def kv4_page_bytes(self, kv_heads: int, depth: int, group: int, page_rows: int) -> int:
+        nbytes = C.c_size_t()
+        self._check_free(self._lib.krm_kv4_page_bytes(kv_heads, depth, group, page_rows,
+                                                      C.byref(nbytes)))
+        return int(nbytes.value)
+
+    def kv4_append(self, k: BufferLike, v: BufferLike, cache: BufferLike, page_table: BufferLike,
+                   cu_rows: BufferLike, lens: BufferLike, *, nseq: int, max_query: int,
+                   total_rows: int, kv_heads: int, depth: int, group: int, page_rows: int,
+                   pages: int, table_stride: int, heads: int = 0, q: BufferLike = None,
+                   q_out: BufferLike = None, positions: BufferLike = None,
+                   cos_table: BufferLike = None, sin_table: BufferLike = None, rotary_dim: int = 0,
+                   layout: int = ROPE_HALF, table_rows: int = 0,
+                   table_width: Optional[int] = None, q_stride: Optional[int] = None,
+                   k_stride: Optional[int] = None, v_stride: Optional[int] = None,
+                   fault: BufferLike = None, io_dtype: int = F32) -> None:
+        """Turn and quantise a step's keys, quantise its values, write both to their pages; with q,
+        turn its query rows into q_out."""
+        packed = kv_heads * depth
+        self._check(self._lib.krm_kv4_append(
+            self._handle, _addr(q), _addr(k), _addr(v), _addr(q_out), _addr(positions),
+            _addr(cos_table), _addr(sin_table), _addr(cache), _addr(page_table), _addr(cu_rows),
+            _addr(lens), _addr(fault), nseq, max_query, total_rows, heads, kv_heads, depth, group,
+            page_rows, pages, table_stride, heads * depth if q_stride is None else q_stride,
+            packed if k_stride is None else k_stride, packed if v_stride is None else v_stride,
+            rotary_dim, layout, table_rows,
+            rotary_dim // 2 if table_width is None else table_width, io_dtype))
+
+    def kv4_read(self, cache: BufferLike, page_table: BufferLike, cu_rows: BufferLike,
+                 lens: BufferLike, k_out: BufferLike, v_out: BufferLike, *, nseq: int,
+                 max_query: int, total_rows: int, kv_heads: int, depth: int, group: int,
+                 page_rows: int, pages: int, table_stride: int, fault: BufferLike = None,
+                 out_dtype: int = F32) -> None:
+        """The last rows of each sequence as the values that the cache holds for them."""
+        self._check(self._lib.krm_kv4_read(
+            self._handle, _addr(cache), _addr(page_table), _addr(cu_rows), _addr(lens),
+            _addr(k_out), _addr(v_out), _addr(fault), nseq, max_query, total_rows, kv_heads, depth,
+            group, page_rows, pages, table_stride, out_dtype))
+
+    def kv4_attention_workspace(self, *, nseq: int, max_query: int, max_columns: int,
+                                total_rows: int, heads: int, kv_heads: int, depth: int,
+                                window: int = 0, io_dtype: int = F32, **_shape: int) -> int:
+        """Bytes of workspace (the other words of the cache's shape may be given too)."""
+        nbytes = C.c_size_t()
+        self._check_free(self._lib.krm_kv4_attention_workspace(
+            nseq, max_query, max_columns, total_rows, heads, kv_heads, depth, window, io_dtype,
+            C.byref(nbytes)))
+        return int(nbytes.value)
+
+    def kv4_attention(self, q: BufferLike, cache: BufferLike, page_table: BufferLike,
+                      cu_rows: BufferLike, lens: BufferLike, out: BufferLike, *, nseq: int,
+                      max_query: int, max_columns: int, total_rows: int, heads: int, kv_heads: int,
+                      depth: int, group: int, page_rows: int, pages: int, table_stride: int,
+                      half_scale: float, window: int = 0, fault: BufferLike = None,
+                      io_dtype: int = F32, workspace: BufferLike = None,
+                      workspace_bytes: int = 0) -> None:
+        """Causal attention of a step's rows (one a sequence or many) over the paged cache, their
+        own columns included."""
+        if isinstance(workspace, DeviceBuffer) and not workspace_bytes:
+            workspace_bytes = workspace.nbytes
+        self._check(self._lib.krm_kv4_attention(
+            self._handle, _addr(q), _addr(cache), _addr(page_table), _addr(cu_rows), _addr(lens),
+            _addr(out), _addr(fault), nseq, max_query, max_columns, total_rows, heads, kv_heads,
+            depth, group, page_rows, pages, table_stride, window, float(half_scale), io_dtype,
+            _addr(workspace), workspace_bytes))
 
 
 def acquire_gpu(device: int = 0, stream: Optional[int] = None) -> GpuContext:
