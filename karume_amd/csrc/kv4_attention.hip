@@ -2,8 +2,11 @@
 //
 // Row r of a sequence stands at column p = len - rows + r and sees columns max(0, p - window + 1) .. p:
 //   out = sum_c softmax_c(scale^2 q . k_c) v_c,   k_c = step * code + minimum, v_c alike.
+#include "i4_codes.h"
 #include "kv4_plan.h"
 #include "krm_internal.h"
+#include "lds_stream.h"
+#include "rows8.h"
 
 #include <cmath>
 
@@ -11,131 +14,678 @@ using namespace krm;
 
 namespace {
 
-constexpr int kThreads = 256;
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
 
-template <typename T>
-__device__ inline float ld(const T* p, size_t i);
-template <>
-__device__ inline float ld<float>(const float* p, size_t i) { return p[i]; }
-template <>
-__device__ inline float ld<__half>(const __half* p, size_t i) { return __half2float(p[i]); }
-template <typename T>
-__device__ inline void st(T* p, size_t i, float v);
-template <>
-__device__ inline void st<float>(float* p, size_t i, float v) { p[i] = v; }
-template <>
-__device__ inline void st<__half>(__half* p, size_t i, float v) { p[i] = __float2half_rn(v); }
+constexpr int kStages = 2;         // tiles of a wave on their way
+constexpr int kTile = 32;          // columns a wave takes at a time
+constexpr int kJoin = 32;           // parts whose sums are asked for together
+constexpr int kRows = 16;          // (row, head) pairs of a workgroup
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttentionArgs {
   Kv4Layout layout;
   Kv4Limits limits;
-  uint32_t heads, pages, window;
-  float scale;   // half_scale^2 * log2 e: scores are kept in base 2
+  uint32_t nseq, heads, pages, window;
+  uint32_t share;          // query heads of a kv head
+  float share_inverse, row_tiles_inverse, of_sequence_inverse;
+  uint32_t row_tiles;      // blocks of kRows (row, head) pairs of a kv head
+  uint32_t max_splits;     // workgroups that one block's columns are dealt to at most
+  uint32_t partial_rows;   // rows that a partial has room for
+  uint32_t least;          // tiles, at least, of a split
+  float share_of_work;     // of all sequences' tiles, in one workgroup
+  float scale;             // half_scale^2 * log2 e: scores are kept in base 2
+  float* partials;         // [unit][split]: partial_rows x D sums, then partial_rows x (max, sum)
+  uint32_t* tickets;
 };
 
-__device__ inline float half_at(const uint8_t* p) {
-  return __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t*>(p)));
+// Device-scope store / load of one float: written through to (read from) memory that every XCD sees.
+__device__ inline void publish(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ inline float observe(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+__device__ inline float2_t observe2(const float* p) {
+  return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// One workgroup a (row, head): 256 columns at a time, a score a thread, then an output element a thread
-// (256 / D threads share its columns).
-template <typename XT, int D>
-__global__ __launch_bounds__(kThreads) void kv4_attention_kernel(
+// Over the lanes 16, 32 and 48 apart.
+template <typename F>
+__device__ inline float across_quarters(float x, F join) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = join(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return join(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float quarters_max(float x) {
+  return across_quarters(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ inline float quarters_sum(float x) {
+  return across_quarters(x, [](float a, float b) { return a + b; });
+}
+
+__device__ inline half2_t half2_of(uint32_t w) { return __builtin_bit_cast(half2_t, w); }
+__device__ inline half8_t join8(half2_t a, half2_t b, half2_t c, half2_t d) {
+  return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+// Codes at the bottom (u) or four bits up (16 u) of the halves of a word, as the exact integers.
+__device__ inline half2_t low_codes(uint32_t x) {
+  return half2_of(and_or(x, 0x000F000Fu, 0x64006400u)) - half2_t{(_Float16)1024.0f, (_Float16)1024.0f};
+}
+__device__ inline half2_t high_codes(uint32_t x) {
+  return __builtin_elementwise_fma(half2_of(and_or(x, 0x00F000F0u, 0x64006400u)),
+                                   half2_t{(_Float16)0.0625f, (_Float16)0.0625f},
+                                   half2_t{(_Float16)-64.0f, (_Float16)-64.0f});
+}
+// step * x + sum with a step in fp16 (one mixed instruction).
+__device__ inline float scaled(uint32_t params, float x, float sum) { return fmaf((float)half2_of(params).x, x, sum); }
+
+template <int N>
+__device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    w[0] = a.x; w[1] = a.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 a = *reinterpret_cast<const uint4*>(p + 16 * i);
+      w[4 * i] = a.x; w[4 * i + 1] = a.y; w[4 * i + 2] = a.z; w[4 * i + 3] = a.w;
+    }
+  }
+}
+
+// What a wave needs of 32 columns, two halves of 16, and where it lies in the wave's part of LDS.  Lane (i = lane %
+// 16, c = lane / 16) of an operand needs of each half
+//   keys    words (c, .) of row i, all parameters of rows i and 4 c .. 4 c + 3
+//   values  rows 4 c .. 4 c + 3: word columns i (+ 16) and the parameters of their groups
+// (a depth of 64 has eight word columns: lanes 8 .. 15 carry the upper half words of columns 0 .. 7).  Codes come in
+// 16-byte pieces that a lane asks for and reads itself, so LDS is only where they wait; parameters are shared.
+template <int D, int NG>
+struct Stage {
+  static constexpr int kSteps = D / 32;
+  static constexpr int kColumns = D <= 128 ? 1 : D / 128;     // word columns of a lane
+  static constexpr int kParts = kColumns;                     // pieces of a half's key row that a lane has
+  static constexpr int kWords = NG <= 4 ? 1 : 2;              // dwords a lane of a half's parameters
+  static constexpr uint32_t kParams = 256 * kWords;           // bytes of a half's parameters
+  static constexpr uint32_t kKeys = 0, kValues = 2 * kParts * 1024, kKeyParams = 4 * kParts * 1024,
+                            kValueParams = kKeyParams + 2 * kParams, kBytes = kValueParams + 2 * kParams;
+  static constexpr int kLoads = 4 * kParts + 4 * kWords;      // that fill it
+};
+
+// The same address in every lane, in scalar registers whatever the compiler made of it.
+__device__ inline const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t at = (uint64_t)p;
+  return (const uint8_t*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at));
+}
+// x / d for x up to 2^24, `inverse` = 1 / d: the quotient in floating point, put right by the remainder.
+__device__ inline uint32_t divided(uint32_t x, uint32_t d, float inverse) {
+  const uint32_t guess = (uint32_t)((float)x * inverse);
+  const int32_t rest = (int32_t)(x - guess * d);
+  return rest < 0 ? guess - 1 : rest >= (int32_t)d ? guess + 1 : guess;
+}
+// Over all lanes.
+__device__ inline float wave_sum(float x) {
+#define KRM_ADD_DPP(CTRL, ROWS) \
+  x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false))
+  KRM_ADD_DPP(0x111, 0xf);   // row_shr:1
+  KRM_ADD_DPP(0x112, 0xf);
+  KRM_ADD_DPP(0x114, 0xf);
+  KRM_ADD_DPP(0x118, 0xf);
+  KRM_ADD_DPP(0x142, 0xa);   // row_bcast:15
+  KRM_ADD_DPP(0x143, 0xc);   // row_bcast:31
+#undef KRM_ADD_DPP
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+template <typename XT, int D, int NG, int kWaves>
+__global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
     const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table,
     const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens, XT* __restrict__ out,
     uint32_t* __restrict__ fault, AttentionArgs a) {
-  constexpr int kParts = kThreads / D;
-  __shared__ float s_q[D], s_p[kThreads], s_acc[kThreads], s_red[kThreads / kWave];
-  const uint32_t seq = blockIdx.y, tid = threadIdx.x;
-  const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+  constexpr bool kF32 = sizeof(XT) == 4;
+  constexpr int kThreads = kWaves * kWave;
+  using S = Stage<D, NG>;
+  constexpr int kSteps = S::kSteps, kColumns = S::kColumns;
+  constexpr int kPerGroup = kSteps / NG;
+  constexpr int kOuts = D == 64 ? 4 : 8;        // elements of a word column that a lane's rows carry
+  constexpr int kStride = D + 4;                // of a row in LDS
+  extern __shared__ __align__(16) uint8_t s_ring[];   // [wave][stage]; behind the tiles [wave][partial_rows][kStride] f32
+  __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
+  __shared__ uint32_t s_ticket;
+
+  const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  // Workgroups go to the XCDs in turn: a unit (sequence, kv head, block of rows) has its next split on the next XCD,
+  // so that neither first splits nor a long sequence gather on one of them.
+  const uint32_t split = blockIdx.y, units = gridDim.x, of_sequence = a.layout.kv_heads * a.row_tiles;
+  uint32_t unit = blockIdx.x;
+  if (split) {
+    unit += units > split ? split : split % units;
+    if (unit >= units) unit -= units;
+  }
+  const uint32_t seq = divided(unit, of_sequence, a.of_sequence_inverse), in_sequence = unit - seq * of_sequence;
+  const uint32_t kv_head = divided(in_sequence, a.row_tiles, a.row_tiles_inverse);
+  const uint32_t pair0 = (in_sequence - kv_head * a.row_tiles) * kRows;   // first (row, head) pair of this workgroup
+  // ---- everything that its place alone tells: the sequence's words, its first 64 pages, the step's lengths
+  const int32_t* table = page_table + (size_t)seq * a.limits.table_stride;
+  const uint32_t entry = (uint32_t)table[min(lane, a.limits.table_stride - 1)];
+  float work = 0.f;
+  if (a.max_splits > 1) {
+    for (uint32_t i = lane; i < a.nseq; i += kWave) {
+      const uint32_t n = min((uint32_t)max(lens[i], 0), a.limits.max_columns);
+      work += (float)((a.window ? min(n, a.window) : n) / kTile + 1);
+    }
+  }
   const int32_t cu0 = cu_rows[seq], cu1 = cu_rows[seq + 1];
   const Kv4Sequence s = kv4_sequence(cu0, cu1, lens[seq], a.limits);
-  const bool in_rows = cu0 >= 0 && cu1 >= cu0 && (uint32_t)cu1 <= a.limits.total_rows && row < (uint32_t)(cu1 - cu0);
-  if (!s.ok && fault && blockIdx.x == 0 && tid == 0) *fault = 1u;
+  const bool in_rows = cu0 >= 0 && cu1 >= cu0 && (uint32_t)cu1 <= a.limits.total_rows;
+  if (!s.ok && fault && split == 0 && tid == 0) *fault = 1u;
   if (!in_rows) return;
-  const size_t base = (((size_t)s.first + row) * a.heads + head) * D;
+  const uint32_t pairs = (uint32_t)(cu1 - cu0) * a.share;
+  if (pair0 >= pairs) return;
+  const uint32_t count = min((uint32_t)kRows, pairs - pair0);
+  const uint32_t row0 = divided(pair0, a.share, a.share_inverse), head0 = pair0 - row0 * a.share;
+  auto row_of = [&](uint32_t m) { return divided(head0 + m, a.share, a.share_inverse); };   // of pair m, from row0 on
+  auto out_row = [&](uint32_t m) -> size_t {   // of pair m: its first element
+    const uint32_t row = row_of(m), head = kv_head * a.share + head0 + m - row * a.share;
+    return (((size_t)(uint32_t)cu0 + row0 + row) * a.heads + head) * D;
+  };
   if (!s.ok) {
-    if (tid < D) st<XT>(out, base + tid, NAN);
+    if (split == 0)
+      for (uint32_t e = tid; e < count * D; e += kThreads) out[out_row(e / D) + e % D] = from_f32<XT>(NAN);
     return;
   }
-  if (tid < D) s_q[tid] = ld<XT>(q, base + tid) * a.scale;
-  const int32_t position = s.len - s.rows + (int32_t)row;
-  const int32_t first = kv4_first_column(position, a.window);
-  const uint32_t kv_head = head / (a.heads / a.layout.kv_heads);
-  const int32_t* table = page_table + (size_t)seq * a.limits.table_stride;
-  const uint32_t groups = a.layout.groups();
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  bool bad = false;
-  const uint32_t d = tid % D, part = tid / D;
-  __syncthreads();
-  for (int32_t c0 = first; c0 <= position; c0 += kThreads) {
-    const int32_t c = c0 + (int32_t)tid;
-    float score = -INFINITY;
-    if (c <= position) {
-      const int32_t page = table[c / a.layout.page_rows];
-      if (page < 0 || (uint32_t)page >= a.pages) {
-        bad = true;
-      } else {
-        const uint8_t* block = cache + (size_t)page * a.layout.page() + (size_t)kv_head * a.layout.block();
-        const uint32_t in_page = c & (a.layout.page_rows - 1);
-        score = 0.f;
-        for (uint32_t g = 0; g < groups; ++g) {
-          float codes = 0.f, sum = 0.f;
-          for (uint32_t w = g * a.layout.group / 8; w < (g + 1) * a.layout.group / 8; ++w) {
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(block + a.layout.key_word(in_page, w));
-            for (int i = 0; i < 8; ++i) {
-              const float qi = s_q[w * 8 + i];
-              codes = fmaf(qi, (float)((word >> (4 * ((i & 1) * 4 + i / 2))) & 15u), codes);
-              sum += qi;
-            }
+  // columns that any of the rows sees, and their tiles
+  const int32_t first_row = s.len - s.rows + (int32_t)row0, last_row = first_row + (int32_t)row_of(count - 1);
+  const int32_t low = kv4_first_column(first_row, a.window), high = last_row;
+  const int32_t tile0 = low / kTile;
+  const uint32_t tiles = (uint32_t)(high / kTile - tile0 + 1);
+  uint32_t per = tiles, nsplit = 1;
+  if (a.max_splits > 1) {
+    // the step's tiles, as far as they go by the lengths, are dealt evenly to the workgroups that fit the machine
+    per = max((uint32_t)(wave_sum(work) * a.share_of_work), a.least) + kWaves - 1;
+    per = max(per / kWaves * kWaves, (tiles + a.max_splits - 1) / a.max_splits);
+    nsplit = (tiles + per - 1) / per;
+    if (split >= nsplit) return;
+  }
+  const int32_t begin = tile0 + (int32_t)min(split * per, tiles);
+  const int32_t end = tile0 + (int32_t)min((split + 1) * per, tiles);
+  // this wave's tiles are mine0, mine0 + kWaves, .. (the waves' next tiles lie together: in one long run for each wave
+  // 131000 columns took 44.4 us, so 39.8)
+  const int32_t mine0 = begin + (int32_t)wave;
+  const int32_t mine = mine0 < end ? (int32_t)((uint32_t)(end - mine0 + kWaves - 1) / kWaves) : 0;
+
+  // ---- the queries: lane (m = lane % 16, c): elements 32 s + 8 c .. + 7 of pair m for each step s
+  const uint32_t m = lane & 15, c = lane >> 4;
+  const bool live = m < count;
+  const int32_t position = first_row + (int32_t)(live ? row_of(m) : 0);
+  const int32_t from = kv4_first_column(position, a.window);
+  float x[kSteps][8];
+  {
+    const XT* src = q + out_row(live ? m : 0) + 8 * c;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) load8(src + 32 * st, x[st]);
+  }
+  // Pages of 64 of this wave's tiles, a tile a lane.  kBad: outside the cache (page 0 is read in its place, its scores
+  // become NaN and its values 0).  A half that no row sees has no page: page 0 is read, and nothing of it is used.
+  const uint32_t page_shift = 31 - __builtin_clz(a.layout.page_rows);
+  constexpr uint32_t kBad = 0x80000000u;
+  uint32_t ids[2];
+  auto find_pages = [&](int32_t index) {
+    const bool near = (uint32_t)high >> page_shift < kWave;   // all in the entries that every wave has
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int32_t column = (mine0 + (index + (int32_t)lane) * kWaves) * kTile + 16 * h;
+      const bool seen = index + (int32_t)lane < mine && column <= high && column + 15 >= low;
+      const uint32_t at = seen ? (uint32_t)column >> page_shift : 0u;
+      uint32_t id = near ? (uint32_t)__builtin_amdgcn_ds_bpermute((int)at * 4, (int)entry) : (uint32_t)table[at];
+      if (!seen) id = 0;
+      ids[h] = id < a.pages ? id : kBad;
+    }
+  };
+  find_pages(0);
+
+  // ---- a wave's ring: kStages tiles on their way
+  auto lds_address = [](const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
+  };
+  uint8_t* const ring = s_ring + wave * (kStages * S::kBytes);
+  const uint32_t ring_at = lds_address(ring);
+  const uint64_t page_bytes = a.layout.page();
+  const uint8_t* head_base = cache + (size_t)kv_head * a.layout.block();
+  const uint32_t column_of_lane = D == 64 ? (m & 7) : m;
+  const uint32_t lane_k = m * (D / 2) + (D == 64 ? (c / 2) * 16 : c * (D / 8));
+  const uint32_t lane_v = (c * (D / 8) + column_of_lane) * 16;
+  uint32_t bad_halves = 0;   // two bits a stage
+  auto ask = [&](int32_t index, uint32_t stage) {   // of this wave's tile `index`
+    bad_halves &= ~(3u << (2 * stage));
+    const uint32_t at = ring_at + stage * S::kBytes;
+    const int32_t tile = mine0 + index * kWaves;
+    if (index > 0 && (index & 63) == 0) find_pages(index);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int32_t column = tile * kTile + 16 * h;
+      const uint32_t found = __builtin_amdgcn_readlane(ids[h], index & 63), id = found & ~kBad;
+      if (found & kBad) bad_halves |= 1u << (2 * stage + h);
+      const uint32_t in_page = (uint32_t)column & (a.layout.page_rows - 1);
+      const uint8_t* block = uniform(head_base + id * page_bytes);
+      const uint8_t* keys = block + in_page * (D / 2);
+      const uint8_t* values = keys + a.layout.value_codes();
+#pragma unroll
+      for (int i = 0; i < S::kParts; ++i) {
+        stream_to_lds(at + S::kKeys + (h * S::kParts + i) * 1024, lane_k + 16 * i, keys);
+        stream_to_lds(at + S::kValues + (h * S::kParts + i) * 1024, lane_v + 256 * i, values);
+      }
+      const uint8_t* key_params = block + a.layout.key_params() + in_page * (NG * 4);
+      const uint8_t* value_params = block + a.layout.value_params() + in_page * (NG * 4);
+#pragma unroll
+      for (int i = 0; i < S::kWords; ++i) {   // (16 rows' parameters are 64 NG bytes: lanes past them repeat the last)
+        const uint32_t offset = min(lane * 4 + 256 * i, 64u * NG - 4);
+        stream_word_to_lds(at + S::kKeyParams + h * S::kParams + 256 * i, offset, key_params, false);
+        stream_word_to_lds(at + S::kValueParams + h * S::kParams + 256 * i, offset, value_params, false);
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kStages; ++i)
+    if (i < mine) ask(i, i);
+
+  // ---- queries as operands.  x * 2^e has its row's largest magnitude in [2^5, 2^6).  Codes enter the matrix cores
+  // as they are masked out of a word: the fp16 subnormals u 2^-24 and 16 u 2^-24, exact; their queries are x 2^(e+8)
+  // and x 2^(e+4).  A group's sum of products is then 2^(e-16) times its own; steps multiply it in f32, and the
+  // minima meet the group's sum of queries (fp16 hi + lo: 22 bits) in an instruction of their own.
+  half8_t qh[kSteps], ql[kF32 ? kSteps : 1], qs_h, qs_l;
+  float scale;
+  {
+    float most = 0.f;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[st][i] = live ? x[st][i] : 0.f;
+        most = fmaxf(most, fabsf(x[st][i]));
+      }
+    most = quarters_max(most);
+    int e = 0;
+    // (queries so small or large that the scale would leave f32's range with them are not normalised any further)
+    if (most > 0.f && most < INFINITY) e = max(min(6 - __builtin_amdgcn_frexp_expf(most), 100), __builtin_amdgcn_frexp_expf(a.scale) - 110);
+    scale = ldexpf(a.scale, (kF32 ? 2 : 16) - e);
+    float sums[NG] = {};
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float z = ldexpf(x[st][i], e), y = z * (!kF32 && (i & 2) ? 16.0f : 256.0f);   // elements 2, 3, 6, 7 lie four bits up
+        qh[st][i] = (_Float16)y;
+        if constexpr (kF32) ql[st][i] = (_Float16)(y - (float)qh[st][i]);
+        sum += z;
+      }
+      sums[st / kPerGroup] += quarters_sum(sum);
+    }
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {   // the groups along the contracted index, in lanes c = 0
+      const float y = c == 0 && g < NG ? sums[g < NG ? g : 0] : 0.f;
+      qs_h[g] = (_Float16)y;
+      qs_l[g] = (_Float16)(y - (float)qs_h[g]);
+    }
+  }
+
+  float4_t acc[kColumns][kOuts] = {}, base[kF32 ? kColumns : 1] = {};
+  float top = -INFINITY, sum = 0.f;
+  bool lost = false;   // a page outside the cache was seen
+
+  auto consume = [&](int32_t index, uint32_t stage, bool more) {
+    const int32_t column0 = (mine0 + index * kWaves) * kTile;
+    const uint8_t* at = ring + stage * S::kBytes;
+    uint32_t k[2][kSteps], own[2][NG], theirs[2][4 * NG];
+    uint4 v[2][kColumns], vp[2][kColumns];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < S::kParts; ++i) {
+        const uint8_t* piece = at + S::kKeys + (h * S::kParts + i) * 1024 + lane * 16;
+        if constexpr (D == 64) {
+          const uint2 w = *reinterpret_cast<const uint2*>(piece + (c & 1) * 8);
+          k[h][0] = w.x; k[h][1] = w.y;
+        } else {
+          const uint4 w = *reinterpret_cast<const uint4*>(piece);
+          k[h][4 * i] = w.x; k[h][4 * i + 1] = w.y; k[h][4 * i + 2] = w.z; k[h][4 * i + 3] = w.w;
+        }
+        v[h][i] = *reinterpret_cast<const uint4*>(at + S::kValues + (h * S::kParts + i) * 1024 + lane * 16);
+        vp[h][i] = *reinterpret_cast<const uint4*>(at + S::kValueParams + h * S::kParams + c * (NG * 16) +
+                                                   (column_of_lane + 16 * i) * 8 * NG / D * 16);
+      }
+      const uint8_t* params = at + S::kKeyParams + h * S::kParams;
+      load_words(params + m * (NG * 4), own[h]);
+      load_words(params + c * (NG * 16), theirs[h]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read before the stage is filled again
+    const bool bad[2] = {(bad_halves >> (2 * stage) & 1) != 0, (bad_halves >> (2 * stage) & 2) != 0};
+    if (more) ask(index + kStages, stage);
+
+    // some row does not see some column, or a page is bad
+    const bool edge = column0 < kv4_first_column(last_row, a.window) || column0 + kTile - 1 > first_row || bad[0] || bad[1];
+    if (edge) {
+      lost = lost || bad[0] || bad[1];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (bad[h]) {
+#pragma unroll
+          for (int g = 0; g < 4 * NG; ++g) theirs[h][g] = 0x7e007e00u;
+        }
+#pragma unroll
+        for (int i = 0; i < kColumns; ++i) {
+          uint32_t w[4] = {vp[h][i].x, vp[h][i].y, vp[h][i].z, vp[h][i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {   // columns that no row sees hold anything: 0 times it has to be 0
+            const int32_t column = column0 + 16 * h + 4 * (int32_t)c + j;
+            const uint32_t keep = column >= low && column <= high && !bad[h] ? 0xffffffffu : 0xffff0000u >> (16 * (j & 1));
+            w[j / 2] &= keep;
+            w[2 + j / 2] &= keep;
           }
-          const uint8_t* param = block + a.layout.key_param(in_page, g);
-          score = fmaf(half_at(param), codes, score);
-          score = fmaf(half_at(param + 2), sum, score);
+          vp[h][i] = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
     }
-    if (__syncthreads_or(bad)) {   // a page that is none of the cache's
-      if (tid < D) st<XT>(out, base + tid, NAN);
-      if (fault && tid == 0) *fault = 1u;
-      return;
+
+    float4_t sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      half8_t minima = {};
+#pragma unroll
+      for (int g = 0; g < NG; ++g) minima[g] = half2_of(own[h][g]).y;   // (lanes c > 0: times 0)
+      float4_t total = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, qs_l, float4_t{}, 0, 0, 0);
+      total = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, qs_h, total, 0, 0, 0);
+      total *= kF32 ? 0x1p-2f : 0x1p-16f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float4_t part = {};
+#pragma unroll
+        for (int st = g * kPerGroup; st < (g + 1) * kPerGroup; ++st) {
+          const uint32_t word = k[h][st], upper = word >> 8;
+          half2_t u[4] = {half2_of(word & 0x000F000Fu), half2_of(word & 0x00F000F0u), half2_of(upper & 0x000F000Fu),
+                          half2_of(upper & 0x00F000F0u)};
+          if constexpr (kF32) {
+            const half2_t low2 = {(_Float16)16384.0f, (_Float16)16384.0f}, high2 = {(_Float16)1024.0f, (_Float16)1024.0f};
+            u[0] *= low2;
+            u[1] *= high2;
+            u[2] *= low2;
+            u[3] *= high2;
+          }
+          const half8_t codes = join8(u[0], u[1], u[2], u[3]);
+          if constexpr (kF32) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, ql[st], part, 0, 0, 0);
+          part = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, qh[st], part, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) total[r] = scaled(theirs[h][r * NG + g], part[r], total[r]);
+      }
+      sc[h] = total;
     }
-    float top = score;
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
-    if (tid % kWave == 0) s_red[tid / kWave] = top;
-    __syncthreads();
-    top = m;
-    for (int w = 0; w < kThreads / kWave; ++w) top = fmaxf(top, s_red[w]);
-    const float keep = __builtin_amdgcn_exp2f(m - top);
-    m = top;
-    const float p = c <= position ? __builtin_amdgcn_exp2f(score - m) : 0.f;
-    s_p[tid] = p;
-    __syncthreads();
-    acc *= keep;
-    l *= keep;
-    for (uint32_t j = part; j < (uint32_t)kThreads && c0 + (int32_t)j <= position; j += kParts) {
-      const uint32_t cj = (uint32_t)c0 + j, in_page = cj & (a.layout.page_rows - 1);
-      const uint8_t* block =
-          cache + (size_t)table[cj / a.layout.page_rows] * a.layout.page() + (size_t)kv_head * a.layout.block();
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(block + a.layout.value_word(in_page, d / 8));
-      const uint8_t* param = block + a.layout.value_param(in_page, d / a.layout.group);
-      acc = fmaf(s_p[j], fmaf(half_at(param), (float)((word >> (4 * (d % 8))) & 15u), half_at(param + 8)), acc);
-      l += s_p[j];
+    // ---- softmax: lane (m, c) has columns 4 c .. 4 c + 3 of each half
+    if (edge) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int32_t column = column0 + 16 * h + 4 * (int32_t)c + r;
+          if (column < from || column > position) sc[h][r] = -INFINITY;
+        }
     }
-    __syncthreads();
+    float here = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                       fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    here = quarters_max(here) * scale;
+    if (__any(here > top)) {
+      const float now = fmaxf(here, top);
+      const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      sum *= keep;
+#pragma unroll
+      for (int i = 0; i < kColumns; ++i) {
+        if constexpr (kF32) base[i] *= keep;
+#pragma unroll
+        for (int f = 0; f < kOuts; ++f) acc[i][f] *= keep;
+      }
+    }
+    // f32 rows: weights are 2^10 times what they would be, so that their low parts are no subnormal numbers
+    const float shift = (top == -INFINITY ? 0.f : top) - (kF32 ? 10.0f : 0.0f);
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4], scale, -shift));
+      sum += p[j];
+    }
+    half8_t ph, pl;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ph[j] = (_Float16)p[j];
+      pl[j] = (_Float16)(p[j] - (float)ph[j]);
+    }
+
+    // ---- values: lane (i, c) has rows 4 c .. 4 c + 3 of each half, the same order as the weights
+#pragma unroll
+    for (int i = 0; i < kColumns; ++i) {
+      half2_t step[4], least[4];   // of rows (0, 1), (2, 3) of each half
+      step[0] = half2_of(vp[0][i].x); step[1] = half2_of(vp[0][i].y);
+      step[2] = half2_of(vp[1][i].x); step[3] = half2_of(vp[1][i].y);
+      least[0] = half2_of(vp[0][i].z); least[1] = half2_of(vp[0][i].w);
+      least[2] = half2_of(vp[1][i].z); least[3] = half2_of(vp[1][i].w);
+      half8_t fix = {};
+      bool any_fix = false;
+      if (edge) {
+        // a row that does not see a column of no numbers must not meet it as 0 * NaN: the column enters as 0
+        // and the rows that do see it are marked afterwards
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool sound = fabsf((float)step[j][e]) < INFINITY && fabsf((float)least[j][e]) < INFINITY;
+            fix[2 * j + e] = sound ? (_Float16)0.0f : (_Float16)1.0f;
+            if (!sound) step[j][e] = least[j][e] = (_Float16)0.0f;
+            any_fix = any_fix || !sound;
+          }
+        }
+      }
+      const uint32_t words[8] = {v[0][i].x, v[0][i].y, v[0][i].z, v[0][i].w,
+                                 v[1][i].x, v[1][i].y, v[1][i].z, v[1][i].w};
+#pragma unroll
+      for (int b = 0; b < kOuts / 2; ++b) {
+        const uint32_t byte = D == 64 ? b + (m >> 3) * 2 : b;
+        const uint32_t select = byte | 0x0c000c00u | (4 + byte) << 16;
+        half2_t lo2[4], hi2[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x = __builtin_amdgcn_perm(words[2 * j + 1], words[2 * j], select);
+          lo2[j] = low_codes(x);
+          hi2[j] = high_codes(x);
+        }
+        if constexpr (!kF32) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            lo2[j] = __builtin_elementwise_fma(lo2[j], step[j], least[j]);
+            hi2[j] = __builtin_elementwise_fma(hi2[j], step[j], least[j]);
+          }
+          const half8_t lo8 = join8(lo2[0], lo2[1], lo2[2], lo2[3]), hi8 = join8(hi2[0], hi2[1], hi2[2], hi2[3]);
+          acc[i][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo8, pl, acc[i][2 * b], 0, 0, 0);
+          acc[i][2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo8, ph, acc[i][2 * b], 0, 0, 0);
+          acc[i][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi8, pl, acc[i][2 * b + 1], 0, 0, 0);
+          acc[i][2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi8, ph, acc[i][2 * b + 1], 0, 0, 0);
+        } else {
+          half2_t rest[4];
+          auto add = [&](half2_t(&u)[4], float4_t& to) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const half2_t whole = u[j] * step[j];
+              rest[j] = __builtin_elementwise_fma(u[j], step[j], -whole);
+              u[j] = whole;
+            }
+            const half8_t hi = join8(u[0], u[1], u[2], u[3]);
+            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(join8(rest[0], rest[1], rest[2], rest[3]), ph, to, 0, 0, 0);
+            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pl, to, 0, 0, 0);
+            to = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ph, to, 0, 0, 0);
+          };
+          add(lo2, acc[i][2 * b]);
+          add(hi2, acc[i][2 * b + 1]);
+        }
+      }
+      if constexpr (kF32) {
+        const half8_t minima = join8(least[0], least[1], least[2], least[3]);
+        base[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, pl, base[i], 0, 0, 0);
+        base[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, ph, base[i], 0, 0, 0);
+      }
+      if (edge && __any(any_fix)) {
+        half8_t sees;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int32_t column = column0 + 16 * (j / 4) + 4 * (int32_t)c + j % 4;
+          sees[j] = column < from || column > position ? (_Float16)0.0f : (_Float16)1.0f;
+        }
+        const float4_t hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(fix, sees, float4_t{}, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (hits[r] > 0.f)
+#pragma unroll
+            for (int f = 0; f < kOuts; ++f) acc[i][f][r] = __builtin_nanf("");
+      }
+    }
+  };
+
+  for (int32_t i = 0; i < mine; ++i) {
+    const int32_t behind = min(mine - 1 - i, (int32_t)kStages - 1);   // tiles asked for behind this one
+    if (behind >= 2) wait_vm<2 * S::kLoads>();
+    else if (behind == 1) wait_vm<S::kLoads>();
+    else wait_vm<0>();
+    consume(i, (uint32_t)i % kStages, i + kStages < mine);
   }
-  s_acc[tid] = acc;
-  s_p[tid] = l;
+  if (lost && fault && lane == 0) *fault = 1u;
+  sum = quarters_sum(sum);
+
+  // ---- the waves' states become one, in order
+  __syncthreads();   // (every wave is through its ring)
+  float* s_acc = reinterpret_cast<float*>(s_ring);
+  if (c == 0) {
+    s_max[wave][m] = top;
+    s_sum[wave][m] = sum;
+  }
+  if (live) {
+    float* row = s_acc + (wave * a.partial_rows + m) * kStride;
+#pragma unroll
+    for (int i = 0; i < kColumns; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t n = 4 * c + r;
+        const uint32_t d = D == 64 ? 8 * (n & 7) + 4 * (n >> 3) : 8 * (n + 16 * i);
+#pragma unroll
+        for (int f = 0; f < kOuts; f += 4) {
+          float4_t o = {acc[i][f][r], acc[i][f + 1][r], acc[i][f + 2][r], acc[i][f + 3][r]};
+          if constexpr (kF32) o += base[i][r];
+          *reinterpret_cast<float4_t*>(row + d + f) = o;
+        }
+      }
+  }
   __syncthreads();
-  if (tid < D) {
-    float total = 0.f, sum = 0.f;
-    for (int w = 0; w < kParts; ++w) {
-      total += s_acc[w * D + tid];
-      sum += s_p[w * D + tid];
+  // a part: partial_rows x D sums, then (max, sum) of each row
+  const size_t part_size = (size_t)a.partial_rows * (D + 2);
+  float* const parts = a.partials + (size_t)unit * a.max_splits * part_size;
+  float* const part = parts + split * part_size;
+  for (uint32_t e = tid; e < count * D; e += kThreads) {
+    const uint32_t row = e / D, d = e % D;
+    float most = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_max[w][row]);
+    const float ref = most == -INFINITY ? 0.f : most;
+    float total = 0.f, weight = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float k = __builtin_amdgcn_exp2f(s_max[w][row] - ref);
+      total = fmaf(k, s_acc[(w * a.partial_rows + row) * kStride + d], total);
+      weight = fmaf(k, s_sum[w][row], weight);
     }
-    st<XT>(out, base + tid, total / sum);
+    if (nsplit == 1) {
+      out[out_row(row) + d] = from_f32<XT>(total / weight);
+    } else {
+      publish(part + e, total);
+      if (d == 0) {
+        publish(part + a.partial_rows * D + 2 * row, most);
+        publish(part + a.partial_rows * D + 2 * row + 1, weight);
+      }
+    }
+  }
+  if (nsplit == 1) return;
+  // the workgroup that arrives last joins the parts in order, whichever it is
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  uint32_t* ticket = a.tickets + (size_t)unit * kTicketStride;
+  if (tid == 0) s_ticket = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (s_ticket + 1 != nsplit) return;
+  if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  float* s_part = s_acc;   // [row][nsplit] (max, sum)
+  for (uint32_t i = tid; i < nsplit * count; i += kThreads) {
+    const float* state = parts + (i / count) * part_size + a.partial_rows * D + 2 * (i % count);
+    float* to = s_part + ((i % count) * nsplit + i / count) * 2;
+    to[0] = observe(state);
+    to[1] = observe(state + 1);
+  }
+  __syncthreads();
+  for (uint32_t e = 2 * tid; e < count * D; e += 2 * kThreads) {
+    const float* states = s_part + (e / D) * nsplit * 2;
+    float most = -INFINITY, weight = 0.f;
+    float2_t total = {0.f, 0.f};
+    for (uint32_t p = 0; p < nsplit; ++p) most = fmaxf(most, states[2 * p]);
+    const float ref = most == -INFINITY ? 0.f : most;
+    for (uint32_t p0 = 0; p0 < nsplit; p0 += kJoin) {
+      float2_t o[kJoin];
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i) o[i] = observe2(parts + min(p0 + i, nsplit - 1) * part_size + e);
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i) {
+        if (p0 + i < nsplit) {
+          const float k = __builtin_amdgcn_exp2f(states[2 * (p0 + i)] - ref);
+          total[0] = fmaf(k, o[i][0], total[0]);
+          total[1] = fmaf(k, o[i][1], total[1]);
+          weight = fmaf(k, states[2 * (p0 + i) + 1], weight);
+        }
+      }
+    }
+    XT* to = out + out_row(e / D) + e % D;
+    to[0] = from_f32<XT>(total[0] / weight);
+    to[1] = from_f32<XT>(total[1] / weight);
   }
 }
+
+// How a call's columns are dealt.
+struct AttentionPlan {
+  uint32_t rows, row_tiles, units, max_splits, partial_rows, least;
+  float share_of_work;
+  size_t bytes;
+};
+// Eight waves (two a SIMD) while their registers allow it: half as many parts to join as with four, twice a CU.
+constexpr int waves_of(int depth) { return depth == 256 ? 4 : 8; }
+// One workgroup a CU: with 512 and 1024 of them 131000 columns took 49.4 us, with 256 39.8.
+constexpr uint32_t kFill = 256;
+constexpr uint32_t kMostGroups = 2048;   // in a grid, those without a split among them
+constexpr uint32_t kMostSplits = 64;
+AttentionPlan plan_attention(const Kv4Shape& s, uint32_t max_columns) {
+  AttentionPlan p;
+  p.rows = kv4_rows(s.max_query, s.total_rows);
+  const uint64_t pairs = (uint64_t)p.rows * (s.heads / s.kv_heads);
+  p.row_tiles = (uint32_t)((pairs + kRows - 1) / kRows);
+  p.partial_rows = pairs < kRows ? (uint32_t)pairs : kRows;
+  const uint64_t units = (uint64_t)s.nseq * s.kv_heads * p.row_tiles;
+  p.units = (uint32_t)(units < 0xffffffffu ? units : 0xffffffffu);
+  // a split has two tiles a wave at least: joining two parts costs about as much as a tile more
+  p.least = 2 * waves_of(s.depth);
+  const uint64_t tiles = ((uint64_t)max_columns + kTile - 1) / kTile + 1, most = (tiles + p.least - 1) / p.least;
+  uint64_t splits = units ? kMostGroups / units : 1;
+  splits = splits > kMostSplits ? kMostSplits : splits;
+  splits = splits > most ? most : splits;
+  p.max_splits = splits < 1 ? 1 : (uint32_t)splits;   // (with more units than kMostGroups, and so than counters: one)
+  p.share_of_work = (float)s.kv_heads * (float)p.row_tiles / kFill;
+  p.bytes = splits > 1 ? (size_t)units * splits * p.partial_rows * (s.depth + 2) * sizeof(float) : 0;
+  return p;
+}
+static_assert(kMostGroups <= kTicketSlots, "a counter a unit");
 
 }  // namespace
 
@@ -151,7 +701,7 @@ int32_t krm_kv4_attention_workspace(uint32_t nseq, uint32_t max_query, uint32_t 
   KRM_REQUIRE(nullptr, kv4_shape_ok(shape, why, sizeof why), "krm_kv4_attention_workspace: %s", why);
   KRM_REQUIRE(nullptr, max_columns <= 0x7fffffffu, "krm_kv4_attention_workspace: max_columns %u", max_columns);
   (void)window;
-  *bytes = 0;
+  *bytes = plan_attention(shape, max_columns).bytes;
   return KRM_OK;
 }
 
@@ -166,7 +716,8 @@ int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_t
   const Kv4Shape shape{nseq, max_query, total_rows, heads, kv_heads, depth, group, page_rows, pages, table_stride};
   char why[128];
   KRM_REQUIRE(ctx, kv4_shape_ok(shape, why, sizeof why), "krm_kv4_attention: %s", why);
-  KRM_REQUIRE(ctx, std::isfinite(half_scale * half_scale), "krm_kv4_attention: half_scale");
+  const float scale = half_scale * half_scale * kLog2e;
+  KRM_REQUIRE(ctx, std::isnormal(scale), "krm_kv4_attention: half_scale");
   KRM_REQUIRE(ctx, max_columns <= 0x7fffffffu && (max_columns >= kv4_rows(max_query, total_rows)),
               "krm_kv4_attention: max_columns %u beside max_query %u", max_columns, max_query);
   if (nseq == 0 || total_rows == 0) return KRM_OK;
@@ -176,24 +727,43 @@ int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_t
                        aligned(workspace, 16),
               "krm_kv4_attention: misaligned buffer (rows, cache and workspace: 16 bytes)");
   KRM_REQUIRE(ctx, q != out, "krm_kv4_attention: out is q");
-  (void)workspace_bytes;
+  const AttentionPlan plan = plan_attention(shape, max_columns);
+  const uint32_t share = heads / kv_heads;
+  KRM_REQUIRE(ctx, plan.units <= 0x7fffffu && (uint64_t)plan.rows * share <= 1u << 24,
+              "krm_kv4_attention: %u sequences of %u rows of %u heads are more than one call takes", nseq, plan.rows, heads);
+  if (plan.max_splits > 1) {
+    KRM_REQUIRE(ctx, workspace && workspace_bytes >= plan.bytes, "krm_kv4_attention: workspace of %zu bytes, %zu needed",
+                workspace ? workspace_bytes : (size_t)0, plan.bytes);
+    KRM_TRY(needs_serial_scratch(ctx, "krm_kv4_attention"));
+  }
   const AttentionArgs a{{depth, group, page_rows, kv_heads},
                         {total_rows, max_query, max_columns, table_stride, page_rows},
-                        heads, pages, window, half_scale * half_scale * 1.4426950408889634f};
-  const uint32_t rows = kv4_rows(max_query, total_rows);
-  KRM_REQUIRE(ctx, (uint64_t)rows * heads <= 0x7fffffu, "krm_kv4_attention: %u rows of %u heads", rows, heads);
-#define KRM_ATTENTION(XT, D)                                                                                    \
-  kv4_attention_kernel<XT, D><<<dim3(rows * heads, nseq), dim3(kThreads), 0, ctx->stream>>>(                \
-      ptr<const XT>(q), ptr<const uint8_t>(cache), ptr<const int32_t>(page_table_i32),                           \
+                        nseq, heads, pages, window, share, 1.0f / share, 1.0f / plan.row_tiles,
+                        1.0f / ((float)kv_heads * plan.row_tiles), plan.row_tiles, plan.max_splits, plan.partial_rows,
+                        plan.least, plan.share_of_work, scale, ptr<float>(workspace), ctx->tickets};
+  const dim3 grid(plan.units, plan.max_splits);
+  const int waves = waves_of(depth);
+  const size_t joined = (size_t)waves * plan.partial_rows * (depth + 4) * sizeof(float);
+#define KRM_ATTENTION(XT, D, NG)                                                                                 \
+  const size_t ring = (size_t)waves * kStages * Stage<D, NG>::kBytes, lds = ring > joined ? ring : joined;       \
+  kv4_decode_kernel<XT, D, NG, waves_of(D)><<<grid, dim3(waves * kWave), lds, ctx->stream>>>(                                       \
+      ptr<const XT>(q), ptr<const uint8_t>(cache), ptr<const int32_t>(page_table_i32),                            \
       ptr<const int32_t>(cu_rows_i32), ptr<const int32_t>(lens_i32), ptr<XT>(out), ptr<uint32_t>(fault_u32), a)
-#define KRM_ATTENTION_D(XT)                      \
-  if (depth == 64) KRM_ATTENTION(XT, 64);        \
-  else if (depth == 128) KRM_ATTENTION(XT, 128); \
-  else KRM_ATTENTION(XT, 256)
-  if (io_dtype == KRM_F32) { KRM_ATTENTION_D(float); } else { KRM_ATTENTION_D(__half); }
+#define KRM_ATTENTION_D(XT)                                                              \
+  switch (depth * 16 + depth / group) {                                                  \
+    case 64 * 16 + 1: { KRM_ATTENTION(XT, 64, 1); break; }                                  \
+    case 64 * 16 + 2: { KRM_ATTENTION(XT, 64, 2); break; }                                  \
+    case 128 * 16 + 1: { KRM_ATTENTION(XT, 128, 1); break; }                                \
+    case 128 * 16 + 2: { KRM_ATTENTION(XT, 128, 2); break; }                                \
+    case 128 * 16 + 4: { KRM_ATTENTION(XT, 128, 4); break; }                                \
+    case 256 * 16 + 2: { KRM_ATTENTION(XT, 256, 2); break; }                                \
+    case 256 * 16 + 4: { KRM_ATTENTION(XT, 256, 4); break; }                                \
+    default: { KRM_ATTENTION(XT, 256, 8); }                                          \
+  }
+  if (io_dtype == KRM_F32) { KRM_ATTENTION_D(float) } else { KRM_ATTENTION_D(__half) }
 #undef KRM_ATTENTION_D
 #undef KRM_ATTENTION
-  return launched(ctx, "kv4_attention_kernel");
+  return launched(ctx, "kv4_decode_kernel");
 }
 
 }  // extern "C"

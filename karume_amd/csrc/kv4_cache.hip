@@ -8,6 +8,7 @@
 #include "kv4_plan.h"
 #include "krm_internal.h"
 #include "rotary.h"
+#include "rows8.h"
 
 using namespace krm;
 
@@ -15,32 +16,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kPiece = 8;   // elements of a thread: one word of codes
-
-__device__ inline void load8(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ inline void load8(const __half* p, float (&v)[8]) {
-  const uint4 raw = *reinterpret_cast<const uint4*>(p);
-  const __half2* h = reinterpret_cast<const __half2*>(&raw);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __low2float(h[i]);
-    v[2 * i + 1] = __high2float(h[i]);
-  }
-}
-__device__ inline void store8(float* p, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ inline void store8(__half* p, const float (&v)[8]) {
-  uint4 raw;
-  __half2* h = reinterpret_cast<__half2*>(&raw);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __halves2half2(__float2half_rn(v[2 * i]), __float2half_rn(v[2 * i + 1]));
-  *reinterpret_cast<uint4*>(p) = raw;
-}
 
 __device__ inline uint16_t bits_of(__half h) { return __half_as_ushort(h); }
 __device__ inline float value_of(uint16_t b) { return __half2float(__ushort_as_half(b)); }
