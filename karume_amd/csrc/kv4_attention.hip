@@ -66,14 +66,17 @@ __device__ inline half2_t half2_of(uint32_t w) { return __builtin_bit_cast(half2
 __device__ inline half8_t join8(half2_t a, half2_t b, half2_t c, half2_t d) {
   return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
-// Codes at the bottom (u) or four bits up (16 u) of the halves of a word, as the exact integers.
+// Codes at the bottom (u) or four bits up (16 u) of the halves of a word, as the exact integers u - LESS.
+template <int LESS>
 __device__ inline half2_t low_codes(uint32_t x) {
-  return half2_of(and_or(x, 0x000F000Fu, 0x64006400u)) - half2_t{(_Float16)1024.0f, (_Float16)1024.0f};
+  return half2_of(and_or(x, 0x000F000Fu, 0x64006400u)) -
+         half2_t{(_Float16)(1024.0f + LESS), (_Float16)(1024.0f + LESS)};
 }
+template <int LESS>
 __device__ inline half2_t high_codes(uint32_t x) {
   return __builtin_elementwise_fma(half2_of(and_or(x, 0x00F000F0u, 0x64006400u)),
                                    half2_t{(_Float16)0.0625f, (_Float16)0.0625f},
-                                   half2_t{(_Float16)-64.0f, (_Float16)-64.0f});
+                                   half2_t{(_Float16)(-64.0f - LESS), (_Float16)(-64.0f - LESS)});
 }
 // step * x + sum with a step in fp16 (one mixed instruction).
 __device__ inline float scaled(uint32_t params, float x, float sum) { return fmaf((float)half2_of(params).x, x, sum); }
@@ -395,7 +398,18 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
       half8_t minima = {};
 #pragma unroll
       for (int g = 0; g < NG; ++g) minima[g] = half2_of(own[h][g]).y;   // (lanes c > 0: times 0)
-      float4_t total = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, qs_l, float4_t{}, 0, 0, 0);
+      float4_t total = {};
+      if constexpr (kF32) {   // step * 8 + minimum = hi + lo
+        half8_t rest = {};
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float x = scaled(own[h][g], 8.0f, (float)minima[g]);
+          minima[g] = (_Float16)x;
+          rest[g] = (_Float16)(x - (float)minima[g]);
+        }
+        total = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, qs_h, total, 0, 0, 0);
+      }
+      total = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, qs_l, total, 0, 0, 0);
       total = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, qs_h, total, 0, 0, 0);
       total *= kF32 ? 0x1p-2f : 0x1p-16f;
 #pragma unroll
@@ -407,11 +421,14 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
           half2_t u[4] = {half2_of(word & 0x000F000Fu), half2_of(word & 0x00F000F0u), half2_of(upper & 0x000F000Fu),
                           half2_of(upper & 0x00F000F0u)};
           if constexpr (kF32) {
+            // (u - 8) / 1024: the matrix cores drop low bits of sums with subnormal numbers, and sums around zero
+            // lose less to the minima's
             const half2_t low2 = {(_Float16)16384.0f, (_Float16)16384.0f}, high2 = {(_Float16)1024.0f, (_Float16)1024.0f};
-            u[0] *= low2;
-            u[1] *= high2;
-            u[2] *= low2;
-            u[3] *= high2;
+            const half2_t middle = {(_Float16)-0.0078125f, (_Float16)-0.0078125f};
+            u[0] = __builtin_elementwise_fma(u[0], low2, middle);
+            u[1] = __builtin_elementwise_fma(u[1], high2, middle);
+            u[2] = __builtin_elementwise_fma(u[2], low2, middle);
+            u[3] = __builtin_elementwise_fma(u[3], high2, middle);
           }
           const half8_t codes = join8(u[0], u[1], u[2], u[3]);
           if constexpr (kF32) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, ql[st], part, 0, 0, 0);
@@ -496,8 +513,9 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t x = __builtin_amdgcn_perm(words[2 * j + 1], words[2 * j], select);
-          lo2[j] = low_codes(x);
-          hi2[j] = high_codes(x);
+          // (f32 rows: sums around zero, beside which the minima's are small; a mean of many values is far below 8 steps)
+          lo2[j] = low_codes<kF32 ? 8 : 0>(x);
+          hi2[j] = high_codes<kF32 ? 8 : 0>(x);
         }
         if constexpr (!kF32) {
 #pragma unroll
@@ -529,7 +547,14 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
         }
       }
       if constexpr (kF32) {
-        const half8_t minima = join8(least[0], least[1], least[2], least[3]);
+        half8_t minima, rest2;   // step * 8 + minimum = hi + lo
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float x = fmaf((float)step[j / 2][j % 2], 8.0f, (float)least[j / 2][j % 2]);
+          minima[j] = (_Float16)x;
+          rest2[j] = (_Float16)(x - (float)minima[j]);
+        }
+        base[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest2, ph, base[i], 0, 0, 0);
         base[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, pl, base[i], 0, 0, 0);
         base[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, ph, base[i], 0, 0, 0);
       }
