@@ -2,9 +2,7 @@
 //
 // Row r of a sequence stands at column p = len - rows + r and sees columns max(0, p - window + 1) .. p:
 //   out = sum_c softmax_c(scale^2 q . k_c) v_c,   k_c = step * code + minimum, v_c alike.
-#include "i4_codes.h"
-#include "kv4_plan.h"
-#include "krm_internal.h"
+#include "kv4_attention.h"
 #include "lds_stream.h"
 #include "rows8.h"
 
@@ -14,88 +12,10 @@ using namespace krm;
 
 namespace {
 
-typedef float float4_t __attribute__((ext_vector_type(4)));
-typedef float float2_t __attribute__((ext_vector_type(2)));
-
 constexpr int kStages = 2;         // tiles of a wave on their way
 constexpr int kTile = 32;          // columns a wave takes at a time
-constexpr int kJoin = 32;           // parts whose sums are asked for together
 constexpr int kRows = 16;          // (row, head) pairs of a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
-
-struct AttentionArgs {
-  Kv4Layout layout;
-  Kv4Limits limits;
-  uint32_t nseq, heads, pages, window;
-  uint32_t share;          // query heads of a kv head
-  float share_inverse, row_tiles_inverse, of_sequence_inverse;
-  uint32_t row_tiles;      // blocks of kRows (row, head) pairs of a kv head
-  uint32_t max_splits;     // workgroups that one block's columns are dealt to at most
-  uint32_t partial_rows;   // rows that a partial has room for
-  uint32_t least;          // tiles, at least, of a split
-  float share_of_work;     // of all sequences' tiles, in one workgroup
-  float scale;             // half_scale^2 * log2 e: scores are kept in base 2
-  float* partials;         // [unit][split]: partial_rows x D sums, then partial_rows x (max, sum)
-  uint32_t* tickets;
-};
-
-// Device-scope store / load of one float: written through to (read from) memory that every XCD sees.
-__device__ inline void publish(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ inline float observe(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
-__device__ inline float2_t observe2(const float* p) {
-  return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
-
-// Over the lanes 16, 32 and 48 apart.
-template <typename F>
-__device__ inline float across_quarters(float x, F join) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = join(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return join(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ inline float quarters_max(float x) {
-  return across_quarters(x, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ inline float quarters_sum(float x) {
-  return across_quarters(x, [](float a, float b) { return a + b; });
-}
-
-__device__ inline half2_t half2_of(uint32_t w) { return __builtin_bit_cast(half2_t, w); }
-__device__ inline half8_t join8(half2_t a, half2_t b, half2_t c, half2_t d) {
-  return half8_t{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-// Codes at the bottom (u) or four bits up (16 u) of the halves of a word, as the exact integers u - LESS.
-template <int LESS>
-__device__ inline half2_t low_codes(uint32_t x) {
-  return half2_of(and_or(x, 0x000F000Fu, 0x64006400u)) -
-         half2_t{(_Float16)(1024.0f + LESS), (_Float16)(1024.0f + LESS)};
-}
-template <int LESS>
-__device__ inline half2_t high_codes(uint32_t x) {
-  return __builtin_elementwise_fma(half2_of(and_or(x, 0x00F000F0u, 0x64006400u)),
-                                   half2_t{(_Float16)0.0625f, (_Float16)0.0625f},
-                                   half2_t{(_Float16)(-64.0f - LESS), (_Float16)(-64.0f - LESS)});
-}
-// step * x + sum with a step in fp16 (one mixed instruction).
-__device__ inline float scaled(uint32_t params, float x, float sum) { return fmaf((float)half2_of(params).x, x, sum); }
-
-template <int N>
-__device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
-  if constexpr (N == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  } else if constexpr (N == 2) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
-    w[0] = a.x; w[1] = a.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 a = *reinterpret_cast<const uint4*>(p + 16 * i);
-      w[4 * i] = a.x; w[4 * i + 1] = a.y; w[4 * i + 2] = a.z; w[4 * i + 3] = a.w;
-    }
-  }
-}
 
 // What a wave needs of 32 columns, two halves of 16, and where it lies in the wave's part of LDS.  Lane (i = lane %
 // 16, c = lane / 16) of an operand needs of each half
@@ -115,37 +35,11 @@ struct Stage {
   static constexpr int kLoads = 4 * kParts + 4 * kWords;      // that fill it
 };
 
-// The same address in every lane, in scalar registers whatever the compiler made of it.
-__device__ inline const uint8_t* uniform(const uint8_t* p) {
-  const uint64_t at = (uint64_t)p;
-  return (const uint8_t*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
-                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at));
-}
-// x / d for x up to 2^24, `inverse` = 1 / d: the quotient in floating point, put right by the remainder.
-__device__ inline uint32_t divided(uint32_t x, uint32_t d, float inverse) {
-  const uint32_t guess = (uint32_t)((float)x * inverse);
-  const int32_t rest = (int32_t)(x - guess * d);
-  return rest < 0 ? guess - 1 : rest >= (int32_t)d ? guess + 1 : guess;
-}
-// Over all lanes.
-__device__ inline float wave_sum(float x) {
-#define KRM_ADD_DPP(CTRL, ROWS) \
-  x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false))
-  KRM_ADD_DPP(0x111, 0xf);   // row_shr:1
-  KRM_ADD_DPP(0x112, 0xf);
-  KRM_ADD_DPP(0x114, 0xf);
-  KRM_ADD_DPP(0x118, 0xf);
-  KRM_ADD_DPP(0x142, 0xa);   // row_bcast:15
-  KRM_ADD_DPP(0x143, 0xc);   // row_bcast:31
-#undef KRM_ADD_DPP
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
-}
-
 template <typename XT, int D, int NG, int kWaves>
 __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
     const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table,
     const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens, XT* __restrict__ out,
-    uint32_t* __restrict__ fault, AttentionArgs a) {
+    uint32_t* __restrict__ fault, Kv4Attention a) {
   constexpr bool kF32 = sizeof(XT) == 4;
   constexpr int kThreads = kWaves * kWave;
   using S = Stage<D, NG>;
@@ -155,77 +49,30 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
   constexpr int kStride = D + 4;                // of a row in LDS
   extern __shared__ __align__(16) uint8_t s_ring[];   // [wave][stage]; behind the tiles [wave][partial_rows][kStride] f32
   __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
-  __shared__ uint32_t s_ticket;
 
   const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  // Workgroups go to the XCDs in turn: a unit (sequence, kv head, block of rows) has its next split on the next XCD,
-  // so that neither first splits nor a long sequence gather on one of them.
-  const uint32_t split = blockIdx.y, units = gridDim.x, of_sequence = a.layout.kv_heads * a.row_tiles;
-  uint32_t unit = blockIdx.x;
-  if (split) {
-    unit += units > split ? split : split % units;
-    if (unit >= units) unit -= units;
-  }
-  const uint32_t seq = divided(unit, of_sequence, a.of_sequence_inverse), in_sequence = unit - seq * of_sequence;
-  const uint32_t kv_head = divided(in_sequence, a.row_tiles, a.row_tiles_inverse);
-  const uint32_t pair0 = (in_sequence - kv_head * a.row_tiles) * kRows;   // first (row, head) pair of this workgroup
-  // ---- everything that its place alone tells: the sequence's words, its first 64 pages, the step's lengths
-  const int32_t* table = page_table + (size_t)seq * a.limits.table_stride;
+  Work w;
+  uint32_t block;
+  find_unit(a, w, block);
+  // the sequence's first 64 pages are asked for beside its lengths
+  const int32_t* table = page_table + (size_t)w.seq * a.limits.table_stride;
   const uint32_t entry = (uint32_t)table[min(lane, a.limits.table_stride - 1)];
-  float work = 0.f;
-  if (a.max_splits > 1) {
-    for (uint32_t i = lane; i < a.nseq; i += kWave) {
-      const uint32_t n = min((uint32_t)max(lens[i], 0), a.limits.max_columns);
-      work += (float)((a.window ? min(n, a.window) : n) / kTile + 1);
-    }
-  }
-  const int32_t cu0 = cu_rows[seq], cu1 = cu_rows[seq + 1];
-  const Kv4Sequence s = kv4_sequence(cu0, cu1, lens[seq], a.limits);
-  const bool in_rows = cu0 >= 0 && cu1 >= cu0 && (uint32_t)cu1 <= a.limits.total_rows;
-  if (!s.ok && fault && split == 0 && tid == 0) *fault = 1u;
-  if (!in_rows) return;
-  const uint32_t pairs = (uint32_t)(cu1 - cu0) * a.share;
-  if (pair0 >= pairs) return;
-  const uint32_t count = min((uint32_t)kRows, pairs - pair0);
-  const uint32_t row0 = divided(pair0, a.share, a.share_inverse), head0 = pair0 - row0 * a.share;
-  auto row_of = [&](uint32_t m) { return divided(head0 + m, a.share, a.share_inverse); };   // of pair m, from row0 on
-  auto out_row = [&](uint32_t m) -> size_t {   // of pair m: its first element
-    const uint32_t row = row_of(m), head = kv_head * a.share + head0 + m - row * a.share;
-    return (((size_t)(uint32_t)cu0 + row0 + row) * a.heads + head) * D;
-  };
-  if (!s.ok) {
-    if (split == 0)
-      for (uint32_t e = tid; e < count * D; e += kThreads) out[out_row(e / D) + e % D] = from_f32<XT>(NAN);
-    return;
-  }
-  // columns that any of the rows sees, and their tiles
-  const int32_t first_row = s.len - s.rows + (int32_t)row0, last_row = first_row + (int32_t)row_of(count - 1);
-  const int32_t low = kv4_first_column(first_row, a.window), high = last_row;
-  const int32_t tile0 = low / kTile;
-  const uint32_t tiles = (uint32_t)(high / kTile - tile0 + 1);
-  uint32_t per = tiles, nsplit = 1;
-  if (a.max_splits > 1) {
-    // the step's tiles, as far as they go by the lengths, are dealt evenly to the workgroups that fit the machine
-    per = max((uint32_t)(wave_sum(work) * a.share_of_work), a.least) + kWaves - 1;
-    per = max(per / kWaves * kWaves, (tiles + a.max_splits - 1) / a.max_splits);
-    nsplit = (tiles + per - 1) / per;
-    if (split >= nsplit) return;
-  }
-  const int32_t begin = tile0 + (int32_t)min(split * per, tiles);
-  const int32_t end = tile0 + (int32_t)min((split + 1) * per, tiles);
+  if (!find_work<XT, D, kThreads, kRows, kTile, kWaves>(a, w, block, cu_rows, lens, out, fault)) return;
+  const uint32_t count = w.count;
+  const int32_t first_row = w.first_row, last_row = w.last_row, low = w.low, high = w.high;
   // this wave's tiles are mine0, mine0 + kWaves, .. (the waves' next tiles lie together: in one long run for each wave
   // 131000 columns took 44.4 us, so 39.8)
-  const int32_t mine0 = begin + (int32_t)wave;
-  const int32_t mine = mine0 < end ? (int32_t)((uint32_t)(end - mine0 + kWaves - 1) / kWaves) : 0;
+  const int32_t mine0 = w.begin + (int32_t)wave;
+  const int32_t mine = mine0 < w.end ? (int32_t)((uint32_t)(w.end - mine0 + kWaves - 1) / kWaves) : 0;
 
   // ---- the queries: lane (m = lane % 16, c): elements 32 s + 8 c .. + 7 of pair m for each step s
   const uint32_t m = lane & 15, c = lane >> 4;
   const bool live = m < count;
-  const int32_t position = first_row + (int32_t)(live ? row_of(m) : 0);
+  const int32_t position = first_row + (int32_t)row_of(a, w, live ? m : 0);
   const int32_t from = kv4_first_column(position, a.window);
   float x[kSteps][8];
   {
-    const XT* src = q + out_row(live ? m : 0) + 8 * c;
+    const XT* src = q + row_at(a, w, live ? m : 0, D) + 8 * c;
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) load8(src + 32 * st, x[st]);
   }
@@ -255,7 +102,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
   uint8_t* const ring = s_ring + wave * (kStages * S::kBytes);
   const uint32_t ring_at = lds_address(ring);
   const uint64_t page_bytes = a.layout.page();
-  const uint8_t* head_base = cache + (size_t)kv_head * a.layout.block();
+  const uint8_t* head_base = cache + (size_t)w.kv_head * a.layout.block();
   const uint32_t column_of_lane = D == 64 ? (m & 7) : m;
   const uint32_t lane_k = m * (D / 2) + (D == 64 ? (c / 2) * 16 : c * (D / 8));
   const uint32_t lane_v = (c * (D / 8) + column_of_lane) * 16;
@@ -405,7 +252,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
         for (int g = 0; g < NG; ++g) {
           const float x = scaled(own[h][g], 8.0f, (float)minima[g]);
           minima[g] = (_Float16)x;
-          rest[g] = (_Float16)(x - (float)minima[g]);
+          rest[g] = less(x, minima[g]);
         }
         total = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest, qs_h, total, 0, 0, 0);
       }
@@ -476,7 +323,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       ph[j] = (_Float16)p[j];
-      pl[j] = (_Float16)(p[j] - (float)ph[j]);
+      pl[j] = less(p[j], ph[j]);
     }
 
     // ---- values: lane (i, c) has rows 4 c .. 4 c + 3 of each half, the same order as the weights
@@ -552,7 +399,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
         for (int j = 0; j < 8; ++j) {
           const float x = fmaf((float)step[j / 2][j % 2], 8.0f, (float)least[j / 2][j % 2]);
           minima[j] = (_Float16)x;
-          rest2[j] = (_Float16)(x - (float)minima[j]);
+          rest2[j] = less(x, minima[j]);
         }
         base[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(rest2, ph, base[i], 0, 0, 0);
         base[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(minima, pl, base[i], 0, 0, 0);
@@ -611,8 +458,8 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
   __syncthreads();
   // a part: partial_rows x D sums, then (max, sum) of each row
   const size_t part_size = (size_t)a.partial_rows * (D + 2);
-  float* const parts = a.partials + (size_t)unit * a.max_splits * part_size;
-  float* const part = parts + split * part_size;
+  float* const parts = a.partials + (size_t)w.unit * a.max_splits * part_size;
+  float* const part = parts + w.split * part_size;
   for (uint32_t e = tid; e < count * D; e += kThreads) {
     const uint32_t row = e / D, d = e % D;
     float most = -INFINITY;
@@ -626,8 +473,8 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
       total = fmaf(k, s_acc[(w * a.partial_rows + row) * kStride + d], total);
       weight = fmaf(k, s_sum[w][row], weight);
     }
-    if (nsplit == 1) {
-      out[out_row(row) + d] = from_f32<XT>(total / weight);
+    if (w.nsplit == 1) {
+      out[row_at(a, w, row, D) + d] = from_f32<XT>(total / weight);
     } else {
       publish(part + e, total);
       if (d == 0) {
@@ -636,81 +483,71 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
       }
     }
   }
-  if (nsplit == 1) return;
-  // the workgroup that arrives last joins the parts in order, whichever it is
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  uint32_t* ticket = a.tickets + (size_t)unit * kTicketStride;
-  if (tid == 0) s_ticket = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  if (s_ticket + 1 != nsplit) return;
-  if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  float* s_part = s_acc;   // [row][nsplit] (max, sum)
-  for (uint32_t i = tid; i < nsplit * count; i += kThreads) {
-    const float* state = parts + (i / count) * part_size + a.partial_rows * D + 2 * (i % count);
-    float* to = s_part + ((i % count) * nsplit + i / count) * 2;
-    to[0] = observe(state);
-    to[1] = observe(state + 1);
-  }
-  __syncthreads();
-  for (uint32_t e = 2 * tid; e < count * D; e += 2 * kThreads) {
-    const float* states = s_part + (e / D) * nsplit * 2;
-    float most = -INFINITY, weight = 0.f;
-    float2_t total = {0.f, 0.f};
-    for (uint32_t p = 0; p < nsplit; ++p) most = fmaxf(most, states[2 * p]);
-    const float ref = most == -INFINITY ? 0.f : most;
-    for (uint32_t p0 = 0; p0 < nsplit; p0 += kJoin) {
-      float2_t o[kJoin];
-#pragma unroll
-      for (int i = 0; i < kJoin; ++i) o[i] = observe2(parts + min(p0 + i, nsplit - 1) * part_size + e);
-#pragma unroll
-      for (int i = 0; i < kJoin; ++i) {
-        if (p0 + i < nsplit) {
-          const float k = __builtin_amdgcn_exp2f(states[2 * (p0 + i)] - ref);
-          total[0] = fmaf(k, o[i][0], total[0]);
-          total[1] = fmaf(k, o[i][1], total[1]);
-          weight = fmaf(k, states[2 * (p0 + i) + 1], weight);
-        }
-      }
-    }
-    XT* to = out + out_row(e / D) + e % D;
-    to[0] = from_f32<XT>(total[0] / weight);
-    to[1] = from_f32<XT>(total[1] / weight);
-  }
+  if (w.nsplit > 1) join_parts<XT, D, kThreads>(a, w, out, s_acc);
 }
 
-// How a call's columns are dealt.
-struct AttentionPlan {
-  uint32_t rows, row_tiles, units, max_splits, partial_rows, least;
-  float share_of_work;
-  size_t bytes;
+// How the columns of a launch are dealt.
+struct LaunchPlan {
+  uint32_t row_tiles = 0, units = 0, max_splits = 0, partial_rows = 0, least = 0, least_pairs = 0, most_pairs = 0xffffffffu;
+  float share_of_work = 0;
+  size_t bytes = 0;
 };
 // Eight waves (two a SIMD) while their registers allow it: half as many parts to join as with four, twice a CU.
 constexpr int waves_of(int depth) { return depth == 256 ? 4 : 8; }
 // One workgroup a CU: with 512 and 1024 of them 131000 columns took 49.4 us, with 256 39.8.
 constexpr uint32_t kFill = 256;
 constexpr uint32_t kMostGroups = 2048;   // in a grid, those without a split among them
-constexpr uint32_t kMostSplits = 64;
-AttentionPlan plan_attention(const Kv4Shape& s, uint32_t max_columns) {
-  AttentionPlan p;
-  p.rows = kv4_rows(s.max_query, s.total_rows);
-  const uint64_t pairs = (uint64_t)p.rows * (s.heads / s.kv_heads);
-  p.row_tiles = (uint32_t)((pairs + kRows - 1) / kRows);
-  p.partial_rows = pairs < kRows ? (uint32_t)pairs : kRows;
-  const uint64_t units = (uint64_t)s.nseq * s.kv_heads * p.row_tiles;
+static_assert(kMostGroups <= kTicketSlots, "a counter a unit");
+LaunchPlan plan_launch(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs, uint32_t tile_pairs, uint32_t tile_columns,
+                       uint32_t least, uint32_t most_splits, size_t part_floats) {
+  LaunchPlan p;
+  const uint64_t row_tiles = (pairs + tile_pairs - 1) / tile_pairs, units = (uint64_t)s.nseq * s.kv_heads * row_tiles;
+  p.row_tiles = (uint32_t)row_tiles;
+  p.partial_rows = pairs < tile_pairs ? (uint32_t)pairs : tile_pairs;
   p.units = (uint32_t)(units < 0xffffffffu ? units : 0xffffffffu);
-  // a split has two tiles a wave at least: joining two parts costs about as much as a tile more
-  p.least = 2 * waves_of(s.depth);
-  const uint64_t tiles = ((uint64_t)max_columns + kTile - 1) / kTile + 1, most = (tiles + p.least - 1) / p.least;
+  p.least = least;
+  const uint64_t tiles = ((uint64_t)max_columns + tile_columns - 1) / tile_columns + 1, most = (tiles + least - 1) / least;
   uint64_t splits = units ? kMostGroups / units : 1;
-  splits = splits > kMostSplits ? kMostSplits : splits;
+  splits = splits > most_splits ? most_splits : splits;
   splits = splits > most ? most : splits;
   p.max_splits = splits < 1 ? 1 : (uint32_t)splits;   // (with more units than kMostGroups, and so than counters: one)
-  p.share_of_work = (float)s.kv_heads * (float)p.row_tiles / kFill;
-  p.bytes = splits > 1 ? (size_t)units * splits * p.partial_rows * (s.depth + 2) * sizeof(float) : 0;
+  p.share_of_work = (float)s.kv_heads * (float)row_tiles / kFill;
+  p.bytes = splits > 1 ? (size_t)units * splits * part_floats * sizeof(float) : 0;
   return p;
 }
-static_assert(kMostGroups <= kTicketSlots, "a counter a unit");
+// Which kernel has which sequences.  kv4_decode_kernel takes blocks of 16 (row, head) pairs and reads the columns again for
+// each, kv4_chunk_kernel up to 256 of them with one turn of the codes, which pays where blocks of 16 are several times
+// the CUs (us, decode / chunk, 8 kv heads x 4, D 128, fp16, columns 1024 and 8192: 512 rows of one sequence 51 / 36 and
+// 236 / 128; 128 rows 17 / 34 and 70 / 73; 64 rows of eight 58 / 37 and 242 / 127; 16 rows of eight 19 / 33 and 71 / 101;
+// 1 kv head x 8, D 256: 512 rows 26 / 65 and 124 / 153, of eight 168 / 117 and 946 / 802).
+// A step may hold both kinds: sequences of up to kFewPairs pairs then stay with the decode kernel, in a launch of its own.
+constexpr uint64_t kFewPairs = 32;
+struct AttentionPlan {
+  bool few = true, many = false;   // which launches there are
+  LaunchPlan rows, chunk;
+  size_t bytes = 0;
+};
+AttentionPlan plan_attention(const Kv4Shape& s, uint32_t max_columns) {
+  AttentionPlan p;
+  const uint32_t rows = kv4_rows(s.max_query, s.total_rows);
+  const uint64_t pairs = (uint64_t)rows * (s.heads / s.kv_heads);
+  const uint64_t blocks = (uint64_t)s.nseq * s.kv_heads * ((pairs + kRows - 1) / kRows);
+  p.many = pairs > kFewPairs && blocks >= (s.depth == 256 ? 4u : 2u) * kFill;
+  p.few = !p.many || (s.nseq > 1 && s.total_rows < (uint64_t)s.nseq * rows);
+  if (p.few) {
+    // a split has two tiles a wave at least: joining two parts costs about as much as a tile more
+    p.rows = plan_launch(s, max_columns, p.many ? kFewPairs : pairs, kRows, kTile, 2 * waves_of(s.depth), 64,
+                         (size_t)(pairs < kRows ? pairs : kRows) * (s.depth + 2));
+    if (p.many) p.rows.most_pairs = kFewPairs;
+  }
+  if (p.many) {
+    p.chunk = plan_launch(s, max_columns, pairs, kv4_chunk_pairs(s.depth), kv4_chunk_columns(s.depth), 4, 16,
+                          (size_t)kv4_chunk_pairs(s.depth) * (s.depth + 4));
+    if (p.few) p.chunk.least_pairs = kFewPairs + 1;
+  }
+  p.bytes = p.rows.bytes > p.chunk.bytes ? p.rows.bytes : p.chunk.bytes;
+  return p;
+}
 
 }  // namespace
 
@@ -754,21 +591,47 @@ int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_t
   KRM_REQUIRE(ctx, q != out, "krm_kv4_attention: out is q");
   const AttentionPlan plan = plan_attention(shape, max_columns);
   const uint32_t share = heads / kv_heads;
-  KRM_REQUIRE(ctx, plan.units <= 0x7fffffu && (uint64_t)plan.rows * share <= 1u << 24,
-              "krm_kv4_attention: %u sequences of %u rows of %u heads are more than one call takes", nseq, plan.rows, heads);
-  if (plan.max_splits > 1) {
+  KRM_REQUIRE(ctx, plan.rows.units <= 0x7fffffu && plan.chunk.units <= 0x7fffffu &&
+                       (uint64_t)kv4_rows(max_query, total_rows) * share <= 1u << 24,
+              "krm_kv4_attention: %u sequences of %u rows of %u heads are more than one call takes", nseq, max_query, heads);
+  if (plan.bytes) {
     KRM_REQUIRE(ctx, workspace && workspace_bytes >= plan.bytes, "krm_kv4_attention: workspace of %zu bytes, %zu needed",
                 workspace ? workspace_bytes : (size_t)0, plan.bytes);
     KRM_TRY(needs_serial_scratch(ctx, "krm_kv4_attention"));
   }
-  const AttentionArgs a{{depth, group, page_rows, kv_heads},
-                        {total_rows, max_query, max_columns, table_stride, page_rows},
-                        nseq, heads, pages, window, share, 1.0f / share, 1.0f / plan.row_tiles,
-                        1.0f / ((float)kv_heads * plan.row_tiles), plan.row_tiles, plan.max_splits, plan.partial_rows,
-                        plan.least, plan.share_of_work, scale, ptr<float>(workspace), ctx->tickets};
-  const dim3 grid(plan.units, plan.max_splits);
+  auto arguments = [&](const LaunchPlan& p) {
+    Kv4Attention a;
+    a.layout = {depth, group, page_rows, kv_heads};
+    a.limits = {total_rows, max_query, max_columns, table_stride, page_rows};
+    a.nseq = nseq;
+    a.heads = heads;
+    a.pages = pages;
+    a.window = window;
+    a.share = share;
+    a.row_tiles = p.row_tiles;
+    a.share_inverse = 1.0f / share;
+    a.row_tiles_inverse = 1.0f / p.row_tiles;
+    a.of_sequence_inverse = 1.0f / ((float)kv_heads * p.row_tiles);
+    a.max_splits = p.max_splits;
+    a.partial_rows = p.partial_rows;
+    a.least = p.least;
+    a.least_pairs = p.least_pairs;
+    a.most_pairs = p.most_pairs;
+    a.share_of_work = p.share_of_work;
+    a.scale = scale;
+    a.partials = ptr<float>(workspace);
+    a.tickets = ctx->tickets;
+    return a;
+  };
+  if (plan.many) {
+    KRM_TRY(launch_kv4_chunk(ctx, arguments(plan.chunk), {q, cache, page_table_i32, cu_rows_i32, lens_i32, out, fault_u32},
+                             plan.chunk.units, io_dtype));
+    if (!plan.few) return KRM_OK;
+  }
+  const Kv4Attention a = arguments(plan.rows);
+  const dim3 grid(plan.rows.units, plan.rows.max_splits);
   const int waves = waves_of(depth);
-  const size_t joined = (size_t)waves * plan.partial_rows * (depth + 4) * sizeof(float);
+  const size_t joined = (size_t)waves * a.partial_rows * (depth + 4) * sizeof(float);
 #define KRM_ATTENTION(XT, D, NG)                                                                                 \
   const size_t ring = (size_t)waves * kStages * Stage<D, NG>::kBytes, lds = ring > joined ? ring : joined;       \
   kv4_decode_kernel<XT, D, NG, waves_of(D)><<<grid, dim3(waves * kWave), lds, ctx->stream>>>(                                       \

@@ -1,0 +1,537 @@
+// Attention of many rows over the pages of the 4-bit K/V cache: kv4_attention.hip's operator where a sequence has
+// chunks of rows.
+//
+// What bounds it is arithmetic, so a tile's codes are turned into fp16 once for all rows of a workgroup: it has kPairs
+// (row, head) pairs, 32 a wave, and for each tile of columns half of the waves make keys and half values, in LDS, two
+// tiles by turns; every wave then multiplies its rows with all of it.
+//   keys    k = hi + lo, two fp16 planes (22 bits): the products with fp16 queries are off by no more than f32 sums;
+//           f32 queries are hi + lo too
+//   weights p = hi + lo; values rounded to fp16 once (f32 rows: hi + lo)
+// The scores are formed as K Q^T: a lane has one pair's scores, so its maximum and sum stay in the lane, and the weights
+// leave the product in the order in which the next one takes them.
+#include "kv4_attention.h"
+#include "rows8.h"
+
+using namespace krm;
+
+namespace {
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+__device__ inline float16_t product(half8_t a, half8_t b, float16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// The same of the lane 32 apart, joined.
+template <typename F>
+__device__ inline float across_halves(float x, F join) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return join(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+// The 16-byte chunks of a row of keys in LDS are exchanged by its number (chunk ^ this), so that 16 rows read at one
+// chunk, and four (a depth of 64: eight) rows written at four (two) chunks, lie on different banks.
+template <int D>
+__device__ inline uint32_t exchanged(uint32_t row) {
+  const uint32_t x = row >> 1;
+  return D == 64 ? (x & 1) | (x & 2) << 1 | (x & 4) >> 1 : (row & 3) << 2 | (row >> 2 & 3);
+}
+
+template <typename XT, int D>
+struct Chunk {
+  static constexpr bool kF32 = sizeof(XT) == 4;
+  static constexpr int kWaves = D == 256 ? 4 : 8;
+  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kPairs = kWaves * 32;
+  static constexpr int kColumns = kWaves * 8;        // of a tile: 16 for each wave that makes keys
+  static constexpr int kBlocks = kColumns / 16;
+  static constexpr int kKeyPlanes = 2, kValuePlanes = kF32 ? 2 : 1;
+  static constexpr uint32_t kPlane = kColumns * D * 2;
+  static constexpr uint32_t kTileBytes = (kKeyPlanes + kValuePlanes) * kPlane;
+};
+
+template <typename XT, int D, int NG>
+__global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
+    const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table,
+    const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens, XT* __restrict__ out,
+    uint32_t* __restrict__ fault, Kv4Attention a) {
+  using C = Chunk<XT, D>;
+  constexpr bool kF32 = C::kF32;
+  constexpr int kThreads = C::kThreads, kPairs = C::kPairs, kColumns = C::kColumns, kBlocks = C::kBlocks;
+  constexpr int kSteps = D / 16, kSubs = kColumns / 32, kOuts = D / 32;
+  constexpr int kPieces = D <= 128 ? 1 : D / 128;    // 16-byte pieces of codes that a lane turns
+  extern __shared__ __align__(16) uint8_t s_tiles[];  // [2][keys hi, keys lo, values hi (, values lo)]
+  __shared__ uint32_t s_unsound[2][kColumns];         // groups of a column's values that are no numbers (edge tiles)
+  __shared__ uint32_t s_any[2];
+
+  const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  Work w;
+  uint32_t block;
+  find_unit(a, w, block);
+  block = a.row_tiles - 1 - block;   // late rows, which see the most columns, begin first
+  if (!find_work<XT, D, kThreads, kPairs, kColumns, 1>(a, w, block, cu_rows, lens, out, fault)) return;
+  const int32_t low = w.low, high = w.high;
+
+  // ---- this wave's rows: lane (m = lane % 32, half)
+  const uint32_t m = lane & 31, half = lane >> 5, pair = wave * 32 + m;
+  const bool live = pair < w.count;
+  const int32_t position = w.first_row + (int32_t)row_of(a, w, live ? pair : 0);
+  const int32_t from = kv4_first_column(position, a.window);
+  // columns that this wave's rows see (none: it only makes keys or values)
+  const bool has_rows = wave * 32 < w.count;
+  const int32_t wave_low = kv4_first_column(w.first_row + (int32_t)row_of(a, w, has_rows ? wave * 32 : 0), a.window);
+  const int32_t wave_high =
+      has_rows ? w.first_row + (int32_t)row_of(a, w, min(wave * 32 + 31, w.count - 1)) : wave_low - 1;
+  half8_t qh[kSteps], ql[kF32 ? kSteps : 1];
+  float scale = a.scale;
+  {
+    const XT* src = q + row_at(a, w, live ? pair : 0, D) + 8 * half;
+    if constexpr (!kF32) {
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        const half8_t x = *reinterpret_cast<const half8_t*>(src + 16 * st);
+        qh[st] = live ? x : half8_t{};
+      }
+    } else {
+      // x * 2^e = hi + lo with the row's largest magnitude in [2^5, 2^6)
+      float x[kSteps][8], most = 0.f;
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        load8(src + 16 * st, x[st]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[st][i] = live ? x[st][i] : 0.f;
+          most = fmaxf(most, fabsf(x[st][i]));
+        }
+      }
+      most = across_halves(most, [](float x, float y) { return fmaxf(x, y); });
+      int e = 0;
+      if (most > 0.f && most < INFINITY)
+        e = max(min(6 - __builtin_amdgcn_frexp_expf(most), 100), __builtin_amdgcn_frexp_expf(a.scale) - 110);
+      scale = ldexpf(a.scale, -e);
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float y = ldexpf(x[st][i], e);
+          qh[st][i] = (_Float16)y;
+          ql[st][i] = (_Float16)(y - (float)qh[st][i]);
+        }
+    }
+  }
+
+  // ---- the other work of a wave: codes of 16 columns of each tile, keys (waves below kBlocks) or values
+  const bool makes_values = wave >= kBlocks;
+  const uint32_t my_block = makes_values ? wave - kBlocks : wave;
+  const int32_t* table = page_table + (size_t)w.seq * a.limits.table_stride;
+  const uint32_t page_shift = 31 - __builtin_clz(a.layout.page_rows);
+  const uint64_t page_bytes = a.layout.page();
+  const uint8_t* head_base = cache + (size_t)w.kv_head * a.layout.block();
+  // keys: lane (row r, piece c): words (c, .) of row r; values: lane (rows 4 b .. 4 b + 3, word column).  A depth of 64
+  // has half as many pieces: lanes 32 .. 63 repeat those of 0 .. 31 and write nothing.
+  const uint32_t at_lane = D == 64 ? lane & 31 : lane;
+  const bool idle = D == 64 && lane >= 32;
+  const uint32_t key_row = D == 64 ? at_lane / 2 : at_lane / 4, key_piece = D == 64 ? at_lane & 1 : at_lane & 3;
+  constexpr uint32_t kWordColumns = D / 8;
+  struct Raw {
+    uint4 codes[kPieces];
+    uint32_t params[NG > 4 ? NG : 4];   // keys: of the row's groups; values: 16 bytes of a piece's group
+    uint4 more[kPieces > 1 ? kPieces - 1 : 1];
+    uint32_t bad;
+  };
+  auto fetch = [&](int32_t tile) __attribute__((always_inline)) -> Raw {
+    Raw r;
+    const int32_t column = tile * kColumns + 16 * (int32_t)my_block;
+    uint32_t id = 0;
+    r.bad = 0;
+    if (column <= high && column + 15 >= low) {   // (a block that no row sees has no page: page 0, and nothing is used)
+      id = (uint32_t)table[(uint32_t)column >> page_shift];
+      if (id >= a.pages) {
+        r.bad = 1;
+        id = 0;
+      }
+    }
+    const uint32_t in_page = (uint32_t)column & (a.layout.page_rows - 1);
+    const uint8_t* base = uniform(head_base + id * page_bytes);
+    if (!makes_values) {
+      const uint8_t* codes = base + in_page * (D / 2) + key_row * (D / 2);
+      if constexpr (D == 64) {
+        r.codes[0] = *reinterpret_cast<const uint4*>(codes + key_piece * 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+          r.codes[i] = *reinterpret_cast<const uint4*>(codes + key_piece * (D / 8) + 16 * i);
+      }
+      uint32_t p[NG];
+      load_words(base + a.layout.key_params() + (in_page + key_row) * (NG * 4), p);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) r.params[g] = p[g];
+    } else {
+      const uint8_t* codes = base + a.layout.value_codes() + in_page * (D / 2);
+      const uint8_t* params = base + a.layout.value_params() + in_page * (NG * 4);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint32_t piece = at_lane + kWave * i, four = piece / kWordColumns, column_of = piece % kWordColumns;
+        r.codes[i] = *reinterpret_cast<const uint4*>(codes + piece * 16);
+        const uint4 p = *reinterpret_cast<const uint4*>(params + four * (NG * 16) + column_of * 8 * NG / D * 16);
+        if (i == 0) {
+          r.params[0] = p.x; r.params[1] = p.y; r.params[2] = p.z; r.params[3] = p.w;
+        } else {
+          r.more[i - 1] = p;
+        }
+      }
+    }
+    return r;
+  };
+  // Whether a tile has a column that some row does not see, or that lies on no page.
+  auto tile_edge = [&](int32_t tile) {
+    const int32_t column0 = tile * kColumns;
+    return column0 < kv4_first_column(w.last_row, a.window) || column0 + kColumns - 1 > w.first_row;
+  };
+  bool lost = false;
+  auto make = [&](const Raw& r, int32_t tile, uint32_t buffer) __attribute__((always_inline)) {
+    uint8_t* const to = s_tiles + buffer * C::kTileBytes;
+    const int32_t column0 = tile * kColumns;
+    lost = lost || r.bad;
+    if (!makes_values) {
+      const uint32_t row = 16 * my_block + key_row;
+      if (idle) return;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint32_t words[4] = {r.codes[i].x, r.codes[i].y, r.codes[i].z, r.codes[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // word (c, s) of the row: elements 32 s + 8 c .. + 7, chunk 4 s + c
+          const int at = D == 64 ? j & 1 : 4 * i + j;                               // s
+          const uint32_t c = D == 64 ? 2 * key_piece + (j >> 1) : key_piece;
+          const half2_t p = half2_of(r.bad ? 0x7e007e00u : r.params[at * NG / (D / 32)]);
+          const float step = (float)p.x, least = (float)p.y;
+          uint32_t even = words[j] & 0x0f0f0f0fu, odd = (words[j] >> 4) & 0x0f0f0f0fu;
+          asm("" : "+v"(even), "+v"(odd));   // (bytes of these, not nibbles of the word, become numbers in one step each)
+          // nibble i: element 2 i, nibble 4 + i: element 2 i + 1
+          const uint32_t code[8] = {even & 255, even >> 16 & 255, odd & 255, odd >> 16 & 255,
+                                    even >> 8 & 255, even >> 24, odd >> 8 & 255, odd >> 24};
+          half8_t hi, lo;
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float2_t x = {fmaf(step, (float)code[e], least), fmaf(step, (float)code[e + 1], least)};
+            const half2_t h2 = rounded2(x);
+            hi[e] = h2.x;
+            hi[e + 1] = h2.y;
+            lo[e] = less(x[0], h2.x);
+            lo[e + 1] = less(x[1], h2.y);
+          }
+          const uint32_t place = row * (D * 2) + ((4 * (uint32_t)at + c) ^ exchanged<D>(row)) * 16;
+          *reinterpret_cast<half8_t*>(to + place) = hi;
+          *reinterpret_cast<half8_t*>(to + C::kPlane + place) = lo;
+        }
+      }
+    } else {
+      const bool edge = tile_edge(tile) || r.bad;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint32_t piece = at_lane + kWave * i, four = piece / kWordColumns, column_of = piece % kWordColumns;
+        uint32_t p[4];
+        if (i == 0) {
+          p[0] = r.params[0]; p[1] = r.params[1]; p[2] = r.params[2]; p[3] = r.params[3];
+        } else {
+          p[0] = r.more[i - 1].x; p[1] = r.more[i - 1].y; p[2] = r.more[i - 1].z; p[3] = r.more[i - 1].w;
+        }
+        if (edge) {
+          // columns that no row sees hold anything, and 0 times it has to be 0; a column of no numbers that some row
+          // does not see enters as 0, and the rows that do see it are marked behind the product
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int32_t column = column0 + 16 * (int32_t)my_block + 4 * (int32_t)four + j;
+            const uint32_t mine = 0xffffu << (16 * (j & 1));
+            const bool none = column < low || column > high || r.bad;
+            const half2_t s2 = half2_of(p[j / 2]), l2 = half2_of(p[2 + j / 2]);
+            const bool sound = fabsf((float)s2[j & 1]) < INFINITY && fabsf((float)l2[j & 1]) < INFINITY;
+            if (!none && !sound && !idle) {
+              atomicOr(&s_unsound[buffer][column - column0], 1u << (column_of * 8 * NG / D));
+              s_any[buffer] = 1;
+            }
+            if (none || !sound) {
+              p[j / 2] &= ~mine;
+              p[2 + j / 2] &= ~mine;
+            }
+          }
+        }
+        if (idle) continue;
+        const uint32_t words[4] = {r.codes[i].x, r.codes[i].y, r.codes[i].z, r.codes[i].w};
+        // rows 4 four .. + 3 of a block of 16: the operand's lanes of `half` four & 1, elements 4 (four / 2) ..
+        // (element e of word column x lies at e ^ (x & 7), so that neighbouring columns lie on different banks)
+        uint8_t* const at = to + 2 * C::kPlane + ((my_block * 2 + (four & 1)) * D + 8 * column_of) * 16 + (four / 2) * 8;
+        const uint32_t turn = (column_of & 7) * 16;
+        if constexpr (!kF32) {
+          const half2_t s01 = half2_of(p[0]), s23 = half2_of(p[1]), l01 = half2_of(p[2]), l23 = half2_of(p[3]);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const uint32_t select = (uint32_t)b | 0x0c000c00u | (4u + b) << 16;
+            const uint32_t x = __builtin_amdgcn_perm(words[1], words[0], select);
+            const uint32_t y = __builtin_amdgcn_perm(words[3], words[2], select);
+            const half2_t e0 = __builtin_elementwise_fma(low_codes<0>(x), s01, l01);
+            const half2_t e1 = __builtin_elementwise_fma(low_codes<0>(y), s23, l23);
+            const half2_t o0 = __builtin_elementwise_fma(high_codes<0>(x), s01, l01);
+            const half2_t o1 = __builtin_elementwise_fma(high_codes<0>(y), s23, l23);
+            *reinterpret_cast<uint2*>(at + ((2 * b) * 16 ^ turn)) =
+                make_uint2(__builtin_bit_cast(uint32_t, e0), __builtin_bit_cast(uint32_t, e1));
+            *reinterpret_cast<uint2*>(at + ((2 * b + 1) * 16 ^ turn)) =
+                make_uint2(__builtin_bit_cast(uint32_t, o0), __builtin_bit_cast(uint32_t, o1));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            half2_t h[2], l[2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float x = fmaf((float)half2_of(p[j / 2])[j & 1], (float)(words[j] >> (4 * e) & 15u),
+                                   (float)half2_of(p[2 + j / 2])[j & 1]);
+              h[j / 2][j & 1] = (_Float16)x;
+              l[j / 2][j & 1] = less(x, h[j / 2][j & 1]);
+            }
+            *reinterpret_cast<uint2*>(at + (e * 16 ^ turn)) =
+                make_uint2(__builtin_bit_cast(uint32_t, h[0]), __builtin_bit_cast(uint32_t, h[1]));
+            *reinterpret_cast<uint2*>(at + C::kPlane + (e * 16 ^ turn)) =
+                make_uint2(__builtin_bit_cast(uint32_t, l[0]), __builtin_bit_cast(uint32_t, l[1]));
+          }
+        }
+      }
+    }
+  };
+
+  // ---- a tile's rows
+  float16_t acc[kOuts] = {};
+  float top = -INFINITY, sum = 0.f;
+  const uint32_t key_lane = m * (D * 2);
+  const uint32_t value_lane[2] = {((m & 24) | ((m & 7) ^ (m >> 3))) * 16, ((m & 24) | ((m & 7) ^ (4 + (m >> 3)))) * 16};
+  auto consume = [&](int32_t tile, uint32_t buffer) __attribute__((always_inline)) {
+    const int32_t column0 = tile * kColumns;
+    const uint8_t* keys = s_tiles + buffer * C::kTileBytes;
+    const uint8_t* values = keys + 2 * C::kPlane + half * D * 16;
+    float16_t sc[kSubs];
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub) sc[sub] = float16_t{};
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const uint32_t chunk = 2 * st + half;
+      half8_t hi[kSubs], lo[kSubs];
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub) {
+        const uint32_t at = sub * 32 * (D * 2) + key_lane + (chunk ^ exchanged<D>(m)) * 16;
+        hi[sub] = *reinterpret_cast<const half8_t*>(keys + at);
+        lo[sub] = *reinterpret_cast<const half8_t*>(keys + C::kPlane + at);
+      }
+      // (neighbouring products are of different sums, so that none waits for the one before it)
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub) sc[sub] = product(lo[sub], qh[st], sc[sub]);
+      if constexpr (kF32) {
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub) sc[sub] = product(hi[sub], ql[st], sc[sub]);
+      }
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub) sc[sub] = product(hi[sub], qh[st], sc[sub]);
+    }
+    // lane (m, half): columns 8 (r / 4) + 4 half + r % 4 of each 32
+    if (tile_edge(tile)) {
+      int32_t first = column0 + 4 * (int32_t)half;
+      asm volatile("" : "+v"(first));   // (stays behind the branch: in every tile these are a fifth of its instructions)
+#pragma unroll
+      for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int32_t column = first + 32 * sub + 8 * (r / 4) + r % 4;
+          if (column < from || column > position) sc[sub][r] = -INFINITY;
+        }
+    }
+    float here = sc[0][0];
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) here = fmaxf(here, sc[sub][r]);
+    here = across_halves(here, [](float x, float y) { return fmaxf(x, y); }) * scale;
+    // weights may grow to 2^(4 + 10) before the sums are brought to a new maximum
+    if (__any(here > top + 4.0f)) {
+      const float now = fmaxf(here, top);
+      const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      sum *= keep;
+#pragma unroll
+      for (int o = 0; o < kOuts; ++o) acc[o] *= keep;
+    }
+    const float shift = (top == -INFINITY ? 0.f : top) - 10.0f;
+#pragma unroll
+    for (int sub = 0; sub < kSubs; ++sub) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        half8_t ph, pl;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float2_t p = {__builtin_amdgcn_exp2f(fmaf(sc[sub][8 * ks + j], scale, -shift)),
+                              __builtin_amdgcn_exp2f(fmaf(sc[sub][8 * ks + j + 1], scale, -shift))};
+          const half2_t hi = rounded2(p);
+          sum += p[0] + p[1];
+          ph[j] = hi.x;
+          ph[j + 1] = hi.y;
+          pl[j] = less(p[0], hi.x);
+          pl[j + 1] = less(p[1], hi.y);
+        }
+#pragma unroll
+        for (int o = 0; o < kOuts; o += 2) {
+          half8_t hi[2], lo[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint8_t* at = values + ((2 * sub + ks) * 2 * D + 32 * (o + i)) * 16 + value_lane[i];
+            hi[i] = *reinterpret_cast<const half8_t*>(at);
+            if constexpr (kF32) lo[i] = *reinterpret_cast<const half8_t*>(at + C::kPlane);
+          }
+          if constexpr (kF32) {
+            acc[o] = product(lo[0], ph, acc[o]);
+            acc[o + 1] = product(lo[1], ph, acc[o + 1]);
+          }
+          acc[o] = product(hi[0], pl, acc[o]);
+          acc[o + 1] = product(hi[1], pl, acc[o + 1]);
+          acc[o] = product(hi[0], ph, acc[o]);
+          acc[o + 1] = product(hi[1], ph, acc[o + 1]);
+        }
+      }
+    }
+    if (s_any[buffer]) {
+      for (int i = 0; i < kColumns; ++i) {
+        const uint32_t groups = s_unsound[buffer][i];
+        const int32_t column = column0 + i;
+        if (groups == 0 || column < from || column > position) continue;
+#pragma unroll
+        for (int o = 0; o < kOuts; ++o)
+          if (groups >> (32 * o * NG / D) & 1u) acc[o] = float16_t{} + __builtin_nanf("");
+      }
+    }
+  };
+
+  for (uint32_t i = tid; i < 2 * kColumns; i += kThreads) s_unsound[i / kColumns][i % kColumns] = 0;
+  if (tid < 2) s_any[tid] = 0;
+  __syncthreads();
+  Raw raw = fetch(w.begin);
+  make(raw, w.begin, 0);
+  if (w.begin + 1 < w.end) raw = fetch(w.begin + 1);
+  __syncthreads();
+  for (int32_t tile = w.begin; tile < w.end; ++tile) {
+    const uint32_t buffer = (uint32_t)(tile - w.begin) & 1u;
+    // The two waves of a SIMD are a key maker and a value maker: one makes before it multiplies and the other behind, so
+    // that one's conversions and exponentials run beside the other's products.
+    auto next = [&]() __attribute__((always_inline)) {
+      if (tile + 1 < w.end) {
+        make(raw, tile + 1, buffer ^ 1u);
+        if (tile + 2 < w.end) raw = fetch(tile + 2);
+      }
+    };
+    const bool sees = tile * kColumns <= wave_high && tile * kColumns + kColumns > wave_low;
+    if (makes_values) next();
+    if (sees) consume(tile, buffer);
+    if (!makes_values) next();
+    __syncthreads();
+    if (s_any[buffer]) {   // everyone is through with the tile: its marks are cleared before it is made again
+      for (uint32_t i = tid; i < (uint32_t)kColumns; i += kThreads) s_unsound[buffer][i] = 0;
+      __syncthreads();
+      if (tid == 0) s_any[buffer] = 0;
+      __syncthreads();
+    }
+  }
+  if (lost && fault && lane == 0) *fault = 1u;
+  sum = across_halves(sum, [](float x, float y) { return x + y; });
+
+  // ---- parts: as the lanes hold them, (max, sum) of every lane behind the sums; whoever arrives last joins them in
+  // order in the same lanes
+  if (w.nsplit > 1) {
+    __shared__ uint32_t s_ticket;
+    constexpr uint32_t kState = kOuts * 16 * kThreads;          // floats before the states
+    constexpr size_t kPart = kState + 2 * kThreads;
+    float* const parts = a.partials + (size_t)w.unit * a.max_splits * kPart;
+    float* const mine = parts + w.split * kPart + 2 * tid;
+#pragma unroll
+    for (int o = 0; o < kOuts; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2)
+        publish2(mine + (o * 16 + r) * kThreads, float2_t{acc[o][r], acc[o][r + 1]});
+    publish2(mine + kState, float2_t{top, sum});
+    // every store of this workgroup is through before it is counted (a release fence would write the whole L2 back)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint32_t* ticket = a.tickets + (size_t)w.unit * kTicketStride;
+    if (tid == 0) s_ticket = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (s_ticket + 1 != w.nsplit) return;
+    if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    top = -INFINITY;
+    sum = 0.f;
+#pragma unroll
+    for (int o = 0; o < kOuts; ++o) acc[o] = float16_t{};
+    for (uint32_t p = 0; p < w.nsplit; ++p) {
+      const float* from_part = parts + p * kPart + 2 * tid;
+      const float2_t state = observe2(from_part + kState);
+      float2_t x[kOuts * 8];
+#pragma unroll
+      for (int i = 0; i < kOuts * 8; ++i) x[i] = observe2(from_part + 2 * i * kThreads);
+      const float now = fmaxf(top, state[0]), ref = now == -INFINITY ? 0.f : now;
+      const float keep = __builtin_amdgcn_exp2f(top - ref), take = __builtin_amdgcn_exp2f(state[0] - ref);
+      top = now;
+      sum = fmaf(sum, keep, state[1] * take);
+#pragma unroll
+      for (int o = 0; o < kOuts; ++o)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[o][r] = fmaf(acc[o][r], keep, x[(o * 16 + r) / 2][r & 1] * take);
+    }
+  }
+  // ---- out: lane (m, half) has elements 32 o + 8 (r / 4) + 4 half + r % 4 of its pair
+  if (live) {
+    XT* to = out + row_at(a, w, pair, D) + 4 * half;
+    const float inverse = 1.0f / sum;
+#pragma unroll
+    for (int o = 0; o < kOuts; ++o)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        XT x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = from_f32<XT>(acc[o][r + i] * inverse);
+        if constexpr (kF32) *reinterpret_cast<float4*>(to + 32 * o + 2 * r) = *reinterpret_cast<const float4*>(x);
+        else *reinterpret_cast<uint2*>(to + 32 * o + 2 * r) = *reinterpret_cast<const uint2*>(x);
+      }
+  }
+}
+
+template <typename XT, int D, int NG>
+void launch(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& b, uint32_t units) {
+  using C = Chunk<XT, D>;
+  kv4_chunk_kernel<XT, D, NG><<<dim3(units, a.max_splits), dim3(C::kThreads), 2 * C::kTileBytes, ctx->stream>>>(
+      ptr<const XT>(b.q), ptr<const uint8_t>(b.cache), ptr<const int32_t>(b.page_table),
+      ptr<const int32_t>(b.cu_rows), ptr<const int32_t>(b.lens), ptr<XT>(b.out), ptr<uint32_t>(b.fault), a);
+}
+template <typename XT>
+void launch_depth(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& b, uint32_t units) {
+  switch (a.layout.depth * 16 + a.layout.groups()) {
+    case 64 * 16 + 1: return launch<XT, 64, 1>(ctx, a, b, units);
+    case 64 * 16 + 2: return launch<XT, 64, 2>(ctx, a, b, units);
+    case 128 * 16 + 1: return launch<XT, 128, 1>(ctx, a, b, units);
+    case 128 * 16 + 2: return launch<XT, 128, 2>(ctx, a, b, units);
+    case 128 * 16 + 4: return launch<XT, 128, 4>(ctx, a, b, units);
+    case 256 * 16 + 2: return launch<XT, 256, 2>(ctx, a, b, units);
+    case 256 * 16 + 4: return launch<XT, 256, 4>(ctx, a, b, units);
+    default: return launch<XT, 256, 8>(ctx, a, b, units);
+  }
+}
+
+}  // namespace
+
+namespace krm {
+
+uint32_t kv4_chunk_pairs(uint32_t depth) { return depth == 256 ? Chunk<float, 256>::kPairs : Chunk<float, 64>::kPairs; }
+uint32_t kv4_chunk_columns(uint32_t depth) {
+  return depth == 256 ? Chunk<float, 256>::kColumns : Chunk<float, 64>::kColumns;
+}
+
+int32_t launch_kv4_chunk(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& b, uint32_t units, int32_t io_dtype) {
+  if (io_dtype == KRM_F32) launch_depth<float>(ctx, a, b, units);
+  else launch_depth<__half>(ctx, a, b, units);
+  return launched(ctx, "kv4_chunk_kernel");
+}
+
+}  // namespace krm

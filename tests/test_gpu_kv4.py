@@ -268,6 +268,21 @@ def test_chunks_of_rows(gpu_ctx, io, depth, group, page, hkv, share, rows, lens)
 
 
 @pytest.mark.parametrize("io", [np.float16, np.float32])
+@pytest.mark.parametrize("depth,group,page", LAYOUTS)
+def test_many_rows_of_many_heads(gpu_ctx, io, depth, group, page):
+    """Steps with blocks enough for the kernel that turns a tile's codes once for many rows: with whole and part waves and
+    workgroups of rows, columns that are split and joined, and sequences of few rows and of none among them."""
+    rng = np.random.default_rng(depth * group + page)
+    hkv = 8 if depth < 256 else 4
+    rows, lens = (260, 1, 0, 75, 8), (700, 333, 0, 75, 129)
+    step = ref.Step.make(ref.Layout(hkv, depth, group, page), rows, lens, rng)
+    check(gpu_ctx, step, hkv * 4, io, rng)
+    check(gpu_ctx, step, hkv * 4, io, rng, window=100)
+    whole = ref.Step.make(ref.Layout(hkv, depth, group, page), (150,), (150,), rng)
+    check(gpu_ctx, whole, hkv * 7, io, rng)
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
 def test_limits_larger_than_the_step_needs(gpu_ctx, io):
     """What a recorded call is made with: more rows and columns than the sequences have yet."""
     rng = np.random.default_rng(6)
@@ -362,9 +377,10 @@ def test_refused_sequences_are_nan_and_the_others_are_not(gpu_ctx, io, case):
 def test_pages_outside_the_cache(gpu_ctx, io, page, chunk):
     """Rows that see such a page are NaN, rows of a window that does not are as before."""
     rng = np.random.default_rng(78)
+    heads = 256 if chunk else 4
     step = ref.Step.make(ref.Layout(2, 64, 32, 16), (1, 40 if chunk else 3, 3), (40, 90, 8), rng)
     raw = step.random_cache(rng)
-    q = rng.normal(size=(step.total, 4, 64))
+    q = rng.normal(size=(step.total, heads, 64))
     good = {}
     for window in (0, 20):
         a = Attention(gpu_ctx, step, raw, q, io, window)
@@ -414,10 +430,12 @@ def test_nan_in_a_seen_column_shows_and_in_an_unseen_one_does_not(gpu_ctx, io, d
     """A key's NaN is its row's, a value's its group's, in the rows that see the column and in no others."""
     rng = np.random.default_rng(80)
     for rows, lens, window in (((1, 1), (50, 70), 0), ((1, 1), (50, 70), 5), ((20, 30), (50, 70), 0),
-                               ((40, 30), (50, 70), 7), ((2, 3), (60, 46), 12)):
+                               ((40, 30), (50, 70), 7), ((2, 3), (60, 46), 12), ((200, 3), (230, 60), 0),
+                               ((200, 300), (230, 300), 9)):
         lay = ref.Layout(2, depth, group, 16)
         step = ref.Step.make(lay, rows, lens, rng)
         raw = step.random_cache(rng)
+        share = 8 * share if rows[0] == 200 else share    # (blocks enough for the kernel of many rows)
         q = rng.normal(size=(sum(rows), 2 * share, depth))
         for name in ("params", "vparams"):
             held = raw.copy()
