@@ -6,6 +6,7 @@
 // Both parameters are rounded outwards, so no element is clipped and every one is off by step / 2 at most
 // (beside the roundings of the f32 operations).  A group that is constant has step 0 and codes 0.
 #include "kv4_plan.h"
+#include "i4_codes.h"
 #include "krm_internal.h"
 #include "rotary.h"
 #include "rows8.h"
@@ -39,68 +40,95 @@ struct AppendArgs {
   uint64_t q_stride, k_stride, v_stride;   // elements between rows
 };
 
-// A thread has 8 elements of one head's row, D / 8 neighbouring lanes the row; a wave has 512 / D rows.
-// The work of a sequence is its rows x (H + 2 Hkv) heads: queries are turned and stored, keys turned,
+// A thread has 8 elements of one head's row, D / 8 neighbouring lanes the row.  A workgroup has 256 * 8 / D of the
+// (H + 2 Hkv) heads of one row of the step, whose angles it holds in LDS: queries are turned and stored, keys turned,
 // quantised and stored, values quantised and stored.
-template <typename XT, int D>
+// PIECES: a thread's elements are turned as whole pieces (pairs within 8 elements, or 8 pairs across two pieces).
+template <typename XT, int D, bool PIECES>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(
     const XT* __restrict__ k, const XT* __restrict__ v, uint8_t* __restrict__ cache,
     const int32_t* __restrict__ page_table, const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens,
     const XT* q, XT* q_out, const int32_t* __restrict__ positions, const float* __restrict__ cos_table,
     const float* __restrict__ sin_table, uint32_t* __restrict__ fault, AppendArgs a) {
   constexpr int kLanes = D / kPiece;
-  __shared__ __align__(16) float s_row[kThreads * kPiece];
-  const uint32_t seq = blockIdx.y;
+  __shared__ __align__(16) float s_cos[D / 2], s_sin[D / 2];
+  const uint32_t seq = blockIdx.z, row = blockIdx.x;
   const Kv4Sequence s = kv4_sequence(cu_rows[seq], cu_rows[seq + 1], lens[seq], a.limits);
   if (!s.ok) {
-    if (fault && blockIdx.x == 0 && threadIdx.x == 0) *fault = 1u;
+    if (fault && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *fault = 1u;
     return;
   }
-  const uint32_t hkv = a.layout.kv_heads;
-  const uint32_t units = a.heads + 2 * hkv;
-  const uint64_t item = (blockIdx.x * (uint64_t)kThreads + threadIdx.x) / kLanes;
-  const uint64_t items = (uint64_t)s.rows * units;
-  if (item - threadIdx.x % 64 / kLanes >= items) return;   // the whole wave has nothing
-  const bool live = item < items;
-  const uint32_t row = (uint32_t)((live ? item : 0) / units);
-  const uint32_t unit = (uint32_t)((live ? item : 0) % units);
+  if (row >= (uint32_t)s.rows) return;
+  const uint32_t hkv = a.layout.kv_heads, units = a.heads + 2 * hkv;
+  const uint32_t sub = threadIdx.x % kLanes, mine = blockIdx.y * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const bool live = mine < units;
+  const uint32_t unit = live ? mine : units - 1;
   const bool is_q = unit < a.heads, is_v = unit >= a.heads + hkv;
   const uint32_t head = is_q ? unit : is_v ? unit - a.heads - hkv : unit - a.heads;
-  const uint32_t sub = threadIdx.x % kLanes;
   const uint64_t token = (uint64_t)s.first + row;
   const uint32_t column = (uint32_t)(s.len - s.rows) + row;
-  const XT* src = (is_q ? q + token * a.q_stride : is_v ? v + token * a.v_stride : k + token * a.k_stride) +
-                  (size_t)head * D + sub * kPiece;
-  float x[8];
-  load8(src, x);
-
-  if (a.turn.rotary_dim) {
-    // partners of a rotation may be in other lanes of the row: exchanged through LDS (a wave's own part)
-    float* mine = s_row + (threadIdx.x - sub) * kPiece;
-    store8(mine + sub * kPiece, x);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  const XT* src = (is_q ? q + token * a.q_stride : is_v ? v + token * a.v_stride : k + token * a.k_stride) + (size_t)head * D;
+  const uint32_t pairs = a.turn.rotary_dim / 2, d0 = sub * kPiece;
+  const bool by_half = a.turn.layout == KRM_ROPE_HALF;
+  const bool turns = !is_v && d0 < a.turn.rotary_dim, second = by_half && d0 >= pairs;   // (PIECES: of the whole piece)
+  float x[8], other[8];
+  load8(src + d0, x);
+  if constexpr (PIECES) {
+    if (by_half && turns) load8(src + (second ? d0 - pairs : d0 + pairs), other);   // (before any lane of the row stores)
+  }
+  const int32_t in_table = (int32_t)column / (int32_t)a.layout.page_rows;
+  const int32_t page = page_table[(size_t)seq * a.limits.table_stride + in_table];
+  if (pairs) {
     const int32_t pos = positions ? positions[token] : (int32_t)column;
     const bool known = pos >= 0 && (uint32_t)pos < a.turn.table_rows;
-    const uint32_t pairs = a.turn.rotary_dim / 2;
+    const size_t at = (size_t)(known ? pos : 0) * a.turn.table_width;
+    if (threadIdx.x < pairs) {
+      s_cos[threadIdx.x] = known ? cos_table[at + threadIdx.x] : __builtin_nanf("");
+      s_sin[threadIdx.x] = known ? sin_table[at + threadIdx.x] : __builtin_nanf("");
+    }
+    __syncthreads();
+    if constexpr (PIECES) {
+      if (turns && by_half) {
+        const uint32_t j = second ? d0 - pairs : d0;
+        float c[8], sn[8];
+        load8(s_cos + j, c);
+        load8(s_sin + j, sn);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t d = sub * kPiece + i;
-      if (is_v || d >= a.turn.rotary_dim) continue;
-      const bool second = a.turn.layout == KRM_ROPE_HALF ? d >= pairs : d & 1;
-      const uint32_t j = a.turn.layout == KRM_ROPE_HALF ? (second ? d - pairs : d) : d / 2;
-      const uint32_t other = a.turn.layout == KRM_ROPE_HALF ? (second ? d - pairs : d + pairs) : d ^ 1;
-      const size_t at = (size_t)(known ? pos : 0) * a.turn.table_width + j;
-      const float c = cos_table[at], sn = sin_table[at], o = mine[other];
-      float ta, tb;
-      if (second) turn_pair(o, x[i], c, sn, ta, tb);
-      else turn_pair(x[i], o, c, sn, ta, tb);
-      x[i] = !known ? __builtin_nanf("") : second ? tb : ta;
+        for (int i = 0; i < 8; ++i) {
+          float ta, tb;
+          turn_pair(second ? other[i] : x[i], second ? x[i] : other[i], c[i], sn[i], ta, tb);
+          x[i] = second ? tb : ta;
+        }
+      } else if (turns) {
+        const float4 c = *reinterpret_cast<const float4*>(s_cos + d0 / 2), sn = *reinterpret_cast<const float4*>(s_sin + d0 / 2);
+        const float co[4] = {c.x, c.y, c.z, c.w}, si[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float ta, tb;
+          turn_pair(x[2 * i], x[2 * i + 1], co[i], si[i], ta, tb);
+          x[2 * i] = ta;
+          x[2 * i + 1] = tb;
+        }
+      }
+    } else {
+      // any even rotary_dim: partners from the row itself, all read before any lane of the row stores
+      float turned[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t d = d0 + i;
+        const bool pair = !is_v && d < a.turn.rotary_dim, late = by_half ? d >= pairs : d & 1;
+        const uint32_t j = !pair ? 0 : by_half ? (late ? d - pairs : d) : d / 2;
+        const float o = pair ? to_f32<XT>(src[by_half ? (late ? d - pairs : d + pairs) : d ^ 1]) : 0.f;
+        float ta, tb;
+        turn_pair(late ? o : x[i], late ? x[i] : o, s_cos[j], s_sin[j], ta, tb);
+        turned[i] = !pair ? x[i] : late ? tb : ta;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = turned[i];
     }
   }
   if (is_q) {
-    if (live) store8(q_out + (token * a.heads + head) * D + sub * kPiece, x);
+    if (live) store8(q_out + (token * a.heads + head) * D + d0, x);
     return;   // (rows of a head lie in one wave's neighbouring lanes: no group below spans a query row)
   }
 
@@ -135,13 +163,12 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(
   }
   if (!live) return;
   const uint32_t in_page = column & (a.layout.page_rows - 1);
-  const int32_t page = page_table[(size_t)seq * a.limits.table_stride + column / a.layout.page_rows];
   if (page < 0 || (uint32_t)page >= a.pages) {
     if (fault && sub == 0) *fault = 1u;
     return;
   }
   uint8_t* block = cache + (size_t)page * a.layout.page() + (size_t)head * a.layout.block();
-  const uint32_t g = sub * kPiece / a.layout.group;
+  const uint32_t g = d0 / a.layout.group;
   if (is_v) {
     *reinterpret_cast<uint32_t*>(block + a.layout.value_word(in_page, sub)) = word;
     if (sub % lanes == 0) {
@@ -250,21 +277,24 @@ int32_t krm_kv4_append(krm_ctx* ctx, krm_buf q, krm_buf k, krm_buf v, krm_buf q_
                      {total_rows, max_query, 0x7fffffffu, table_stride, page_rows},
                      {depth, rotary_dim, table_rows, table_width, layout},
                      q ? heads : 0u, pages, q_stride, k_stride, v_stride};
-  const uint64_t threads = (uint64_t)kv4_rows(max_query, total_rows) * (a.heads + 2 * kv_heads) * (depth / kPiece);
-  const uint64_t blocks = (threads + kThreads - 1) / kThreads;
-  KRM_REQUIRE(ctx, blocks <= 0x7fffffu, "krm_kv4_append: %u rows of a sequence are more than one call takes", max_query);
-#define KRM_APPEND(XT, D)                                                                                       \
-  kv4_append_kernel<XT, D><<<dim3((uint32_t)blocks, nseq), dim3(kThreads), 0, ctx->stream>>>(                    \
+  const uint32_t rows = kv4_rows(max_query, total_rows);
+  KRM_REQUIRE(ctx, rows <= 0x7fffffu, "krm_kv4_append: %u rows of a sequence are more than one call takes", rows);
+  const dim3 grid(rows, ((a.heads + 2 * kv_heads) * (depth / kPiece) + kThreads - 1) / kThreads, nseq);
+  const bool pieces = rotary_dim % (layout == KRM_ROPE_HALF ? 16 : 8) == 0;
+#define KRM_APPEND(XT, D) { if (pieces) KRM_APPEND_P(XT, D, true); else KRM_APPEND_P(XT, D, false); }
+#define KRM_APPEND_P(XT, D, PIECES)                                                                             \
+  kv4_append_kernel<XT, D, PIECES><<<grid, dim3(kThreads), 0, ctx->stream>>>(                                    \
       ptr<const XT>(k), ptr<const XT>(v), ptr<uint8_t>(cache), ptr<const int32_t>(page_table_i32),               \
       ptr<const int32_t>(cu_rows_i32), ptr<const int32_t>(lens_i32), ptr<const XT>(q), ptr<XT>(q_out),           \
       ptr<const int32_t>(positions_i32), ptr<const float>(cos_table_f32), ptr<const float>(sin_table_f32),       \
       ptr<uint32_t>(fault_u32), a)
 #define KRM_APPEND_D(XT)                      \
-  if (depth == 64) KRM_APPEND(XT, 64);        \
-  else if (depth == 128) KRM_APPEND(XT, 128); \
+  if (depth == 64) KRM_APPEND(XT, 64)         \
+  else if (depth == 128) KRM_APPEND(XT, 128)  \
   else KRM_APPEND(XT, 256)
-  if (io_dtype == KRM_F32) { KRM_APPEND_D(float); } else { KRM_APPEND_D(__half); }
+  if (io_dtype == KRM_F32) { KRM_APPEND_D(float) } else { KRM_APPEND_D(__half) }
 #undef KRM_APPEND_D
+#undef KRM_APPEND_P
 #undef KRM_APPEND
   return launched(ctx, "kv4_append_kernel");
 }
