@@ -299,7 +299,9 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
     float here = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                        fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
     here = quarters_max(here) * scale;
-    if (__any(here > top)) {
+    // The sums are brought to a new maximum where one has grown by more than 2^4; weights are 2^10 times what they would
+    // be, so that their low parts are no subnormal numbers, and at most 2^14.
+    if (__any(here > top + 4.0f)) {
       const float now = fmaxf(here, top);
       const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
       top = now;
@@ -311,19 +313,18 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
         for (int f = 0; f < kOuts; ++f) acc[i][f] *= keep;
       }
     }
-    // f32 rows: weights are 2^10 times what they would be, so that their low parts are no subnormal numbers
-    const float shift = (top == -INFINITY ? 0.f : top) - (kF32 ? 10.0f : 0.0f);
-    float p[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4], scale, -shift));
-      sum += p[j];
-    }
+    const float shift = (top == -INFINITY ? 0.f : top) - 10.0f;
     half8_t ph, pl;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      ph[j] = (_Float16)p[j];
-      pl[j] = less(p[j], ph[j]);
+    for (int j = 0; j < 8; j += 2) {
+      const float2_t p = {__builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4], scale, -shift)),
+                          __builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4 + 1], scale, -shift))};
+      const half2_t hi = rounded2(p);
+      sum += p[0] + p[1];
+      ph[j] = hi.x;
+      ph[j + 1] = hi.y;
+      pl[j] = less(p[0], hi.x);
+      pl[j + 1] = less(p[1], hi.y);
     }
 
     // ---- values: lane (i, c) has rows 4 c .. 4 c + 3 of each half, the same order as the weights
