@@ -35,11 +35,139 @@ struct Stage {
   static constexpr int kLoads = 4 * kParts + 4 * kWords;      // that fill it
 };
 
+struct DecodeAttention : Kv4Attention {
+  uint32_t row_tiles;      // blocks of kRows pairs of a kv head, a workgroup each
+  float row_tiles_inverse, of_sequence_inverse;
+  uint32_t max_splits;     // workgroups that one block's columns are dealt to at most
+  uint32_t partial_rows;   // pairs that a part has room for; parts are [unit][split]: sums of all pairs, their (max, sum)
+  uint32_t least;          // tiles, at least, of a split
+  float share_of_work;     // of all sequences' tiles, in one workgroup
+};
+struct DecodeWork : Work {
+  uint32_t unit, split, nsplit;
+};
+// Over all lanes.
+__device__ inline float wave_sum(float x) {
+#define KRM_ADD_DPP(CTRL, ROWS) \
+  x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false))
+  KRM_ADD_DPP(0x111, 0xf);   // row_shr:1
+  KRM_ADD_DPP(0x112, 0xf);
+  KRM_ADD_DPP(0x114, 0xf);
+  KRM_ADD_DPP(0x118, 0xf);
+  KRM_ADD_DPP(0x142, 0xa);   // row_bcast:15
+  KRM_ADD_DPP(0x143, 0xc);   // row_bcast:31
+#undef KRM_ADD_DPP
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+// Grid (units, splits): workgroups go to the XCDs in turn, and a unit (sequence, kv head, block of pairs) has its
+// next split on the next XCD, so that neither first splits nor a long sequence gather on one of them (32 sequences
+// of up to 4096 columns with splits along x, two XCDs at work: 182 us, so 42.6).
+__device__ inline void find_unit(const DecodeAttention& a, DecodeWork& w, uint32_t& block) {
+  const uint32_t units = gridDim.x, of_sequence = a.layout.kv_heads * a.row_tiles;
+  w.split = blockIdx.y;
+  w.unit = blockIdx.x;
+  if (w.split) {
+    w.unit += units > w.split ? w.split : w.split % units;
+    if (w.unit >= units) w.unit -= units;
+  }
+  w.seq = divided(w.unit, of_sequence, a.of_sequence_inverse);
+  const uint32_t in_sequence = w.unit - w.seq * of_sequence;
+  w.kv_head = divided(in_sequence, a.row_tiles, a.row_tiles_inverse);
+  block = in_sequence - w.kv_head * a.row_tiles;
+}
+// False: nothing to do (or done: rows of a refused sequence are NaN).
+template <typename XT, int D, int kWaves>
+__device__ inline bool find_work(const DecodeAttention& a, DecodeWork& w, uint32_t block, const int32_t* __restrict__ cu_rows,
+                                 const int32_t* __restrict__ lens, XT* __restrict__ out, uint32_t* __restrict__ fault) {
+  constexpr int kThreads = kWaves * kWave;
+  const uint32_t tid = threadIdx.x, pair0 = block * kRows;
+  float work = 0.f;
+  if (a.max_splits > 1) {
+    for (uint32_t i = tid % kWave; i < a.nseq; i += kWave) {
+      const uint32_t n = min((uint32_t)max(lens[i], 0), a.limits.max_columns);
+      work += (float)((a.window ? min(n, a.window) : n) / kTile + 1);
+    }
+  }
+  const int32_t cu1 = cu_rows[w.seq + 1];
+  w.cu0 = cu_rows[w.seq];
+  const Kv4Sequence s = kv4_sequence(w.cu0, cu1, lens[w.seq], a.limits);
+  if (!s.ok && fault && w.split == 0 && tid == 0) *fault = 1u;   // (whichever launch its rows belong to)
+  if (w.cu0 < 0 || cu1 < w.cu0 || (uint32_t)cu1 > a.limits.total_rows) return false;
+  const uint64_t pairs = (uint64_t)(uint32_t)(cu1 - w.cu0) * a.share;
+  if (pair0 >= pairs || pairs < a.least_pairs || pairs > a.most_pairs) return false;
+  if (!s.ok) {
+    if (w.split == 0 && block == 0) refuse<XT, D, kThreads>(a, w.kv_head, w.cu0, cu1, out);
+    return false;
+  }
+  w.count = min((uint64_t)kRows, pairs - pair0);
+  w.row0 = divided(pair0, a.share, a.share_inverse);
+  w.head0 = pair0 - w.row0 * a.share;
+  w.first_row = s.len - s.rows + (int32_t)w.row0;
+  w.last_row = w.first_row + (int32_t)row_of(a, w, w.count - 1);
+  w.low = kv4_first_column(w.first_row, a.window);
+  w.high = w.last_row;
+  const int32_t tile0 = w.low / kTile;
+  const uint32_t tiles = (uint32_t)(w.high / kTile - tile0 + 1);
+  uint32_t per = tiles;
+  w.nsplit = 1;
+  if (a.max_splits > 1) {
+    // the step's tiles, as far as they go by the lengths, are dealt evenly to the workgroups that fit the machine
+    per = max((uint32_t)(wave_sum(work) * a.share_of_work), a.least) + kWaves - 1;
+    per = max(per / kWaves * kWaves, (tiles + a.max_splits - 1) / a.max_splits);
+    w.nsplit = (tiles + per - 1) / per;
+    if (w.split >= w.nsplit) return false;
+  }
+  w.begin = tile0 + (int32_t)min(w.split * per, tiles);
+  w.end = tile0 + (int32_t)min((w.split + 1) * per, tiles);
+  return true;
+}
+
+// A workgroup's part of its rows is published; the workgroup that arrives last joins the parts in order, whichever it
+// is.  `s_part`: nsplit * count * 2 floats of LDS that nobody needs any more.
+template <typename XT, int D, int kThreads>
+__device__ inline void join_parts(const DecodeAttention& a, const DecodeWork& w, XT* __restrict__ out, float* s_part) {
+  const uint32_t tid = threadIdx.x, nsplit = w.nsplit, count = w.count;
+  const size_t part_size = (size_t)a.partial_rows * (D + 2);
+  const float* const parts = a.partials + (size_t)w.unit * a.max_splits * part_size;
+  if (!arrived_last(a.tickets + (size_t)w.unit * kTicketStride, nsplit)) return;
+  for (uint32_t i = tid; i < nsplit * count; i += kThreads) {   // [row][nsplit] (max, sum)
+    const float* state = parts + (i / count) * part_size + a.partial_rows * D + 2 * (i % count);
+    float* to = s_part + ((i % count) * nsplit + i / count) * 2;
+    to[0] = observe(state);
+    to[1] = observe(state + 1);
+  }
+  __syncthreads();
+  for (uint32_t e = 2 * tid; e < count * D; e += 2 * kThreads) {
+    const float* states = s_part + (e / D) * nsplit * 2;
+    float most = -INFINITY, weight = 0.f;
+    float2_t total = {0.f, 0.f};
+    for (uint32_t p = 0; p < nsplit; ++p) most = fmaxf(most, states[2 * p]);
+    const float ref = most == -INFINITY ? 0.f : most;
+    for (uint32_t p0 = 0; p0 < nsplit; p0 += kJoin) {
+      float2_t o[kJoin];
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i) o[i] = observe2(parts + min(p0 + i, nsplit - 1) * part_size + e);
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i) {
+        if (p0 + i < nsplit) {
+          const float k = __builtin_amdgcn_exp2f(states[2 * (p0 + i)] - ref);
+          total[0] = fmaf(k, o[i][0], total[0]);
+          total[1] = fmaf(k, o[i][1], total[1]);
+          weight = fmaf(k, states[2 * (p0 + i) + 1], weight);
+        }
+      }
+    }
+    XT* to = out + row_at(a, w, e / D, D) + e % D;
+    to[0] = from_f32<XT>(total[0] / weight);
+    to[1] = from_f32<XT>(total[1] / weight);
+  }
+}
+
 template <typename XT, int D, int NG, int kWaves>
 __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
     const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table,
     const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens, XT* __restrict__ out,
-    uint32_t* __restrict__ fault, Kv4Attention a) {
+    uint32_t* __restrict__ fault, DecodeAttention a) {
   constexpr bool kF32 = sizeof(XT) == 4;
   constexpr int kThreads = kWaves * kWave;
   using S = Stage<D, NG>;
@@ -51,13 +179,13 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
   __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
 
   const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  Work w;
+  DecodeWork w;
   uint32_t block;
   find_unit(a, w, block);
   // the sequence's first 64 pages are asked for beside its lengths
   const int32_t* table = page_table + (size_t)w.seq * a.limits.table_stride;
   const uint32_t entry = (uint32_t)table[min(lane, a.limits.table_stride - 1)];
-  if (!find_work<XT, D, kThreads, kRows, kTile, kWaves>(a, w, block, cu_rows, lens, out, fault)) return;
+  if (!find_work<XT, D, kWaves>(a, w, block, cu_rows, lens, out, fault)) return;
   const uint32_t count = w.count;
   const int32_t first_row = w.first_row, last_row = w.last_row, low = w.low, high = w.high;
   // this wave's tiles are mine0, mine0 + kWaves, .. (the waves' next tiles lie together: in one long run for each wave
@@ -487,33 +615,31 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
   if (w.nsplit > 1) join_parts<XT, D, kThreads>(a, w, out, s_acc);
 }
 
-// How the columns of a launch are dealt.
-struct LaunchPlan {
-  uint32_t row_tiles = 0, units = 0, max_splits = 0, partial_rows = 0, least = 0, least_pairs = 0, most_pairs = 0xffffffffu;
+// How the columns of a launch of kv4_decode_kernel are dealt.
+struct DecodePlan {
+  uint32_t row_tiles = 0, units = 0, max_splits = 0, partial_rows = 0, least = 0;
   float share_of_work = 0;
   size_t bytes = 0;
 };
 // Eight waves (two a SIMD) while their registers allow it: half as many parts to join as with four, twice a CU.
 constexpr int waves_of(int depth) { return depth == 256 ? 4 : 8; }
-// One workgroup a CU: with 512 and 1024 of them 131000 columns took 49.4 us, with 256 39.8.
-constexpr uint32_t kFill = 256;
 constexpr uint32_t kMostGroups = 2048;   // in a grid, those without a split among them
+constexpr uint32_t kMostSplits = 64;
 static_assert(kMostGroups <= kTicketSlots, "a counter a unit");
-LaunchPlan plan_launch(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs, uint32_t tile_pairs, uint32_t tile_columns,
-                       uint32_t least, uint32_t most_splits, size_t part_floats) {
-  LaunchPlan p;
-  const uint64_t row_tiles = (pairs + tile_pairs - 1) / tile_pairs, units = (uint64_t)s.nseq * s.kv_heads * row_tiles;
+DecodePlan plan_decode(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs) {
+  DecodePlan p;
+  const uint64_t row_tiles = (pairs + kRows - 1) / kRows, units = (uint64_t)s.nseq * s.kv_heads * row_tiles;
   p.row_tiles = (uint32_t)row_tiles;
-  p.partial_rows = pairs < tile_pairs ? (uint32_t)pairs : tile_pairs;
+  p.partial_rows = pairs < kRows ? (uint32_t)pairs : kRows;
   p.units = (uint32_t)(units < 0xffffffffu ? units : 0xffffffffu);
-  p.least = least;
-  const uint64_t tiles = ((uint64_t)max_columns + tile_columns - 1) / tile_columns + 1, most = (tiles + least - 1) / least;
+  p.least = 2 * waves_of(s.depth);   // two a wave: joining two parts costs about as much as a tile more
+  const uint64_t tiles = ((uint64_t)max_columns + kTile - 1) / kTile + 1, most = (tiles + p.least - 1) / p.least;
   uint64_t splits = units ? kMostGroups / units : 1;
-  splits = splits > most_splits ? most_splits : splits;
+  splits = splits > kMostSplits ? kMostSplits : splits;
   splits = splits > most ? most : splits;
   p.max_splits = splits < 1 ? 1 : (uint32_t)splits;   // (with more units than kMostGroups, and so than counters: one)
-  p.share_of_work = (float)s.kv_heads * (float)row_tiles / kFill;
-  p.bytes = splits > 1 ? (size_t)units * splits * part_floats * sizeof(float) : 0;
+  p.share_of_work = (float)s.kv_heads * (float)row_tiles / kKv4Groups;
+  p.bytes = splits > 1 ? (size_t)units * splits * p.partial_rows * (s.depth + 2) * sizeof(float) : 0;
   return p;
 }
 // Which kernel has which sequences.  kv4_decode_kernel takes blocks of 16 (row, head) pairs and reads the columns again for
@@ -525,7 +651,7 @@ LaunchPlan plan_launch(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs, 
 constexpr uint64_t kFewPairs = 32;
 struct AttentionPlan {
   bool few = true, many = false;   // which launches there are
-  LaunchPlan rows, chunk;
+  DecodePlan decode;
   size_t bytes = 0;
 };
 AttentionPlan plan_attention(const Kv4Shape& s, uint32_t max_columns) {
@@ -533,20 +659,14 @@ AttentionPlan plan_attention(const Kv4Shape& s, uint32_t max_columns) {
   const uint32_t rows = kv4_rows(s.max_query, s.total_rows);
   const uint64_t pairs = (uint64_t)rows * (s.heads / s.kv_heads);
   const uint64_t blocks = (uint64_t)s.nseq * s.kv_heads * ((pairs + kRows - 1) / kRows);
-  p.many = pairs > kFewPairs && blocks >= (s.depth == 256 ? 4u : 2u) * kFill;
+  p.many = pairs > kFewPairs && blocks >= (s.depth == 256 ? 4u : 2u) * kKv4Groups;
   p.few = !p.many || (s.nseq > 1 && s.total_rows < (uint64_t)s.nseq * rows);
-  if (p.few) {
-    // a split has two tiles a wave at least: joining two parts costs about as much as a tile more
-    p.rows = plan_launch(s, max_columns, p.many ? kFewPairs : pairs, kRows, kTile, 2 * waves_of(s.depth), 64,
-                         (size_t)(pairs < kRows ? pairs : kRows) * (s.depth + 2));
-    if (p.many) p.rows.most_pairs = kFewPairs;
-  }
+  if (p.few) p.decode = plan_decode(s, max_columns, p.many ? kFewPairs : pairs);
+  p.bytes = p.decode.bytes;
   if (p.many) {
-    p.chunk = plan_launch(s, max_columns, pairs, kv4_chunk_pairs(s.depth), kv4_chunk_columns(s.depth), 4, 16,
-                          (size_t)kv4_chunk_pairs(s.depth) * (s.depth + 4));
-    if (p.few) p.chunk.least_pairs = kFewPairs + 1;
+    const size_t chunk = kv4_chunk_workspace(s.depth, max_columns);
+    if (chunk > p.bytes) p.bytes = chunk;
   }
-  p.bytes = p.rows.bytes > p.chunk.bytes ? p.rows.bytes : p.chunk.bytes;
   return p;
 }
 
@@ -592,45 +712,42 @@ int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_t
   KRM_REQUIRE(ctx, q != out, "krm_kv4_attention: out is q");
   const AttentionPlan plan = plan_attention(shape, max_columns);
   const uint32_t share = heads / kv_heads;
-  KRM_REQUIRE(ctx, plan.rows.units <= 0x7fffffu && plan.chunk.units <= 0x7fffffu &&
-                       (uint64_t)kv4_rows(max_query, total_rows) * share <= 1u << 24,
+  const uint64_t blocks = (uint64_t)nseq * kv_heads * ((uint64_t)kv4_rows(max_query, total_rows) * share / kRows + 1);
+  KRM_REQUIRE(ctx, blocks <= 0x7fffffu && (uint64_t)kv4_rows(max_query, total_rows) * share <= 1u << 24,
               "krm_kv4_attention: %u sequences of %u rows of %u heads are more than one call takes", nseq, max_query, heads);
   if (plan.bytes) {
     KRM_REQUIRE(ctx, workspace && workspace_bytes >= plan.bytes, "krm_kv4_attention: workspace of %zu bytes, %zu needed",
                 workspace ? workspace_bytes : (size_t)0, plan.bytes);
     KRM_TRY(needs_serial_scratch(ctx, "krm_kv4_attention"));
   }
-  auto arguments = [&](const LaunchPlan& p) {
-    Kv4Attention a;
-    a.layout = {depth, group, page_rows, kv_heads};
-    a.limits = {total_rows, max_query, max_columns, table_stride, page_rows};
-    a.nseq = nseq;
-    a.heads = heads;
-    a.pages = pages;
-    a.window = window;
-    a.share = share;
-    a.row_tiles = p.row_tiles;
-    a.share_inverse = 1.0f / share;
-    a.row_tiles_inverse = 1.0f / p.row_tiles;
-    a.of_sequence_inverse = 1.0f / ((float)kv_heads * p.row_tiles);
-    a.max_splits = p.max_splits;
-    a.partial_rows = p.partial_rows;
-    a.least = p.least;
-    a.least_pairs = p.least_pairs;
-    a.most_pairs = p.most_pairs;
-    a.share_of_work = p.share_of_work;
-    a.scale = scale;
-    a.partials = ptr<float>(workspace);
-    a.tickets = ctx->tickets;
-    return a;
-  };
+  DecodeAttention a;
+  a.layout = {depth, group, page_rows, kv_heads};
+  a.limits = {total_rows, max_query, max_columns, table_stride, page_rows};
+  a.nseq = nseq;
+  a.heads = heads;
+  a.pages = pages;
+  a.window = window;
+  a.share = share;
+  a.share_inverse = 1.0f / share;
+  a.scale = scale;
+  a.partials = ptr<float>(workspace);
+  a.tickets = ctx->tickets;
   if (plan.many) {
-    KRM_TRY(launch_kv4_chunk(ctx, arguments(plan.chunk), {q, cache, page_table_i32, cu_rows_i32, lens_i32, out, fault_u32},
-                             plan.chunk.units, io_dtype));
+    a.least_pairs = plan.few ? (uint32_t)kFewPairs + 1 : 0;
+    a.most_pairs = 0xffffffffu;
+    KRM_TRY(launch_kv4_chunk(ctx, a, {q, cache, page_table_i32, cu_rows_i32, lens_i32, out, fault_u32}, io_dtype));
     if (!plan.few) return KRM_OK;
   }
-  const Kv4Attention a = arguments(plan.rows);
-  const dim3 grid(plan.rows.units, plan.rows.max_splits);
+  a.least_pairs = 0;
+  a.most_pairs = plan.many ? (uint32_t)kFewPairs : 0xffffffffu;
+  a.row_tiles = plan.decode.row_tiles;
+  a.row_tiles_inverse = 1.0f / a.row_tiles;
+  a.of_sequence_inverse = 1.0f / ((float)kv_heads * a.row_tiles);
+  a.max_splits = plan.decode.max_splits;
+  a.partial_rows = plan.decode.partial_rows;
+  a.least = plan.decode.least;
+  a.share_of_work = plan.decode.share_of_work;
+  const dim3 grid(plan.decode.units, a.max_splits);
   const int waves = waves_of(depth);
   const size_t joined = (size_t)waves * a.partial_rows * (depth + 4) * sizeof(float);
 #define KRM_ATTENTION(XT, D, NG)                                                                                 \

@@ -49,11 +49,148 @@ struct Chunk {
   static constexpr uint32_t kTileBytes = (kKeyPlanes + kValuePlanes) * kPlane;
 };
 
+// The inclusive sums over the lanes.
+__device__ inline uint32_t wave_through(uint32_t x) {
+#define KRM_THROUGH(CTRL, ROWS) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false)
+  KRM_THROUGH(0x111, 0xf);   // row_shr:1
+  KRM_THROUGH(0x112, 0xf);
+  KRM_THROUGH(0x114, 0xf);
+  KRM_THROUGH(0x118, 0xf);
+  KRM_THROUGH(0x142, 0xa);   // row_bcast:15
+  KRM_THROUGH(0x143, 0xc);   // row_bcast:31
+#undef KRM_THROUGH
+  return x;
+}
+
+// A launch's work is one long row of units of 2^grain columns: for each sequence, kv head and block of kPairs pairs those
+// that its rows see.  Each of kKv4Groups workgroups has an equal run of it (in a grid of blocks times splits, 352
+// workgroups of up to 45 tiles, four prompts of 512 rows behind 200 to 4100 columns took 190 us, so 178), which may end one block's columns and begin
+// another's.  Every wave reads the step's words itself, 64 sequences at a time.
+struct ChunkAttention : Kv4Attention {
+  uint32_t grain;
+  uint32_t least;   // units, at least, of a run
+};
+struct ChunkWork : Work {
+  bool refused;                       // the sequence's words break the limits
+  int32_t cu1;
+  uint32_t first_group, parts, part;  // workgroups that have some of these pairs, and which of them this is
+};
+// Where the parts lie: the first part of some pairs is its workgroup's last piece, any other one the first.
+__device__ inline uint32_t part_slot(const ChunkWork& w, uint32_t part) { return 2 * (w.first_group + part) + (part == 0); }
+
+template <int kPairs, int kTile>
+struct Deal {
+  struct Sequence {
+    uint32_t through;   // work up to the sequence's end
+    Kv4Blocks blocks;
+    int32_t cu0, cu1, len;
+    uint32_t ok;
+  };
+  const ChunkAttention& a;
+  const int32_t* cu_rows;
+  const int32_t* lens;
+  Sequence* at_hand;               // 64 sequences, in LDS (every wave writes all of them, the same words)
+  uint32_t group, per, at, end;
+  uint32_t base = 0, before = 0;   // of the sequences at hand: the first one, and the work before them
+
+  __device__ static inline uint32_t lane_id() {
+    uint32_t tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));   // (see the kernel's)
+    return tid % kWave;
+  }
+  // A lane's sequence of the 64 from `first` on.
+  __device__ inline Sequence read(uint32_t first) const {
+    const uint32_t seq = first + lane_id(), i = min(seq, a.nseq - 1);
+    Sequence s;
+    s.cu0 = cu_rows[i];
+    s.cu1 = cu_rows[i + 1];
+    s.len = lens[i];
+    s.ok = kv4_sequence(s.cu0, s.cu1, s.len, a.limits).ok;
+    s.blocks = {0, 1, 0};
+    if (seq < a.nseq && s.cu0 >= 0 && s.cu1 > s.cu0 && (uint32_t)s.cu1 <= a.limits.total_rows) {
+      const uint64_t pairs = (uint64_t)(uint32_t)(s.cu1 - s.cu0) * a.share;
+      if (pairs >= a.least_pairs && pairs <= a.most_pairs) {
+        s.blocks.blocks = 1;   // (all rows of a refused sequence)
+        if (s.ok) s.blocks = kv4_blocks(pairs, a.share, kPairs, s.len, a.window, a.grain);
+      }
+    }
+    s.through = wave_through(a.layout.kv_heads * s.blocks.all());
+    return s;
+  }
+  __device__ static inline uint32_t last_lane(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, kWave - 1);
+  }
+
+  __device__ inline Deal(const ChunkAttention& args, const int32_t* cu, const int32_t* l, uint32_t* fault)
+      : a(args), cu_rows(cu), lens(l) {
+    __shared__ Sequence s_sequences[kWave];
+    at_hand = s_sequences;
+    // neighbouring runs, which may share a kv head's columns, lie on one XCD
+    group = (blockIdx.x % 8) * (kKv4Groups / 8) + blockIdx.x / 8;
+    uint32_t total = 0;
+    Sequence s;
+    for (uint32_t first = 0; first < a.nseq; first += kWave) {
+      s = read(first);
+      total += last_lane(s.through);
+      if (fault && blockIdx.x == 0 && !s.ok) *fault = 1u;
+    }
+    if (a.nseq > kWave) s = read(0);
+    at_hand[lane_id()] = s;
+    per = max((total + kKv4Groups - 1) / kKv4Groups, a.least);
+    at = min(group * per, total);
+    end = min(at + per, total);
+  }
+  // The next piece of this workgroup's run; false at its end.
+  __device__ inline bool next(ChunkWork& w) {
+    if (at >= end) return false;
+    uint32_t through = at_hand[lane_id()].through;
+    while (at - before >= last_lane(through)) {
+      before += last_lane(through);
+      base += kWave;
+      __syncthreads();
+      const Sequence s = read(base);
+      at_hand[lane_id()] = s;
+      through = s.through;
+    }
+    const uint32_t lane = (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(through > at - before));
+    const auto of = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+    const Sequence& s = at_hand[lane];
+    const Kv4Blocks blocks = {of(s.blocks.blocks), of(s.blocks.first), of(s.blocks.step)};
+    const uint32_t of_head = blocks.all(), start = before + of(s.through) - a.layout.kv_heads * of_head;
+    w.seq = base + lane;
+    w.kv_head = of((at - start) / of_head);
+    const uint32_t head_at = start + w.kv_head * of_head, block = of(blocks.block_at(at - head_at));
+    const uint32_t block_at = head_at + blocks.before(block), width = blocks.of(block);
+    const uint32_t from = at - block_at, to = min(width, from + (end - at));
+    at += to - from;
+    w.cu0 = (int32_t)of((uint32_t)s.cu0);
+    w.cu1 = (int32_t)of((uint32_t)s.cu1);
+    w.refused = of(s.ok) == 0;
+    const int32_t rows = w.cu1 - w.cu0;
+    const uint32_t pair0 = block * kPairs;
+    w.count = (uint32_t)min((uint64_t)kPairs, (uint64_t)(uint32_t)rows * a.share - pair0);
+    w.row0 = of(divided(pair0, a.share, a.share_inverse));
+    w.head0 = pair0 - w.row0 * a.share;
+    w.first_row = (int32_t)of((uint32_t)s.len) - rows + (int32_t)w.row0;
+    w.last_row = w.first_row + (int32_t)of(row_of(a, w, w.count - 1));
+    w.low = kv4_first_column(w.first_row, a.window);
+    w.high = w.last_row;
+    // the units are an estimate (rounded, of a window's widest block): what it leaves or lacks is the last part's
+    const int32_t tile0 = w.low / kTile, tiles = w.high / kTile - tile0 + 1;
+    w.begin = tile0 + (int32_t)min(((uint64_t)from << a.grain) / kTile, (uint64_t)tiles);
+    w.end = tile0 + (to == width ? tiles : (int32_t)min(((uint64_t)to << a.grain) / kTile, (uint64_t)tiles));
+    w.first_group = of(block_at / per);
+    w.parts = of((block_at + width - 1) / per) - w.first_group + 1;
+    w.part = group - w.first_group;
+    return true;
+  }
+};
+
 template <typename XT, int D, int NG>
 __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
     const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table,
     const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens, XT* __restrict__ out,
-    uint32_t* __restrict__ fault, Kv4Attention a) {
+    uint32_t* __restrict__ fault, ChunkAttention a) {
   using C = Chunk<XT, D>;
   constexpr bool kF32 = C::kF32;
   constexpr int kThreads = C::kThreads, kPairs = C::kPairs, kColumns = C::kColumns, kBlocks = C::kBlocks;
@@ -63,12 +200,16 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
   __shared__ uint32_t s_unsound[2][kColumns];         // groups of a column's values that are no numbers (edge tiles)
   __shared__ uint32_t s_any[2];
 
-  const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  Work w;
-  uint32_t block;
-  find_unit(a, w, block);
-  block = a.row_tiles - 1 - block;   // late rows, which see the most columns, begin first
-  if (!find_work<XT, D, kThreads, kPairs, kColumns, 1>(a, w, block, cu_rows, lens, out, fault)) return;
+  Deal<kPairs, kColumns> deal(a, cu_rows, lens, fault);
+  ChunkWork w;
+  while (deal.next(w)) {
+  if (w.refused) {
+    refuse<XT, D, kThreads>(a, w.kv_head, w.cu0, w.cu1, out);
+    continue;
+  }
+  uint32_t tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));   // (what hangs on it alone is found for each piece, and not kept beside all of them)
+  const uint32_t lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int32_t low = w.low, high = w.high;
 
   // ---- this wave's rows: lane (m = lane % 32, half)
@@ -83,6 +224,7 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
       has_rows ? w.first_row + (int32_t)row_of(a, w, min(wave * 32 + 31, w.count - 1)) : wave_low - 1;
   half8_t qh[kSteps], ql[kF32 ? kSteps : 1];
   float scale = a.scale;
+  asm volatile("" : "+v"(scale));
   {
     const XT* src = q + row_at(a, w, live ? pair : 0, D) + 8 * half;
     if constexpr (!kF32) {
@@ -106,8 +248,8 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
       most = across_halves(most, [](float x, float y) { return fmaxf(x, y); });
       int e = 0;
       if (most > 0.f && most < INFINITY)
-        e = max(min(6 - __builtin_amdgcn_frexp_expf(most), 100), __builtin_amdgcn_frexp_expf(a.scale) - 110);
-      scale = ldexpf(a.scale, -e);
+        e = max(min(6 - __builtin_amdgcn_frexp_expf(most), 100), __builtin_amdgcn_frexp_expf(scale) - 110);
+      scale = ldexpf(scale, -e);
 #pragma unroll
       for (int st = 0; st < kSteps; ++st)
 #pragma unroll
@@ -139,7 +281,7 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
     uint32_t bad;
   };
   auto fetch = [&](int32_t tile) __attribute__((always_inline)) -> Raw {
-    Raw r;
+    Raw r = {};
     const int32_t column = tile * kColumns + 16 * (int32_t)my_block;
     uint32_t id = 0;
     r.bad = 0;
@@ -410,11 +552,9 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
   for (uint32_t i = tid; i < 2 * kColumns; i += kThreads) s_unsound[i / kColumns][i % kColumns] = 0;
   if (tid < 2) s_any[tid] = 0;
   __syncthreads();
-  Raw raw = fetch(w.begin);
-  make(raw, w.begin, 0);
-  if (w.begin + 1 < w.end) raw = fetch(w.begin + 1);
-  __syncthreads();
-  for (int32_t tile = w.begin; tile < w.end; ++tile) {
+  Raw raw = {};   // (undefined, it would be kept from piece to piece)
+  if (w.begin < w.end) raw = fetch(w.begin);
+  for (int32_t tile = w.begin - 1; tile < w.end; ++tile) {   // (the first turn makes the first tile, and has none to multiply)
     const uint32_t buffer = (uint32_t)(tile - w.begin) & 1u;
     // The two waves of a SIMD are a key maker and a value maker: one makes before it multiplies and the other behind, so
     // that one's conversions and exponentials run beside the other's products.
@@ -424,7 +564,7 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
         if (tile + 2 < w.end) raw = fetch(tile + 2);
       }
     };
-    const bool sees = tile * kColumns <= wave_high && tile * kColumns + kColumns > wave_low;
+    const bool sees = tile >= w.begin && tile * kColumns <= wave_high && tile * kColumns + kColumns > wave_low;
     if (makes_values) next();
     if (sees) consume(tile, buffer);
     if (!makes_values) next();
@@ -441,32 +581,25 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
 
   // ---- parts: as the lanes hold them, (max, sum) of every lane behind the sums; whoever arrives last joins them in
   // order in the same lanes
-  if (w.nsplit > 1) {
-    __shared__ uint32_t s_ticket;
+  bool mine_to_write = true;
+  if (w.parts > 1) {
     constexpr uint32_t kState = kOuts * 16 * kThreads;          // floats before the states
     constexpr size_t kPart = kState + 2 * kThreads;
-    float* const parts = a.partials + (size_t)w.unit * a.max_splits * kPart;
-    float* const mine = parts + w.split * kPart + 2 * tid;
+    float* const mine = a.partials + part_slot(w, w.part) * kPart + 2 * tid;
 #pragma unroll
     for (int o = 0; o < kOuts; ++o)
 #pragma unroll
       for (int r = 0; r < 16; r += 2)
         publish2(mine + (o * 16 + r) * kThreads, float2_t{acc[o][r], acc[o][r + 1]});
     publish2(mine + kState, float2_t{top, sum});
-    // every store of this workgroup is through before it is counted (a release fence would write the whole L2 back)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    uint32_t* ticket = a.tickets + (size_t)w.unit * kTicketStride;
-    if (tid == 0) s_ticket = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (s_ticket + 1 != w.nsplit) return;
-    if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    mine_to_write = arrived_last(a.tickets + (size_t)w.first_group * kTicketStride, w.parts);
+    if (mine_to_write) {
     top = -INFINITY;
     sum = 0.f;
 #pragma unroll
     for (int o = 0; o < kOuts; ++o) acc[o] = float16_t{};
-    for (uint32_t p = 0; p < w.nsplit; ++p) {
-      const float* from_part = parts + p * kPart + 2 * tid;
+    for (uint32_t p = 0; p < w.parts; ++p) {
+      const float* from_part = a.partials + part_slot(w, p) * kPart + 2 * tid;
       const float2_t state = observe2(from_part + kState);
       float2_t x[kOuts * 8];
 #pragma unroll
@@ -480,9 +613,10 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[o][r] = fmaf(acc[o][r], keep, x[(o * 16 + r) / 2][r & 1] * take);
     }
+    }
   }
   // ---- out: lane (m, half) has elements 32 o + 8 (r / 4) + 4 half + r % 4 of its pair
-  if (live) {
+  if (live && mine_to_write) {
     XT* to = out + row_at(a, w, pair, D) + 4 * half;
     const float inverse = 1.0f / sum;
 #pragma unroll
@@ -496,26 +630,28 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
         else *reinterpret_cast<uint2*>(to + 32 * o + 2 * r) = *reinterpret_cast<const uint2*>(x);
       }
   }
+  __syncthreads();   // (LDS is the next piece's)
+  }
 }
 
 template <typename XT, int D, int NG>
-void launch(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& b, uint32_t units) {
+void launch(krm_ctx* ctx, const ChunkAttention& a, const Kv4Buffers& b) {
   using C = Chunk<XT, D>;
-  kv4_chunk_kernel<XT, D, NG><<<dim3(units, a.max_splits), dim3(C::kThreads), 2 * C::kTileBytes, ctx->stream>>>(
+  kv4_chunk_kernel<XT, D, NG><<<dim3(kKv4Groups), dim3(C::kThreads), 2 * C::kTileBytes, ctx->stream>>>(
       ptr<const XT>(b.q), ptr<const uint8_t>(b.cache), ptr<const int32_t>(b.page_table),
       ptr<const int32_t>(b.cu_rows), ptr<const int32_t>(b.lens), ptr<XT>(b.out), ptr<uint32_t>(b.fault), a);
 }
 template <typename XT>
-void launch_depth(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& b, uint32_t units) {
+void launch_depth(krm_ctx* ctx, const ChunkAttention& a, const Kv4Buffers& b) {
   switch (a.layout.depth * 16 + a.layout.groups()) {
-    case 64 * 16 + 1: return launch<XT, 64, 1>(ctx, a, b, units);
-    case 64 * 16 + 2: return launch<XT, 64, 2>(ctx, a, b, units);
-    case 128 * 16 + 1: return launch<XT, 128, 1>(ctx, a, b, units);
-    case 128 * 16 + 2: return launch<XT, 128, 2>(ctx, a, b, units);
-    case 128 * 16 + 4: return launch<XT, 128, 4>(ctx, a, b, units);
-    case 256 * 16 + 2: return launch<XT, 256, 2>(ctx, a, b, units);
-    case 256 * 16 + 4: return launch<XT, 256, 4>(ctx, a, b, units);
-    default: return launch<XT, 256, 8>(ctx, a, b, units);
+    case 64 * 16 + 1: return launch<XT, 64, 1>(ctx, a, b);
+    case 64 * 16 + 2: return launch<XT, 64, 2>(ctx, a, b);
+    case 128 * 16 + 1: return launch<XT, 128, 1>(ctx, a, b);
+    case 128 * 16 + 2: return launch<XT, 128, 2>(ctx, a, b);
+    case 128 * 16 + 4: return launch<XT, 128, 4>(ctx, a, b);
+    case 256 * 16 + 2: return launch<XT, 256, 2>(ctx, a, b);
+    case 256 * 16 + 4: return launch<XT, 256, 4>(ctx, a, b);
+    default: return launch<XT, 256, 8>(ctx, a, b);
   }
 }
 
@@ -523,14 +659,29 @@ void launch_depth(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& b, uint
 
 namespace krm {
 
-uint32_t kv4_chunk_pairs(uint32_t depth) { return depth == 256 ? Chunk<float, 256>::kPairs : Chunk<float, 64>::kPairs; }
-uint32_t kv4_chunk_columns(uint32_t depth) {
-  return depth == 256 ? Chunk<float, 256>::kColumns : Chunk<float, 64>::kColumns;
+static_assert(kKv4Groups <= kTicketSlots, "a counter a workgroup");
+
+size_t kv4_chunk_workspace(uint32_t depth, uint32_t max_columns) {
+  const uint32_t tile = depth == 256 ? Chunk<float, 256>::kColumns : Chunk<float, 64>::kColumns;
+  if (max_columns <= tile) return 0;   // (blocks of one tile are in one piece: see launch_kv4_chunk)
+  const uint32_t pairs = depth == 256 ? Chunk<float, 256>::kPairs : Chunk<float, 64>::kPairs;
+  return 2 * (size_t)kKv4Groups * pairs * (depth + 4) * sizeof(float);
 }
 
-int32_t launch_kv4_chunk(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& b, uint32_t units, int32_t io_dtype) {
-  if (io_dtype == KRM_F32) launch_depth<float>(ctx, a, b, units);
-  else launch_depth<__half>(ctx, a, b, units);
+int32_t launch_kv4_chunk(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& b, int32_t io_dtype) {
+  const uint32_t pairs = a.layout.depth == 256 ? Chunk<float, 256>::kPairs : Chunk<float, 64>::kPairs;
+  const uint32_t tile = a.layout.depth == 256 ? Chunk<float, 256>::kColumns : Chunk<float, 64>::kColumns;
+  ChunkAttention c;
+  static_cast<Kv4Attention&>(c) = a;
+  // Units of four columns, of a tile where no block has more; or as many as keep a launch's work in 31 bits.
+  const uint64_t rows = kv4_rows(a.limits.max_query, a.limits.total_rows);
+  const uint64_t blocks = (uint64_t)a.nseq * a.layout.kv_heads * ((rows * a.share + pairs - 1) / pairs);
+  c.grain = a.limits.max_columns <= tile ? 31 - __builtin_clz(tile) : 2;
+  while (blocks * ((((uint64_t)a.limits.max_columns + pairs) >> c.grain) + 1) >= 1ull << 31) ++c.grain;
+  // a run has two tiles at least: joining two parts costs more
+  c.least = 2 * tile >> c.grain ? 2 * tile >> c.grain : 1;
+  if (io_dtype == KRM_F32) launch_depth<float>(ctx, c, b);
+  else launch_depth<__half>(ctx, c, b);
   return launched(ctx, "kv4_chunk_kernel");
 }
 

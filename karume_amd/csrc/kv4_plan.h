@@ -76,6 +76,42 @@ KRM_HD inline Kv4Sequence kv4_sequence(int32_t cu0, int32_t cu1, int32_t len, co
          (uint64_t)(uint32_t)len <= (uint64_t)a.table_stride * a.page_rows;
   return s;
 }
+
+// Work of one kv head of a sequence in blocks of rows, each of which sees some more columns than the one before it:
+// block b has first + b * step units.  All of them together are less than 2^31.
+struct Kv4Blocks {
+  uint32_t blocks, first, step;
+  KRM_HD uint32_t of(uint32_t b) const { return first + b * step; }
+  KRM_HD uint32_t before(uint32_t b) const { return b * first + (step ? b * (b - 1) / 2 * step : 0); }
+  KRM_HD uint32_t all() const { return before(blocks); }
+  // The block that unit `at` (less than all()) is in.
+  KRM_HD uint32_t block_at(uint32_t at) const {
+    const float x = (float)first - 0.5f * (float)step;   // the root of before(b) = at
+    uint32_t b = (uint32_t)(2.0f * (float)at / (x + sqrtf(x * x + 2.0f * (float)step * (float)at)));
+    if (b > blocks - 1) b = blocks - 1;
+    while (before(b) > at) --b;
+    while (b + 1 < blocks && before(b + 1) <= at) ++b;
+    return b;
+  }
+};
+// Units of 2^grain columns.  `pairs` (row, head) pairs, in blocks of `block_pairs`, of a sequence of `len` columns.
+KRM_HD inline Kv4Blocks kv4_blocks(uint64_t pairs, uint32_t share, uint32_t block_pairs, int32_t len, uint32_t window,
+                                   uint32_t grain) {
+  Kv4Blocks b;
+  const uint32_t rows = (uint32_t)(pairs / share);
+  b.blocks = (uint32_t)((pairs + block_pairs - 1) / block_pairs);
+  const uint32_t last = (uint32_t)((pairs < block_pairs ? pairs : block_pairs) - 1) / share;   // of the first block
+  b.first = (((uint32_t)len - rows + last) >> grain) + 1;
+  b.step = b.blocks > 1 ? block_pairs / share >> grain : 0;
+  if (window) {   // blocks that all see a window are alike, and are all taken for such ones where some do
+    const uint64_t most = (((uint64_t)window + block_pairs) >> grain) + 1;
+    if (b.of(b.blocks - 1) > most) {
+      b.first = (uint32_t)most;
+      b.step = 0;
+    }
+  }
+  return b;
+}
 // First column that a row at `position` sees.
 KRM_HD inline int32_t kv4_first_column(int32_t position, uint32_t window) {
   return window == 0 || (uint32_t)position < window ? 0 : position - (int32_t)window + 1;
