@@ -644,9 +644,9 @@ DecodePlan plan_decode(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs) 
 }
 // Which kernel has which sequences.  kv4_decode_kernel takes blocks of 16 (row, head) pairs and reads the columns again for
 // each, kv4_chunk_kernel up to 256 of them with one turn of the codes, which pays where blocks of 16 are several times
-// the CUs (us, decode / chunk, 8 kv heads x 4, D 128, fp16, columns 1024 and 8192: 512 rows of one sequence 51 / 36 and
-// 236 / 128; 128 rows 17 / 34 and 70 / 73; 64 rows of eight 58 / 37 and 242 / 127; 16 rows of eight 19 / 33 and 71 / 101;
-// 1 kv head x 8, D 256: 512 rows 26 / 65 and 124 / 153, of eight 168 / 117 and 946 / 802).
+// the CUs (us, decode / chunk, 8 kv heads x 4, D 128, fp16, columns 1024 and 8192: 512 rows of one sequence 51 / 38 and
+// 236 / 127; 128 rows 17 / 34 and 70 / 73; 64 rows of eight 58 / 39 and 242 / 121; 16 rows of eight 19 / 33 and 71 / 101;
+// 1 kv head x 8, D 256: 512 rows 26 / 65 and 124 / 153, of eight 168 / 117 and 946 / 844).
 // A step may hold both kinds: sequences of up to kFewPairs pairs then stay with the decode kernel, in a launch of its own.
 constexpr uint64_t kFewPairs = 32;
 struct AttentionPlan {

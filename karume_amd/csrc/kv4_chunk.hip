@@ -62,23 +62,44 @@ __device__ inline uint32_t wave_through(uint32_t x) {
   return x;
 }
 
-// A launch's work is one long row of units of 2^grain columns: for each sequence, kv head and block of kPairs pairs those
-// that its rows see.  Each of kKv4Groups workgroups has an equal run of it (in a grid of blocks times splits, 352
-// workgroups of up to 45 tiles, four prompts of 512 rows behind 200 to 4100 columns took 190 us, so 178), which may end one block's columns and begin
-// another's.  Every wave reads the step's words itself, 64 sequences at a time.
+// Values that are the same in every lane.
+__device__ inline uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
+template <typename T>
+__device__ inline T scalars(const T& from) {
+  struct Words {
+    uint32_t w[sizeof(T) / 4];
+  };
+  Words x = __builtin_bit_cast(Words, from);
+#pragma unroll
+  for (uint32_t i = 0; i < sizeof(T) / 4; ++i) x.w[i] = scalar(x.w[i]);
+  return __builtin_bit_cast(T, x);
+}
+
+// How blocks of kPairs (row, head) pairs are dealt to kKv4Groups workgroups, one a CU.  Every wave reads the step's words
+// itself, 64 sequences at a time.
+// A launch's work is one long row of units of 2^grain columns: for each sequence, kv head and block those that its rows see.
+// Each workgroup has an equal run of it, which may end one block's columns and begin another's.  (A grid of blocks times
+// equal splits: four prompts of 512 rows behind 200 to 4100 columns 190 us, so 178; three of 512 of 2048 104 us, so 96.)
+// Beginning a block costs a workgroup as much as kBegin tiles, which its work counts, and joining a block's parts several
+// times that, so that a run's end less than kSnap tiles away from a block's is moved there (2048 rows of 2048 columns, 4 kv
+// heads x 8, D 64, f32: without both 119.9 us, so 76.5).
+// If whole blocks, or equal parts of them, can be dealt one a workgroup, and none has kDearer tiles more than a run, they
+// are (512 rows of 1024 columns, 8 kv heads x 4, D 128: runs 44.6 us, parts 38.3).
+constexpr uint32_t kBegin = 2, kSnap = 3, kDearer = 8;
 struct ChunkAttention : Kv4Attention {
   uint32_t grain;
   uint32_t least;   // units, at least, of a run
 };
 struct ChunkWork : Work {
-  bool refused;                       // the sequence's words break the limits
+  uint32_t refused;                   // the sequence's words break the limits
   int32_t cu1;
   uint32_t first_group, parts, part;  // workgroups that have some of these pairs, and which of them this is
 };
 // Where the parts lie: the first part of some pairs is its workgroup's last piece, any other one the first.
 __device__ inline uint32_t part_slot(const ChunkWork& w, uint32_t part) { return 2 * (w.first_group + part) + (part == 0); }
 
-template <int kPairs, int kTile>
+// (in LDS: a tile's loop has no registers for it)
+template <int kWaves, int kPairs, int kTile>
 struct Deal {
   struct Sequence {
     uint32_t through;   // work up to the sequence's end
@@ -86,21 +107,23 @@ struct Deal {
     int32_t cu0, cu1, len;
     uint32_t ok;
   };
-  const ChunkAttention& a;
-  const int32_t* cu_rows;
-  const int32_t* lens;
-  Sequence* at_hand;               // 64 sequences, in LDS (every wave writes all of them, the same words)
-  uint32_t group, per, at, end;
-  uint32_t base = 0, before = 0;   // of the sequences at hand: the first one, and the work before them
+  struct Run : Kv4Run {
+    uint32_t base, before;   // of the sequences at hand: the first one, and the work before them
+  };
+  Sequence sequences[kWave];   // at hand (every wave writes all of them, the same words)
+  Run runs[kWaves];            // each wave's, the same
 
-  __device__ static inline uint32_t lane_id() {
+  // neighbouring runs, which may join parts, lie on one XCD
+  __device__ static inline uint32_t group() { return blockIdx.x % 8 * (kKv4Groups / 8) + blockIdx.x / 8; }
+  __device__ static inline uint32_t thread() {
     uint32_t tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));   // (see the kernel's)
-    return tid % kWave;
+    asm volatile("" : "+v"(tid));   // (what hangs on it alone is found anew, and not kept beside all of a kernel's work)
+    return tid;
   }
   // A lane's sequence of the 64 from `first` on.
-  __device__ inline Sequence read(uint32_t first) const {
-    const uint32_t seq = first + lane_id(), i = min(seq, a.nseq - 1);
+  __device__ static inline Sequence read(const ChunkAttention& a, const int32_t* __restrict__ cu_rows,
+                                         const int32_t* __restrict__ lens, uint32_t begin, uint32_t first) {
+    const uint32_t seq = first + thread() % kWave, i = min(seq, a.nseq - 1);
     Sequence s;
     s.cu0 = cu_rows[i];
     s.cu1 = cu_rows[i + 1];
@@ -112,6 +135,7 @@ struct Deal {
       if (pairs >= a.least_pairs && pairs <= a.most_pairs) {
         s.blocks.blocks = 1;   // (all rows of a refused sequence)
         if (s.ok) s.blocks = kv4_blocks(pairs, a.share, kPairs, s.len, a.window, a.grain);
+        s.blocks.first += begin;
       }
     }
     s.through = wave_through(a.layout.kv_heads * s.blocks.all());
@@ -121,68 +145,100 @@ struct Deal {
     return (uint32_t)__builtin_amdgcn_readlane((int)x, kWave - 1);
   }
 
-  __device__ inline Deal(const ChunkAttention& args, const int32_t* cu, const int32_t* l, uint32_t* fault)
-      : a(args), cu_rows(cu), lens(l) {
-    __shared__ Sequence s_sequences[kWave];
-    at_hand = s_sequences;
-    // neighbouring runs, which may share a kv head's columns, lie on one XCD
-    group = (blockIdx.x % 8) * (kKv4Groups / 8) + blockIdx.x / 8;
+  __device__ inline void start(const ChunkAttention& a, const int32_t* __restrict__ cu_rows,
+                               const int32_t* __restrict__ lens, uint32_t* __restrict__ fault) {
+    Run r;
+    r.begin = a.nseq > kWave ? kBegin * kTile >> a.grain : 0;
+    r.snap = max(kSnap * kTile >> a.grain, 1u);
+    r.even = 0;
     uint32_t total = 0;
     Sequence s;
     for (uint32_t first = 0; first < a.nseq; first += kWave) {
-      s = read(first);
+      s = read(a, cu_rows, lens, r.begin, first);
       total += last_lane(s.through);
       if (fault && blockIdx.x == 0 && !s.ok) *fault = 1u;
     }
-    if (a.nseq > kWave) s = read(0);
-    at_hand[lane_id()] = s;
-    per = max((total + kKv4Groups - 1) / kKv4Groups, a.least);
-    at = min(group * per, total);
-    end = min(at + per, total);
+    r.per = max((total + kKv4Groups - 1) / kKv4Groups, a.least);
+    if (a.nseq > kWave) {
+      s = read(a, cu_rows, lens, r.begin, 0);
+    } else {
+      const uint32_t widest = s.blocks.blocks ? s.blocks.of(s.blocks.blocks - 1) : 0;
+      for (uint32_t more = 0; more <= kDearer && !r.even; ++more) {
+        const uint32_t most = r.per + (more * kTile >> a.grain), parts = (widest + most - 1) / most;
+        const uint32_t to = wave_through(a.layout.kv_heads * s.blocks.blocks * parts);
+        if (last_lane(to) <= kKv4Groups) {
+          r.even = 1;
+          s.blocks.first = parts;
+          s.blocks.step = 0;
+          s.through = to;
+        }
+      }
+      if (r.even) {
+        r.per = r.snap = 1;
+      } else {
+        r.begin = kBegin * kTile >> a.grain;
+        s.blocks.first += r.begin;
+        s.through = wave_through(a.layout.kv_heads * s.blocks.all());
+        r.per = max((last_lane(s.through) + kKv4Groups - 1) / kKv4Groups, a.least);
+      }
+      total = last_lane(s.through);
+    }
+    sequences[thread() % kWave] = s;
+    r.at = min(group() * r.per, total);
+    r.end = min(r.at + r.per, total);
+    r.base = r.before = 0;
+    r.fresh = 1;
+    runs[scalar(thread() / kWave)] = r;
   }
   // The next piece of this workgroup's run; false at its end.
-  __device__ inline bool next(ChunkWork& w) {
-    if (at >= end) return false;
-    uint32_t through = at_hand[lane_id()].through;
-    while (at - before >= last_lane(through)) {
-      before += last_lane(through);
-      base += kWave;
+  __device__ inline bool next(const ChunkAttention& a, const int32_t* __restrict__ cu_rows,
+                              const int32_t* __restrict__ lens, ChunkWork& w) {
+    Run& run = runs[scalar(thread() / kWave)];
+    Run r = scalars(run);
+    for (;;) {
+    if (r.at >= r.end) return false;
+    uint32_t through = sequences[thread() % kWave].through;
+    while (r.at - r.before >= last_lane(through)) {
+      r.before += last_lane(through);
+      r.base += kWave;
       __syncthreads();
-      const Sequence s = read(base);
-      at_hand[lane_id()] = s;
+      const Sequence s = read(a, cu_rows, lens, r.begin, r.base);
+      sequences[thread() % kWave] = s;
       through = s.through;
     }
-    const uint32_t lane = (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(through > at - before));
-    const auto of = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
-    const Sequence& s = at_hand[lane];
-    const Kv4Blocks blocks = {of(s.blocks.blocks), of(s.blocks.first), of(s.blocks.step)};
-    const uint32_t of_head = blocks.all(), start = before + of(s.through) - a.layout.kv_heads * of_head;
-    w.seq = base + lane;
-    w.kv_head = of((at - start) / of_head);
-    const uint32_t head_at = start + w.kv_head * of_head, block = of(blocks.block_at(at - head_at));
+    const uint32_t lane = (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(through > r.at - r.before));
+    const Sequence& s = sequences[lane];
+    const Kv4Blocks blocks = {scalar(s.blocks.blocks), scalar(s.blocks.first), scalar(s.blocks.step)};
+    const uint32_t of_head = blocks.all(), start = r.before + scalar(s.through) - a.layout.kv_heads * of_head;
+    w.seq = r.base + lane;
+    w.kv_head = scalar((r.at - start) / of_head);
+    const uint32_t head_at = start + w.kv_head * of_head, block = scalar(blocks.block_at(r.at - head_at));
     const uint32_t block_at = head_at + blocks.before(block), width = blocks.of(block);
-    const uint32_t from = at - block_at, to = min(width, from + (end - at));
-    at += to - from;
-    w.cu0 = (int32_t)of((uint32_t)s.cu0);
-    w.cu1 = (int32_t)of((uint32_t)s.cu1);
-    w.refused = of(s.ok) == 0;
+    Kv4Cut cut;
+    const Kv4Dealt dealt = kv4_cut(r, block_at, width, cut);
+    if (dealt == kRunEnds) return false;
+    if (dealt == kBlockSkipped) continue;
+    run = r;
+    w.cu0 = (int32_t)scalar((uint32_t)s.cu0);
+    w.cu1 = (int32_t)scalar((uint32_t)s.cu1);
+    w.refused = scalar(s.ok) == 0;
     const int32_t rows = w.cu1 - w.cu0;
     const uint32_t pair0 = block * kPairs;
     w.count = (uint32_t)min((uint64_t)kPairs, (uint64_t)(uint32_t)rows * a.share - pair0);
-    w.row0 = of(divided(pair0, a.share, a.share_inverse));
+    w.row0 = scalar(divided(pair0, a.share, a.share_inverse));
     w.head0 = pair0 - w.row0 * a.share;
-    w.first_row = (int32_t)of((uint32_t)s.len) - rows + (int32_t)w.row0;
-    w.last_row = w.first_row + (int32_t)of(row_of(a, w, w.count - 1));
+    w.first_row = (int32_t)scalar((uint32_t)s.len) - rows + (int32_t)w.row0;
+    w.last_row = w.first_row + (int32_t)scalar(row_of(a, w, w.count - 1));
     w.low = kv4_first_column(w.first_row, a.window);
     w.high = w.last_row;
-    // the units are an estimate (rounded, of a window's widest block): what it leaves or lacks is the last part's
     const int32_t tile0 = w.low / kTile, tiles = w.high / kTile - tile0 + 1;
-    w.begin = tile0 + (int32_t)min(((uint64_t)from << a.grain) / kTile, (uint64_t)tiles);
-    w.end = tile0 + (to == width ? tiles : (int32_t)min(((uint64_t)to << a.grain) / kTile, (uint64_t)tiles));
-    w.first_group = of(block_at / per);
-    w.parts = of((block_at + width - 1) / per) - w.first_group + 1;
-    w.part = group - w.first_group;
+    w.begin = tile0 + (int32_t)scalar(kv4_tile(r, cut.from, width, tiles, a.grain, kTile));
+    w.end = tile0 + (int32_t)scalar(kv4_tile(r, cut.to, width, tiles, a.grain, kTile));
+    w.parts = scalar(cut.parts);
+    w.first_group = scalar(cut.first);
+    w.part = group() - w.first_group;
     return true;
+    }
   }
 };
 
@@ -190,7 +246,7 @@ template <typename XT, int D, int NG>
 __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
     const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table,
     const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens, XT* __restrict__ out,
-    uint32_t* __restrict__ fault, ChunkAttention a) {
+    uint32_t* __restrict__ fault, ChunkAttention given) {
   using C = Chunk<XT, D>;
   constexpr bool kF32 = C::kF32;
   constexpr int kThreads = C::kThreads, kPairs = C::kPairs, kColumns = C::kColumns, kBlocks = C::kBlocks;
@@ -200,16 +256,23 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
   __shared__ uint32_t s_unsound[2][kColumns];         // groups of a column's values that are no numbers (edge tiles)
   __shared__ uint32_t s_any[2];
 
-  Deal<kPairs, kColumns> deal(a, cu_rows, lens, fault);
+  // the call's numbers and the piece's wait in LDS while its tiles have the registers
+  __shared__ ChunkAttention s_numbers;
+  __shared__ ChunkWork s_work;
+  __shared__ Deal<kThreads / kWave, kPairs, kColumns> deal;
+  if (threadIdx.x == 0) s_numbers = given;
+  deal.start(given, cu_rows, lens, fault);
+  __syncthreads();
+  for (;;) {
+  const ChunkAttention a = scalars(s_numbers);
   ChunkWork w;
-  while (deal.next(w)) {
+  if (!deal.next(a, cu_rows, lens, w)) break;
+  s_work = w;   // (every wave writes the same words)
   if (w.refused) {
     refuse<XT, D, kThreads>(a, w.kv_head, w.cu0, w.cu1, out);
     continue;
   }
-  uint32_t tid = threadIdx.x;
-  asm volatile("" : "+v"(tid));   // (what hangs on it alone is found for each piece, and not kept beside all of them)
-  const uint32_t lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const uint32_t tid = deal.thread(), lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int32_t low = w.low, high = w.high;
 
   // ---- this wave's rows: lane (m = lane % 32, half)
@@ -538,6 +601,7 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
       }
     }
     if (s_any[buffer]) {
+#pragma unroll 1
       for (int i = 0; i < kColumns; ++i) {
         const uint32_t groups = s_unsound[buffer][i];
         const int32_t column = column0 + i;
@@ -581,25 +645,27 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
 
   // ---- parts: as the lanes hold them, (max, sum) of every lane behind the sums; whoever arrives last joins them in
   // order in the same lanes
+  const ChunkAttention numbers = scalars(s_numbers);
+  const ChunkWork piece = scalars(s_work);
   bool mine_to_write = true;
-  if (w.parts > 1) {
+  if (piece.parts > 1) {
     constexpr uint32_t kState = kOuts * 16 * kThreads;          // floats before the states
     constexpr size_t kPart = kState + 2 * kThreads;
-    float* const mine = a.partials + part_slot(w, w.part) * kPart + 2 * tid;
+    float* const mine = given.partials + part_slot(piece, piece.part) * kPart + 2 * tid;
 #pragma unroll
     for (int o = 0; o < kOuts; ++o)
 #pragma unroll
       for (int r = 0; r < 16; r += 2)
         publish2(mine + (o * 16 + r) * kThreads, float2_t{acc[o][r], acc[o][r + 1]});
     publish2(mine + kState, float2_t{top, sum});
-    mine_to_write = arrived_last(a.tickets + (size_t)w.first_group * kTicketStride, w.parts);
+    mine_to_write = arrived_last(given.tickets + (size_t)piece.first_group * kTicketStride, piece.parts);
     if (mine_to_write) {
     top = -INFINITY;
     sum = 0.f;
 #pragma unroll
     for (int o = 0; o < kOuts; ++o) acc[o] = float16_t{};
-    for (uint32_t p = 0; p < w.parts; ++p) {
-      const float* from_part = a.partials + part_slot(w, p) * kPart + 2 * tid;
+    for (uint32_t p = 0; p < piece.parts; ++p) {
+      const float* from_part = given.partials + part_slot(piece, p) * kPart + 2 * tid;
       const float2_t state = observe2(from_part + kState);
       float2_t x[kOuts * 8];
 #pragma unroll
@@ -616,8 +682,8 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
     }
   }
   // ---- out: lane (m, half) has elements 32 o + 8 (r / 4) + 4 half + r % 4 of its pair
-  if (live && mine_to_write) {
-    XT* to = out + row_at(a, w, pair, D) + 4 * half;
+  if (pair < piece.count && mine_to_write) {
+    XT* to = out + row_at(numbers, piece, pair, D) + 4 * half;
     const float inverse = 1.0f / sum;
 #pragma unroll
     for (int o = 0; o < kOuts; ++o)
@@ -677,7 +743,7 @@ int32_t launch_kv4_chunk(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& 
   const uint64_t rows = kv4_rows(a.limits.max_query, a.limits.total_rows);
   const uint64_t blocks = (uint64_t)a.nseq * a.layout.kv_heads * ((rows * a.share + pairs - 1) / pairs);
   c.grain = a.limits.max_columns <= tile ? 31 - __builtin_clz(tile) : 2;
-  while (blocks * ((((uint64_t)a.limits.max_columns + pairs) >> c.grain) + 1) >= 1ull << 31) ++c.grain;
+  while (blocks * (((a.limits.max_columns + (uint64_t)pairs + kBegin * tile) >> c.grain) + 2) >= 1ull << 31) ++c.grain;
   // a run has two tiles at least: joining two parts costs more
   c.least = 2 * tile >> c.grain ? 2 * tile >> c.grain : 1;
   if (io_dtype == KRM_F32) launch_depth<float>(ctx, c, b);

@@ -13,6 +13,7 @@
 // value codes is four rows (the contracted index) of eight output elements.
 #pragma once
 
+#include <cmath>
 #include <cstddef>
 #include <cstdint>
 #include <cstdio>
@@ -111,6 +112,52 @@ KRM_HD inline Kv4Blocks kv4_blocks(uint64_t pairs, uint32_t share, uint32_t bloc
     }
   }
   return b;
+}
+// A workgroup's run of the row of work: units [at, end), of `per` units in all runs but the last.
+struct Kv4Run {
+  uint32_t per, at, end;
+  uint32_t begin, snap;   // units that beginning a block counts as; distance at which a run's end moves to a block's
+  uint32_t even;          // units are equal parts of blocks
+  uint32_t fresh;         // the run has had no piece yet
+};
+// Its piece of the block that unit `at` is in, which has `width` units from `block_at` on.
+struct Kv4Cut {
+  uint32_t from, to;      // of the block's units
+  uint32_t parts, first;  // pieces that the block is in, each in a run of its own; the first one's run
+};
+enum Kv4Dealt { kRunEnds, kBlockSkipped, kPieceDealt };
+KRM_HD inline Kv4Dealt kv4_cut(Kv4Run& r, uint32_t block_at, uint32_t width, Kv4Cut& c) {
+  const bool uncut = width < 2 * r.snap;
+  const uint32_t near = uncut ? (width + 1) / 2 : r.snap, behind = block_at + width;
+  c.from = r.at - block_at;
+  c.to = width;
+  if (r.fresh) {
+    r.fresh = 0;
+    if (c.from < near) {
+      c.from = 0;
+    } else if (uncut || width - c.from < r.snap) {
+      r.at = behind;
+      return r.at < r.end ? kBlockSkipped : kRunEnds;
+    }
+  }
+  if (r.end < behind) {
+    if (r.end - block_at < near) return kRunEnds;
+    if (!uncut && behind - r.end >= r.snap) c.to = r.end - block_at;
+  }
+  r.at = block_at + c.to;
+  const uint32_t first_cut = (block_at + r.snap + r.per - 1) / r.per, last_cut = (behind - r.snap) / r.per;
+  c.parts = uncut || last_cut < first_cut ? 1 : last_cut - first_cut + 2;
+  c.first = first_cut - 1;
+  return kPieceDealt;
+}
+// The tile, of a block's `tiles`, at which its unit `unit` begins.  (Units are an estimate, rounded, of a window's widest
+// block: what it leaves or lacks is the last part's.)
+KRM_HD inline uint32_t kv4_tile(const Kv4Run& r, uint32_t unit, uint32_t width, uint32_t tiles, uint32_t grain,
+                                uint32_t tile) {
+  if (r.even) return tiles / width * unit + tiles % width * unit / width;
+  if (unit == width) return tiles;
+  const uint64_t at = ((uint64_t)(unit < r.begin ? 0 : unit - r.begin) << grain) / tile;
+  return at < tiles ? (uint32_t)at : tiles;
 }
 // First column that a row at `position` sees.
 KRM_HD inline int32_t kv4_first_column(int32_t position, uint32_t window) {

@@ -283,6 +283,51 @@ def test_many_rows_of_many_heads(gpu_ctx, io, depth, group, page):
 
 
 @pytest.mark.parametrize("io", [np.float16, np.float32])
+@pytest.mark.parametrize("depth,group", [(64, 32), (128, 128), (256, 64)])
+def test_many_sequences_of_many_rows(gpu_ctx, io, depth, group):
+    """More sequences than a wave reads at a time, chunks and single rows in one step, and one long sequence among them."""
+    rng = np.random.default_rng(depth)
+    rows = [(40, 1, 0, 17, 9)[i % 5] for i in range(133)]
+    lens = [r + int(rng.integers(0, 90)) if r else 0 for r in rows]
+    lens[130] = 1500
+    step = ref.Step.make(ref.Layout(2, depth, group, 32), rows, lens, rng)
+    check(gpu_ctx, step, 8, io, rng)
+    check(gpu_ctx, step, 8, io, rng, window=33)
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+@pytest.mark.parametrize("depth,rows,lens", [(64, (512,), (512,)), (128, (700, 260), (700, 5000)),
+                                             (256, (300, 300), (300, 1200))])
+def test_whole_prompts(gpu_ctx, io, depth, rows, lens):
+    """Rows that see nothing but each other: blocks of rows with few columns beside ones with all of them."""
+    rng = np.random.default_rng(depth)
+    step = ref.Step.make(ref.Layout(4, depth, 64, 64), rows, lens, rng)
+    check(gpu_ctx, step, 16, io, rng)
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+def test_all_rows_of_a_refused_chunk_are_nan(gpu_ctx, io):
+    rng = np.random.default_rng(3)
+    rows, lens = (70, 90, 1, 64), (70, 300, 40, 500)
+    step = ref.Step.make(ref.Layout(8, 64, 32, 16), rows, lens, rng)
+    raw = step.random_cache(rng)
+    q = rng.normal(size=(step.total, 32, 64))
+    a = Attention(gpu_ctx, step, raw, q, io)
+    want, reach, top = step.attention(raw, a.q, a.half_scale, 0)
+    most, _ = tolerance(io, reach, top, 500)
+    refused = np.zeros(step.total, bool)
+    refused[70:160] = True
+    for change, lengths in ((dict(), (70, 89, 40, 500)), (dict(max_query=70), lens)):
+        a.buf["lens"].upload(np.int32(lengths))
+        a.fault.zero()
+        a.run(**change)
+        got = a.result().astype(np.float64)
+        assert a.faulted() == 1 and np.all(np.isnan(got[refused]))
+        assert np.abs(got[~refused] - want[~refused]).max() <= most
+    a.free()
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
 def test_limits_larger_than_the_step_needs(gpu_ctx, io):
     """What a recorded call is made with: more rows and columns than the sequences have yet."""
     rng = np.random.default_rng(6)

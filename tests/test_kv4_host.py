@@ -32,6 +32,47 @@ extern "C" int32_t first_column(int32_t position, uint32_t window) { return kv4_
 extern "C" int shape(const uint32_t* w, char* why) {
   return kv4_shape_ok({w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], w[9]}, why, 128);
 }
+extern "C" void blocks(uint64_t pairs, uint32_t share, uint32_t of, int32_t len, uint32_t window, uint32_t grain,
+                       uint32_t* out) {
+  const Kv4Blocks b = kv4_blocks(pairs, share, of, len, window, grain);
+  out[0] = b.blocks; out[1] = b.first; out[2] = b.step;
+}
+extern "C" int64_t lost_block(uint32_t blocks, uint32_t first, uint32_t step) {   // the first unit found in a wrong one
+  const Kv4Blocks b{blocks, first, step};
+  for (uint32_t i = 0; i < blocks; ++i) {
+    const uint32_t at = b.before(i), last = at + b.of(i) - 1;
+    if (b.block_at(at) != i) return at;
+    if (b.block_at(last) != i || b.block_at(at + b.of(i) / 2) != i) return last;
+  }
+  return b.before(blocks) == b.all() ? -1 : -2;
+}
+// The pieces of all runs, one after the other: run, block, from, to, parts, first run.
+extern "C" int deal(const uint32_t* width, int blocks, uint32_t runs, uint32_t least, uint32_t begin, uint32_t snap,
+                    uint32_t* out) {
+  uint32_t total = 0, n = 0;
+  for (int i = 0; i < blocks; ++i) total += width[i];
+  uint32_t per = (total + runs - 1) / runs;
+  if (per < least) per = least;
+  for (uint32_t g = 0; g < runs; ++g) {
+    Kv4Run r{per, g * per < total ? g * per : total, 0, begin, snap, 0, 1};
+    r.end = r.at + per < total ? r.at + per : total;
+    while (r.at < r.end) {
+      uint32_t at = 0, i = 0;
+      while (at + width[i] <= r.at) at += width[i++];
+      Kv4Cut c;
+      const Kv4Dealt dealt = kv4_cut(r, at, width[i], c);
+      if (dealt == kRunEnds) break;
+      if (dealt == kBlockSkipped) continue;
+      const uint32_t piece[6] = {g, i, c.from, c.to, c.parts, c.first};
+      for (uint32_t x : piece) out[n++] = x;
+    }
+  }
+  return (int)n / 6;
+}
+extern "C" uint32_t tile(uint32_t begin, uint32_t even, uint32_t unit, uint32_t width, uint32_t tiles, uint32_t grain,
+                         uint32_t of) {
+  return kv4_tile({1, 0, 0, begin, 1, even, 0}, unit, width, tiles, grain, of);
+}
 extern "C" int turn(uint32_t depth, uint32_t rotary, int32_t layout, uint32_t rows, uint32_t width, char* why) {
   return kv4_turn_ok(depth, rotary, layout, rows, width, why, 128);
 }
@@ -133,6 +174,84 @@ def test_a_sequence_ends_where_its_table_does(plan):
     assert plan.sequence(0, 1, 640, limits(10), C.byref(got)) == 1
     assert plan.sequence(0, 1, 641, limits(10), C.byref(got)) == 0
     assert plan.sequence(0, 1, 2**31 - 1, limits(2**31 - 1), C.byref(got)) == 1   # the product passes 32 bits
+
+
+@pytest.mark.parametrize("runs,least,begin,snap", [(256, 1, 0, 1), (256, 32, 32, 48), (8, 32, 32, 48), (5, 3, 2, 3),
+                                                   (256, 1, 1, 1), (7, 1, 0, 4)])
+@pytest.mark.parametrize("seed", range(12))
+def test_runs_of_work_cover_every_block_once(plan, runs, least, begin, snap, seed):
+    """Pieces join up to whole blocks, each cut block's in neighbouring runs, one a run; a run begins a cut block with its
+    last piece and goes on with one in its first, so that two places a run hold all parts."""
+    rng = np.random.default_rng(seed)
+    most = (3, 40, 900, 5000)[seed % 4]
+    width = (rng.integers(1, most + 1, size=rng.integers(1, 400)) + begin).astype(np.uint32)
+    if seed % 3 == 0:
+        width[rng.integers(len(width))] = 100000
+    out = np.zeros((runs + len(width) + 8, 6), np.uint32)
+    n = plan.deal(width.ctypes.data_as(C.c_void_p), len(width), runs, least, begin, snap,
+                  out.ctypes.data_as(C.c_void_p))
+    pieces, places = [tuple(map(int, p)) for p in out[:n]], set()
+    for block, w in enumerate(width):
+        mine = [p for p in pieces if p[1] == block]
+        assert mine[0][2] == 0 and mine[-1][3] == w and all(a[3] == b[2] for a, b in zip(mine, mine[1:]))
+        assert all(p[2] < p[3] and p[4] == len(mine) for p in mine)
+        if len(mine) > 1:
+            assert [p[0] for p in mine] == list(range(mine[0][5], mine[0][5] + len(mine)))
+            assert all(p[5] == mine[0][5] and min(p[3] - p[2], w - p[3] or w) >= min(snap, w) // 2 for p in mine)
+            for i, p in enumerate(mine):
+                place = 2 * p[0] + (i == 0)
+                assert place not in places
+                places.add(place)
+                of_run = [x for x in pieces if x[0] == p[0]]
+                assert of_run[-1 if i == 0 else 0] == p
+    # no run has more than its share and what the two ends move
+    per = max(-(-int(width.sum()) // runs), least)
+    for g in range(runs):
+        assert sum(p[3] - p[2] for p in pieces if p[0] == g) <= per + 2 * snap
+
+
+@pytest.mark.parametrize("blocks,first,step", [(1, 7, 0), (1, 1, 5), (300, 5, 0), (4000, 1, 1), (64, 16, 8),
+                                               (20000, 3, 10), (2**15, 1, 3), (46000, 1, 2), (1500, 1400000, 3),
+                                               (2, 2**30 - 5, 1)])
+def test_every_unit_is_found_in_its_block(plan, blocks, first, step):
+    assert blocks * first + step * blocks * (blocks - 1) // 2 < 2**31
+    plan.lost_block.restype = C.c_int64
+    assert plan.lost_block(blocks, first, step) == -1
+
+
+@pytest.mark.parametrize("pairs,share,of,length,window,grain", [
+    (1, 1, 256, 1, 0, 2), (2048, 4, 256, 1024, 0, 2), (4096, 8, 128, 9000, 0, 2), (700, 7, 256, 150, 0, 2),
+    (1040, 4, 256, 700, 100, 2), (4096, 8, 256, 512, 5000, 2), (2**20, 64, 256, 2**20, 0, 4), (640, 1, 128, 640, 1, 2)])
+def test_blocks_count_the_columns_that_their_rows_see(plan, pairs, share, of, length, window, grain):
+    out = (C.c_uint32 * 3)()
+    plan.blocks(C.c_uint64(pairs), share, of, length, window, grain, out)
+    blocks, first, step = out
+    assert blocks == -(-pairs // of)
+    rows = pairs // share
+    for b in range(blocks):
+        last = min((b + 1) * of, pairs) - 1
+        seen = length - rows + last // share + 1
+        if window:
+            seen = min(seen, window + last // share - b * of // share)
+        units = first + b * step
+        # at least one; rounding loses less than a unit and a row a block; a window's blocks are all taken for the widest
+        assert units >= 1 and units <= ((length + of) >> grain) + 1
+        if not window:
+            assert (seen - (b + 1) * (1 + (1 << grain))) >> grain <= units <= ((seen + of) >> grain) + 1
+        else:
+            assert units * 2**grain >= min(seen, window)
+
+
+def test_tiles_of_the_parts_of_a_block(plan):
+    for tiles in (1, 2, 7, 64, 10**6):
+        for parts in (1, 2, 3, 8, 256):   # equal parts
+            at = [plan.tile(0, 1, u, parts, tiles, 2, 64) for u in range(parts + 1)]
+            assert at[0] == 0 and at[-1] == tiles and all(0 <= b - a <= -(-tiles // parts) + 1 for a, b in zip(at, at[1:]))
+    for begin in (0, 32):   # units of four columns, 16 a tile, behind what beginning counts as
+        width = 16 * 10 + begin + 3
+        at = [plan.tile(begin, 0, u, width, 11, 2, 64) for u in range(width + 1)]
+        assert at[0] == 0 and at[-1] == 11 and at == sorted(at) and at[begin + 16] == 1 and at[begin + 159] == 9
+    assert plan.tile(0, 0, 2**31 - 2, 2**31 - 1, 2**25, 2, 64) == 2**25
 
 
 def test_first_column_of_a_window(plan):
