@@ -617,12 +617,17 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
 
 // How the columns of a launch of kv4_decode_kernel are dealt.
 struct DecodePlan {
-  uint32_t row_tiles = 0, units = 0, max_splits = 0, partial_rows = 0, least = 0;
+  uint32_t waves = 0, row_tiles = 0, units = 0, max_splits = 0, partial_rows = 0, least = 0;
   float share_of_work = 0;
   size_t bytes = 0;
 };
-// Eight waves (two a SIMD) while their registers allow it: half as many parts to join as with four, twice a CU.
-constexpr int waves_of(int depth) { return depth == 256 ? 4 : 8; }
+// Waves of a workgroup.  With eight a CU has one workgroup, two waves a SIMD, and as few parts to join as can be.  With four
+// it has two or three, and one's first loads and last sums run beside another's tiles, which pays where many sequences'
+// pieces are unequal or more than the CUs (us, eight / four, 8 kv heads x 4, D 128, fp16: 16 sequences of 128 to 4096
+// columns 28 / 24, 32 of them 41 / 37, 128 of 300 28 / 23, 128 of 2000 90 / 76; but 16 of 4000 28 / 31, 131000 columns 40 /
+// 54), or where all pieces together are few (one sequence of 700 or 4096 columns 11.7 / 10.8, 12.2 / 11.1).
+constexpr uint32_t kFewWaves = 4, kManyWaves = 8;
+constexpr uint32_t kManyUnits = 96, kManyGroups = kKv4Groups * 3 / 2;
 constexpr uint32_t kMostGroups = 2048;   // in a grid, those without a split among them
 constexpr uint32_t kMostSplits = 64;
 static_assert(kMostGroups <= kTicketSlots, "a counter a unit");
@@ -632,13 +637,17 @@ DecodePlan plan_decode(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs) 
   p.row_tiles = (uint32_t)row_tiles;
   p.partial_rows = pairs < kRows ? (uint32_t)pairs : kRows;
   p.units = (uint32_t)(units < 0xffffffffu ? units : 0xffffffffu);
-  p.least = 2 * waves_of(s.depth);   // two a wave: joining two parts costs about as much as a tile more
-  const uint64_t tiles = ((uint64_t)max_columns + kTile - 1) / kTile + 1, most = (tiles + p.least - 1) / p.least;
+  const uint64_t tiles = ((uint64_t)max_columns + kTile - 1) / kTile + 1;
+  const bool many = s.depth < 256 && (uint64_t)s.nseq * s.kv_heads >= kManyUnits;
+  const bool small = tiles > 2 * kManyWaves + 1 && units * tiles <= 2 * kManyWaves * kKv4Groups;
+  p.waves = s.depth == 256 || many || small ? kFewWaves : kManyWaves;
+  p.least = 2 * (many ? kManyWaves : p.waves);   // two a wave: joining two parts costs about as much as a tile more
+  const uint64_t most = (tiles + p.least - 1) / p.least;
   uint64_t splits = units ? kMostGroups / units : 1;
   splits = splits > kMostSplits ? kMostSplits : splits;
   splits = splits > most ? most : splits;
   p.max_splits = splits < 1 ? 1 : (uint32_t)splits;   // (with more units than kMostGroups, and so than counters: one)
-  p.share_of_work = (float)s.kv_heads * (float)row_tiles / kKv4Groups;
+  p.share_of_work = (float)s.kv_heads * (float)row_tiles / (many ? kManyGroups : kKv4Groups);
   p.bytes = splits > 1 ? (size_t)units * splits * p.partial_rows * (s.depth + 2) * sizeof(float) : 0;
   return p;
 }
@@ -748,26 +757,33 @@ int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_t
   a.least = plan.decode.least;
   a.share_of_work = plan.decode.share_of_work;
   const dim3 grid(plan.decode.units, a.max_splits);
-  const int waves = waves_of(depth);
+  const uint32_t waves = plan.decode.waves;
   const size_t joined = (size_t)waves * a.partial_rows * (depth + 4) * sizeof(float);
-#define KRM_ATTENTION(XT, D, NG)                                                                                 \
-  const size_t ring = (size_t)waves * kStages * Stage<D, NG>::kBytes, lds = ring > joined ? ring : joined;       \
-  kv4_decode_kernel<XT, D, NG, waves_of(D)><<<grid, dim3(waves * kWave), lds, ctx->stream>>>(                                       \
-      ptr<const XT>(q), ptr<const uint8_t>(cache), ptr<const int32_t>(page_table_i32),                            \
+#define KRM_ATTENTION(XT, D, NG, WAVES)                                                                    \
+  const size_t ring = (size_t)WAVES * kStages * Stage<D, NG>::kBytes, lds = ring > joined ? ring : joined; \
+  kv4_decode_kernel<XT, D, NG, WAVES><<<grid, dim3(WAVES * kWave), lds, ctx->stream>>>(                    \
+      ptr<const XT>(q), ptr<const uint8_t>(cache), ptr<const int32_t>(page_table_i32),                     \
       ptr<const int32_t>(cu_rows_i32), ptr<const int32_t>(lens_i32), ptr<XT>(out), ptr<uint32_t>(fault_u32), a)
-#define KRM_ATTENTION_D(XT)                                                              \
-  switch (depth * 16 + depth / group) {                                                  \
-    case 64 * 16 + 1: { KRM_ATTENTION(XT, 64, 1); break; }                                  \
-    case 64 * 16 + 2: { KRM_ATTENTION(XT, 64, 2); break; }                                  \
-    case 128 * 16 + 1: { KRM_ATTENTION(XT, 128, 1); break; }                                \
-    case 128 * 16 + 2: { KRM_ATTENTION(XT, 128, 2); break; }                                \
-    case 128 * 16 + 4: { KRM_ATTENTION(XT, 128, 4); break; }                                \
-    case 256 * 16 + 2: { KRM_ATTENTION(XT, 256, 2); break; }                                \
-    case 256 * 16 + 4: { KRM_ATTENTION(XT, 256, 4); break; }                                \
-    default: { KRM_ATTENTION(XT, 256, 8); }                                          \
+#define KRM_ATTENTION_W(XT, D, NG)                                           \
+  {                                                                          \
+    if (waves == kManyWaves) { KRM_ATTENTION(XT, D, NG, kManyWaves); }       \
+    else { KRM_ATTENTION(XT, D, NG, kFewWaves); }                            \
+    break;                                                                   \
+  }
+#define KRM_ATTENTION_D(XT)                                  \
+  switch (depth * 16 + depth / group) {                      \
+    case 64 * 16 + 1: KRM_ATTENTION_W(XT, 64, 1)             \
+    case 64 * 16 + 2: KRM_ATTENTION_W(XT, 64, 2)             \
+    case 128 * 16 + 1: KRM_ATTENTION_W(XT, 128, 1)           \
+    case 128 * 16 + 2: KRM_ATTENTION_W(XT, 128, 2)           \
+    case 128 * 16 + 4: KRM_ATTENTION_W(XT, 128, 4)           \
+    case 256 * 16 + 2: { KRM_ATTENTION(XT, 256, 2, kFewWaves); break; } \
+    case 256 * 16 + 4: { KRM_ATTENTION(XT, 256, 4, kFewWaves); break; } \
+    default: { KRM_ATTENTION(XT, 256, 8, kFewWaves); }       \
   }
   if (io_dtype == KRM_F32) { KRM_ATTENTION_D(float) } else { KRM_ATTENTION_D(__half) }
 #undef KRM_ATTENTION_D
+#undef KRM_ATTENTION_W
 #undef KRM_ATTENTION
   return launched(ctx, "kv4_decode_kernel");
 }
