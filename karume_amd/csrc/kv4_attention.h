@@ -35,16 +35,12 @@ namespace {
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
 
-constexpr int kJoin = 32;           // parts whose sums are asked for together
+constexpr int kJoin = 16;           // parts whose sums are asked for together
 
-// Device-scope store / load of one float: written through to (read from) memory that every XCD sees.
-__device__ inline void publish(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ inline float observe(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
+// Device-scope load / store of two floats: read from (written through to) memory that every XCD sees.
 __device__ inline float2_t observe2(const float* p) {
   return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
-
 __device__ inline void publish2(float* p, float2_t v) {
   __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }

@@ -122,6 +122,12 @@ __device__ inline bool find_work(const DecodeAttention& a, DecodeWork& w, uint32
   return true;
 }
 
+__device__ inline void store4(float* to, float4_t x) { *reinterpret_cast<float4_t*>(to) = x; }
+__device__ inline void store4(__half* to, float4_t x) {
+  const half2_t a = {(_Float16)x[0], (_Float16)x[1]}, b = {(_Float16)x[2], (_Float16)x[3]};
+  *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+}
+
 // A workgroup's part of its rows is published; the workgroup that arrives last joins the parts in order, whichever it
 // is.  `s_part`: nsplit * count * 2 floats of LDS that nobody needs any more.
 template <typename XT, int D, int kThreads>
@@ -130,36 +136,37 @@ __device__ inline void join_parts(const DecodeAttention& a, const DecodeWork& w,
   const size_t part_size = (size_t)a.partial_rows * (D + 2);
   const float* const parts = a.partials + (size_t)w.unit * a.max_splits * part_size;
   if (!arrived_last(a.tickets + (size_t)w.unit * kTicketStride, nsplit)) return;
-  for (uint32_t i = tid; i < nsplit * count; i += kThreads) {   // [row][nsplit] (max, sum)
-    const float* state = parts + (i / count) * part_size + a.partial_rows * D + 2 * (i % count);
-    float* to = s_part + ((i % count) * nsplit + i / count) * 2;
-    to[0] = observe(state);
-    to[1] = observe(state + 1);
-  }
+  for (uint32_t i = tid; i < nsplit * count; i += kThreads)   // [row][nsplit] (max, sum)
+    *reinterpret_cast<float2_t*>(s_part + ((i % count) * nsplit + i / count) * 2) =
+        observe2(parts + (i / count) * part_size + a.partial_rows * D + 2 * (i % count));
   __syncthreads();
-  for (uint32_t e = 2 * tid; e < count * D; e += 2 * kThreads) {
+  for (uint32_t e = 4 * tid; e < count * D; e += 4 * kThreads) {
     const float* states = s_part + (e / D) * nsplit * 2;
     float most = -INFINITY, weight = 0.f;
-    float2_t total = {0.f, 0.f};
+    float4_t total = {};
     for (uint32_t p = 0; p < nsplit; ++p) most = fmaxf(most, states[2 * p]);
     const float ref = most == -INFINITY ? 0.f : most;
     for (uint32_t p0 = 0; p0 < nsplit; p0 += kJoin) {
-      float2_t o[kJoin];
+      float2_t o[kJoin][2] = {};
 #pragma unroll
-      for (int i = 0; i < kJoin; ++i) o[i] = observe2(parts + min(p0 + i, nsplit - 1) * part_size + e);
+      for (int i = 0; i < kJoin; ++i) {
+        if (p0 + i < nsplit) {
+          const float* from = parts + (p0 + i) * part_size + e;
+          o[i][0] = observe2(from);
+          o[i][1] = observe2(from + 2);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < kJoin; ++i) {
         if (p0 + i < nsplit) {
           const float k = __builtin_amdgcn_exp2f(states[2 * (p0 + i)] - ref);
-          total[0] = fmaf(k, o[i][0], total[0]);
-          total[1] = fmaf(k, o[i][1], total[1]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) total[j] = fmaf(k, o[i][j / 2][j % 2], total[j]);
           weight = fmaf(k, states[2 * (p0 + i) + 1], weight);
         }
       }
     }
-    XT* to = out + row_at(a, w, e / D, D) + e % D;
-    to[0] = from_f32<XT>(total[0] / weight);
-    to[1] = from_f32<XT>(total[1] / weight);
+    store4(out + row_at(a, w, e / D, D) + e % D, total / weight);
   }
 }
 
@@ -589,27 +596,28 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
   const size_t part_size = (size_t)a.partial_rows * (D + 2);
   float* const parts = a.partials + (size_t)w.unit * a.max_splits * part_size;
   float* const part = parts + w.split * part_size;
-  for (uint32_t e = tid; e < count * D; e += kThreads) {
+  for (uint32_t e = 4 * tid; e < count * D; e += 4 * kThreads) {
     const uint32_t row = e / D, d = e % D;
     float most = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_max[w][row]);
     const float ref = most == -INFINITY ? 0.f : most;
-    float total = 0.f, weight = 0.f;
+    float4_t total = {};
+    float weight = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const float k = __builtin_amdgcn_exp2f(s_max[w][row] - ref);
-      total = fmaf(k, s_acc[(w * a.partial_rows + row) * kStride + d], total);
+      const float4_t x = *reinterpret_cast<const float4_t*>(s_acc + (w * a.partial_rows + row) * kStride + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total[i] = fmaf(k, x[i], total[i]);
       weight = fmaf(k, s_sum[w][row], weight);
     }
     if (w.nsplit == 1) {
-      out[row_at(a, w, row, D) + d] = from_f32<XT>(total / weight);
+      store4(out + row_at(a, w, row, D) + d, total / weight);
     } else {
-      publish(part + e, total);
-      if (d == 0) {
-        publish(part + a.partial_rows * D + 2 * row, most);
-        publish(part + a.partial_rows * D + 2 * row + 1, weight);
-      }
+      publish2(part + e, float2_t{total[0], total[1]});
+      publish2(part + e + 2, float2_t{total[2], total[3]});
+      if (d == 0) publish2(part + a.partial_rows * D + 2 * row, float2_t{most, weight});
     }
   }
   if (w.nsplit > 1) join_parts<XT, D, kThreads>(a, w, out, s_acc);
