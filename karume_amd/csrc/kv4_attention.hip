@@ -128,42 +128,41 @@ __device__ inline void store4(__half* to, float4_t x) {
   *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
 }
 
-// A workgroup's part of its rows is published; the workgroup that arrives last joins the parts in order, whichever it
-// is.  `s_part`: nsplit * count * 2 floats of LDS that nobody needs any more.
+// A workgroup's part of its rows is published; the workgroup that arrives last joins the parts in order, whichever it is.
 template <typename XT, int D, int kThreads>
-__device__ inline void join_parts(const DecodeAttention& a, const DecodeWork& w, XT* __restrict__ out, float* s_part) {
+__device__ inline void join_parts(const DecodeAttention& a, const DecodeWork& w, XT* __restrict__ out) {
   const uint32_t tid = threadIdx.x, nsplit = w.nsplit, count = w.count;
   const size_t part_size = (size_t)a.partial_rows * (D + 2);
   const float* const parts = a.partials + (size_t)w.unit * a.max_splits * part_size;
   if (!arrived_last(a.tickets + (size_t)w.unit * kTicketStride, nsplit)) return;
-  for (uint32_t i = tid; i < nsplit * count; i += kThreads)   // [row][nsplit] (max, sum)
-    *reinterpret_cast<float2_t*>(s_part + ((i % count) * nsplit + i / count) * 2) =
-        observe2(parts + (i / count) * part_size + a.partial_rows * D + 2 * (i % count));
-  __syncthreads();
   for (uint32_t e = 4 * tid; e < count * D; e += 4 * kThreads) {
-    const float* states = s_part + (e / D) * nsplit * 2;
-    float most = -INFINITY, weight = 0.f;
+    float top = -INFINITY, weight = 0.f;
     float4_t total = {};
-    for (uint32_t p = 0; p < nsplit; ++p) most = fmaxf(most, states[2 * p]);
-    const float ref = most == -INFINITY ? 0.f : most;
     for (uint32_t p0 = 0; p0 < nsplit; p0 += kJoin) {
-      float2_t o[kJoin][2] = {};
+      float2_t o[kJoin][2] = {}, state[kJoin];
 #pragma unroll
       for (int i = 0; i < kJoin; ++i) {
+        state[i] = {-INFINITY, 0.f};
         if (p0 + i < nsplit) {
-          const float* from = parts + (p0 + i) * part_size + e;
-          o[i][0] = observe2(from);
-          o[i][1] = observe2(from + 2);
+          const float* from = parts + (p0 + i) * part_size;
+          state[i] = observe2(from + a.partial_rows * D + 2 * (e / D));
+          o[i][0] = observe2(from + e);
+          o[i][1] = observe2(from + e + 2);
         }
       }
+      float now = top;
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i) now = fmaxf(now, state[i][0]);
+      const float ref = now == -INFINITY ? 0.f : now, keep = __builtin_amdgcn_exp2f(top - ref);
+      top = now;
+      weight *= keep;
+      total *= keep;
 #pragma unroll
       for (int i = 0; i < kJoin; ++i) {
-        if (p0 + i < nsplit) {
-          const float k = __builtin_amdgcn_exp2f(states[2 * (p0 + i)] - ref);
+        const float k = __builtin_amdgcn_exp2f(state[i][0] - ref);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) total[j] = fmaf(k, o[i][j / 2][j % 2], total[j]);
-          weight = fmaf(k, states[2 * (p0 + i) + 1], weight);
-        }
+        for (int j = 0; j < 4; ++j) total[j] = fmaf(k, o[i][j / 2][j % 2], total[j]);
+        weight = fmaf(k, state[i][1], weight);
       }
     }
     store4(out + row_at(a, w, e / D, D) + e % D, total / weight);
@@ -620,7 +619,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
       if (d == 0) publish2(part + a.partial_rows * D + 2 * row, float2_t{most, weight});
     }
   }
-  if (w.nsplit > 1) join_parts<XT, D, kThreads>(a, w, out, s_acc);
+  if (w.nsplit > 1) join_parts<XT, D, kThreads>(a, w, out);
 }
 
 // How the columns of a launch of kv4_decode_kernel are dealt.
