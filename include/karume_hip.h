@@ -72,7 +72,7 @@ typedef struct krm_event krm_event;
 
 /* ---- context (acquireGpu / GpuContext.destroy, packages/runtime/mod.ts:13-113) ---------- */
 /* A context owns, besides its stream, 1 MiB of pinned host staging and device scratch that its
- * kernels share: 8 MiB of arrival counters (split attention, shared GEMM tiles), two 128 x 256 f32
+ * kernels share: 8 MiB of arrival counters (split attentions, shared GEMM tiles), two 128 x 256 f32
  * tile partials per CU (64 MiB on 256 CUs), 64 MiB of fp16 planes of f32 activations and 512 KiB of
  * per-row scales for the prefill GEMM.  Calls on one context are ordered on its stream; two contexts
  * never share scratch. */
@@ -133,7 +133,7 @@ int32_t krm_graph_begin(krm_ctx* ctx);
  * Ops that use the context's own scratch share it in launch order and therefore belong on the
  * main branch; while a side branch is selected they fail with KRM_ERR_VALIDATION and record
  * nothing: the decode attention when it splits the columns (more than four chunks),
- * krm_attention_varlen / _planned and every f32-class (KRM_COMPUTE_F32 with f32 x) MFMA product in
+ * krm_attention_varlen / _planned, krm_kv4_attention with a workspace and every f32-class (KRM_COMPUTE_F32 with f32 x) MFMA product in
  * groups of 64 and more.  krm_linear_i4 of fp16 x, or of f32 x under KRM_COMPUTE_F16, uses that
  * scratch on the main branch only (large products share tiles through it; f32 rows may be rounded
  * into it by a launch of their own) and takes the forms without it on a side branch: the same class
@@ -603,10 +603,14 @@ int32_t krm_rope_rows(krm_ctx* ctx, krm_buf x, krm_buf positions_i32, krm_buf co
  * krm_kv4_attention: each row attends to columns max(0, p - window + 1) .. p of its sequence (p its own
  * column; window 0 = all), which krm_kv4_append must have written, with scores half_scale^2 q . k:
  *   q, out [total_rows, H, D] io_dtype (out is not q); H a multiple of Hkv.
- * fp16 rows: keys, values and weights are rounded to fp16, sums are f32; f32 rows: f32 class throughout.
- * A refused sequence's rows, and rows that see a page outside the cache, are NaN.  `workspace`
- * (krm_kv4_attention_workspace bytes, 16-byte aligned; 0 bytes: may be 0) belongs to one call at a
- * time; its contents need no preparation. */
+ * fp16 rows: the values that codes stand for are rounded to fp16, once, and so is the result; keys,
+ * weights and sums keep 22 bits and more.  f32 rows: f32 class throughout (queries up to 1e33).  A
+ * refused sequence's rows, and rows that see a page outside the cache, are NaN; so is a row that sees a
+ * column of NaN, and no other.  Columns are dealt to workgroups by all of a step's lengths, and parts of a
+ * row joined in a fixed order: the same call gives the same bits, a row beside other sequences maybe
+ * other last bits.  `workspace` (krm_kv4_attention_workspace bytes of the same arguments, 16-byte aligned;
+ * 0 bytes: may be 0) belongs to one call at a time; its contents need no preparation.  A call that has one
+ * counts its parts in the context's scratch too. */
 int32_t krm_kv4_page_bytes(uint32_t kv_heads, uint32_t depth, uint32_t group, uint32_t page_rows,
                            size_t* bytes);
 int32_t krm_kv4_append(krm_ctx* ctx, krm_buf q, krm_buf k, krm_buf v, krm_buf q_out,

@@ -631,8 +631,8 @@ struct DecodePlan {
 // Waves of a workgroup.  With eight a CU has one workgroup, two waves a SIMD, and as few parts to join as can be.  With four
 // it has two or three, and one's first loads and last sums run beside another's tiles, which pays where many sequences'
 // pieces are unequal or more than the CUs (us, eight / four, 8 kv heads x 4, D 128, fp16: 16 sequences of 128 to 4096
-// columns 28 / 24, 32 of them 41 / 37, 128 of 300 28 / 23, 128 of 2000 90 / 76; but 16 of 4000 28 / 31, 131000 columns 40 /
-// 54), or where all pieces together are few (one sequence of 700 or 4096 columns 11.7 / 10.8, 12.2 / 11.1).
+// columns 26 / 22, 32 of them 40 / 36, 128 of 300 29 / 22, 128 of 2000 90 / 76; but 16 of 4000 27 / 29, 131000 columns 40 /
+// 54), or where all pieces together are few (one sequence of 700 or 4096 columns 10.6 / 9.5, 11.1 / 9.9).
 constexpr uint32_t kFewWaves = 4, kManyWaves = 8;
 constexpr uint32_t kManyUnits = 96, kManyGroups = kKv4Groups * 3 / 2;
 constexpr uint32_t kMostGroups = 2048;   // in a grid, those without a split among them

@@ -652,6 +652,69 @@ def test_two_recorded_calls_share_a_workspace(gpu_ctx):
         a.free()
 
 
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+def test_recorded_chunks_replay_with_other_rows_and_lengths(gpu_ctx, io):
+    """One graph with room for 300 rows a sequence: chunks that grow, shrink, end and are refused between replays, which
+    changes what every workgroup does; each replay has the bits of the eager call."""
+    ctx, rng = gpu_ctx, np.random.default_rng(93)
+    lay, heads = ref.Layout(4, 64, 64, 32), 32
+    full = ref.Step.make(lay, (300, 300, 300), (1000, 700, 300), rng)
+    raw, q = full.random_cache(rng), rng.normal(size=(full.total, heads, 64))
+    a = Attention(ctx, full, raw, q, io)
+    with ctx.record() as rec:
+        a.run()
+    for rows, lens, bad in (((300, 300, 300), (1000, 700, 300), False), ((1, 300, 2), (999, 300, 50), False),
+                            ((0, 0, 200), (7, 0, 280), False), ((130, 0, 31), (130, 3, 31), False),
+                            ((200, 300, 40), (1000, 299, 300), True), ((1, 1, 1), (5, 640, 1), False)):
+        step = ref.Step(lay, list(rows), list(lens), full.pages, full.table)
+        got = []
+        for run in (rec.graph.launch, a.run):
+            a.buf["cu"].upload(step.cu)
+            a.buf["lens"].upload(np.int32(lens))
+            a.out.upload(np.full(a.out.nbytes // np.dtype(io).itemsize, 77, io))
+            a.fault.zero()
+            run()
+            ctx.sync()
+            got.append(a.out.download(io, (full.total + 1, heads, 64)))
+            assert a.faulted() == bad
+        assert got[0].tobytes() == got[1].tobytes(), rows
+        assert np.all(got[0][step.total:] == 77)
+        if not bad:
+            want, reach, top = step.attention(raw, a.q[:step.total], a.half_scale)
+            assert np.abs(got[0][:step.total] - want).max() <= tolerance(io, reach, top, 1000)[0]
+        else:
+            assert np.all(np.isnan(got[0][200:500])) and np.all(np.isfinite(got[0][:200]))
+    rec.graph.destroy()
+    a.free()
+
+
+def test_side_branches_have_calls_without_a_workspace_only(gpu_ctx):
+    ctx, rng = gpu_ctx, np.random.default_rng(94)
+    calls = []
+    for lens in ((30, 9), (800, 90)):
+        step = ref.Step.make(ref.Layout(2, 64, 32, 16), (1, 1), lens, rng)
+        calls.append(Attention(ctx, step, step.random_cache(rng), rng.normal(size=(2, 4, 64)), np.float16))
+    short, long = calls
+    assert short.need == 0 < long.need
+    with ctx.record() as rec:
+        rec.branch(1)
+        with pytest.raises(ka.GpuValidationError):
+            long.run()
+        short.run()
+        rec.branch(0)
+        long.run()
+    for _ in range(3):
+        rec.graph.launch()
+        ctx.sync()
+    got = [a.result().tobytes() for a in calls]
+    for a, g in zip(calls, got):
+        a.run()
+        assert a.result().tobytes() == g
+    rec.graph.destroy()
+    short.free()
+    long.free()
+
+
 def test_refusals(gpu_ctx):
     ctx, rng = gpu_ctx, np.random.default_rng(1)
     step = ref.Step.make(ref.Layout(2, 64, 32, 16), (1, 2), (700, 80), rng)
