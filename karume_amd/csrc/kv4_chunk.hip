@@ -644,7 +644,7 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
   sum = across_halves(sum, [](float x, float y) { return x + y; });
 
   // ---- parts: as the lanes hold them, (max, sum) of every lane behind the sums; whoever arrives last joins them in
-  // order in the same lanes
+  // order in the same lanes, its own from registers
   const ChunkAttention numbers = scalars(s_numbers);
   const ChunkWork piece = scalars(s_work);
   bool mine_to_write = true;
@@ -659,17 +659,28 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
         publish2(mine + (o * 16 + r) * kThreads, float2_t{acc[o][r], acc[o][r + 1]});
     publish2(mine + kState, float2_t{top, sum});
     mine_to_write = arrived_last(given.tickets + (size_t)piece.first_group * kTicketStride, piece.parts);
+    constexpr bool kKeepsOwn = D < 256 || !kF32;   // (registers: there its own part is read back too)
     if (mine_to_write) {
+    const float2_t own_state = {top, sum};
+    float16_t own[kOuts];
     top = -INFINITY;
     sum = 0.f;
 #pragma unroll
-    for (int o = 0; o < kOuts; ++o) acc[o] = float16_t{};
+    for (int o = 0; o < kOuts; ++o) {
+      own[o] = acc[o];
+      acc[o] = float16_t{};
+    }
     for (uint32_t p = 0; p < piece.parts; ++p) {
       const float* from_part = given.partials + part_slot(piece, p) * kPart + 2 * tid;
-      const float2_t state = observe2(from_part + kState);
-      float2_t x[kOuts * 8];
+      float2_t state = own_state, x[kOuts * 8];
+      if (kKeepsOwn && p == piece.part) {
 #pragma unroll
-      for (int i = 0; i < kOuts * 8; ++i) x[i] = observe2(from_part + 2 * i * kThreads);
+        for (int i = 0; i < kOuts * 8; ++i) x[i] = {own[i / 8][2 * i % 16], own[i / 8][2 * i % 16 + 1]};
+      } else {
+        state = observe2(from_part + kState);
+#pragma unroll
+        for (int i = 0; i < kOuts * 8; ++i) x[i] = observe2(from_part + 2 * i * kThreads);
+      }
       const float now = fmaxf(top, state[0]), ref = now == -INFINITY ? 0.f : now;
       const float keep = __builtin_amdgcn_exp2f(top - ref), take = __builtin_amdgcn_exp2f(state[0] - ref);
       top = now;
