@@ -659,12 +659,14 @@ DecodePlan plan_decode(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs) 
   return p;
 }
 // Which kernel has which sequences.  kv4_decode_kernel takes blocks of 16 (row, head) pairs and reads the columns again for
-// each, kv4_chunk_kernel up to 256 of them with one turn of the codes, which pays where blocks of 16 are several times
-// the CUs (us, decode / chunk, 8 kv heads x 4, D 128, fp16, columns 1024 and 8192: 512 rows of one sequence 51 / 38 and
-// 236 / 127; 128 rows 17 / 34 and 70 / 73; 64 rows of eight 58 / 39 and 242 / 121; 16 rows of eight 19 / 33 and 71 / 101;
-// 1 kv head x 8, D 256: 512 rows 26 / 65 and 124 / 153, of eight 168 / 117 and 946 / 844).
+// each, kv4_chunk_kernel up to 256 of them with one turn of the codes, which pays where blocks of 16 are four times the
+// CUs, or twice over long columns (us, decode / chunk, 1024 and 8192 columns; 8 kv heads x 4, D 128, fp16: 128 rows 17 / 40
+// and 71 / 76; 256 rows 29 / 40 and 123 / 83, of 2048 columns 46 / 47; 512 rows 46 / 36 and 229 / 118; eight sequences of 64
+// rows 53 / 38 and 234 / 121; 4 kv heads x 4, D 256: 512 rows 42 / 52 and 233 / 237, eight sequences of 128 86 / 73 and 464 /
+// 441; eight of 128 rows of 128 columns, D 128 42 / 21, D 256 33 / 28).
 // A step may hold both kinds: sequences of up to kFewPairs pairs then stay with the decode kernel, in a launch of its own.
 constexpr uint64_t kFewPairs = 32;
+constexpr uint32_t kLongColumns = 2048;
 struct AttentionPlan {
   bool few = true, many = false;   // which launches there are
   DecodePlan decode;
@@ -675,7 +677,8 @@ AttentionPlan plan_attention(const Kv4Shape& s, uint32_t max_columns) {
   const uint32_t rows = kv4_rows(s.max_query, s.total_rows);
   const uint64_t pairs = (uint64_t)rows * (s.heads / s.kv_heads);
   const uint64_t blocks = (uint64_t)s.nseq * s.kv_heads * ((pairs + kRows - 1) / kRows);
-  p.many = pairs > kFewPairs && blocks >= (s.depth == 256 ? 4u : 2u) * kKv4Groups;
+  p.many = pairs > kFewPairs &&
+           blocks >= (s.depth < 256 && max_columns >= kLongColumns ? 2u : 4u) * kKv4Groups;
   p.few = !p.many || (s.nseq > 1 && s.total_rows < (uint64_t)s.nseq * rows);
   if (p.few) p.decode = plan_decode(s, max_columns, p.many ? kFewPairs : pairs);
   p.bytes = p.decode.bytes;

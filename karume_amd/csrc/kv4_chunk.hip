@@ -84,7 +84,7 @@ __device__ inline T scalars(const T& from) {
 // times that, so that a run's end less than kSnap tiles away from a block's is moved there (2048 rows of 2048 columns, 4 kv
 // heads x 8, D 64, f32: without both 119.9 us, so 76.5).
 // If whole blocks, or equal parts of them, can be dealt one a workgroup, and none has kDearer tiles more than a run, they
-// are (512 rows of 1024 columns, 8 kv heads x 4, D 128: runs 44.6 us, parts 38.3).
+// are (512 rows of 1024 columns, 8 kv heads x 4, D 128: runs 44.6 us, parts 38.3; since 36.4).
 constexpr uint32_t kBegin = 2, kSnap = 3, kDearer = 8;
 struct ChunkAttention : Kv4Attention {
   uint32_t grain;

@@ -251,6 +251,7 @@ int32_t krm_rope_rows(krm_ctx* ctx, krm_buf x, krm_buf positions_i32, krm_buf co
   char why[128];
   KRM_REQUIRE(ctx, head_dim >= 1 && kv4_turn_ok(head_dim, rotary_dim, layout, table_rows, table_width, why, sizeof why),
               "krm_rope_rows: %s", head_dim ? why : "head_dim 0");
+  KRM_REQUIRE(ctx, rows <= 0x7fffffffu, "krm_rope_rows: %u rows", rows);
   if (rows == 0 || heads == 0) return KRM_OK;
   const uint64_t packed = (uint64_t)heads * head_dim;
   KRM_REQUIRE(ctx, x && out && (rotary_dim == 0 || (positions_i32 && cos_table_f32 && sin_table_f32)),
@@ -277,7 +278,7 @@ int32_t krm_rope_rows(krm_ctx* ctx, krm_buf x, krm_buf positions_i32, krm_buf co
     const uint32_t heads_most = 4 * kThreads / per_head ? 4 * kThreads / per_head : 1;
     const uint32_t block_heads = heads < heads_most ? heads : heads_most;
     const dim3 grid((rows + block_rows - 1) / block_rows, (heads + block_heads - 1) / block_heads), block(kThreads);
-    if (grid.y <= 65535) {
+    if (grid.x <= 0x7fffffu && grid.y <= 65535) {
 #define KRM_PIECES(XT, HALF)                                                                                         \
   rope_pieces_kernel<XT, HALF><<<grid, block, (size_t)block_rows * rotary_dim * sizeof(float), ctx->stream>>>(       \
       ptr<const XT>(x), ptr<const int32_t>(positions_i32), ptr<const float>(cos_table_f32),                          \

@@ -280,6 +280,9 @@ def test_many_rows_of_many_heads(gpu_ctx, io, depth, group, page):
     check(gpu_ctx, step, hkv * 4, io, rng, window=100)
     whole = ref.Step.make(ref.Layout(hkv, depth, group, page), (150,), (150,), rng)
     check(gpu_ctx, whole, hkv * 7, io, rng)
+    check(gpu_ctx, whole, hkv * 7, io, rng, max_columns=2048)
+    more = ref.Step.make(ref.Layout(8, depth, group, page), (300,), (301,), rng)
+    check(gpu_ctx, more, 8 * 7, io, rng)
 
 
 @pytest.mark.parametrize("io", [np.float16, np.float32])
@@ -296,8 +299,9 @@ def test_many_sequences_of_many_rows(gpu_ctx, io, depth, group):
 
 
 @pytest.mark.parametrize("io", [np.float16, np.float32])
-@pytest.mark.parametrize("depth,rows,lens", [(64, (512,), (512,)), (128, (700, 260), (700, 5000)),
-                                             (256, (300, 300), (300, 1200))])
+@pytest.mark.parametrize("depth,rows,lens", [(64, (512,), (512,)), (64, (512, 512), (512, 512)),
+                                             (128, (700, 260), (700, 5000)), (256, (300, 300), (300, 1200)),
+                                             (256, (300, 300, 1, 77), (300, 1200, 5, 77))])
 def test_whole_prompts(gpu_ctx, io, depth, rows, lens):
     """Rows that see nothing but each other: blocks of rows with few columns beside ones with all of them."""
     rng = np.random.default_rng(depth)
@@ -311,7 +315,7 @@ def test_all_rows_of_a_refused_chunk_are_nan(gpu_ctx, io):
     rows, lens = (70, 90, 1, 64), (70, 300, 40, 500)
     step = ref.Step.make(ref.Layout(8, 64, 32, 16), rows, lens, rng)
     raw = step.random_cache(rng)
-    q = rng.normal(size=(step.total, 32, 64))
+    q = rng.normal(size=(step.total, 64, 64))
     a = Attention(gpu_ctx, step, raw, q, io)
     want, reach, top = step.attention(raw, a.q, a.half_scale, 0)
     most, _ = tolerance(io, reach, top, 500)

@@ -113,7 +113,7 @@ def test_refusals(gpu_ctx):
     buf = ctx.alloc(4096)
     rows = dict(rows=2, heads=2, head_dim=64, rotary_dim=64, table_rows=4)
     for change in (dict(rotary_dim=66), dict(rotary_dim=63), dict(layout=2), dict(table_width=31), dict(table_rows=0),
-                   dict(x_stride=127), dict(out_stride=127), dict(io_dtype=5), dict(head_dim=0)):
+                   dict(x_stride=127), dict(out_stride=127), dict(io_dtype=5), dict(head_dim=0), dict(rows=2**31)):
         with pytest.raises(ka.GpuValidationError):
             ctx.rope_rows(buf, buf, buf, buf, buf.offset(2048), **{**rows, **change})
     for name, change in (("in place", dict(to_head_major=True)), ("in place", dict(out_stride=130))):
