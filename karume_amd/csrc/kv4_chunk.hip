@@ -755,7 +755,7 @@ int32_t launch_kv4_chunk(krm_ctx* ctx, const Kv4Attention& a, const Kv4Buffers& 
   const uint64_t blocks = (uint64_t)a.nseq * a.layout.kv_heads * ((rows * a.share + pairs - 1) / pairs);
   c.grain = a.limits.max_columns <= tile ? 31 - __builtin_clz(tile) : 2;
   while (blocks * (((a.limits.max_columns + (uint64_t)pairs + kBegin * tile) >> c.grain) + 2) >= 1ull << 31) ++c.grain;
-  // a run has two tiles at least: joining two parts costs more
+  // a run has two tiles at least (45 steps of 16 to 1024 rows: four 1.5 % more time, one 0.2 %)
   c.least = 2 * tile >> c.grain ? 2 * tile >> c.grain : 1;
   if (io_dtype == KRM_F32) launch_depth<float>(ctx, c, b);
   else launch_depth<__half>(ctx, c, b);
