@@ -19,8 +19,8 @@ struct Kv4Attention {
   float* partials;                    // parts of rows, as each kernel lays them out
   uint32_t* tickets;
 };
-// Workgroups that share a launch's columns, one a CU: with 512 and 1024 of them a decode step of 131000 columns took 49.4
-// us, with 256 39.8.
+// Workgroups that share a launch's columns, one a CU: with 512 and 1024 of them a decode step of 131000 columns took
+// 49.4 us, with 256 39.8.
 constexpr uint32_t kKv4Groups = 256;
 struct Kv4Buffers {
   krm_buf q, cache, page_table, cu_rows, lens, out, fault;
@@ -39,10 +39,12 @@ constexpr int kJoin = 16;           // parts whose sums are asked for together
 
 // Device-scope load / store of two floats: read from (written through to) memory that every XCD sees.
 __device__ inline float2_t observe2(const float* p) {
-  return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT));
 }
 __device__ inline void publish2(float* p, float2_t v) {
-  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
 }
 // Both rounded to nearest, in one step (and not a second time where a single one of them is used).
 __device__ inline half2_t rounded2(float2_t x) {

@@ -2,6 +2,10 @@
 //
 // Row r of a sequence stands at column p = len - rows + r and sees columns max(0, p - window + 1) .. p:
 //   out = sum_c softmax_c(scale^2 q . k_c) v_c,   k_c = step * code + minimum, v_c alike.
+// This is the kernel for few rows.  A long sequence is bound by memory (131000 columns, 8 kv heads x 4, D 128, groups of
+// 64, 151 MB: 38 us, 4.0 TB/s), ragged batches by the vector instructions that turn codes (about 330 a tile of 32 columns
+// beside 28 matrix ones) and by unequal pieces (32 sequences of 128 to 4096 columns 36.5 us), short ones by the chain
+// lengths, pages, columns, waves' join (500 columns 8.8 us).
 #include "kv4_attention.h"
 #include "lds_stream.h"
 #include "rows8.h"
@@ -128,7 +132,8 @@ __device__ inline void store4(__half* to, float4_t x) {
   *reinterpret_cast<uint2*>(to) = make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
 }
 
-// A workgroup's part of its rows is published; the workgroup that arrives last joins the parts in order, whichever it is.
+// A workgroup's part of its rows is published; the workgroup that arrives last joins the parts in order, whichever it
+// is.
 template <typename XT, int D, int kThreads>
 __device__ inline void join_parts(const DecodeAttention& a, const DecodeWork& w, XT* __restrict__ out) {
   const uint32_t tid = threadIdx.x, nsplit = w.nsplit, count = w.count;
@@ -292,7 +297,8 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
     most = quarters_max(most);
     int e = 0;
     // (queries so small or large that the scale would leave f32's range with them are not normalised any further)
-    if (most > 0.f && most < INFINITY) e = max(min(6 - __builtin_amdgcn_frexp_expf(most), 100), __builtin_amdgcn_frexp_expf(a.scale) - 110);
+    if (most > 0.f && most < INFINITY)
+      e = max(min(6 - __builtin_amdgcn_frexp_expf(most), 100), __builtin_amdgcn_frexp_expf(a.scale) - 110);
     scale = ldexpf(a.scale, (kF32 ? 2 : 16) - e);
     float sums[NG] = {};
 #pragma unroll
@@ -300,7 +306,8 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float z = ldexpf(x[st][i], e), y = z * (!kF32 && (i & 2) ? 16.0f : 256.0f);   // elements 2, 3, 6, 7 lie four bits up
+        const float z = ldexpf(x[st][i], e);
+        const float y = z * (!kF32 && (i & 2) ? 16.0f : 256.0f);   // elements 2, 3, 6, 7 lie four bits up
         qh[st][i] = (_Float16)y;
         if constexpr (kF32) ql[st][i] = (_Float16)(y - (float)qh[st][i]);
         sum += z;
@@ -433,8 +440,8 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
     float here = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                        fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
     here = quarters_max(here) * scale;
-    // The sums are brought to a new maximum where one has grown by more than 2^4; weights are 2^10 times what they would
-    // be, so that their low parts are no subnormal numbers, and at most 2^14.
+    // The sums are brought to a new maximum where one has grown by more than 2^4; weights are 2^10 times what they
+    // would be, so that their low parts are no subnormal numbers, and at most 2^14.
     if (__any(here > top + 4.0f)) {
       const float now = fmaxf(here, top);
       const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
@@ -495,7 +502,8 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t x = __builtin_amdgcn_perm(words[2 * j + 1], words[2 * j], select);
-          // (f32 rows: sums around zero, beside which the minima's are small; a mean of many values is far below 8 steps)
+          // (f32 rows: sums around zero, beside which the minima's are small; a mean of many values is far below 8
+          // steps)
           lo2[j] = low_codes<kF32 ? 8 : 0>(x);
           hi2[j] = high_codes<kF32 ? 8 : 0>(x);
         }
@@ -628,11 +636,12 @@ struct DecodePlan {
   float share_of_work = 0;
   size_t bytes = 0;
 };
-// Waves of a workgroup.  With eight a CU has one workgroup, two waves a SIMD, and as few parts to join as can be.  With four
-// it has two or three, and one's first loads and last sums run beside another's tiles, which pays where many sequences'
-// pieces are unequal or more than the CUs (us, eight / four, 8 kv heads x 4, D 128, fp16: 16 sequences of 128 to 4096
-// columns 26 / 22, 32 of them 40 / 36, 128 of 300 29 / 22, 128 of 2000 90 / 76; but 16 of 4000 27 / 29, 131000 columns 40 /
-// 54), or where all pieces together are few (one sequence of 700 or 4096 columns 10.6 / 9.5, 11.1 / 9.9).
+// Waves of a workgroup.  With eight a CU has one workgroup, two waves a SIMD, and as few parts to join as can be.  With
+// four it has two or three, and one's first loads and last sums run beside another's tiles, which pays where many
+// sequences' pieces are unequal or more than the CUs (us, eight / four, 8 kv heads x 4, D 128, fp16: 16 sequences of
+// 128 to 4096 columns 26 / 22, 32 of them 40 / 36, 128 of 300 29 / 22, 128 of 2000 90 / 76; but 16 of 4000 27 / 29,
+// 131000 columns 40 / 54), or where all pieces together are few (one sequence of 700 or 4096 columns 10.6 / 9.5, 11.1 /
+// 9.9).
 constexpr uint32_t kFewWaves = 4, kManyWaves = 8;
 constexpr uint32_t kManyUnits = 96, kManyGroups = kKv4Groups * 3 / 2;
 constexpr uint32_t kMostGroups = 2048;   // in a grid, those without a split among them
@@ -658,13 +667,14 @@ DecodePlan plan_decode(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs) 
   p.bytes = splits > 1 ? (size_t)units * splits * p.partial_rows * (s.depth + 2) * sizeof(float) : 0;
   return p;
 }
-// Which kernel has which sequences.  kv4_decode_kernel takes blocks of 16 (row, head) pairs and reads the columns again for
-// each, kv4_chunk_kernel up to 256 of them with one turn of the codes, which pays where blocks of 16 are four times the
-// CUs, or twice over long columns (us, decode / chunk, 1024 and 8192 columns; 8 kv heads x 4, D 128, fp16: 128 rows 17 / 40
-// and 71 / 76; 256 rows 29 / 40 and 123 / 83, of 2048 columns 46 / 47; 512 rows 46 / 36 and 229 / 118; eight sequences of 64
-// rows 53 / 38 and 234 / 121; 4 kv heads x 4, D 256: 512 rows 42 / 52 and 233 / 237, eight sequences of 128 86 / 73 and 464 /
-// 441; eight of 128 rows of 128 columns, D 128 42 / 21, D 256 33 / 28).
-// A step may hold both kinds: sequences of up to kFewPairs pairs then stay with the decode kernel, in a launch of its own.
+// Which kernel has which sequences.  kv4_decode_kernel takes blocks of 16 (row, head) pairs and reads the columns again
+// for each, kv4_chunk_kernel up to 256 of them with one turn of the codes, which pays where blocks of 16 are four times
+// the CUs, or twice over long columns (us, decode / chunk, 1024 and 8192 columns; 8 kv heads x 4, D 128, fp16: 128 rows
+// 17 / 40 and 71 / 76; 256 rows 29 / 40 and 123 / 83, of 2048 columns 46 / 47; 512 rows 46 / 36 and 229 / 118; eight
+// sequences of 64 rows 53 / 38 and 234 / 121; 4 kv heads x 4, D 256: 512 rows 42 / 52 and 233 / 237, eight sequences of
+// 128 86 / 73 and 464 / 441; eight of 128 rows of 128 columns, D 128 42 / 21, D 256 33 / 28).
+// A step may hold both kinds: sequences of up to kFewPairs pairs then stay with the decode kernel, in a launch of its
+// own.
 constexpr uint64_t kFewPairs = 32;
 constexpr uint32_t kLongColumns = 2048;
 struct AttentionPlan {

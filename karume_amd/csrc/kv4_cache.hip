@@ -43,6 +43,9 @@ struct AppendArgs {
 // A thread has 8 elements of one head's row, D / 8 neighbouring lanes the row.  A workgroup has 256 * 8 / D of the
 // (H + 2 Hkv) heads of one row of the step, whose angles it holds in LDS: queries are turned and stored, keys turned,
 // quantised and stored, values quantised and stored.
+// What bounds it is memory: 8100 f32 rows of 32 + 2 x 8 heads of 128, 342 MB, take 65 us (5.2 TB/s, some of it from the
+// last-level cache); with angles fetched by every head and divisions to find its place 84.  One row of 64 sequences: 3.9
+// us, less than its launch takes the host.
 // PIECES: a thread's elements are turned as whole pieces (pairs within 8 elements, or 8 pairs across two pieces).
 template <typename XT, int D, bool PIECES>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(
@@ -184,7 +187,8 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(
 }
 
 // The last rows of each sequence as the values they stand for: step * code is exact in f32 and the sum is
-// rounded once.  Rows on a page that is none of the cache's are NaN.
+// rounded once.  Rows on a page that is none of the cache's are NaN.  (8100 rows of 2 x 8 heads of 128 to fp16, 43 MB:
+// 12.4 us.)
 template <typename OT, int D>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(
     const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table, const int32_t* __restrict__ cu_rows,

@@ -7,6 +7,9 @@
 //   keys    k = hi + lo, two fp16 planes (22 bits): the products with fp16 queries are off by no more than f32 sums;
 //           f32 queries are hi + lo too
 //   weights p = hi + lo; values rounded to fp16 once (f32 rows: hi + lo)
+// Both hi and lo planes double the products: four prompts of 512 rows behind 200 to 4100 columns (8 kv heads x 4, D 128,
+// fp16; 80 GFLOP without them) take 170 to 178 us, 143 of them at the rate of a large product; matrix and vector
+// instructions each have about half of a SIMD's time and hardly overlap.
 // The scores are formed as K Q^T: a lane has one pair's scores, so its maximum and sum stay in the lane, and the weights
 // leave the product in the order in which the next one takes them.
 #include "kv4_attention.h"
@@ -62,6 +65,12 @@ __device__ inline uint32_t wave_through(uint32_t x) {
   return x;
 }
 
+// The thread's number.  (What hangs on it alone is found anew, and not kept beside all of a kernel's work.)
+__device__ inline uint32_t thread_id() {
+  uint32_t tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
 // Values that are the same in every lane.
 __device__ inline uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 template <typename T>
@@ -75,16 +84,16 @@ __device__ inline T scalars(const T& from) {
   return __builtin_bit_cast(T, x);
 }
 
-// How blocks of kPairs (row, head) pairs are dealt to kKv4Groups workgroups, one a CU.  Every wave reads the step's words
-// itself, 64 sequences at a time.
-// A launch's work is one long row of units of 2^grain columns: for each sequence, kv head and block those that its rows see.
-// Each workgroup has an equal run of it, which may end one block's columns and begin another's.  (A grid of blocks times
-// equal splits: four prompts of 512 rows behind 200 to 4100 columns 190 us, so 178; three of 512 of 2048 104 us, so 96.)
-// Beginning a block costs a workgroup as much as kBegin tiles, which its work counts, and joining a block's parts several
-// times that, so that a run's end less than kSnap tiles away from a block's is moved there (2048 rows of 2048 columns, 4 kv
-// heads x 8, D 64, f32: without both 119.9 us, so 76.5).
-// If whole blocks, or equal parts of them, can be dealt one a workgroup, and none has kDearer tiles more than a run, they
-// are (512 rows of 1024 columns, 8 kv heads x 4, D 128: runs 44.6 us, parts 38.3; since 36.4).
+// How blocks of kPairs (row, head) pairs are dealt to kKv4Groups workgroups, one a CU.  Every wave reads the step's
+// words itself, 64 sequences at a time.
+// A launch's work is one long row of units of 2^grain columns: for each sequence, kv head and block those that its rows
+// see. Each workgroup has an equal run of it, which may end one block's columns and begin another's.  (A grid of blocks
+// times equal splits: four prompts of 512 rows behind 200 to 4100 columns 190 us, so 178; three of 512 of 2048 104 us,
+// so 96.) Beginning a block costs a workgroup as much as kBegin tiles, which its work counts, and joining a block's
+// parts several times that, so that a run's end less than kSnap tiles away from a block's is moved there (2048 rows of
+// 2048 columns, 4 kv heads x 8, D 64, f32: without both 119.9 us, so 76.5).
+// If whole blocks, or equal parts of them, can be dealt one a workgroup, and none has kDearer tiles more than a run,
+// they are (512 rows of 1024 columns, 8 kv heads x 4, D 128: runs 44.6 us, parts 38.3; since 36.4).
 constexpr uint32_t kBegin = 2, kSnap = 3, kDearer = 8;
 struct ChunkAttention : Kv4Attention {
   uint32_t grain;
@@ -96,7 +105,9 @@ struct ChunkWork : Work {
   uint32_t first_group, parts, part;  // workgroups that have some of these pairs, and which of them this is
 };
 // Where the parts lie: the first part of some pairs is its workgroup's last piece, any other one the first.
-__device__ inline uint32_t part_slot(const ChunkWork& w, uint32_t part) { return 2 * (w.first_group + part) + (part == 0); }
+__device__ inline uint32_t part_slot(const ChunkWork& w, uint32_t part) {
+  return 2 * (w.first_group + part) + (part == 0);
+}
 
 // (in LDS: a tile's loop has no registers for it)
 template <int kWaves, int kPairs, int kTile>
@@ -115,15 +126,10 @@ struct Deal {
 
   // neighbouring runs, which may join parts, lie on one XCD
   __device__ static inline uint32_t group() { return blockIdx.x % 8 * (kKv4Groups / 8) + blockIdx.x / 8; }
-  __device__ static inline uint32_t thread() {
-    uint32_t tid = threadIdx.x;
-    asm volatile("" : "+v"(tid));   // (what hangs on it alone is found anew, and not kept beside all of a kernel's work)
-    return tid;
-  }
   // A lane's sequence of the 64 from `first` on.
   __device__ static inline Sequence read(const ChunkAttention& a, const int32_t* __restrict__ cu_rows,
                                          const int32_t* __restrict__ lens, uint32_t begin, uint32_t first) {
-    const uint32_t seq = first + thread() % kWave, i = min(seq, a.nseq - 1);
+    const uint32_t seq = first + thread_id() % kWave, i = min(seq, a.nseq - 1);
     Sequence s;
     s.cu0 = cu_rows[i];
     s.cu1 = cu_rows[i + 1];
@@ -183,96 +189,81 @@ struct Deal {
       }
       total = last_lane(s.through);
     }
-    sequences[thread() % kWave] = s;
+    sequences[thread_id() % kWave] = s;
     r.at = min(group() * r.per, total);
     r.end = min(r.at + r.per, total);
     r.base = r.before = 0;
     r.fresh = 1;
-    runs[scalar(thread() / kWave)] = r;
+    runs[scalar(thread_id() / kWave)] = r;
   }
   // The next piece of this workgroup's run; false at its end.
   __device__ inline bool next(const ChunkAttention& a, const int32_t* __restrict__ cu_rows,
                               const int32_t* __restrict__ lens, ChunkWork& w) {
-    Run& run = runs[scalar(thread() / kWave)];
+    Run& run = runs[scalar(thread_id() / kWave)];
     Run r = scalars(run);
     for (;;) {
-    if (r.at >= r.end) return false;
-    uint32_t through = sequences[thread() % kWave].through;
-    while (r.at - r.before >= last_lane(through)) {
-      r.before += last_lane(through);
-      r.base += kWave;
-      __syncthreads();
-      const Sequence s = read(a, cu_rows, lens, r.begin, r.base);
-      sequences[thread() % kWave] = s;
-      through = s.through;
-    }
-    const uint32_t lane = (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(through > r.at - r.before));
-    const Sequence& s = sequences[lane];
-    const Kv4Blocks blocks = {scalar(s.blocks.blocks), scalar(s.blocks.first), scalar(s.blocks.step)};
-    const uint32_t of_head = blocks.all(), start = r.before + scalar(s.through) - a.layout.kv_heads * of_head;
-    w.seq = r.base + lane;
-    w.kv_head = scalar((r.at - start) / of_head);
-    const uint32_t head_at = start + w.kv_head * of_head, block = scalar(blocks.block_at(r.at - head_at));
-    const uint32_t block_at = head_at + blocks.before(block), width = blocks.of(block);
-    Kv4Cut cut;
-    const Kv4Dealt dealt = kv4_cut(r, block_at, width, cut);
-    if (dealt == kRunEnds) return false;
-    if (dealt == kBlockSkipped) continue;
-    run = r;
-    w.cu0 = (int32_t)scalar((uint32_t)s.cu0);
-    w.cu1 = (int32_t)scalar((uint32_t)s.cu1);
-    w.refused = scalar(s.ok) == 0;
-    const int32_t rows = w.cu1 - w.cu0;
-    const uint32_t pair0 = block * kPairs;
-    w.count = (uint32_t)min((uint64_t)kPairs, (uint64_t)(uint32_t)rows * a.share - pair0);
-    w.row0 = scalar(divided(pair0, a.share, a.share_inverse));
-    w.head0 = pair0 - w.row0 * a.share;
-    w.first_row = (int32_t)scalar((uint32_t)s.len) - rows + (int32_t)w.row0;
-    w.last_row = w.first_row + (int32_t)scalar(row_of(a, w, w.count - 1));
-    w.low = kv4_first_column(w.first_row, a.window);
-    w.high = w.last_row;
-    const int32_t tile0 = w.low / kTile, tiles = w.high / kTile - tile0 + 1;
-    w.begin = tile0 + (int32_t)scalar(kv4_tile(r, cut.from, width, tiles, a.grain, kTile));
-    w.end = tile0 + (int32_t)scalar(kv4_tile(r, cut.to, width, tiles, a.grain, kTile));
-    w.parts = scalar(cut.parts);
-    w.first_group = scalar(cut.first);
-    w.part = group() - w.first_group;
-    return true;
+      if (r.at >= r.end) return false;
+      uint32_t through = sequences[thread_id() % kWave].through;
+      while (r.at - r.before >= last_lane(through)) {
+        r.before += last_lane(through);
+        r.base += kWave;
+        __syncthreads();
+        const Sequence s = read(a, cu_rows, lens, r.begin, r.base);
+        sequences[thread_id() % kWave] = s;
+        through = s.through;
+      }
+      const uint32_t lane = (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(through > r.at - r.before));
+      const Sequence& s = sequences[lane];
+      const Kv4Blocks blocks = {scalar(s.blocks.blocks), scalar(s.blocks.first), scalar(s.blocks.step)};
+      const uint32_t of_head = blocks.all(), start = r.before + scalar(s.through) - a.layout.kv_heads * of_head;
+      w.seq = r.base + lane;
+      w.kv_head = scalar((r.at - start) / of_head);
+      const uint32_t head_at = start + w.kv_head * of_head, block = scalar(blocks.block_at(r.at - head_at));
+      const uint32_t block_at = head_at + blocks.before(block), width = blocks.of(block);
+      Kv4Cut cut;
+      const Kv4Dealt dealt = kv4_cut(r, block_at, width, cut);
+      if (dealt == kRunEnds) return false;
+      if (dealt == kBlockSkipped) continue;
+      run = r;
+      w.cu0 = (int32_t)scalar((uint32_t)s.cu0);
+      w.cu1 = (int32_t)scalar((uint32_t)s.cu1);
+      w.refused = scalar(s.ok) == 0;
+      const int32_t rows = w.cu1 - w.cu0;
+      const uint32_t pair0 = block * kPairs;
+      w.count = (uint32_t)min((uint64_t)kPairs, (uint64_t)(uint32_t)rows * a.share - pair0);
+      w.row0 = scalar(divided(pair0, a.share, a.share_inverse));
+      w.head0 = pair0 - w.row0 * a.share;
+      w.first_row = (int32_t)scalar((uint32_t)s.len) - rows + (int32_t)w.row0;
+      w.last_row = w.first_row + (int32_t)scalar(row_of(a, w, w.count - 1));
+      w.low = kv4_first_column(w.first_row, a.window);
+      w.high = w.last_row;
+      const int32_t tile0 = w.low / kTile, tiles = w.high / kTile - tile0 + 1;
+      w.begin = tile0 + (int32_t)scalar(kv4_tile(r, cut.from, width, tiles, a.grain, kTile));
+      w.end = tile0 + (int32_t)scalar(kv4_tile(r, cut.to, width, tiles, a.grain, kTile));
+      w.parts = scalar(cut.parts);
+      w.first_group = scalar(cut.first);
+      w.part = group() - w.first_group;
+      return true;
     }
   }
 };
 
+// One piece.  `a` and `w` are in registers, and wait in LDS as s_numbers and s_work for what comes behind the tiles.
 template <typename XT, int D, int NG>
-__global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
+__device__ __forceinline__ void chunk_piece(
     const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table,
-    const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens, XT* __restrict__ out,
-    uint32_t* __restrict__ fault, ChunkAttention given) {
+    XT* __restrict__ out, uint32_t* __restrict__ fault, float* partials, uint32_t* tickets, const ChunkAttention& a,
+    const ChunkWork& w, const ChunkAttention& s_numbers, const ChunkWork& s_work) {
   using C = Chunk<XT, D>;
   constexpr bool kF32 = C::kF32;
-  constexpr int kThreads = C::kThreads, kPairs = C::kPairs, kColumns = C::kColumns, kBlocks = C::kBlocks;
+  constexpr int kThreads = C::kThreads, kColumns = C::kColumns, kBlocks = C::kBlocks;
   constexpr int kSteps = D / 16, kSubs = kColumns / 32, kOuts = D / 32;
   constexpr int kPieces = D <= 128 ? 1 : D / 128;    // 16-byte pieces of codes that a lane turns
   extern __shared__ __align__(16) uint8_t s_tiles[];  // [2][keys hi, keys lo, values hi (, values lo)]
   __shared__ uint32_t s_unsound[2][kColumns];         // groups of a column's values that are no numbers (edge tiles)
   __shared__ uint32_t s_any[2];
 
-  // the call's numbers and the piece's wait in LDS while its tiles have the registers
-  __shared__ ChunkAttention s_numbers;
-  __shared__ ChunkWork s_work;
-  __shared__ Deal<kThreads / kWave, kPairs, kColumns> deal;
-  if (threadIdx.x == 0) s_numbers = given;
-  deal.start(given, cu_rows, lens, fault);
-  __syncthreads();
-  for (;;) {
-  const ChunkAttention a = scalars(s_numbers);
-  ChunkWork w;
-  if (!deal.next(a, cu_rows, lens, w)) break;
-  s_work = w;   // (every wave writes the same words)
-  if (w.refused) {
-    refuse<XT, D, kThreads>(a, w.kv_head, w.cu0, w.cu1, out);
-    continue;
-  }
-  const uint32_t tid = deal.thread(), lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const uint32_t tid = thread_id(), lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int32_t low = w.low, high = w.high;
 
   // ---- this wave's rows: lane (m = lane % 32, half)
@@ -618,10 +609,11 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
   __syncthreads();
   Raw raw = {};   // (undefined, it would be kept from piece to piece)
   if (w.begin < w.end) raw = fetch(w.begin);
-  for (int32_t tile = w.begin - 1; tile < w.end; ++tile) {   // (the first turn makes the first tile, and has none to multiply)
+  // (the first turn makes the first tile, and has none to multiply)
+  for (int32_t tile = w.begin - 1; tile < w.end; ++tile) {
     const uint32_t buffer = (uint32_t)(tile - w.begin) & 1u;
-    // The two waves of a SIMD are a key maker and a value maker: one makes before it multiplies and the other behind, so
-    // that one's conversions and exponentials run beside the other's products.
+    // The two waves of a SIMD are a key maker and a value maker: one makes before it multiplies and the other behind,
+    // so that one's conversions and exponentials run beside the other's products.
     auto next = [&]() __attribute__((always_inline)) {
       if (tile + 1 < w.end) {
         make(raw, tile + 1, buffer ^ 1u);
@@ -651,45 +643,45 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
   if (piece.parts > 1) {
     constexpr uint32_t kState = kOuts * 16 * kThreads;          // floats before the states
     constexpr size_t kPart = kState + 2 * kThreads;
-    float* const mine = given.partials + part_slot(piece, piece.part) * kPart + 2 * tid;
+    float* const mine = partials + part_slot(piece, piece.part) * kPart + 2 * tid;
 #pragma unroll
     for (int o = 0; o < kOuts; ++o)
 #pragma unroll
       for (int r = 0; r < 16; r += 2)
         publish2(mine + (o * 16 + r) * kThreads, float2_t{acc[o][r], acc[o][r + 1]});
     publish2(mine + kState, float2_t{top, sum});
-    mine_to_write = arrived_last(given.tickets + (size_t)piece.first_group * kTicketStride, piece.parts);
+    mine_to_write = arrived_last(tickets + (size_t)piece.first_group * kTicketStride, piece.parts);
     constexpr bool kKeepsOwn = D < 256 || !kF32;   // (registers: there its own part is read back too)
     if (mine_to_write) {
-    const float2_t own_state = {top, sum};
-    float16_t own[kOuts];
-    top = -INFINITY;
-    sum = 0.f;
+      const float2_t own_state = {top, sum};
+      float16_t own[kOuts];
+      top = -INFINITY;
+      sum = 0.f;
 #pragma unroll
-    for (int o = 0; o < kOuts; ++o) {
-      own[o] = acc[o];
-      acc[o] = float16_t{};
-    }
-    for (uint32_t p = 0; p < piece.parts; ++p) {
-      const float* from_part = given.partials + part_slot(piece, p) * kPart + 2 * tid;
-      float2_t state = own_state, x[kOuts * 8];
-      if (kKeepsOwn && p == piece.part) {
-#pragma unroll
-        for (int i = 0; i < kOuts * 8; ++i) x[i] = {own[i / 8][2 * i % 16], own[i / 8][2 * i % 16 + 1]};
-      } else {
-        state = observe2(from_part + kState);
-#pragma unroll
-        for (int i = 0; i < kOuts * 8; ++i) x[i] = observe2(from_part + 2 * i * kThreads);
+      for (int o = 0; o < kOuts; ++o) {
+        own[o] = acc[o];
+        acc[o] = float16_t{};
       }
-      const float now = fmaxf(top, state[0]), ref = now == -INFINITY ? 0.f : now;
-      const float keep = __builtin_amdgcn_exp2f(top - ref), take = __builtin_amdgcn_exp2f(state[0] - ref);
-      top = now;
-      sum = fmaf(sum, keep, state[1] * take);
+      for (uint32_t p = 0; p < piece.parts; ++p) {
+        const float* from_part = partials + part_slot(piece, p) * kPart + 2 * tid;
+        float2_t state = own_state, x[kOuts * 8];
+        if (kKeepsOwn && p == piece.part) {
 #pragma unroll
-      for (int o = 0; o < kOuts; ++o)
+          for (int i = 0; i < kOuts * 8; ++i) x[i] = {own[i / 8][2 * i % 16], own[i / 8][2 * i % 16 + 1]};
+        } else {
+          state = observe2(from_part + kState);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[o][r] = fmaf(acc[o][r], keep, x[(o * 16 + r) / 2][r & 1] * take);
-    }
+          for (int i = 0; i < kOuts * 8; ++i) x[i] = observe2(from_part + 2 * i * kThreads);
+        }
+        const float now = fmaxf(top, state[0]), ref = now == -INFINITY ? 0.f : now;
+        const float keep = __builtin_amdgcn_exp2f(top - ref), take = __builtin_amdgcn_exp2f(state[0] - ref);
+        top = now;
+        sum = fmaf(sum, keep, state[1] * take);
+#pragma unroll
+        for (int o = 0; o < kOuts; ++o)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[o][r] = fmaf(acc[o][r], keep, x[(o * 16 + r) / 2][r & 1] * take);
+      }
     }
   }
   // ---- out: lane (m, half) has elements 32 o + 8 (r / 4) + 4 half + r % 4 of its pair
@@ -708,6 +700,30 @@ __global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
       }
   }
   __syncthreads();   // (LDS is the next piece's)
+}
+
+template <typename XT, int D, int NG>
+__global__ __launch_bounds__((Chunk<XT, D>::kThreads)) void kv4_chunk_kernel(
+    const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table,
+    const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens, XT* __restrict__ out,
+    uint32_t* __restrict__ fault, ChunkAttention given) {
+  using C = Chunk<XT, D>;
+  __shared__ ChunkAttention s_numbers;
+  __shared__ ChunkWork s_work;
+  __shared__ Deal<C::kThreads / kWave, C::kPairs, C::kColumns> deal;
+  if (threadIdx.x == 0) s_numbers = given;
+  deal.start(given, cu_rows, lens, fault);
+  __syncthreads();
+  for (;;) {
+    const ChunkAttention a = scalars(s_numbers);
+    ChunkWork w;
+    if (!deal.next(a, cu_rows, lens, w)) break;
+    if (w.refused) {
+      refuse<XT, D, C::kThreads>(a, w.kv_head, w.cu0, w.cu1, out);
+    } else {
+      s_work = w;   // (every wave writes the same words)
+      chunk_piece<XT, D, NG>(q, cache, page_table, out, fault, given.partials, given.tickets, a, w, s_numbers, s_work);
+    }
   }
 }
 

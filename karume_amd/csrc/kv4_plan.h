@@ -150,8 +150,8 @@ KRM_HD inline Kv4Dealt kv4_cut(Kv4Run& r, uint32_t block_at, uint32_t width, Kv4
   c.first = first_cut - 1;
   return kPieceDealt;
 }
-// The tile, of a block's `tiles`, at which its unit `unit` begins.  (Units are an estimate, rounded, of a window's widest
-// block: what it leaves or lacks is the last part's.)
+// The tile, of a block's `tiles`, at which its unit `unit` begins.  (Units are an estimate, rounded, of a window's
+// widest block: what it leaves or lacks is the last part's.)
 KRM_HD inline uint32_t kv4_tile(const Kv4Run& r, uint32_t unit, uint32_t width, uint32_t tiles, uint32_t grain,
                                 uint32_t tile) {
   if (r.even) return tiles / width * unit + tiles % width * unit / width;

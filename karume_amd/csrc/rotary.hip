@@ -83,10 +83,10 @@ __global__ __launch_bounds__(kThreads) void rope_tables_kernel(const double* __r
   }
 }
 
-// Rows whose pieces of 8 elements are whole and 16-byte aligned: a workgroup has `block_rows` rows (or a part of one row's
-// heads), whose angles it holds in LDS, so that all heads share one trip to the table; a thread has both sides of 8 pairs
-// (interleaved: 4), or 8 elements that are only copied.  What bounds it is memory: 5003 rows of 40 heads of 128 fp16
-// head-major, 105 MB: 22.3 us, 4.7 TB/s (two elements and their angles a thread: 55.9).
+// Rows whose pieces of 8 elements are whole and 16-byte aligned: a workgroup has `block_rows` rows (or a part of one
+// row's heads), whose angles it holds in LDS, so that all heads share one trip to the table; a thread has both sides of
+// 8 pairs (interleaved: 4), or 8 elements that are only copied.  What bounds it is memory: 5003 rows of 40 heads of 128
+// fp16 head-major, 105 MB: 22.3 us, 4.7 TB/s (two elements and their angles a thread: 55.9).
 template <typename XT, bool HALF>
 __global__ __launch_bounds__(kThreads) void rope_pieces_kernel(
     const XT* __restrict__ x, const int32_t* __restrict__ positions, const float* __restrict__ cos_table,
@@ -98,8 +98,8 @@ __global__ __launch_bounds__(kThreads) void rope_pieces_kernel(
   const uint32_t turns = HALF ? t.rotary_dim / 16 : t.rotary_dim / 8;     // items of a head that are turned
   const uint32_t per_head = turns + (t.head_dim - t.rotary_dim) / 8, per_row = my_heads * per_head;
   const uint32_t items = my_rows * per_row;
-  // (the first item's elements are asked for before the angles; an item has both sides of its pairs, so that rows may be
-  // turned in place)
+  // (the first item's elements are asked for before the angles; an item has both sides of its pairs, so that rows may
+  // be turned in place)
   struct Item {
     float a[8], b[8];
     XT* dst;
