@@ -44,8 +44,8 @@ struct AppendArgs {
 // (H + 2 Hkv) heads of one row of the step, whose angles it holds in LDS: queries are turned and stored, keys turned,
 // quantised and stored, values quantised and stored.
 // What bounds it is memory: 8100 f32 rows of 32 + 2 x 8 heads of 128, 342 MB, take 65 us (5.2 TB/s, some of it from the
-// last-level cache); with angles fetched by every head and divisions to find its place 84.  One row of 64 sequences: 3.9
-// us, less than its launch takes the host.
+// last-level cache); with the read-back 79, and 96 with angles fetched by every head and places found by division.  One
+// row of 64 sequences: 3.9 us, less than its launch takes the host.
 // PIECES: a thread's elements are turned as whole pieces (pairs within 8 elements, or 8 pairs across two pieces).
 template <typename XT, int D, bool PIECES>
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(
