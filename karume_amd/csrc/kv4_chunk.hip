@@ -8,7 +8,7 @@
 //           f32 queries are hi + lo too
 //   weights p = hi + lo; values rounded to fp16 once (f32 rows: hi + lo)
 // Both hi and lo planes double the products: four prompts of 512 rows behind 200 to 4100 columns (8 kv heads x 4, D 128,
-// fp16; 80 GFLOP without them) take 170 to 178 us, 143 of them at the rate of a large product; matrix and vector
+// fp16; 80 GFLOP without them) take 170 to 180 us, 143 of them at the rate of a large product; matrix and vector
 // instructions each have about half of a SIMD's time and hardly overlap.
 // The scores are formed as K Q^T: a lane has one pair's scores, so its maximum and sum stay in the lane, and the weights
 // leave the product in the order in which the next one takes them.
@@ -622,7 +622,9 @@ __device__ __forceinline__ void chunk_piece(
     };
     const bool sees = tile >= w.begin && tile * kColumns <= wave_high && tile * kColumns + kColumns > wave_low;
     if (makes_values) next();
+    __builtin_amdgcn_s_setprio(1);   // (products before the other wave's codes: 0.5 % of 39 steps)
     if (sees) consume(tile, buffer);
+    __builtin_amdgcn_s_setprio(0);
     if (!makes_values) next();
     __syncthreads();
     if (s_any[buffer]) {   // everyone is through with the tile: its marks are cleared before it is made again
