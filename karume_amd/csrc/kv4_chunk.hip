@@ -13,6 +13,7 @@
 // The scores are formed as K Q^T: a lane has one pair's scores, so its maximum and sum stay in the lane, and the weights
 // leave the product in the order in which the next one takes them.
 #include "kv4_attention.h"
+#include "kv4_marks.h"
 #include "rows8.h"
 
 using namespace krm;
@@ -260,8 +261,7 @@ __device__ __forceinline__ void chunk_piece(
   constexpr int kSteps = D / 16, kSubs = kColumns / 32, kOuts = D / 32;
   constexpr int kPieces = D <= 128 ? 1 : D / 128;    // 16-byte pieces of codes that a lane turns
   extern __shared__ __align__(16) uint8_t s_tiles[];  // [2][keys hi, keys lo, values hi (, values lo)]
-  __shared__ uint32_t s_unsound[2][kColumns];         // groups of a column's values that are no numbers (edge tiles)
-  __shared__ uint32_t s_any[2];
+  __shared__ Kv4Marks<kColumns> s_marks;              // (of tiles that some row does not see in full)
 
   const uint32_t tid = thread_id(), lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int32_t low = w.low, high = w.high;
@@ -443,8 +443,8 @@ __device__ __forceinline__ void chunk_piece(
             const half2_t s2 = half2_of(p[j / 2]), l2 = half2_of(p[2 + j / 2]);
             const bool sound = fabsf((float)s2[j & 1]) < INFINITY && fabsf((float)l2[j & 1]) < INFINITY;
             if (!none && !sound && !idle) {
-              atomicOr(&s_unsound[buffer][column - column0], 1u << (column_of * 8 * NG / D));
-              s_any[buffer] = 1;
+              atomicOr(&s_marks.groups[buffer][column - column0], 1u << (column_of * 8 * NG / D));
+              s_marks.any[buffer] = 1;
             }
             if (none || !sound) {
               p[j / 2] &= ~mine;
@@ -591,10 +591,10 @@ __device__ __forceinline__ void chunk_piece(
         }
       }
     }
-    if (s_any[buffer]) {
+    if (s_marks.any[buffer]) {
 #pragma unroll 1
       for (int i = 0; i < kColumns; ++i) {
-        const uint32_t groups = s_unsound[buffer][i];
+        const uint32_t groups = s_marks.groups[buffer][i];
         const int32_t column = column0 + i;
         if (groups == 0 || column < from || column > position) continue;
 #pragma unroll
@@ -604,8 +604,7 @@ __device__ __forceinline__ void chunk_piece(
     }
   };
 
-  for (uint32_t i = tid; i < 2 * kColumns; i += kThreads) s_unsound[i / kColumns][i % kColumns] = 0;
-  if (tid < 2) s_any[tid] = 0;
+  s_marks.clear(tid, kThreads);
   __syncthreads();
   Raw raw = {};   // (undefined, it would be kept from piece to piece)
   if (w.begin < w.end) raw = fetch(w.begin);
@@ -626,13 +625,7 @@ __device__ __forceinline__ void chunk_piece(
     if (sees) consume(tile, buffer);
     __builtin_amdgcn_s_setprio(0);
     if (!makes_values) next();
-    __syncthreads();
-    if (s_any[buffer]) {   // everyone is through with the tile: its marks are cleared before it is made again
-      for (uint32_t i = tid; i < (uint32_t)kColumns; i += kThreads) s_unsound[buffer][i] = 0;
-      __syncthreads();
-      if (tid == 0) s_any[buffer] = 0;
-      __syncthreads();
-    }
+    s_marks.end_turn(buffer, tid, kThreads, [] { __syncthreads(); });
   }
   if (lost && fault && lane == 0) *fault = 1u;
   sum = across_halves(sum, [](float x, float y) { return x + y; });

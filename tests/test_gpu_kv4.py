@@ -770,3 +770,42 @@ def test_refusals(gpu_ctx):
     a.run()
     assert np.all(np.isfinite(a.result()))
     a.free()
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+@pytest.mark.parametrize("depth,group,hkv,rows,lens,window", [
+    (64, 32, 8, (2100,), (2100,), 200), (128, 128, 8, (2100,), (2300,), 90), (256, 64, 8, (1100, 1100), (1100, 1300), 40)])
+def test_columns_of_no_numbers_in_most_tiles_of_many_rows(gpu_ctx, io, depth, group, hkv, rows, lens, window):
+    """Windows shorter than a block of rows, so that every tile has a column that some row does not see: tiles with marked
+    columns and without, in every order one and two tiles apart, call after call."""
+    rng = np.random.default_rng(depth + window)
+    lay = ref.Layout(hkv, depth, group, 64)
+    step = ref.Step.make(lay, rows, lens, rng)
+    raw = step.random_cache(rng)
+    q = rng.normal(size=(step.total, hkv, depth))
+    held, groups, wide = raw.copy(), depth // group, 32 if depth == 256 else 64
+    vparams = lay.pages(held)["vparams"]
+    want, cu = np.zeros(q.shape, bool), step.cu
+    for i, n in enumerate(lens):
+        page, row = step.columns_of(i)
+        for head, tile in np.argwhere(rng.random((hkv, n // wide)) < 0.4):
+            column, g = wide * tile + int(rng.integers(wide)), int(rng.integers(groups))
+            vparams[page[column], head, row[column] // 4, g, tile & 1, row[column] % 4] = (np.nan, np.inf)[head & 1]
+            p = np.arange(n - rows[i], n)
+            sees = np.flatnonzero((p >= column) & (p - column < window))
+            want[cu[i] + sees, head, g * group:(g + 1) * group] = True
+    assert 0.05 < want.mean() < 0.95
+    a = Attention(gpu_ctx, step, held, q, io, window)
+    sound, reach, top = step.attention(raw, a.q, a.half_scale, window)
+    most, _ = tolerance(io, reach, top, window)
+    first = None
+    for _ in range(12):
+        a.out.upload(np.full(a.out.nbytes // np.dtype(io).itemsize, 77, io))
+        a.run()
+        got = a.result()
+        assert np.array_equal(np.isfinite(got), ~want)
+        assert np.abs(got.astype(np.float64) - sound)[~want].max() <= most
+        first = got.tobytes() if first is None else first
+        assert got.tobytes() == first
+    assert not a.faulted()
+    a.free()
