@@ -599,7 +599,7 @@ int32_t krm_rope_rows(krm_ctx* ctx, krm_buf x, krm_buf positions_i32, krm_buf co
  * D] (q_out may be q where q_stride = H * D).  A refused sequence writes nothing, a row without its page
  * no keys and values.  Two sequences of one call must not write to one page.
  * krm_kv4_read: the same rows back, as values in out_dtype: k_out, v_out [total_rows, Hkv, D]; with
- * cu_rows = the sums of lens, all columns.  Rows without their page are NaN.
+ * cu_rows = the sums of lens, all columns.  Rows without their page, and a refused sequence's, are NaN.
  * krm_kv4_attention: each row attends to columns max(0, p - window + 1) .. p of its sequence (p its own
  * column; window 0 = all), which krm_kv4_append must have written, with scores half_scale^2 q . k:
  *   q, out [total_rows, H, D] io_dtype (out is not q); H a multiple of Hkv.

@@ -11,6 +11,8 @@
 #include "rotary.h"
 #include "rows8.h"
 
+#include <cmath>
+
 using namespace krm;
 
 namespace {
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(
 }
 
 // The last rows of each sequence as the values they stand for: step * code is exact in f32 and the sum is
-// rounded once.  Rows on a page that is none of the cache's are NaN.  (8100 rows of 2 x 8 heads of 128 to fp16, 43 MB:
+// rounded once.  Rows on a page that is none of the cache's, and all of a refused sequence, are NaN.  (8100 rows of 2 x 8 heads of 128 to fp16, 43 MB:
 // 12.4 us.)
 template <typename OT, int D>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(
@@ -197,11 +199,18 @@ __global__ __launch_bounds__(kThreads) void kv4_read_kernel(
   constexpr int kLanes = D / kPiece;
   const uint32_t seq = blockIdx.y;
   const Kv4Sequence s = kv4_sequence(cu_rows[seq], cu_rows[seq + 1], lens[seq], limits);
+  const uint32_t hkv = layout.kv_heads;
   if (!s.ok) {
     if (fault && blockIdx.x == 0 && threadIdx.x == 0) *fault = 1u;
+    const float none[8] = {NAN, NAN, NAN, NAN, NAN, NAN, NAN, NAN};
+    const uint64_t pieces = (uint64_t)s.rows * hkv * kLanes;   // (rows: 0 where the offsets are none; may pass max_query)
+    const size_t first = (size_t)(uint32_t)s.first * hkv * D;
+    for (uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x; i < pieces; i += (uint64_t)gridDim.x * kThreads) {
+      store8(k_out + first + i * kPiece, none);
+      store8(v_out + first + i * kPiece, none);
+    }
     return;
   }
-  const uint32_t hkv = layout.kv_heads;
   const uint64_t item = (blockIdx.x * (uint64_t)kThreads + threadIdx.x) / kLanes;
   if (item >= (uint64_t)s.rows * hkv * 2) return;
   const uint32_t row = (uint32_t)(item / (2 * hkv));

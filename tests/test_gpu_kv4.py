@@ -809,3 +809,41 @@ def test_columns_of_no_numbers_in_most_tiles_of_many_rows(gpu_ctx, io, depth, gr
         assert got.tobytes() == first
     assert not a.faulted()
     a.free()
+
+
+@pytest.mark.parametrize("out_dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("depth,hkv", [(64, 1), (128, 3), (256, 2)])
+def test_all_rows_of_a_refused_sequence_read_as_nan(gpu_ctx, out_dtype, depth, hkv):
+    """Also those that the call's limit of rows a sequence leaves no workgroup for; others, and rows of no sequence, as
+    they would be."""
+    ctx, rng = gpu_ctx, np.random.default_rng(depth + hkv)
+    rows, lens = (2, 75, 0, 3), (20, 90, 0, 40)
+    step = ref.Step.make(ref.Layout(hkv, depth, 32, 16), rows, lens, rng)
+    cache, table, cu, n = up(ctx, step.random_cache(rng), step.table, step.cu, np.int32(lens))
+    fault, out = ctx.zeros(16), [ctx.alloc((step.total + 1) * hkv * depth * np.dtype(out_dtype).itemsize) for _ in range(2)]
+
+    def read(lengths, offsets=step.cu, **change):
+        n.upload(np.int32(lengths))
+        cu.upload(np.int32(offsets))
+        fault.zero()
+        for o in out:
+            o.upload(np.full((step.total + 1) * hkv * depth, 7, out_dtype))
+        ctx.kv4_read(cache, table, cu, n, *out, fault=fault, out_dtype=IO[out_dtype], **{**step.shape(), **change})
+        return [o.download(out_dtype, (step.total + 1, hkv * depth)) for o in out], fault.download(np.uint32, (1,))[0]
+
+    good, faulted = read(lens)
+    assert not faulted and all(np.all(np.isfinite(g)) and np.all(g[-1] == 7) for g in good)
+    refused = np.r_[np.zeros(2, bool), np.ones(75, bool), np.zeros(4, bool)]
+    for lengths, change in (((20, 74, 0, 40), {}), ((20, 16 * step.table.shape[1] + 1, 0, 40), {}), ((20, -1, 0, 40), {}),
+                            (lens, dict(max_query=3))):
+        got, faulted = read(lengths, **change)
+        assert faulted == 1
+        for g, whole in zip(got, good):
+            assert np.all(np.isnan(g[refused])) and g[~refused].tobytes() == whole[~refused].tobytes(), (lengths, change)
+    for offsets in ((0, 2, 99, 77, 80), (0, 2, -1, 77, 80)):   # no rows of its own
+        got, faulted = read((20, 90, 0, 40), offsets, max_query=3)
+        assert faulted == 1
+        for g, whole in zip(got, good):
+            assert g[:2].tobytes() == whole[:2].tobytes() and g[77:].tobytes() == whole[77:].tobytes()
+            assert np.all(g[2:77] == 7)
+    free(cache, table, cu, n, fault, *out)
