@@ -27,9 +27,12 @@ template <>
 __device__ inline void st<__half>(__half* p, size_t i, float v) { p[i] = __float2half_rn(v); }
 
 // cos and sin of position * frequency.  The angle and its reduction are in 64 bits: at position 1e6 a
-// 32-bit angle is off by 0.03.  a = n pi/2 + r with |r| <= pi/4 (pi/2 in two parts, so that r keeps its
+// 32-bit angle is off by 0.03.  The product is kept whole, as its rounded value a and what that left: past 2^30 the
+// rounding alone would move the angle by up to 2^-23.  a = n pi/2 + r with |r| <= pi/4 (pi/2 in two parts, so that r keeps its
 // bits for any n a position can give), then both series in 32 bits on r: the first terms left out are
-// r^11/11! < 1.8e-9 and r^12/12! < 1.2e-10, below half a step of the result.
+// r^11/11! < 1.8e-9 and r^12/12! < 1.2e-10, below half a step of the result.  In units of 2^-25: r is off by 1, the
+// sine by its own rounding and 0.3 more, the cosine by 2.5 in all at |r| = pi/4 and less nearer to 1; the amplitude's
+// product rounds by 2 of the result.  Together below 4, 2^-23 of the amplitude.
 // A thread keeps VEC frequencies and walks rows, so that it needs no division and stores 16 bytes at a time (with one
 // element a thread and its place by division 131072 x 64 pairs, 67 MB, took 17.7 us; see krm_rope_tables).
 template <int VEC>
@@ -51,8 +54,8 @@ __global__ __launch_bounds__(kThreads) void rope_tables_kernel(const double* __r
     for (int i = 0; i < VEC; ++i) {
       const double angle = position * f[i];
       const double n = rint(angle * 0.63661977236758134308);
-      const double part = fma(-n, 1.57079632679489661923, angle);
-      const float r = (float)fma(-n, 6.12323399573676603587e-17, part);
+      const double part = fma(-n, 1.57079632679489661923, angle), left = fma(position, f[i], -angle);
+      const float r = (float)(fma(-n, 6.12323399573676603587e-17, part) + left);
       const int quarter = (int)(n - 4.0 * floor(n * 0.25));
       const float r2 = r * r;
       float sn = fmaf(r2, 2.7557319e-6f, -1.9841270e-4f);

@@ -132,3 +132,24 @@ def test_refusals(gpu_ctx):
     ctx.rope_tables(None, None, None, rows=0, pairs=8)
     ctx.rope_rows(None, None, None, None, None, **{**rows, "rows": 0})
     buf.free()
+
+
+@pytest.mark.parametrize("pairs,rows,first,base,amplitude", [
+    (64, 16384, 2**31 - 16384, 1.5, 1.0), (63, 8000, 2**31 - 8000, 1.5, 1.2079), (64, 8000, 2**30, 1.1, 0.75),
+    (32, 20000, 0, 10000.0, 1.0), (64, 8000, 131072, 500000.0, 1.2079)])
+def test_tables_are_off_by_a_step_at_most(gpu_ctx, pairs, rows, first, base, amplitude):
+    """What is promised for |angle| < 2^31, 2^-23 of the amplitude, against angles in 64 bits of mantissa (off by 2^-33
+    there): ones in 53 bits are off by as much as the promise themselves."""
+    if np.finfo(np.longdouble).nmant < 63:
+        pytest.skip("no longer numbers than 64 bits")
+    ctx = gpu_ctx
+    freq, _ = ka.rope_frequencies(2 * pairs, base)
+    bufs = [ctx.upload(freq)] + [ctx.alloc(rows * pairs * 4) for _ in range(2)]
+    ctx.rope_tables(*bufs, rows=rows, pairs=pairs, first=first, amplitude=amplitude)
+    angle = (first + np.arange(rows, dtype=np.longdouble))[:, None] * freq.astype(np.longdouble)
+    amplitude = np.longdouble(np.float32(amplitude))
+    for buf, want in zip(bufs[1:], (np.cos(angle), np.sin(angle))):
+        got = buf.download(np.float32, (rows, pairs))
+        assert np.abs(got - want * amplitude).max() <= 2.0**-23 * amplitude
+    for b in bufs:
+        b.free()
