@@ -89,11 +89,12 @@ __global__ __launch_bounds__(kThreads) void rope_tables_kernel(const double* __r
 // Rows whose pieces of 8 elements are whole and 16-byte aligned: a workgroup has `block_rows` rows (or a part of one
 // row's heads), whose angles it holds in LDS, so that all heads share one trip to the table; a thread has both sides of
 // 8 pairs (interleaved: 4), or 8 elements that are only copied.  What bounds it is memory: 5003 rows of 40 heads of 128
-// fp16 head-major, 105 MB: 22.3 us, 4.7 TB/s (two elements and their angles a thread: 55.9).
+// fp16 head-major, 105 MB: 22.3 us, 4.7 TB/s (two elements and their angles a thread: 55.9).  (x and out may be one
+// buffer, and nothing here tells the compiler otherwise.)
 template <typename XT, bool HALF>
 __global__ __launch_bounds__(kThreads) void rope_pieces_kernel(
-    const XT* __restrict__ x, const int32_t* __restrict__ positions, const float* __restrict__ cos_table,
-    const float* __restrict__ sin_table, XT* __restrict__ out, uint32_t rows, uint32_t heads, RotaryArgs t,
+    const XT* x, const int32_t* __restrict__ positions, const float* __restrict__ cos_table,
+    const float* __restrict__ sin_table, XT* out, uint32_t rows, uint32_t heads, RotaryArgs t,
     uint64_t x_stride, uint64_t out_stride, uint32_t to_head_major, uint32_t block_rows, uint32_t block_heads) {
   extern __shared__ __align__(16) float s_angles[];   // [block_rows][2][R/2]
   const uint32_t pairs = t.rotary_dim / 2, row0 = blockIdx.x * block_rows, head0 = blockIdx.y * block_heads;
@@ -166,8 +167,8 @@ __global__ __launch_bounds__(kThreads) void rope_pieces_kernel(
 
 template <typename XT>
 __global__ __launch_bounds__(kThreads) void rope_rows_kernel(
-    const XT* __restrict__ x, const int32_t* __restrict__ positions, const float* __restrict__ cos_table,
-    const float* __restrict__ sin_table, XT* __restrict__ out, uint32_t rows, uint32_t heads, RotaryArgs t,
+    const XT* x, const int32_t* __restrict__ positions, const float* __restrict__ cos_table,
+    const float* __restrict__ sin_table, XT* out, uint32_t rows, uint32_t heads, RotaryArgs t,
     uint64_t x_stride, uint64_t out_stride, uint32_t to_head_major) {
   // a thread has both elements of a pair (or two elements that are only copied), so that rows may be
   // turned in place
