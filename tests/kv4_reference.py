@@ -185,6 +185,45 @@ class Step:
         return out, reach, top
 
 
+def attention_by_row(step, raw, q, half_scale, window=0, values=np.float64):
+    """(out f64 [total, H, D] of values rounded to the given type; by how much, at most, it may be moved by the errors of
+    f32 scores [total, H, 1]; their size [total, H]; max |v|).
+
+    A score is sum q (step * code + minimum) half_scale^2 from products that are exact or known to 2^-22, so its error is
+    counted against m = sum |q| (step * code + |minimum|) half_scale^2: at most 3 D/16 matrix products and 16 other
+    operations come in a row, each rounds by 2^-23 of what it holds at most: e = (3 D/16 + 16) 2^-23 m, m the row's
+    largest.  Every weight is then off by a factor within exp(+-2 e), and all of them together, normalised, move by
+    exp(2 e) - 1; where one column holds nearly all the weight, by twice what the others can have with their scores 2 e
+    nearer.  An output moves by that times the largest value."""
+    lay, out = step.layout, np.zeros(q.shape, dtype=np.float64)
+    moved, size, top, cu = np.zeros((*q.shape[:2], 1)), np.zeros(q.shape[:2]), 0.0, step.cu
+    share, spans = q.shape[1] // lay.kv_heads, raw.copy()
+    minima = lay.pages(spans)["params"][..., 1]
+    minima[...] = np.abs(minima)
+    for i, n in enumerate(step.rows):
+        if not n:
+            continue
+        c = step.lens[i]
+        ids = step.table[i, :-(-c // lay.page_rows)]
+        k, v = (np.repeat(x[:, :c], share, axis=0) for x in lay.values(raw, ids))
+        span, _ = (np.repeat(x[:, :c], share, axis=0) for x in lay.values(spans, ids))
+        v = v.astype(values).astype(np.float64)
+        x = q[cu[i]:cu[i + 1]].astype(np.float64).transpose(1, 0, 2)
+        far = np.arange(c - n, c)[:, None] - np.arange(c)
+        seen = (far >= 0) & (far < (window or c + 1))
+        s = np.where(seen, np.matmul(x, k.swapaxes(1, 2)) * half_scale ** 2, -np.inf)
+        m = np.where(seen, np.matmul(np.abs(x), span.swapaxes(1, 2)) * half_scale ** 2, 0.0).max(-1, keepdims=True)
+        e, most = (3 * lay.depth / 16 + 16) * 2.0**-23 * m, s.max(-1, keepdims=True)
+        with np.errstate(over="ignore"):
+            p = np.exp(s - most)
+            others = np.exp(np.minimum(0.0, s - most + 2 * e)).sum(-1, keepdims=True) - 1.0
+            moves = np.minimum(np.expm1(2 * e), 2 * others) * np.abs(v).max((1, 2), keepdims=True)
+        rows, top = slice(cu[i], cu[i + 1]), max(top, np.abs(v).max())
+        out[rows] = np.matmul(p / p.sum(-1, keepdims=True), v).transpose(1, 0, 2)
+        moved[rows], size[rows] = moves.transpose(1, 0, 2), m[..., 0].T
+    return out, moved, size, top
+
+
 def pack_all(lay, records, k, v):
     """Codes and parameters of [pages, Hkv, P, D] keys and values into page records."""
     codes, step, minimum = k

@@ -847,3 +847,75 @@ def test_all_rows_of_a_refused_sequence_read_as_nan(gpu_ctx, out_dtype, depth, h
             assert g[:2].tobytes() == whole[:2].tobytes() and g[77:].tobytes() == whole[77:].tobytes()
             assert np.all(g[2:77] == 7)
     free(cache, table, cu, n, fault, *out)
+
+
+def check_by_row(step, raw, a, classes):
+    """Each row against its own error, and the 2-norm of each class of rows against what independent roundings give.
+
+    fp16 rows: values are rounded to fp16 once, which the reference does too, and so is the result; f32 rows: values are
+    known to 2^-22.  Beside what the scores' errors move (attention_by_row), weights are known to 2^-22, exp2 and the scale
+    to as much, and at most 64 + log2(columns) sums come in a row, each rounding by 2^-23.
+    2-norm: the result's rounding is that of the reference's result, 10 % more for classes of a thousand elements; the rest
+    is independent roundings of 2^-25 rms, 8 in a row of a score's size and of as many sums as there are columns, whose
+    sizes add up to sqrt(columns) times their sum's.  (A plane of keys or of weights left out, so that they are rounded to
+    fp16, is 1.15 to 1.9 times that and more.)"""
+    half = a.io == np.float16
+    want, moved, size, top = ref.attention_by_row(step, raw, a.q, a.half_scale, a.window, a.io if half else np.float64)
+    got = a.result().astype(np.float64)
+    span = max(step.lens)
+    most = moved + top * (4 * 2.0**-22 + (64 + np.log2(span)) * 2.0**-23)
+    if half:
+        most = most + 2.0**-11 * (np.abs(want) + most) + 2.0**-25
+    assert np.all(np.isfinite(got))
+    assert np.all(np.abs(got - want) <= most), np.argwhere(np.abs(got - want) > most)[:5]
+    told = 0
+    for name in sorted(set(classes)):
+        mine = np.array([c == name for c in classes])
+        other = 2.0**-22 + 2.0**-25 * (8 * np.sqrt((size[mine] ** 2).mean()) + 16 * np.sqrt(span))
+        norm = np.linalg.norm(want[mine])
+        if other > 0.01:   # (scores that f32 cannot tell apart: the rows' own limits are all that there is)
+            told += np.mean(moved[mine] < 1e-6 * top) > 0.5
+            continue
+        share = other + (1.1 * np.linalg.norm(want[mine].astype(np.float16) - want[mine]) / norm if half else 0.0)
+        told += 1
+        assert np.linalg.norm(got[mine] - want[mine]) <= share * norm, (name, share)
+    assert told == len(set(classes))
+    assert not a.faulted()
+
+
+# Rows and heads for the kernel of few rows, and blocks enough for that of many.
+FEW, MANY = (2, 4, (3, 18), (70, 500)), (2, 32, (260, 9), (300, 120))
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+@pytest.mark.parametrize("depth,group,page", [(64, 32, 16), (128, 64, 128), (128, 128, 32), (256, 32, 64)])
+@pytest.mark.parametrize("rows", ["few", "many"])
+def test_each_row_is_within_its_own_error(gpu_ctx, io, depth, group, page, rows):
+    """Rows of queries of all sizes beside each other, zeros among them, in both kernels."""
+    rng = np.random.default_rng(depth + group + page)
+    hkv, share, n, lens = FEW if rows == "few" else MANY
+    step = ref.Step.make(ref.Layout(hkv, depth, group, page), n, lens, rng)
+    raw = step.random_cache(rng)
+    sizes = (1.0, 1e-3, 300.0, 0.0, 8.0) + ((1e4, 1e-6) if io == np.float16 else (1e4, 1e-30))
+    classes = [sizes[i % len(sizes)] for i in range(step.total)]
+    q = np.clip(rng.normal(size=(step.total, hkv * share, depth)), -4.0, 4.0)   # (fp16 ends at 65504)
+    a = Attention(gpu_ctx, step, raw, q * np.array(classes)[:, None, None], io)
+    a.run()
+    check_by_row(step, raw, a, classes)
+    a.free()
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+@pytest.mark.parametrize("depth,group,page", [(64, 64, 64), (128, 32, 16), (256, 128, 256)])
+@pytest.mark.parametrize("rows", ["few", "many"])
+@pytest.mark.parametrize("spread,window", [(1e-4, 0), (1.0, 90), (30.0, 0)])
+def test_keys_and_values_of_all_sizes_in_both_kernels(gpu_ctx, io, depth, group, page, rows, spread, window):
+    """Steps and minima among fp16's subnormals, and in the hundreds."""
+    rng = np.random.default_rng(depth + group)
+    hkv, share, n, lens = FEW if rows == "few" else MANY
+    step = ref.Step.make(ref.Layout(hkv, depth, group, page), n, lens, rng)
+    raw = step.random_cache(rng, spread)
+    a = Attention(gpu_ctx, step, raw, rng.normal(size=(step.total, hkv * share, depth)), io, window)
+    a.run()
+    check_by_row(step, raw, a, ["all"] * step.total)
+    a.free()
