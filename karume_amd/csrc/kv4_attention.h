@@ -16,6 +16,7 @@ struct Kv4Attention {
   float share_inverse;
   uint32_t least_pairs, most_pairs;   // (row, head) pairs of a sequence and kv head that the launch is for
   float scale;                        // half_scale^2 * log2 e: scores are kept in base 2
+  float fraction;                     // scale / 2^frexp_exp(scale), from 0.5 up to 1
   float* partials;                    // parts of rows, as each kernel lays them out
   uint32_t* tickets;
 };
@@ -92,6 +93,19 @@ __device__ inline half2_t high_codes(uint32_t x) {
 }
 // step * x + sum with a step in fp16 (one mixed instruction).
 __device__ inline float scaled(uint32_t params, float x, float sum) { return fmaf((float)half2_of(params).x, x, sum); }
+
+// Weights are 2^(score - shift).  The shift is the largest score less 10, so that the weights' low parts are no subnormal
+// numbers; past 2^24, where f32 does not hold that difference, it is the score itself.  What has been summed goes by the
+// shift, in the lanes, in LDS and in a row's parts.
+__device__ inline float shift_of(float top) { return fabsf(top) > 0x1p24f ? top : top - 10.0f; }
+// The power of two by which a row of queries is multiplied, so that the largest is in [2^5, 2^6).  (Those so small or
+// large that the scale would leave f32's range with them are not normalised any further.)  f32 rows are multiplied with
+// the scale's fraction too: what is left of the scale is a power of two, with which no product is rounded.
+__device__ inline int normal_power(float most, float scale) {
+  if (!(most > 0.f && most < INFINITY)) return 0;
+  const int of_scale = __builtin_amdgcn_frexp_expf(scale);
+  return max(min(6 - __builtin_amdgcn_frexp_expf(most), min(100, of_scale + 100)), of_scale - 110);
+}
 
 template <int N>
 __device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {

@@ -174,8 +174,10 @@ __device__ inline void join_parts(const DecodeAttention& a, const DecodeWork& w,
   }
 }
 
+// (Three waves a SIMD: LDS has room for three workgroups of four waves of fp16 rows, up to D = 128, and so have 168
+// registers.  With 176 and more, two of them, 32 sequences of 128 to 4096 columns take 37 us, so 33.)
 template <typename XT, int D, int NG, int kWaves>
-__global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
+__global__ __launch_bounds__(kWaves* kWave, kWaves == 4 && D <= 128 && sizeof(XT) == 2 ? 3 : 1) void kv4_decode_kernel(
     const XT* __restrict__ q, const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table,
     const int32_t* __restrict__ cu_rows, const int32_t* __restrict__ lens, XT* __restrict__ out,
     uint32_t* __restrict__ fault, DecodeAttention a) {
@@ -279,10 +281,11 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
   for (int i = 0; i < kStages; ++i)
     if (i < mine) ask(i, i);
 
-  // ---- queries as operands.  x * 2^e has its row's largest magnitude in [2^5, 2^6).  Codes enter the matrix cores
-  // as they are masked out of a word: the fp16 subnormals u 2^-24 and 16 u 2^-24, exact; their queries are x 2^(e+8)
-  // and x 2^(e+4).  A group's sum of products is then 2^(e-16) times its own; steps multiply it in f32, and the
-  // minima meet the group's sum of queries (fp16 hi + lo: 22 bits) in an instruction of their own.
+  // ---- queries as operands.  x * 2^e has its row's largest magnitude in [2^5, 2^6) (f32 rows: times the scale's
+  // fraction, so that their scale is a power of two).  Codes enter the matrix cores as they are masked out of a word: the
+  // fp16 subnormals u 2^-24 and 16 u 2^-24, exact; their queries are x 2^(e+8) and x 2^(e+4).  A group's sum of products
+  // is then 2^(e-16) times its own; steps multiply it in f32, and the minima meet the group's sum of queries (fp16 hi +
+  // lo: 22 bits) in an instruction of their own.
   half8_t qh[kSteps], ql[kF32 ? kSteps : 1], qs_h, qs_l;
   float scale;
   {
@@ -295,18 +298,15 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
         most = fmaxf(most, fabsf(x[st][i]));
       }
     most = quarters_max(most);
-    int e = 0;
-    // (queries so small or large that the scale would leave f32's range with them are not normalised any further)
-    if (most > 0.f && most < INFINITY)
-      e = max(min(6 - __builtin_amdgcn_frexp_expf(most), 100), __builtin_amdgcn_frexp_expf(a.scale) - 110);
-    scale = ldexpf(a.scale, (kF32 ? 2 : 16) - e);
+    const int e = normal_power(most, a.scale);
+    scale = kF32 ? ldexpf(1.0f, __builtin_amdgcn_frexp_expf(a.scale) + 2 - e) : ldexpf(a.scale, 16 - e);
     float sums[NG] = {};
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) {
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float z = ldexpf(x[st][i], e);
+        const float z = kF32 ? ldexpf(x[st][i], e) * a.fraction : ldexpf(x[st][i], e);
         const float y = z * (!kF32 && (i & 2) ? 16.0f : 256.0f);   // elements 2, 3, 6, 7 lie four bits up
         qh[st][i] = (_Float16)y;
         if constexpr (kF32) ql[st][i] = (_Float16)(y - (float)qh[st][i]);
@@ -427,7 +427,14 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
       }
       sc[h] = total;
     }
-    // ---- softmax: lane (m, c) has columns 4 c .. 4 c + 3 of each half
+    // ---- softmax: lane (m, c) has columns 4 c .. 4 c + 3 of each half.  (fp16 rows: all products with the scale are
+    // rounded as the maximum is.  In one mixed operation with the shift, a large one's rounding would be the weight's: up
+    // to 2^1 at 2^24, and more than fp16 has room for from 2^26 on.)
+    if constexpr (!kF32) {
+      sc[0] *= scale;
+      sc[1] *= scale;
+    }
+    const float factor = kF32 ? scale : 1.0f;
     if (edge) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -439,12 +446,12 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
     }
     float here = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                        fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-    here = quarters_max(here) * scale;
-    // The sums are brought to a new maximum where one has grown by more than 2^4; weights are 2^10 times what they
-    // would be, so that their low parts are no subnormal numbers, and at most 2^14.
-    if (__any(here > top + 4.0f)) {
+    here = quarters_max(here) * factor;
+    // The sums are brought to a new maximum where one has grown by more than 2^4: weights, with the 2^10 of their shift,
+    // are at most 2^14.
+    if (__any(here - top > 4.0f)) {   // (not top + 4: past 2^26 it rounds to top + 8)
       const float now = fmaxf(here, top);
-      const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+      const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(shift_of(top) - shift_of(now));
       top = now;
       sum *= keep;
 #pragma unroll
@@ -454,12 +461,12 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
         for (int f = 0; f < kOuts; ++f) acc[i][f] *= keep;
       }
     }
-    const float shift = (top == -INFINITY ? 0.f : top) - 10.0f;
+    const float shift = top == -INFINITY ? 0.f : shift_of(top);
     half8_t ph, pl;
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
-      const float2_t p = {__builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4], scale, -shift)),
-                          __builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4 + 1], scale, -shift))};
+      const float2_t p = {__builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4], factor, -shift)),
+                          __builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4 + 1], factor, -shift))};
       const half2_t hi = rounded2(p);
       sum += p[0] + p[1];
       ph[j] = hi.x;
@@ -579,7 +586,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv4_decode_kernel(
   __syncthreads();   // (every wave is through its ring)
   float* s_acc = reinterpret_cast<float*>(s_ring);
   if (c == 0) {
-    s_max[wave][m] = top;
+    s_max[wave][m] = shift_of(top);
     s_sum[wave][m] = sum;
   }
   if (live) {
@@ -758,7 +765,9 @@ int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_t
   a.window = window;
   a.share = share;
   a.share_inverse = 1.0f / share;
+  int power;
   a.scale = scale;
+  a.fraction = std::frexp(scale, &power);
   a.partials = ptr<float>(workspace);
   a.tickets = ctx->tickets;
   if (plan.many) {

@@ -288,7 +288,7 @@ __device__ __forceinline__ void chunk_piece(
         qh[st] = live ? x : half8_t{};
       }
     } else {
-      // x * 2^e = hi + lo with the row's largest magnitude in [2^5, 2^6)
+      // x * 2^e * fraction = hi + lo, x * 2^e with the row's largest magnitude in [2^5, 2^6)
       float x[kSteps][8], most = 0.f;
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) {
@@ -300,15 +300,14 @@ __device__ __forceinline__ void chunk_piece(
         }
       }
       most = across_halves(most, [](float x, float y) { return fmaxf(x, y); });
-      int e = 0;
-      if (most > 0.f && most < INFINITY)
-        e = max(min(6 - __builtin_amdgcn_frexp_expf(most), 100), __builtin_amdgcn_frexp_expf(scale) - 110);
-      scale = ldexpf(scale, -e);
+      const int e = normal_power(most, scale);
+      scale = ldexpf(1.0f, __builtin_amdgcn_frexp_expf(scale) - e);
 #pragma unroll
       for (int st = 0; st < kSteps; ++st)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float y = ldexpf(x[st][i], e);
+          float y = ldexpf(x[st][i], e) * a.fraction;
+          asm("" : "+v"(y));   // (else the product is rounded to fp16 in one step here and in two there)
           qh[st][i] = (_Float16)y;
           ql[st][i] = (_Float16)(y - (float)qh[st][i]);
         }
@@ -546,15 +545,25 @@ __device__ __forceinline__ void chunk_piece(
       for (int r = 0; r < 16; ++r) here = fmaxf(here, sc[sub][r]);
     here = across_halves(here, [](float x, float y) { return fmaxf(x, y); }) * scale;
     // weights may grow to 2^(4 + 10) before the sums are brought to a new maximum
-    if (__any(here > top + 4.0f)) {
+    if (__any(here - top > 4.0f)) {   // (not top + 4: past 2^26 it rounds to top + 8)
       const float now = fmaxf(here, top);
-      const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - now);
+      const float keep = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(shift_of(top) - shift_of(now));
       top = now;
       sum *= keep;
 #pragma unroll
       for (int o = 0; o < kOuts; ++o) acc[o] *= keep;
     }
-    const float shift = (top == -INFINITY ? 0.f : top) - 10.0f;
+    const float shift = top == -INFINITY ? 0.f : shift_of(top);
+    // fp16 rows: a product's rounding is missing from the mixed operation below, and is the weight's: up to 2^1 at 2^24,
+    // and more than fp16 has room for from 2^26 on.  There all of them are rounded first, as the maximum was.
+    float factor = scale;
+    if constexpr (!kF32) {
+      if (__any(fabsf(top) > 0x1p24f && top > -INFINITY)) {
+#pragma unroll
+        for (int sub = 0; sub < kSubs; ++sub) sc[sub] *= scale;
+        factor = 1.0f;
+      }
+    }
 #pragma unroll
     for (int sub = 0; sub < kSubs; ++sub) {
 #pragma unroll
@@ -562,8 +571,8 @@ __device__ __forceinline__ void chunk_piece(
         half8_t ph, pl;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-          const float2_t p = {__builtin_amdgcn_exp2f(fmaf(sc[sub][8 * ks + j], scale, -shift)),
-                              __builtin_amdgcn_exp2f(fmaf(sc[sub][8 * ks + j + 1], scale, -shift))};
+          const float2_t p = {__builtin_amdgcn_exp2f(fmaf(sc[sub][8 * ks + j], factor, -shift)),
+                              __builtin_amdgcn_exp2f(fmaf(sc[sub][8 * ks + j + 1], factor, -shift))};
           const half2_t hi = rounded2(p);
           sum += p[0] + p[1];
           ph[j] = hi.x;
@@ -629,6 +638,7 @@ __device__ __forceinline__ void chunk_piece(
   }
   if (lost && fault && lane == 0) *fault = 1u;
   sum = across_halves(sum, [](float x, float y) { return x + y; });
+  top = shift_of(top);
 
   // ---- parts: as the lanes hold them, (max, sum) of every lane behind the sums; whoever arrives last joins them in
   // order in the same lanes, its own from registers

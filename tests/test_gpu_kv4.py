@@ -919,3 +919,25 @@ def test_keys_and_values_of_all_sizes_in_both_kernels(gpu_ctx, io, depth, group,
     a.run()
     check_by_row(step, raw, a, ["all"] * step.total)
     a.free()
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+@pytest.mark.parametrize("depth,group,page", [(64, 32, 16), (128, 64, 128), (256, 128, 64)])
+@pytest.mark.parametrize("rows", ["few", "many"])
+def test_scores_past_what_f32_can_tell_apart(gpu_ctx, io, depth, group, page, rows):
+    """Up to f32 queries of 1e33, and fp16 ones of 65504 beside keys of thousands: neighbouring f32 numbers are more than a
+    weight's range apart there, and the largest column still has the weight."""
+    rng = np.random.default_rng(depth + page)
+    hkv, share, n, lens = FEW if rows == "few" else MANY
+    step = ref.Step.make(ref.Layout(hkv, depth, group, page), n, lens, rng)
+    sizes = (1.0, 30.0, 100.0, 300.0, 1e3, 3e3, 16376.0) if io == np.float16 else (1.0, 100.0, 1e3, 1e5, 1e7, 1e20, 2.5e31)
+    for spread, half_scale in ((500.0, 1.0), (1.0, None)):
+        raw = step.random_cache(rng, spread)
+        if half_scale is None and io == np.float32:
+            sizes = tuple(10 * x for x in sizes)
+        classes = [sizes[i % len(sizes)] for i in range(step.total)]
+        q = np.clip(rng.normal(size=(step.total, hkv * share, depth)), -4.0, 4.0) * np.array(classes)[:, None, None]
+        a = Attention(gpu_ctx, step, raw, q, io, half_scale=half_scale)
+        a.run()
+        check_by_row(step, raw, a, classes)
+        a.free()

@@ -78,3 +78,15 @@ def test_rows_of_the_gemv_brought_to_lds_are_built_without_a_norm(kernels):
     staged = [arguments(n) for n in kernels if n.startswith("gemv_i4_kernel<") and arguments(n)[5] == "-1"]
     assert len(staged) == 12
     assert {(a[6], a[7]) for a in staged} == {("false", "false")}
+
+
+def test_paged_attention_keeps_its_state_in_registers(kernels):
+    """And fp16 rows of up to 128 elements leave room for a third workgroup of four waves, as LDS does."""
+    forms = {n: k for n, k in kernels.items() if n.startswith(("kv4_decode_kernel<", "kv4_chunk_kernel<"))}
+    assert len(forms) == 26 + 16
+    for name, kernel in forms.items():
+        assert kernel_resources.scratch(kernel) == 0, name
+        kind = arguments(name)
+        if kind[0] == "__half" and kind[1] != "256" and kind[3:] == ["4"]:
+            assert kernel_resources.registers(kernel) <= 168, name
+            assert 3 * (kernel[".group_segment_fixed_size"] + 4 * 2 * 5120) <= 160 * 1024, name
