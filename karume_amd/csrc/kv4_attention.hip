@@ -45,7 +45,7 @@ struct DecodeAttention : Kv4Attention {
   uint32_t max_splits;     // workgroups that one block's columns are dealt to at most
   uint32_t partial_rows;   // pairs that a part has room for; parts are [unit][split]: sums of all pairs, their (max, sum)
   uint32_t least;          // tiles, at least, of a split
-  float share_of_work;     // of all sequences' tiles, in one workgroup
+  float share_of_work;     // of all sequences' tiles of a kv head, in one workgroup
 };
 struct DecodeWork : Work {
   uint32_t unit, split, nsplit;
@@ -88,8 +88,8 @@ __device__ inline bool find_work(const DecodeAttention& a, DecodeWork& w, uint32
   float work = 0.f;
   if (a.max_splits > 1) {
     for (uint32_t i = tid % kWave; i < a.nseq; i += kWave) {
-      const uint32_t n = min((uint32_t)max(lens[i], 0), a.limits.max_columns);
-      work += (float)((a.window ? min(n, a.window) : n) / kTile + 1);
+      work += kv4_tiles((uint32_t)(cu_rows[i + 1] - cu_rows[i]), lens[i], a.share, a.least_pairs, a.most_pairs, kRows,
+                        a.window, a.limits.max_columns, kTile);
     }
   }
   const int32_t cu1 = cu_rows[w.seq + 1];
@@ -670,7 +670,7 @@ DecodePlan plan_decode(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs) 
   splits = splits > kMostSplits ? kMostSplits : splits;
   splits = splits > most ? most : splits;
   p.max_splits = splits < 1 ? 1 : (uint32_t)splits;   // (with more units than kMostGroups, and so than counters: one)
-  p.share_of_work = (float)s.kv_heads * (float)row_tiles / (many ? kManyGroups : kKv4Groups);
+  p.share_of_work = (float)s.kv_heads / (many ? kManyGroups : kKv4Groups);
   p.bytes = splits > 1 ? (size_t)units * splits * p.partial_rows * (s.depth + 2) * sizeof(float) : 0;
   return p;
 }

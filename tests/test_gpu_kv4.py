@@ -941,3 +941,42 @@ def test_scores_past_what_f32_can_tell_apart(gpu_ctx, io, depth, group, page, ro
         a.run()
         check_by_row(step, raw, a, classes)
         a.free()
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+def test_lengths_that_mean_nothing_change_nothing(gpu_ctx, io):
+    """Entries of a padded batch, whatever their lengths say, take no part in how the others' columns are dealt: the same
+    bits, and as many workgroups for the sequences that have rows."""
+    rng = np.random.default_rng(95)
+    rows, lens = (0, 0, 1, 0, 0, 1, 0, 0), (0, 0, 333, 0, 0, 40000, 0, 0)
+    step = ref.Step.make(ref.Layout(2, 64, 32, 64), rows, lens, rng)
+    a = Attention(gpu_ctx, step, step.random_cache(rng), rng.normal(size=(2, 8, 64)), io)
+    a.run()
+    good = a.result()
+    assert np.all(np.isfinite(good))
+    for other in (40000, 2**31 - 1, -7):
+        a.buf["lens"].upload(np.int32([n if r else other for r, n in zip(rows, lens)]))
+        a.run()
+        assert a.result().tobytes() == good.tobytes() and not a.faulted()
+    a.free()
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+def test_single_rows_are_dealt_by_their_own_lengths_beside_prompts(gpu_ctx, io):
+    """In a step of both kinds, single rows' bits do not hang on how far the prompts beside them have come."""
+    rng = np.random.default_rng(96)
+    lay, heads = ref.Layout(8, 64, 32, 64), 32
+    rows, full = (1, 200, 1, 200, 1), (2500, 2600, 40, 2600, 900)
+    step = ref.Step.make(lay, rows, full, rng)
+    raw, q = step.random_cache(rng), rng.normal(size=(step.total, heads, 64))
+    a, singles, got = Attention(gpu_ctx, step, raw, q, io), [0, 201, 402], []
+    for prompts in (200, 1000, 2600):
+        now = ref.Step(lay, rows, [n if r == 1 else prompts for r, n in zip(rows, full)], step.pages, step.table)
+        a.buf["lens"].upload(np.int32(now.lens))
+        a.run()
+        got.append(a.result()[singles])
+        want, reach, top = now.attention(raw, a.q, a.half_scale)
+        assert np.abs(a.result() - want).max() <= tolerance(io, reach, top, 2600)[0]
+        assert got[-1].tobytes() == got[0].tobytes()
+    assert not a.faulted()
+    a.free()
