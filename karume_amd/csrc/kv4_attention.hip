@@ -573,9 +573,8 @@ __global__ __launch_bounds__(kWaves* kWave, kWaves == 4 && D <= 128 && sizeof(XT
   };
 
   for (int32_t i = 0; i < mine; ++i) {
-    const int32_t behind = min(mine - 1 - i, (int32_t)kStages - 1);   // tiles asked for behind this one
-    if (behind >= 2) wait_vm<2 * S::kLoads>();
-    else if (behind == 1) wait_vm<S::kLoads>();
+    static_assert(kStages == 2, "one tile asked for behind this one, or none");
+    if (i + 1 < mine) wait_vm<S::kLoads>();
     else wait_vm<0>();
     consume(i, (uint32_t)i % kStages, i + kStages < mine);
   }
