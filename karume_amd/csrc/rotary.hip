@@ -1,6 +1,7 @@
 // Rotary positions beyond the half-split whole-head form: tables made on the device for any set of
 // frequencies, and the rotation of interleaved or half-split pairs in part of each head.
 #include "kv4_plan.h"
+#include "i4_codes.h"
 #include "krm_internal.h"
 #include "rotary.h"
 #include "rows8.h"
@@ -13,26 +14,13 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T>
-__device__ inline float ld(const T* p, size_t i);
-template <>
-__device__ inline float ld<float>(const float* p, size_t i) { return p[i]; }
-template <>
-__device__ inline float ld<__half>(const __half* p, size_t i) { return __half2float(p[i]); }
-template <typename T>
-__device__ inline void st(T* p, size_t i, float v);
-template <>
-__device__ inline void st<float>(float* p, size_t i, float v) { p[i] = v; }
-template <>
-__device__ inline void st<__half>(__half* p, size_t i, float v) { p[i] = __float2half_rn(v); }
-
-// cos and sin of position * frequency.  The angle and its reduction are in 64 bits: at position 1e6 a
-// 32-bit angle is off by 0.03.  The product is kept whole, as its rounded value a and what that left: past 2^30 the
-// rounding alone would move the angle by up to 2^-23.  a = n pi/2 + r with |r| <= pi/4 (pi/2 in two parts, so that r keeps its
-// bits for any n a position can give), then both series in 32 bits on r: the first terms left out are
-// r^11/11! < 1.8e-9 and r^12/12! < 1.2e-10, below half a step of the result.  In units of 2^-25: r is off by 1, the
-// sine by its own rounding and 0.3 more, the cosine by 2.5 in all at |r| = pi/4 and less nearer to 1; the amplitude's
-// product rounds by 2 of the result.  Together below 4, 2^-23 of the amplitude.
+// cos and sin of position * frequency.  The angle and its reduction are in 64 bits: at position 1e6 a 32-bit angle is off
+// by 0.03.  The product is kept whole, as its rounded value a and what that left: past 2^30 the rounding alone would move
+// the angle by up to 2^-23.  a = n pi/2 + r with |r| <= pi/4 (pi/2 in two parts, so that r keeps its bits for any n a
+// position can give), then both series in 32 bits on r: the first terms left out are r^11/11! < 1.8e-9 and r^12/12! <
+// 1.2e-10, below half a step of the result.  In units of 2^-25: r is off by 1, the sine by its own rounding and 0.3 more,
+// the cosine by 2.5 in all at |r| = pi/4 and less nearer to 1; the amplitude's product rounds by 2 of the result.
+// Together below 4, 2^-23 of the amplitude.
 // A thread keeps VEC frequencies and walks rows, so that it needs no division and stores 16 bytes at a time (with one
 // element a thread and its place by division 131072 x 64 pairs, 67 MB, took 17.7 us; see krm_rope_tables).
 template <int VEC>
@@ -192,8 +180,8 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(
       d0 = 2 * j;
       d1 = 2 * j + 1;
     }
-    const float a = ld<XT>(x, src + d0);
-    const float b = d1 < t.head_dim ? ld<XT>(x, src + d1) : 0.f;
+    const float a = to_f32<XT>(x[src + d0]);
+    const float b = d1 < t.head_dim ? to_f32<XT>(x[src + d1]) : 0.f;
     float ta = a, tb = b;
     if (j < pairs) {
       const int32_t pos = positions[row];
@@ -204,8 +192,8 @@ __global__ __launch_bounds__(kThreads) void rope_rows_kernel(
         turn_pair(a, b, cos_table[at], sin_table[at], ta, tb);
       }
     }
-    st<XT>(out, dst + d0, ta);
-    if (d1 < t.head_dim) st<XT>(out, dst + d1, tb);
+    out[dst + d0] = from_f32<XT>(ta);
+    if (d1 < t.head_dim) out[dst + d1] = from_f32<XT>(tb);
   }
 }
 
