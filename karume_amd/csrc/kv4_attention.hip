@@ -678,10 +678,13 @@ DecodePlan plan_decode(const Kv4Shape& s, uint32_t max_columns, uint64_t pairs) 
 // the CUs, or twice over long columns (us, decode / chunk, 1024 and 8192 columns; 8 kv heads x 4, D 128, fp16: 128 rows
 // 17 / 40 and 71 / 76; 256 rows 29 / 40 and 123 / 83, of 2048 columns 46 / 47; 512 rows 46 / 36 and 229 / 118; eight
 // sequences of 64 rows 53 / 38 and 234 / 121; 4 kv heads x 4, D 256: 512 rows 42 / 52 and 233 / 237, eight sequences of
-// 128 86 / 73 and 464 / 441; eight of 128 rows of 128 columns, D 128 42 / 21, D 256 33 / 28).
+// 128 86 / 73 and 464 / 441; eight of 128 rows of 128 columns, D 128 42 / 21, D 256 33 / 28).  Sequences of up to 64 pairs
+// fill a quarter of its workgroup, however many they are (64 sequences of 40 pairs, D 128, 128, 1024 and 4096 columns: 19 /
+// 26, 54 / 94, 173 / 328; of 64 pairs 23 / 27, 70 / 95, 227 / 329; of up to 72, 32 of them, 14 / 23, 39 / 71, 116 / 172; of
+// up to 128 23 / 22, 65 / 68, 201 / 171; D 256, 64 of 64 pairs 37 / 26, 106 / 115, 313 / 418).
 // A step may hold both kinds: sequences of up to kFewPairs pairs then stay with the decode kernel, in a launch of its
 // own.
-constexpr uint64_t kFewPairs = 32;
+constexpr uint64_t kFewPairs = 32, kManyPairs = 64;
 constexpr uint32_t kLongColumns = 2048;
 struct AttentionPlan {
   bool few = true, many = false;   // which launches there are
@@ -693,7 +696,7 @@ AttentionPlan plan_attention(const Kv4Shape& s, uint32_t max_columns) {
   const uint32_t rows = kv4_rows(s.max_query, s.total_rows);
   const uint64_t pairs = (uint64_t)rows * (s.heads / s.kv_heads);
   const uint64_t blocks = (uint64_t)s.nseq * s.kv_heads * ((pairs + kRows - 1) / kRows);
-  p.many = pairs > kFewPairs &&
+  p.many = pairs > kManyPairs &&
            blocks >= (s.depth < 256 && max_columns >= kLongColumns ? 2u : 4u) * kKv4Groups;
   p.few = !p.many || (s.nseq > 1 && s.total_rows < (uint64_t)s.nseq * rows);
   if (p.few) p.decode = plan_decode(s, max_columns, p.many ? kFewPairs : pairs);

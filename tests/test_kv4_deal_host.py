@@ -6,7 +6,7 @@ import subprocess
 
 import pytest
 
-from karume_amd import build
+from karume_amd import _ffi, build
 
 SHIM = """
 #include "kv4_plan.h"
@@ -53,3 +53,15 @@ def test_the_other_launch_s_sequences_count_nothing(tiles, rows, least, most, co
 
 def test_a_refused_sequence_counts_within_the_limits(tiles):
     assert tiles(1, 2**31 - 1) == 157 and tiles(1, -5) == 1
+
+
+@pytest.mark.parametrize("depth", [64, 128, 256])
+@pytest.mark.parametrize("nseq,rows,share", [(64, 5, 8), (128, 8, 8), (256, 16, 4), (512, 64, 1)])
+def test_many_sequences_of_up_to_64_pairs_have_blocks_of_16(depth, nseq, rows, share):
+    """They need no workspace then: there are workgroups enough without a split, and the kernel for many rows, which has
+    one whatever the step is, would use a quarter of its rows."""
+    lib, size = _ffi.load(), C.c_size_t()
+    assert lib.krm_kv4_attention_workspace(nseq, rows, 4096, nseq * rows, 8 * share, 8, depth, 0, 0, C.byref(size)) == 0
+    assert size.value == 0
+    assert lib.krm_kv4_attention_workspace(nseq, 4 * rows, 4096, nseq * 4 * rows, 8 * share, 8, depth, 0, 0, C.byref(size)) == 0
+    assert size.value > 0
