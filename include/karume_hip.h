@@ -570,7 +570,7 @@ int32_t krm_rope_rows(krm_ctx* ctx, krm_buf x, krm_buf positions_i32, krm_buf co
  * Sequences of a batch grow page by page: `cache` is `pages` pages of krm_kv4_page_bytes each (one such
  * buffer a layer, 16-byte aligned), column c of sequence i lies in row c % page_rows of page
  * page_table[i, c / page_rows] (int32 [nseq, table_stride] on the device; entries past a sequence's
- * columns are not read).  Pages may be shared by sequences that only read them.
+ * columns may be anything).  Pages may be shared by sequences that only read them.
  * Depth is 64, 128 or 256; a group of 32, 64 or 128 elements of a head's row (at most the depth) is held
  * as 4-bit codes and an fp16 (step, minimum):
  *   minimum = largest fp16 <= min(x) (+0 for a zero),

@@ -3,9 +3,12 @@
 // Row r of a sequence stands at column p = len - rows + r and sees columns max(0, p - window + 1) .. p:
 //   out = sum_c softmax_c(scale^2 q . k_c) v_c,   k_c = step * code + minimum, v_c alike.
 // This is the kernel for few rows.  A long sequence is bound by memory (131000 columns, 8 kv heads x 4, D 128, groups of
-// 64, 151 MB: 38 us, 4.0 TB/s), ragged batches by the vector instructions that turn codes (about 330 a tile of 32 columns
-// beside 28 matrix ones) and by unequal pieces (32 sequences of 128 to 4096 columns 36.5 us), short ones by the chain
-// lengths, pages, columns, waves' join (500 columns 8.8 us).
+// 64, 151 MB: 38 us, 4.0 TB/s), ragged batches by the vector instructions that turn codes (about 340 a tile of 32 columns
+// beside 28 matrix ones) and by unequal pieces (32 sequences of 128 to 4096 columns 33 us), short ones by the chain
+// lengths, pages, columns, waves' join (500 columns 9.1 us).
+// What is rounded to fewer than 22 bits: fp16 rows' values, to fp16, once.  Their products with the weights' two parts are
+// half of the matrix instructions, and a low part of the values would make them half as many again.  The result, fp16
+// itself, is off from 64 bits by 2.8e-4 (2-norm); of exact values it would be by 2.0e-4.
 #include "kv4_attention.h"
 #include "lds_stream.h"
 #include "rows8.h"
@@ -645,9 +648,9 @@ struct DecodePlan {
 // Waves of a workgroup.  With eight a CU has one workgroup, two waves a SIMD, and as few parts to join as can be.  With
 // four it has two or three, and one's first loads and last sums run beside another's tiles, which pays where many
 // sequences' pieces are unequal or more than the CUs (us, eight / four, 8 kv heads x 4, D 128, fp16: 16 sequences of
-// 128 to 4096 columns 26 / 22, 32 of them 40 / 36, 128 of 300 29 / 22, 128 of 2000 90 / 76; but 16 of 4000 27 / 29,
-// 131000 columns 40 / 54), or where all pieces together are few (one sequence of 700 or 4096 columns 10.6 / 9.5, 11.1 /
-// 9.9).
+// 128 to 4096 columns 26.3 / 23.7, 32 of them 43 / 33, 128 of 300 28 / 18, 128 of 2000 90 / 67, 16 of 4000 31 / 26; but
+// 131000 columns 38.0 / 47.7, 128 rows of 8192 68 / 84), or where all pieces together are few (one sequence of 700 or
+// 4096 columns 10.6 / 9.2, 11.0 / 9.6).
 constexpr uint32_t kFewWaves = 4, kManyWaves = 8;
 constexpr uint32_t kManyUnits = 96, kManyGroups = kKv4Groups * 3 / 2;
 constexpr uint32_t kMostGroups = 2048;   // in a grid, those without a split among them

@@ -188,9 +188,9 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(
   }
 }
 
-// The last rows of each sequence as the values they stand for: step * code is exact in f32 and the sum is
-// rounded once.  Rows on a page that is none of the cache's, and all of a refused sequence, are NaN.  (8100 rows of 2 x 8 heads of 128 to fp16, 43 MB:
-// 12.4 us.)
+// The last rows of each sequence as the values they stand for: step * code is exact in f32 and the sum is rounded once.
+// Rows on a page that is none of the cache's, and all of a refused sequence, are NaN.  (8100 rows of 2 x 8 heads of 128 to
+// fp16, 43 MB: 12.4 us.)
 template <typename OT, int D>
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(
     const uint8_t* __restrict__ cache, const int32_t* __restrict__ page_table, const int32_t* __restrict__ cu_rows,

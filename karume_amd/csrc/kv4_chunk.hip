@@ -6,7 +6,7 @@
 // tiles by turns; every wave then multiplies its rows with all of it.
 //   keys    k = hi + lo, two fp16 planes (22 bits): the products with fp16 queries are off by no more than f32 sums;
 //           f32 queries are hi + lo too
-//   weights p = hi + lo; values rounded to fp16 once (f32 rows: hi + lo)
+//   weights p = hi + lo; values rounded to fp16 once (f32 rows: hi + lo), as kv4_attention.hip does and for its reason
 // Both hi and lo planes double the products: four prompts of 512 rows behind 200 to 4100 columns (8 kv heads x 4, D 128,
 // fp16; 80 GFLOP without them) take 170 to 180 us, 143 of them at the rate of a large product; matrix and vector
 // instructions each have about half of a SIMD's time and hardly overlap.
