@@ -119,7 +119,8 @@ __device__ inline bool find_work(const DecodeAttention& a, DecodeWork& w, uint32
   w.nsplit = 1;
   if (a.max_splits > 1) {
     // the step's tiles, as far as they go by the lengths, are dealt evenly to the workgroups that fit the machine
-    per = max((uint32_t)(wave_sum(work) * a.share_of_work), a.least) + kWaves - 1;
+    // (sequences that share rows, which no valid offsets give, could add up to any number)
+    per = max((uint32_t)fminf(wave_sum(work) * a.share_of_work, 0x1p30f), a.least) + kWaves - 1;
     per = max(per / kWaves * kWaves, (tiles + a.max_splits - 1) / a.max_splits);
     w.nsplit = (tiles + per - 1) / per;
     if (w.split >= w.nsplit) return false;
@@ -754,7 +755,7 @@ int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_t
   const AttentionPlan plan = plan_attention(shape, max_columns);
   const uint32_t share = heads / kv_heads;
   const uint64_t blocks = (uint64_t)nseq * kv_heads * ((uint64_t)kv4_rows(max_query, total_rows) * share / kRows + 1);
-  KRM_REQUIRE(ctx, blocks <= 0x7fffffu && (uint64_t)kv4_rows(max_query, total_rows) * share <= 1u << 24,
+  KRM_REQUIRE(ctx, blocks <= 0x7fffffu && (uint64_t)kv4_rows(max_query, total_rows) * share <= kKv4MostPairs,
               "krm_kv4_attention: %u sequences of %u rows of %u heads are more than one call takes", nseq, max_query, heads);
   if (plan.bytes) {
     KRM_REQUIRE(ctx, workspace && workspace_bytes >= plan.bytes, "krm_kv4_attention: workspace of %zu bytes, %zu needed",

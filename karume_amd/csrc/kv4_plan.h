@@ -30,6 +30,9 @@ namespace krm {
 // step * 15 + minimum with both rounded outwards, then stay finite in fp16.
 constexpr float kKv4Limit = 32640.0f;
 
+// (row, head) pairs of a sequence and kv head that a call takes.
+constexpr uint32_t kKv4MostPairs = 1u << 24;
+
 struct Kv4Layout {
   uint32_t depth, group, page_rows, kv_heads;
 
@@ -80,12 +83,14 @@ KRM_HD inline Kv4Sequence kv4_sequence(int32_t cu0, int32_t cu1, int32_t len, co
 
 // Tiles of `tile` columns, about, that one kv head of a sequence has in a launch for sequences of least_pairs to
 // most_pairs (row, head) pairs, all blocks of block_pairs of them together: none for an entry without rows (whatever its
-// length says) or one of the other launch.  (A refused sequence counts with what its words say, within max_columns.)
+// length says) or one of the other launch, or more pairs than any call takes, as descending offsets give.  (A refused
+// sequence counts with what else its words say, within max_columns.)
 KRM_HD inline float kv4_tiles(uint32_t rows, int32_t len, uint32_t share, uint32_t least_pairs, uint32_t most_pairs,
                               uint32_t block_pairs, uint32_t window, uint32_t max_columns, uint32_t tile) {
   const uint32_t pairs = rows * share, most = window && window < max_columns ? window : max_columns;
   const uint32_t n = len < 0 ? 0 : (uint32_t)len < most ? (uint32_t)len : most;
-  const uint32_t blocks = pairs < least_pairs || pairs > most_pairs ? 0 : (pairs + block_pairs - 1) / block_pairs;
+  const uint32_t past = most_pairs < kKv4MostPairs ? most_pairs : kKv4MostPairs;
+  const uint32_t blocks = pairs < least_pairs || pairs > past ? 0 : (pairs + block_pairs - 1) / block_pairs;
   return (float)(n / tile + 1) * (float)blocks;
 }
 

@@ -980,3 +980,21 @@ def test_single_rows_are_dealt_by_their_own_lengths_beside_prompts(gpu_ctx, io):
         assert got[-1].tobytes() == got[0].tobytes()
     assert not a.faulted()
     a.free()
+
+
+@pytest.mark.parametrize("io", [np.float16, np.float32])
+@pytest.mark.parametrize("cu", [(0, 1, 30, 5), (0, 1, 30, -2**31), (0, 1, 30, 2**31 - 1)])
+def test_offsets_that_are_none_leave_the_others_their_rows(gpu_ctx, io, cu):
+    """With limits as large as they may be: what the words of such an entry multiply to is no measure of work."""
+    rng = np.random.default_rng(97)
+    step = ref.Step.make(ref.Layout(2, 64, 32, 16), (1, 29, 0), (1500, 40, 0), rng)
+    a = Attention(gpu_ctx, step, step.random_cache(rng), rng.normal(size=(30, 8, 64)), io, max_columns=2**31 - 1)
+    a.run()
+    good = a.result()
+    assert np.all(np.isfinite(good)) and not a.faulted()
+    a.buf["cu"].upload(np.int32(cu))
+    a.buf["lens"].upload(np.int32((1500, 40, 2**31 - 1)))
+    a.out.upload(np.full(a.out.nbytes // np.dtype(io).itemsize, 77, io))
+    a.run()
+    assert a.result().tobytes() == good.tobytes() and a.faulted()
+    a.free()

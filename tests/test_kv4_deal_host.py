@@ -65,3 +65,8 @@ def test_many_sequences_of_up_to_64_pairs_have_blocks_of_16(depth, nseq, rows, s
     assert size.value == 0
     assert lib.krm_kv4_attention_workspace(nseq, 4 * rows, 4096, nseq * 4 * rows, 8 * share, 8, depth, 0, 0, C.byref(size)) == 0
     assert size.value > 0
+
+
+@pytest.mark.parametrize("rows", [-1, -10, -2**30, -2**31, 2**22 + 1, 2**31 - 1])
+def test_rows_that_no_call_takes_count_nothing(tiles, rows):
+    assert tiles(rows & 0xffffffff, 5000) == 0
