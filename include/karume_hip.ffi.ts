@@ -275,6 +275,39 @@ export const KARUME_HIP_SYMBOLS = {
     ],
     result: "i32",
   },
+  krm_quantize_mx4: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u32", "u32", "u64", "i32", "i32"
+    ],
+    result: "i32",
+  },
+  krm_dequant_mx4: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u32", "u32", "i32"
+    ],
+    result: "i32",
+  },
+  krm_linear_mx4: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u32", "u32", "u32",
+      "i32", "i32"
+    ],
+    result: "i32",
+  },
+  krm_linear_mx4_fused: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u32", "u32",
+      "u32", "u64", "i32", "i32", "i32", "i32"
+    ],
+    result: "i32",
+  },
+  krm_block_norm: {
+    parameters: [
+      "pointer", "u64", "u64", "u64", "u64", "u64", "u64", "u64", "u32", "u32", "u32",
+      "i32", "f32", "f32", "f32", "i32", "i32"
+    ],
+    result: "i32",
+  },
 } as const;
 
 export type KarumeHipLibrary = Deno.DynamicLibrary<typeof KARUME_HIP_SYMBOLS>;

@@ -637,6 +637,68 @@ int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_t
                           uint32_t window, float half_scale, int32_t io_dtype, krm_buf workspace,
                           size_t workspace_bytes);
 
+/* ---- microscaled 4-bit floating point (no counterpart in the reference, whose 4-bit weights are
+ *      integers with a float scale a group: packages/runtime/src/format/i4.ts:63-118) ---------------
+ * A row of k elements (k a multiple of 32) is k/2 bytes of codes and k/32 scale bytes.  A code is an e2m1
+ * number (sign, two bits of exponent, one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6), element 2j in the low
+ * nibble of byte j; scale byte E of 32 elements stands for 2^(E - 127), 255 for NaN.  Rows are packed:
+ * codes [rows, k/2] (16-byte aligned), scales [rows, k/32] (any address).
+ * krm_quantize_mx4: with a = the largest magnitude of a block and 2^p <= a < 2^(p+1)
+ *   E = max(p + 125, 0)         KRM_MX4_FLOOR: a comes to stand in [4, 8), above 6 is clipped
+ *                               KRM_MX4_CEIL: one more where a > 1.5 * 2^p, so that nothing is clipped
+ *   code = x / 2^(E - 127) rounded half to even, clipped at 6 (a negative that rounds to zero is -0)
+ * A block that holds an infinity or a NaN has E = 255 and codes 0; one of zeros E = 0.  x rows (f32 or
+ * fp16, 16-byte aligned) are x_stride elements apart.
+ * krm_dequant_mx4: the values back, f32 exact or rounded to fp16 once (past either type's range:
+ * infinite); NaN where E = 255. */
+#define KRM_MX4_FLOOR 0
+#define KRM_MX4_CEIL 1
+int32_t krm_quantize_mx4(krm_ctx* ctx, krm_buf x, krm_buf codes, krm_buf scales, uint32_t rows,
+                         uint32_t dim, uint64_t x_stride, int32_t x_dtype, int32_t scale_rule);
+int32_t krm_dequant_mx4(krm_ctx* ctx, krm_buf codes, krm_buf scales, krm_buf out, uint32_t rows,
+                        uint32_t dim, int32_t out_dtype);
+/* `linear` over rows in that format (the op of krm_linear_i4, packages/runtime/src/kernels/gemm.ts:115,
+ * 315-327, on the matrix cores' own 4-bit products):
+ *   s[m, n] = sum_k x[m, k] * w[n, k] + bias[n]      products exact, sums f32
+ *   out     = s + residual, or with KRM_EPILOGUE_SILU_PAIRS (rows (2i, 2i+1) of w = (gate_i, up_i), n even,
+ *             n_out = n / 2) silu(gate) * up + residual, rounded to out_dtype once
+ *   xq, xs  [m, k] codes and scales        w, w_scales  [n, k]
+ *   bias    [n] f32 or 0                   residual  [m, n_out] out_dtype or 0; may be out
+ * A sum whose terms (with both scales) stay in f32's normal range is of f32 class; terms below it may be
+ * lost.  Results depend on the shape alone; a row may have other last bits beside other rows.
+ * krm_linear_mx4_fused: krm_quantize_mx4 of x [m, k] (f32 or fp16, rows x_stride elements apart, 16-byte
+ * aligned) and the product behind one call, the same result bit for bit.  Few rows are quantised inside the
+ * product's launch; every other shape goes through xq [m, k/2] and xs [m, k/32], which must then be given
+ * (a call without them is refused where it needs them). */
+int32_t krm_linear_mx4(krm_ctx* ctx, krm_buf xq, krm_buf xs, krm_buf w, krm_buf w_scales,
+                       krm_buf bias_f32, krm_buf residual, krm_buf out, uint32_t m, uint32_t n,
+                       uint32_t k, int32_t out_dtype, int32_t epilogue);
+int32_t krm_linear_mx4_fused(krm_ctx* ctx, krm_buf x, krm_buf xq, krm_buf xs, krm_buf w,
+                             krm_buf w_scales, krm_buf bias_f32, krm_buf residual, krm_buf out,
+                             uint32_t m, uint32_t n, uint32_t k, uint64_t x_stride, int32_t x_dtype,
+                             int32_t out_dtype, int32_t scale_rule, int32_t epilogue);
+
+/* ---- between two blocks of a layer -----------------------------------------------------------------
+ * The norm behind a block, its gate, the scaled residual sum and the norm in front of the next block in one
+ * pass (krm_rms_norm, krm_add and krm_rms_norm with their scales; packages/runtime/src/kernels/
+ * rms-norm.ts:35-91, packages/runtime/src/codegen/elementwise.ts):
+ *   t        = y * rsqrt(mean(y^2) + eps) * post_weight       (post_weight 0: t = y)
+ *   t        = t * gate[row / gate_span]                      (KRM_GATE_SIGMOID: its logistic; gate 0: none;
+ *                                                              gate_span 0: one row of gates for all rows)
+ *   s        = residual_scale * residual + block_scale * t    (residual 0: the block alone)
+ *   sum_out  = s                                              (0: not wanted)
+ *   norm_out = s * rsqrt(mean(s^2) + eps) * pre_weight        (both 0: not wanted)
+ * y, residual, sum_out [rows, dim] and gate [ceil(rows / gate_span), dim] are io_dtype, norm_out is
+ * norm_dtype (io_dtype, or KRM_F16 beside f32), weights f32.  f32 arithmetic; nothing is rounded between the
+ * steps (norm_out follows s before it is rounded to sum_out).  sum_out and norm_out may each be y or
+ * residual (norm_out where its type is theirs); other overlaps are not allowed.  dim is at most 16384. */
+#define KRM_GATE_PLAIN 0
+#define KRM_GATE_SIGMOID 1
+int32_t krm_block_norm(krm_ctx* ctx, krm_buf y, krm_buf post_weight_f32, krm_buf gate,
+                       krm_buf residual, krm_buf pre_weight_f32, krm_buf sum_out, krm_buf norm_out,
+                       uint32_t rows, uint32_t dim, uint32_t gate_span, int32_t gate_kind, float eps,
+                       float block_scale, float residual_scale, int32_t io_dtype, int32_t norm_dtype);
+
 /* ==== DIAGNOSTICS ============================================================================
  * Not ops of the runtime: measurement probes that bench.py uses to state what a launch and a
  * read of a given size cost on this machine.  A host binds them only if it wants those floors

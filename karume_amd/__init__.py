@@ -9,8 +9,9 @@ from .format_i4 import I4Error, check_int4, group_scale_shape, pack_int4
 from .format_model import (ContainerError, IrError, KarumeModel, PackedInt4, SafetensorsError,
                            i4_resident_initializers, open_model, packed_int4,
                            parse_safetensors, tensor_bytes)
+from .format_mx4 import Mx4Error, pack_mx4
 from .runtime import (COMPUTE_F16, COMPUTE_F32, EPILOGUE_NONE, EPILOGUE_SILU_PAIRS, F16, F32,
-                      PROBE_EMPTY, PROBE_READ, ROPE_HALF, ROPE_INTERLEAVED, DeviceBuffer,
+                      GATE_PLAIN, GATE_SIGMOID, MX4_CEIL, MX4_FLOOR, PROBE_EMPTY, PROBE_READ, ROPE_HALF, ROPE_INTERLEAVED, DeviceBuffer,
                       ExecutionError, GpuContext, GpuDeviceLostError, GpuEvent, GpuGraph, GpuOutOfMemoryError,
                       GpuValidationError, KarumeError, acquire_gpu, dtype_code, version)
 
@@ -27,6 +28,7 @@ __all__ = [
     "ContainerError", "IrError", "KarumeModel", "PackedInt4", "SafetensorsError",
     "i4_resident_initializers", "open_model", "packed_int4", "parse_safetensors", "tensor_bytes",
     "COMPUTE_F16", "COMPUTE_F32", "EPILOGUE_NONE", "EPILOGUE_SILU_PAIRS", "F16", "F32",
+    "Mx4Error", "pack_mx4", "GATE_PLAIN", "GATE_SIGMOID", "MX4_CEIL", "MX4_FLOOR",
     "PROBE_EMPTY", "PROBE_READ", "ROPE_HALF", "ROPE_INTERLEAVED", "rope_frequencies", "DeviceBuffer", "ExecutionError", "GpuContext",
     "GpuDeviceLostError", "GpuEvent", "GpuGraph", "GpuOutOfMemoryError", "GpuValidationError", "KarumeError",
     "acquire_gpu", "dtype_code", "version",

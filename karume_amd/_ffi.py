@@ -123,6 +123,14 @@ PROTOTYPES = {
     "krm_kv4_attention": (i32, [c_ctx, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, u32, u32,
                                 u32, u32, u32, u32, u32, u32, u32, u32, u32, u32, C.c_float, i32,
                                 c_buf, size_t]),
+    "krm_quantize_mx4": (i32, [c_ctx, c_buf, c_buf, c_buf, u32, u32, u64, i32, i32]),
+    "krm_dequant_mx4": (i32, [c_ctx, c_buf, c_buf, c_buf, u32, u32, i32]),
+    "krm_linear_mx4": (i32, [c_ctx, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, u32, u32, u32,
+                             i32, i32]),
+    "krm_linear_mx4_fused": (i32, [c_ctx, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf,
+                                   u32, u32, u32, u64, i32, i32, i32, i32]),
+    "krm_block_norm": (i32, [c_ctx, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, c_buf, u32, u32, u32,
+                             i32, C.c_float, C.c_float, C.c_float, i32, i32]),
 }
 
 _lib = None

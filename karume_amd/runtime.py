@@ -25,6 +25,8 @@ EPILOGUE_NONE = 0
 CHUNK_OUT_ROW_MAJOR, CHUNK_APPEND, CHUNK_OUT_F16 = 1, 2, 4
 EPILOGUE_SILU_PAIRS = 1
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+MX4_FLOOR, MX4_CEIL = 0, 1
+GATE_PLAIN, GATE_SIGMOID = 0, 1
 
 _NP_DTYPE_CODE = {np.dtype(np.float32): F32, np.dtype(np.float16): F16}
 
@@ -720,6 +722,59 @@ class GpuContext:
             _addr(out), _addr(fault), nseq, max_query, max_columns, total_rows, heads, kv_heads,
             depth, group, page_rows, pages, table_stride, window, float(half_scale), io_dtype,
             _addr(workspace), workspace_bytes))
+
+    # -- microscaled 4-bit floating point --------------------------------------------------------------
+    def quantize_mx4(self, x: BufferLike, codes: BufferLike, scales: BufferLike, *, rows: int,
+                     dim: int, x_stride: Optional[int] = None, x_dtype: int = F32,
+                     scale_rule: int = MX4_FLOOR) -> None:
+        """Rows of floats (x_stride elements apart, default packed) to blocks of 32 e2m1 codes with a
+        scale byte each: codes [rows, dim / 2], scales [rows, dim / 32]."""
+        self._check(self._lib.krm_quantize_mx4(
+            self._handle, _addr(x), _addr(codes), _addr(scales), rows, dim,
+            dim if x_stride is None else x_stride, x_dtype, scale_rule))
+
+    def dequant_mx4(self, codes: BufferLike, scales: BufferLike, out: BufferLike, *, rows: int,
+                    dim: int, out_dtype: int = F32) -> None:
+        """The values that such rows stand for."""
+        self._check(self._lib.krm_dequant_mx4(self._handle, _addr(codes), _addr(scales), _addr(out),
+                                              rows, dim, out_dtype))
+
+    def linear_mx4(self, xq: BufferLike, xs: BufferLike, w: BufferLike, w_scales: BufferLike,
+                   out: BufferLike, m: int, n: int, k: int, *, bias: BufferLike = None,
+                   residual: BufferLike = None, out_dtype: int = F32,
+                   epilogue: int = EPILOGUE_NONE) -> None:
+        """out [m, n] = x w^T + bias (+ residual) of rows in that format; EPILOGUE_SILU_PAIRS takes rows
+        (2i, 2i + 1) of w as (gate, up) and writes [m, n / 2]."""
+        self._check(self._lib.krm_linear_mx4(
+            self._handle, _addr(xq), _addr(xs), _addr(w), _addr(w_scales), _addr(bias),
+            _addr(residual), _addr(out), m, n, k, out_dtype, epilogue))
+
+    def linear_mx4_fused(self, x: BufferLike, w: BufferLike, w_scales: BufferLike, out: BufferLike,
+                         m: int, n: int, k: int, *, xq: BufferLike = None, xs: BufferLike = None,
+                         bias: BufferLike = None, residual: BufferLike = None,
+                         x_stride: Optional[int] = None, x_dtype: int = F32, out_dtype: int = F32,
+                         scale_rule: int = MX4_FLOOR, epilogue: int = EPILOGUE_NONE) -> None:
+        """quantize_mx4 of x and linear_mx4 behind one call; xq [m, k / 2] and xs [m, k / 32] are work
+        buffers that few rows do without."""
+        self._check(self._lib.krm_linear_mx4_fused(
+            self._handle, _addr(x), _addr(xq), _addr(xs), _addr(w), _addr(w_scales), _addr(bias),
+            _addr(residual), _addr(out), m, n, k, k if x_stride is None else x_stride, x_dtype,
+            out_dtype, scale_rule, epilogue))
+
+    # -- between two blocks of a layer -----------------------------------------------------------------
+    def block_norm(self, y: BufferLike, *, rows: int, dim: int, post_weight: BufferLike = None,
+                   gate: BufferLike = None, gate_span: int = 0, gate_kind: int = GATE_PLAIN,
+                   residual: BufferLike = None, pre_weight: BufferLike = None,
+                   sum_out: BufferLike = None, norm_out: BufferLike = None, eps: float = 1e-5,
+                   block_scale: float = 1.0, residual_scale: float = 1.0, io_dtype: int = F32,
+                   norm_dtype: Optional[int] = None) -> None:
+        """The norm behind a block (post_weight), its gate, the scaled residual sum (sum_out) and the norm
+        in front of the next block (pre_weight, norm_out) in one pass."""
+        self._check(self._lib.krm_block_norm(
+            self._handle, _addr(y), _addr(post_weight), _addr(gate), _addr(residual),
+            _addr(pre_weight), _addr(sum_out), _addr(norm_out), rows, dim, gate_span, gate_kind,
+            float(eps), float(block_scale), float(residual_scale), io_dtype,
+            io_dtype if norm_dtype is None else norm_dtype))
 
 
 def acquire_gpu(device: int = 0, stream: Optional[int] = None) -> GpuContext:
