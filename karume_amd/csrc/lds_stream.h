@@ -12,6 +12,14 @@ __device__ inline void stream_to_lds(uint32_t lds, uint32_t offset, const void* 
                "v"(offset), "s"(base)
                : "memory");
 }
+// Two of them: the second from base + offset2 to LDS 1024 bytes on (an instruction's own offset counts in memory and
+// in LDS, so that it names the base less as much).
+__device__ inline void stream_two_to_lds(uint32_t lds, uint32_t offset, uint32_t offset2, const uint8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+               "global_load_lds_dwordx4 %2, %4 offset:1024" ::"s"(lds),
+               "v"(offset), "v"(offset2), "s"(base), "s"(base - 1024)
+               : "memory");
+}
 // The same for a dword or a zero-extended ushort a lane, to LDS at lds + 4 * lane.
 __device__ inline void stream_word_to_lds(uint32_t lds, uint32_t offset, const void* base, bool half) {
   if (half)
@@ -22,6 +30,10 @@ __device__ inline void stream_word_to_lds(uint32_t lds, uint32_t offset, const v
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds),
                  "v"(offset), "s"(base)
                  : "memory");
+}
+// A zero-extended byte a lane to LDS at lds + 4 * lane.
+__device__ inline void stream_byte_to_lds(uint32_t lds, uint32_t offset, const void* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 template <int N>
 __device__ inline void wait_vm() {

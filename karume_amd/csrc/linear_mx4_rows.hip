@@ -1,0 +1,252 @@
+// Products of up to 16 mx4 rows, or rows of floats that are quantised on the way: rows of w are read once and bound
+// the time by their bytes.
+#include "lds_stream.h"
+#include "mx4_tiles.h"
+
+#include <type_traits>
+
+using namespace krm;
+
+namespace {
+
+// Waves that stream and multiply, and waves that bring x.
+constexpr uint32_t kStreams = 8, kBringers = 8, kThreads = 64 * (kStreams + kBringers);
+
+// Where the rows of x come from: codes in memory, or floats.
+struct Mx4Codes {
+  const uint8_t *codes, *scales;
+};
+template <typename XT>
+struct Mx4Floats {
+  const XT* x;
+  uint64_t stride;
+  bool ceil;
+};
+
+// x in LDS: rows of codes 16 bytes apart more than they are long (rows at one column spread over all banks), then their
+// scales in whole quarters of a run.
+__host__ __device__ inline uint32_t code_pitch(uint32_t blocks) { return blocks * 16u + 16u; }
+__host__ __device__ inline uint32_t scale_pitch(uint32_t blocks) { return (blocks + 15u) & ~15u; }
+
+// A turn of a wave is U steps of 128 codes of 16 rows of w: codes, then scales (whole words of a row and step, or a
+// byte a lane), DEPTH of them in LDS.
+template <int U, bool ALIGNED>
+constexpr uint32_t kTurn = U * 1024u + (ALIGNED ? 256u : U * 256u);
+constexpr uint32_t kSums = 2 * kStreams * 1024;
+template <int U, int DEPTH, bool ALIGNED>
+constexpr uint32_t kHeld = 160u * 1024u - kStreams * DEPTH * kTurn<U, ALIGNED> - kSums;  // bytes for x
+
+// One workgroup a CU walks pieces of 16 rows of w.  Eight waves share a piece's turns in a fixed order, each with a ring
+// of its own in LDS that memory fills without registers or barriers, over the ends of pieces too; another eight
+// bring x meanwhile and leave.  The first eight join their sums in LDS, one wave in turn stores a piece.  The order of a row's
+// sums depends on K alone, so that it does not matter where x came from.
+// Bound by w's bytes: what a CU has on its way (96 KiB) is what keeps memory busy.
+template <typename OT, bool PAIRS, typename X, int U, int DEPTH, bool ALIGNED>
+__global__ __launch_bounds__(kThreads) void linear_mx4_rows_kernel(X x, const uint8_t* __restrict__ w,
+                                                                   const uint8_t* __restrict__ ws, uint32_t blocks,
+                                                                   Mx4Out o) {
+  constexpr uint32_t kLoads = U + (ALIGNED ? 1 : U);  // of a turn
+  __shared__ __align__(1024) uint8_t s_ring[kStreams][DEPTH][kTurn<U, ALIGNED>];
+  __shared__ v4f s_sum[2][kStreams][64];
+  __shared__ __align__(16) uint8_t s_x[kHeld<U, DEPTH, ALIGNED>];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t r = lane & 15u, kb = lane >> 4;
+  const uint32_t rows = o.m, x_pitch = code_pitch(blocks), xs_pitch = scale_pitch(blocks);
+  uint8_t* const s_scales = s_x + rows * x_pitch;
+  auto met = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };  // (what streams goes on)
+
+  if (wave >= kStreams) {
+    // blocks of codes or pieces of eight floats, one after the other over all rows, a few of a thread's at once
+    constexpr bool kCopies = std::is_same<X, Mx4Codes>::value;
+    constexpr uint32_t kBringing = kBringers * 64u, kAtOnce = 4;
+    const uint32_t length = kCopies ? blocks : blocks * 4u, count = rows * length;
+    const uint32_t thread = threadIdx.x - kStreams * 64u;
+    uint32_t row = thread / length, at = thread - row * length;
+    for (uint32_t first = thread; first < count; first += kBringing * kAtOnce) {
+      uint32_t rows_of[kAtOnce], at_of[kAtOnce];
+#pragma unroll
+      for (uint32_t i = 0; i < kAtOnce; ++i) {
+        rows_of[i] = least(row, rows - 1u);
+        at_of[i] = at;
+        for (at += kBringing; at >= length; at -= length) ++row;
+      }
+      auto there = [&](uint32_t i) { return first + i * kBringing < count; };
+      if constexpr (kCopies) {
+        v4i codes[kAtOnce];
+        uint8_t scales[kAtOnce];
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+          const size_t from = (size_t)rows_of[i] * blocks + at_of[i];
+          codes[i] = *reinterpret_cast<const v4i*>(x.codes + from * 16u);
+          scales[i] = x.scales[from];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i)
+          if (there(i)) {
+            *reinterpret_cast<v4i*>(s_x + rows_of[i] * x_pitch + at_of[i] * 16u) = codes[i];
+            s_scales[rows_of[i] * xs_pitch + at_of[i]] = scales[i];
+          }
+      } else {
+        decltype(mx4_load8(x.x)) e[kAtOnce];
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) e[i] = mx4_load8(x.x + rows_of[i] * x.stride + (size_t)at_of[i] * 8u);
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+          uint32_t byte;
+          const uint32_t codes = mx4_quantise8(e[i], x.ceil, byte);
+          if (there(i)) {
+            *reinterpret_cast<uint32_t*>(s_x + rows_of[i] * x_pitch + at_of[i] * 4u) = codes;
+            if ((at_of[i] & 3u) == 0) s_scales[rows_of[i] * xs_pitch + at_of[i] / 4u] = (uint8_t)byte;
+          }
+        }
+      }
+    }
+    met();
+    return;  // (a barrier waits for the waves that are left)
+  }
+
+  const uint32_t steps = (blocks + 3u) / 4u, pieces = (o.n + 15u) / 16u;
+  const uint32_t turns = ((steps + U - 1u) / U + kStreams - 1u) / kStreams;  // of a wave and piece
+  const uint32_t my_pieces = (pieces - blockIdx.x + gridDim.x - 1u) / gridDim.x, total = my_pieces * turns;
+  auto lds_address = [](const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
+  };
+  const uint32_t ring_lds = lds_address(&s_ring[wave][0][0]);
+  struct Place {
+    uint32_t piece, turn, slot;
+  };
+  auto advance = [&](Place& at) {
+    if (++at.slot == DEPTH) at.slot = 0;
+    if (++at.turn == turns) at.turn = 0, at.piece += gridDim.x;
+  };
+  auto step_of = [&](const Place& at, uint32_t u) { return (at.turn * kStreams + wave) * U + u; };
+  // Four lanes bring 64 neighbouring bytes of a row; the pieces of 16 turned by the row's number, so that rows that
+  // are read at once spread over all banks.
+  const uint32_t chunk = (lane & 3u) ^ ((lane >> 3) & 3u);
+  auto request = [&](const Place& at) {
+    const uint32_t n0 = at.piece * 16u, n_last = least(o.n - 1u - n0, 15u);
+    const uint8_t* const w_piece = w + (size_t)n0 * blocks * 16u;
+    const uint8_t* const ws_piece = ws + (size_t)n0 * blocks;
+    const uint32_t lds = ring_lds + at.slot * kTurn<U, ALIGNED>;
+    const uint32_t row = least(lane / 4u, n_last) * blocks;
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+      stream_to_lds(lds + u * 1024u, (row + least(step_of(at, u) * 4u + chunk, blocks - 1u)) * 16u, w_piece);
+    if constexpr (ALIGNED) {
+      const uint32_t of_row = least(least(lane / U, 15u), n_last) * blocks;
+      stream_word_to_lds(lds + U * 1024u, of_row + least(step_of(at, lane % U) * 4u, blocks - 4u), ws_piece, false);
+    } else {
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u)
+        stream_byte_to_lds(lds + U * 1024u + u * 256u, least(r, n_last) * blocks + least(step_of(at, u) * 4u + kb, blocks - 1u), ws_piece);
+    }
+  };
+
+  Place at{blockIdx.x, 0, 0}, ahead = at;
+  uint32_t asked = 0;
+  for (; asked < DEPTH && asked < total; ++asked) {
+    request(ahead);
+    advance(ahead);
+  }
+  met();  // x is there
+  const uint32_t code_at = r * 64u + ((kb ^ ((r >> 1) & 3u)) * 16u);
+  const uint32_t x_row = least(r, rows - 1u);
+  v4f sum = {0.f, 0.f, 0.f, 0.f};
+  uint32_t done = 0;  // pieces
+  for (uint32_t t = 0; t < total; ++t) {
+    if (asked - t == DEPTH) wait_vm<(DEPTH - 1) * kLoads>(); else wait_vm<0>();
+    const uint8_t* const turn = s_ring[wave][at.slot];
+    v4i wc[U], xc[U];
+    uint32_t w_scale[U], x_scale[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      wc[u] = *reinterpret_cast<const v4i*>(turn + u * 1024u + code_at);
+      xc[u] = *reinterpret_cast<const v4i*>(s_x + x_row * x_pitch + least(step_of(at, u) * 4u + kb, blocks - 1u) * 16u);
+      if constexpr (ALIGNED) w_scale[u] = *reinterpret_cast<const uint32_t*>(turn + U * 1024u + (r * U + u) * 4u);
+      else w_scale[u] = *reinterpret_cast<const uint32_t*>(turn + U * 1024u + u * 256u + lane * 4u);
+      x_scale[u] = *reinterpret_cast<const uint32_t*>(s_scales + x_row * xs_pitch + least(step_of(at, u) * 4u, xs_pitch - 4u));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the turn's place is free
+    if (asked < total) {
+      request(ahead);
+      advance(ahead);
+      ++asked;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      // past the end of K both scales are 2^-127: their product is below f32's range
+      const bool there = ALIGNED ? step_of(at, u) < steps : step_of(at, u) * 4u + kb < blocks;
+      const uint32_t s_w = ALIGNED ? w_scale[u] >> (8u * kb) : w_scale[u], s_x8 = x_scale[u] >> (8u * kb);
+      sum = mx4_step(wc[u], there ? s_w : 0u, xc[u], there ? s_x8 : 0u, sum);
+    }
+    if (at.turn + 1u == turns) {
+      s_sum[done & 1u][wave][lane] = sum;
+      sum = v4f{0.f, 0.f, 0.f, 0.f};
+      met();
+      if (wave == done % kStreams) {
+        v4f whole[1] = {s_sum[done & 1u][0][lane]};
+#pragma unroll
+        for (uint32_t v = 1; v < kStreams; ++v) whole[0] += s_sum[done & 1u][v][lane];
+        mx4_finish<OT, PAIRS, 1>(o, r, at.piece * 16u + kb * 4u, whole);
+      }
+      ++done;
+    }
+    advance(at);
+  }
+}
+
+// Bytes of x in LDS, and how a K and its scales are walked.
+uint64_t held_bytes(uint32_t m, uint32_t blocks) { return (uint64_t)m * (code_pitch(blocks) + scale_pitch(blocks)); }
+
+// Steps a turn: four, or as many as leave every wave a turn.
+uint32_t steps_a_turn(uint32_t blocks) {
+  const uint32_t steps = (blocks + 3) / 4;
+  return steps > 2 * kStreams ? 4 : steps > kStreams ? 2 : 1;
+}
+
+template <typename X>
+void launch_rows_of(krm_ctx* ctx, const X& x, const Mx4Product& p, bool half, bool pairs) {
+  const bool words = p.blocks % 4 == 0 && aligned((krm_buf)(uintptr_t)p.ws, 4);
+  const uint32_t pieces = (p.out.n + 15) / 16, grid = pieces < (uint32_t)ctx->num_cus ? pieces : ctx->num_cus;
+  const uint32_t u = steps_a_turn(p.blocks);
+  const bool deep = held_bytes(p.out.m, p.blocks) <= (words ? kHeld<4, 3, true> : kHeld<4, 3, false>);
+  auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, ctx->stream>>>(x, p.w, p.ws, p.blocks, p.out); };
+#define KRM_MX4_ROWS_FORM(OT, PAIRS, U, DEPTH)                                                   \
+  do {                                                                                           \
+    if (words) launch(linear_mx4_rows_kernel<OT, PAIRS, X, U, DEPTH, true>);                     \
+    else launch(linear_mx4_rows_kernel<OT, PAIRS, X, U, DEPTH, false>);                          \
+  } while (0)
+#define KRM_MX4_ROWS(OT, PAIRS)                          \
+  do {                                                   \
+    if (u == 1) KRM_MX4_ROWS_FORM(OT, PAIRS, 1, 3);      \
+    else if (u == 2) KRM_MX4_ROWS_FORM(OT, PAIRS, 2, 3); \
+    else if (deep) KRM_MX4_ROWS_FORM(OT, PAIRS, 4, 3);   \
+    else KRM_MX4_ROWS_FORM(OT, PAIRS, 4, 2);             \
+  } while (0)
+  if (half) { if (pairs) KRM_MX4_ROWS(__half, true); else KRM_MX4_ROWS(__half, false); }
+  else { if (pairs) KRM_MX4_ROWS(float, true); else KRM_MX4_ROWS(float, false); }
+#undef KRM_MX4_ROWS
+#undef KRM_MX4_ROWS_FORM
+}
+
+}  // namespace
+
+namespace krm {
+
+bool mx4_rows_fit(uint32_t m, uint32_t k) {
+  return m <= 16 && k <= (1u << 24) && held_bytes(m, k / kMx4Block) <= kHeld<4, 2, false>;
+}
+
+int32_t launch_mx4_rows(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs) {
+  launch_rows_of(ctx, Mx4Codes{p.xq, p.xs}, p, half, pairs);
+  return launched(ctx, "linear_mx4_rows_kernel");
+}
+
+int32_t launch_mx4_rows_of(krm_ctx* ctx, const Mx4Product& p, krm_buf x, uint64_t stride, int32_t x_dtype, bool ceil,
+                           bool half, bool pairs) {
+  if (x_dtype == KRM_F16) launch_rows_of(ctx, Mx4Floats<__half>{ptr<const __half>(x), stride, ceil}, p, half, pairs);
+  else launch_rows_of(ctx, Mx4Floats<float>{ptr<const float>(x), stride, ceil}, p, half, pairs);
+  return launched(ctx, "linear_mx4_rows_kernel");
+}
+
+}  // namespace krm

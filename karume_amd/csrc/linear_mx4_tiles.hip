@@ -1,0 +1,268 @@
+// Products of many mx4 rows: tiles of rows of x by rows of w, streamed through a ring of stages in LDS.
+#include "lds_stream.h"
+#include "mx4_product.h"
+#include "mx4_tiles.h"
+
+#include <type_traits>
+
+using namespace krm;
+
+namespace {
+
+// mx4_step with the sum in place, in accumulation registers (as the builtin, hundreds of such sums cross a loop's turn in
+// other registers than they began in, with a copy each).  What the compiler cannot know is up to the kernel: two
+// waits between a vector instruction that writes an operand and the product, sixteen between the last product and a
+// sum's reader (settled()).  Inside the loop nothing but LDS writes operands, scales apart, behind which operands_stand().
+template <int STEP>
+__device__ inline void mx4_step_in_place(v4i w, uint32_t w_scale, v4i x, uint32_t x_scale, v4f& sum) {
+#define KRM_MX4_STEP(SELECT)                                                                          \
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SELECT " cbsz:4 blgp:4"     \
+               : "+a"(sum) : "v"(w), "v"(x), "v"(w_scale), "v"(x_scale))
+  if constexpr (STEP == 0) KRM_MX4_STEP("op_sel_hi:[0,0,0]");
+  else if constexpr (STEP == 1) KRM_MX4_STEP("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
+  else if constexpr (STEP == 2) KRM_MX4_STEP("op_sel_hi:[1,1,0]");
+  else KRM_MX4_STEP("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
+#undef KRM_MX4_STEP
+}
+__device__ inline void operands_stand() { asm volatile("s_nop 1"); }
+template <bool WAIT>
+__device__ inline void settled(v4f& sum) {
+  if constexpr (WAIT) asm volatile("s_nop 15" : "+a"(sum)); else asm volatile("" : "+a"(sum));
+}
+
+// A workgroup of WM x WN waves has a tile of WM FM 16 rows of x by WN FN 16 rows of w; a wave FM x FN pieces of 16 x 16.
+//
+// A stage is 128 codes of every row (64 bytes), four stages in LDS.  At step t the waves meet, ask for stage t + 3 in
+// the place of stage t - 1, multiply stage t, its pieces of w read from LDS a little ahead of their products, and
+// read the pieces of x of stage t + 1 beside them.
+// Scales come in runs of 16 blocks (four steps), a quarter of a run to come asked for with every stage;
+// a lane picks the four bytes of its block out of a run's words, and the product instruction one of the four.
+// Scales that are no whole words in memory (ALIGNED false) come as the words that they lie in: a run's sixteen bytes
+// may end in the first word of the next run, so that runs are asked for one earlier.
+// Past the end of K both scales are set to 2^-127: their product is below f32's range, so that whatever codes lie there
+// add nothing.
+// Rows of w lie in LDS so that a lane's sums of four pieces are 16 neighbouring columns.
+template <typename OT, bool PAIRS, int FM, int FN, int WM, int WN, bool ALIGNED>
+__global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
+    const uint8_t* __restrict__ xq, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w,
+    const uint8_t* __restrict__ ws, uint32_t blocks, uint32_t m_tiles, uint32_t n_tiles, Mx4Out o) {
+  static_assert(FN % 4 == 0, "a lane's columns are made of four pieces");
+  constexpr uint32_t kWaves = WM * WN, kThreads = 64 * kWaves;
+  constexpr uint32_t BM = WM * FM * 16, BN = WN * FN * 16;
+  constexpr uint32_t kPlaces = 4;
+  constexpr uint32_t kXLoads = BM / 16 / kWaves, kWLoads = BN / 16 / kWaves;   // of a wave and stage
+  static_assert(kXLoads * kWaves * 16 == BM && kWLoads * kWaves * 16 == BN, "whole loads");
+  // words of scales: four a row and run, four threads a row
+  constexpr uint32_t kXWords = BM * 4 / kThreads, kWWords = BN * 4 / kThreads, kWords = kXWords + kWWords;
+  static_assert(kXWords * kThreads == BM * 4 && kWWords * kThreads == BN * 4, "whole loads");
+  constexpr uint32_t kScaleLoads = (kWords + 3) / 4;                           // of a wave and step
+  constexpr uint32_t kRun = (BM + BN) * 16;                                    // bytes of a run in LDS
+  constexpr uint32_t kLead = ALIGNED ? 1 : 2, kRuns = kLead + 1;               // runs asked for ahead, runs in LDS
+  constexpr uint32_t kGroup = kXLoads + kWLoads + kScaleLoads;                 // loads of a step
+  __shared__ __align__(1024) uint8_t s_x[kPlaces * BM * 64];
+  __shared__ __align__(1024) uint8_t s_w[kPlaces * BN * 64];
+  __shared__ __align__(1024) uint8_t s_scales[kRuns * kRun];
+
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t r = lane & 15u, kb = lane >> 4;
+  uint32_t mt, nt;
+  if (!mx4_tile_of(blockIdx.x, m_tiles, n_tiles, mt, nt)) return;  // the whole workgroup leaves
+  const uint32_t m0 = mt * BM, n0 = nt * BN;
+  const uint32_t wm = wave / WN, wn = wave % WN;
+  const uint32_t steps = (blocks + 3u) / 4u;
+  const uint32_t m_last = o.m - 1u - m0, n_last = o.n - 1u - n0;  // rows past it: itself again, not stored
+  const uint8_t* const x_tile = xq + (size_t)m0 * blocks * 16u;
+  const uint8_t* const w_tile = w + (size_t)n0 * blocks * 16u;
+  auto lds_address = [](const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
+  };
+  const uint32_t x_lds = lds_address(s_x), w_lds = lds_address(s_w), scales_lds = lds_address(s_scales);
+  // the row of w at a row of LDS: piece i of four has rows 4 i .. 4 i + 3 of each 16
+  auto w_row_at = [](uint32_t at) { return (at & ~63u) + ((at >> 2) & 3u) * 16u + ((at >> 4) & 3u) * 4u + (at & 3u); };
+
+  // A load of a wave brings 16 rows of a stage; their four pieces are turned by the row's number, so that the rows
+  // that are read at once spread over all banks.  A wave's loads are neighbours in LDS, two to an instruction's base.
+  constexpr uint32_t kLoads = kXLoads + kWLoads;
+  uint32_t code_row[kLoads];
+#pragma unroll
+  for (uint32_t i = 0; i < kLoads; ++i)
+    code_row[i] = (i < kXLoads ? least((wave * kXLoads + i) * 16u + lane / 4u, m_last)
+                               : least(w_row_at((wave * kWLoads + i - kXLoads) * 16u + lane / 4u), n_last)) * blocks * 16u;
+  const uint32_t piece = (lane & 3u) ^ ((lane >> 3) & 3u);
+  auto code_part = [&](uint32_t asked) { return least(least(asked, steps - 1u) * 4u + piece, blocks - 1u) * 16u; };
+  // loads `first` and, where there is one of the same rows, the next: how many
+  auto pair = [](uint32_t first) { return first + 1 < (first < kXLoads ? kXLoads : kLoads) ? 2u : 1u; };
+  auto request = [&](uint32_t part, uint32_t place, uint32_t i) {
+    const bool is_x = i < kXLoads;
+    const uint32_t lds = is_x ? x_lds + place * BM * 64u + (wave * kXLoads + i) * 1024u
+                              : w_lds + place * BN * 64u + (wave * kWLoads + i - kXLoads) * 1024u;
+    const uint8_t* const tile = is_x ? x_tile : w_tile;
+    if (pair(i) == 2u) stream_two_to_lds(lds, code_row[i] + part, code_row[i + 1] + part, tile);
+    else stream_to_lds(lds, code_row[i] + part, tile);
+  };
+  // Scales are asked for as words from the one that holds the tile's first; a word that is asked for holds a
+  // scale of its row.
+  const uint8_t* const xs_tile = xs + (size_t)m0 * blocks;
+  const uint8_t* const ws_tile = ws + (size_t)n0 * blocks;
+  const uint32_t xs_low = ALIGNED ? 0u : (uint32_t)(uintptr_t)xs_tile & 3u;
+  const uint32_t ws_low = ALIGNED ? 0u : (uint32_t)(uintptr_t)ws_tile & 3u;
+  uint32_t scale_row[kWords];  // where this thread's rows begin
+#pragma unroll
+  for (uint32_t i = 0; i < kWords; ++i)
+    scale_row[i] = i < kXWords ? least(i * kThreads / 4u + threadIdx.x / 4u, m_last) * blocks + xs_low
+                               : least(w_row_at((i - kXWords) * kThreads / 4u + threadIdx.x / 4u), n_last) * blocks + ws_low;
+  auto word_of = [&](uint32_t first, uint32_t run, uint32_t part) {
+    const uint32_t at = run * 16u + part * 4u;
+    if constexpr (ALIGNED) return first + least(at, blocks - 4u);
+    return least((first & ~3u) + at, (first + blocks - 1u) & ~3u);
+  };
+  auto request_scales = [&](uint32_t run, uint32_t i) {
+    const uint32_t load = least(i, kWords - 1u);  // (the last loads of a run may be spare: its last again)
+    stream_word_to_lds(scales_lds + run % kRuns * kRun + wave * 256u + load * kThreads * 4u,
+                       word_of(scale_row[load], run, threadIdx.x & 3u),
+                       load < kXWords ? xs_tile - xs_low : ws_tile - ws_low, false);
+  };
+
+  v4f sum[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j) sum[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+
+  const uint32_t code_at = r * 64u + ((kb ^ ((r >> 1) & 3u)) * 16u);
+  const uint8_t* const w_piece = s_w + wn * FN * 1024u + code_at;
+  const uint8_t* const x_piece = s_x + wm * FM * 1024u + code_at;
+  auto read_w = [&](uint32_t place, int i) { return *reinterpret_cast<const v4i*>(w_piece + place * BN * 64u + i * 1024); };
+  auto read_x = [&](uint32_t place, int j) { return *reinterpret_cast<const v4i*>(x_piece + place * BM * 64u + j * 1024); };
+  // byte kb of four words, one a step; `row`: of x, or BM + of w
+  const uint32_t pick = 0x0c0c0400u + kb * 0x0101u;
+  const uint32_t x_low = (r & 3u) * blocks + xs_low, w_low = (r & 3u) * blocks + ws_low;  // where a row begins in its word
+  auto read_scales = [&](uint32_t run, uint32_t row, uint32_t low, uint32_t keep) {
+    const v4i v = *reinterpret_cast<const v4i*>(s_scales + run % kRuns * kRun + row * 16u);
+    uint32_t d[5] = {(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3], 0u};
+    if constexpr (!ALIGNED) {
+      d[4] = *reinterpret_cast<const uint32_t*>(s_scales + (run + 1u) % kRuns * kRun + row * 16u);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) d[s] = __builtin_amdgcn_alignbyte(d[s + 1], d[s], low);
+    }
+    const uint32_t a = __builtin_amdgcn_perm(d[1], d[0], pick), b = __builtin_amdgcn_perm(d[3], d[2], pick);
+    return __builtin_amdgcn_perm(b, a, 0x05040100u) & keep;
+  };
+  uint32_t w_scale[FN], x_scale[FM];
+  auto read_run = [&](uint32_t run) {
+    // bytes of a lane's words that are there
+    const int32_t count = (int32_t)(blocks + 3u - kb - run * 16u) >> 2;
+    const uint32_t keep = (uint32_t)((1ull << (8u * (uint32_t)max(min(count, 4), 0))) - 1ull);
+#pragma unroll
+    for (uint32_t i = 0; i < FN; ++i) w_scale[i] = read_scales(run, BM + wn * FN * 16u + i * 16u + r, w_low, keep);
+#pragma unroll
+    for (uint32_t j = 0; j < FM; ++j) x_scale[j] = read_scales(run, wm * FM * 16u + j * 16u + r, x_low, keep);
+  };
+
+#pragma unroll
+  for (uint32_t i = 0; i < kLead * 4 * kScaleLoads; ++i) request_scales(i / (4 * kScaleLoads), i % (4 * kScaleLoads));
+#pragma unroll
+  for (uint32_t s = 0; s < 3; ++s) {
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; i += pair(i)) request(code_part(s), s, i);
+#pragma unroll
+    for (uint32_t i = 0; i < kScaleLoads; ++i) request_scales(kLead, s * kScaleLoads + i);
+  }
+  wait_vm<2 * kGroup>();
+  __builtin_amdgcn_s_barrier();
+  // operands: all pieces of x of a step and of the one behind it, pieces of w as they come
+  constexpr int kRing = 4, kAhead = 2;
+  v4i x_held[2][FM], w_ring[kRing];
+  read_run(0);
+#pragma unroll
+  for (int j = 0; j < FM; ++j) x_held[0][j] = read_x(0, j);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) w_ring[i] = read_w(0, i);
+  // (steps past the end: codes of the last stage, scales of nothing)
+  for (uint32_t run = 0; run * 4u < steps; ++run) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      wait_vm<kGroup>();                                  // stage t + 1 is there
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and stage t - 1 has been read
+      __builtin_amdgcn_s_barrier();
+      const uint32_t part = code_part(run * 4u + s + 3u);
+      if (s == 0) operands_stand();
+      // Between the products, one every few of them: the step's loads, its reads of pieces of w two rows of pieces
+      // ahead and of pieces of x a step ahead.
+      constexpr int kProducts = FN * FM, kReads = FN + FM, kAsks = kLoads + kScaleLoads;
+#pragma unroll
+      for (int p = 0; p < kProducts; ++p) {
+        const int i = p / FM, j = p % FM;
+#pragma unroll
+        for (int q = p * kAsks / kProducts; q < (p + 1) * kAsks / kProducts; ++q) {
+          if (q >= (int)kLoads) request_scales(run + kLead + (s + 3) / 4, ((s + 3) & 3) * kScaleLoads + q - kLoads);
+          else if ((q < (int)kXLoads ? q : q - (int)kXLoads) % 2 == 0) request(part, (s + 3) & 3, q);
+        }
+#pragma unroll
+        for (int q = p * kReads / kProducts; q < (p + 1) * kReads / kProducts; ++q) {
+          // (in the order in which they are needed: w of this row + 2, then x)
+          const int row = q * FN / kReads;
+          const bool is_w = q == (row * kReads + FN - 1) / FN;
+          if (is_w) w_ring[(row + kAhead) % kRing] = row + kAhead < FN ? read_w(s, row + kAhead) : read_w((s + 1) & 3, row + kAhead - FN);
+          else x_held[(s + 1) & 1][q - row - 1] = read_x((s + 1) & 3, q - row - 1);
+        }
+        const v4i wi = w_ring[i % kRing];
+        const v4i xj = x_held[s & 1][j];
+        if (s == 0) mx4_step_in_place<0>(wi, w_scale[i], xj, x_scale[j], sum[i][j]);
+        if (s == 1) mx4_step_in_place<1>(wi, w_scale[i], xj, x_scale[j], sum[i][j]);
+        if (s == 2) mx4_step_in_place<2>(wi, w_scale[i], xj, x_scale[j], sum[i][j]);
+        if (s == 3) mx4_step_in_place<3>(wi, w_scale[i], xj, x_scale[j], sum[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    read_run(run + 1);
+  }
+  wait_vm<0>();  // (nothing may land in LDS that is another workgroup's)
+#pragma unroll
+  for (int g = 0; g < FN / 4; ++g)
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const uint32_t row = m0 + wm * FM * 16u + j * 16u + r, col = n0 + wn * FN * 16u + g * 64u + kb * 16u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (g == 0 && j == 0 && i == 0) settled<true>(sum[0][0]); else settled<false>(sum[4 * g + i][j]);
+      }
+      const v4f sums[4] = {sum[4 * g][j], sum[4 * g + 1][j], sum[4 * g + 2][j], sum[4 * g + 3][j]};
+      mx4_finish<OT, PAIRS, 4>(o, row, col, sums);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+template <int FM, int FN, int WM, int WN>
+void launch_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs) {
+  constexpr uint32_t BM = WM * FM * 16, BN = WN * FN * 16;
+  const uint32_t m_tiles = (p.out.m + BM - 1) / BM, n_tiles = (p.out.n + BN - 1) / BN;
+  const bool aligned = p.blocks % 4 == 0 && krm::aligned((krm_buf)(uintptr_t)p.xs | (krm_buf)(uintptr_t)p.ws, 4);
+  const dim3 grid(mx4_tile_grid(m_tiles, n_tiles));
+  auto launch = [&](auto kernel) {
+    kernel<<<grid, 64 * WM * WN, 0, ctx->stream>>>(p.xq, p.xs, p.w, p.ws, p.blocks, m_tiles, n_tiles, p.out);
+  };
+#define KRM_MX4_TILES(OT, PAIRS)                                                       \
+  do {                                                                                 \
+    if (aligned) launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, true>);   \
+    else launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, false>);          \
+  } while (0)
+  if (half) { if (pairs) KRM_MX4_TILES(__half, true); else KRM_MX4_TILES(__half, false); }
+  else { if (pairs) KRM_MX4_TILES(float, true); else KRM_MX4_TILES(float, false); }
+#undef KRM_MX4_TILES
+}
+
+}  // namespace
+
+namespace krm {
+
+int32_t launch_mx4_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, Mx4Form form) {
+  switch (form) {
+    case Mx4Form::kTiles256: launch_tiles<8, 8, 2, 2>(ctx, p, half, pairs); break;
+    case Mx4Form::kTiles128: launch_tiles<4, 4, 2, 2>(ctx, p, half, pairs); break;
+    default: launch_tiles<2, 4, 2, 2>(ctx, p, half, pairs); break;
+  }
+  return launched(ctx, "linear_mx4_tile_kernel");
+}
+
+}  // namespace krm

@@ -6,6 +6,8 @@
 namespace krm {
 namespace {
 
+__device__ inline uint32_t least(uint32_t a, uint32_t b) { return a < b ? a : b; }
+
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -24,55 +26,75 @@ struct Mx4Out {
   const void* residual;  // [m, n_out] or 0; may be out
   void* out;             // [m, n_out]
   uint32_t m, n;
-  bool wide;             // four (pairs: two) neighbouring results of a row are stored at once
+  bool wide;             // a lane's neighbouring results are stored as whole packs
 };
 
+// g / (1 + 2^(-g log2 e)) on the exponential and reciprocal of the hardware, off by a step each.  An f32 result takes the
+// low part of the exponent's product and a Newton step of the reciprocal with it: four steps at most.  Without them
+// the exponential is off by |g| 2^-23, 2^-18 where an fp16 result is not zero, which moves one rounding in a hundred.
+template <typename OT>
 __device__ inline float mx4_silu(float g) {
-  const float t = expf(-fabsf(g));
-  return g * (g < 0.f ? t / (1.0f + t) : 1.0f / (1.0f + t));
+  constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147182f;
+  const float y = -g * kLog2e;
+  float t = __builtin_amdgcn_exp2f(y);
+  if constexpr (sizeof(OT) == 2) return g * __builtin_amdgcn_rcpf(1.0f + t);
+  const float low = fmaf(-g, kLog2eLow, fmaf(-g, kLog2e, -y)) * kLn2;
+  t = fminf(t, 0x1p126f);  // (past it the result is below f32's range, and infinities make no sum)
+  const float d = 1.0f + fmaf(t, low, t);
+  const float r = __builtin_amdgcn_rcpf(d);
+  return g * fmaf(fmaf(-d, r, 1.0f), r, r);
 }
 __device__ inline float mx4_load(const float* p) { return *p; }
 __device__ inline float mx4_load(const __half* p) { return __half2float(*p); }
 __device__ inline void mx4_store(float* p, float v) { *p = v; }
 __device__ inline void mx4_store(__half* p, float v) { *p = __float2half_rn(v); }
 
-// The sums of row `row` and columns col .. col + 3 (col a multiple of 4): bias, silu(gate) * up where the columns are
-// such pairs, residual, one rounding to the stored type.
-template <typename OT, bool PAIRS>
-__device__ inline void mx4_finish(const Mx4Out& o, uint32_t row, uint32_t col, v4f sum) {
+// Four or sixteen neighbouring sums of row `row` from column col on (a multiple of as many): bias, silu(gate) * up where
+// the columns are such pairs, residual, one rounding to the stored type.
+template <typename OT, bool PAIRS, int PIECES>
+__device__ inline void mx4_finish(const Mx4Out& o, uint32_t row, uint32_t col, const v4f (&sum)[PIECES]) {
   if (row >= o.m || col >= o.n) return;
-  constexpr int kCount = PAIRS ? 2 : 4;
+  constexpr int kSums = 4 * PIECES, kCount = PAIRS ? kSums / 2 : kSums;
+  float v[kSums];
+#pragma unroll
+  for (int i = 0; i < kSums; ++i) v[i] = sum[i / 4][i % 4];
   if (o.bias) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += o.bias[min(col + i, o.n - 1)];
+    for (int i = 0; i < kSums; ++i) v[i] += o.bias[least(col + i, o.n - 1)];
   }
-  float v[kCount];
   if constexpr (PAIRS) {
-    v[0] = mx4_silu(sum[0]) * sum[1];
-    v[1] = mx4_silu(sum[2]) * sum[3];
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = sum[i];
+    for (int i = 0; i < kCount; ++i) v[i] = mx4_silu<OT>(v[2 * i]) * v[2 * i + 1];
   }
   const uint32_t width = PAIRS ? o.n / 2 : o.n, first = PAIRS ? col / 2 : col;
   const size_t at = (size_t)row * width + first;
   OT* out = static_cast<OT*>(o.out) + at;
   const OT* residual = static_cast<const OT*>(o.residual) + at;
-  if (o.wide) {  // (the width is a multiple of kCount)
-    struct alignas(kCount * sizeof(OT)) Pack { OT e[kCount]; } pack;
-    if (o.residual) {
-      pack = *reinterpret_cast<const Pack*>(residual);
+  if (o.wide) {  // (the width is a multiple of kCount, rows are aligned to a pack)
+    constexpr int kPack = kCount * sizeof(OT) > 16 ? 16 / sizeof(OT) : kCount;
+    struct alignas(kPack * sizeof(OT)) Pack { OT e[kPack]; };
 #pragma unroll
-      for (int i = 0; i < kCount; ++i) v[i] += mx4_load(&pack.e[i]);
+    for (int p = 0; p < kCount / kPack; ++p) {
+      Pack pack;
+      if (o.residual) {
+        pack = reinterpret_cast<const Pack*>(residual)[p];
+#pragma unroll
+        for (int i = 0; i < kPack; ++i) v[p * kPack + i] += mx4_load(&pack.e[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kPack; ++i) mx4_store(&pack.e[i], v[p * kPack + i]);
+      reinterpret_cast<Pack*>(out)[p] = pack;
     }
-#pragma unroll
-    for (int i = 0; i < kCount; ++i) mx4_store(&pack.e[i], v[i]);
-    *reinterpret_cast<Pack*>(out) = pack;
     return;
   }
 #pragma unroll
   for (int i = 0; i < kCount; ++i)
     if (first + i < width) mx4_store(out + i, o.residual ? v[i] + mx4_load(residual + i) : v[i]);
+}
+// Whether rows of `width` results can be stored `count` (of eb bytes) at once.
+inline bool mx4_wide(uint32_t width, uint32_t count, krm_buf out, krm_buf residual, size_t eb) {
+  const size_t pack = count * eb < 16 ? count * eb : 16;
+  return width % count == 0 && aligned(out | residual, pack);
 }
 
 }  // namespace

@@ -20,10 +20,8 @@ __global__ __launch_bounds__(kThreads) void quantize_mx4_kernel(const XT* __rest
   const uint32_t at = blockIdx.x * kThreads + threadIdx.x;
   if (at >= eighths) return;  // (eighths is a multiple of four: a block's threads leave together)
   for (uint32_t row = blockIdx.y; row < rows; row += gridDim.y) {
-    float v[8];
-    load8(x + row * x_stride + (size_t)at * 8, v);
     uint32_t byte;
-    const uint32_t packed = mx4_quantise8(v, ceil, byte);
+    const uint32_t packed = mx4_quantise8(mx4_load8(x + row * x_stride + (size_t)at * 8), ceil, byte);
     codes[(size_t)row * eighths + at] = packed;
     if ((at & 3u) == 0) scales[(size_t)row * (eighths / 4) + at / 4] = (uint8_t)byte;
   }
@@ -54,23 +52,26 @@ __global__ __launch_bounds__(kThreads) void dequant_mx4_kernel(const uint32_t* _
 
 }  // namespace
 
+int32_t krm::check_mx4_rows(krm_ctx* ctx, const char* what, krm_buf x, uint32_t dim, uint64_t x_stride, int32_t x_dtype,
+                            int32_t scale_rule) {
+  KRM_REQUIRE(ctx, valid_dtype(x_dtype), "%s: unknown dtype %d", what, x_dtype);
+  KRM_REQUIRE(ctx, scale_rule == KRM_MX4_FLOOR || scale_rule == KRM_MX4_CEIL, "%s: unknown scale rule %d", what, scale_rule);
+  KRM_REQUIRE(ctx, dim > 0 && dim % kMx4Block == 0, "%s: dim must be a positive multiple of 32 (%u)", what, dim);
+  KRM_REQUIRE(ctx, x_stride >= dim && x_stride <= (1ull << 40) && x_stride * dtype_bytes(x_dtype) % 16 == 0,
+              "%s: x_stride %llu must be at least dim (%u) and keep rows 16-byte aligned", what,
+              (unsigned long long)x_stride, dim);
+  KRM_REQUIRE(ctx, aligned(x, 16), "%s: x needs 16-byte alignment", what);
+  return KRM_OK;
+}
+
 extern "C" int32_t krm_quantize_mx4(krm_ctx* ctx, krm_buf x, krm_buf codes, krm_buf scales,
                                     uint32_t rows, uint32_t dim, uint64_t x_stride, int32_t x_dtype,
                                     int32_t scale_rule) {
   KRM_TRY(enter(ctx));
-  KRM_REQUIRE(ctx, valid_dtype(x_dtype), "quantize mx4: unknown dtype %d", x_dtype);
-  KRM_REQUIRE(ctx, scale_rule == KRM_MX4_FLOOR || scale_rule == KRM_MX4_CEIL,
-              "quantize mx4: unknown scale rule %d", scale_rule);
-  KRM_REQUIRE(ctx, dim > 0 && dim % kMx4Block == 0,
-              "quantize mx4: dim must be a positive multiple of 32 (%u)", dim);
+  KRM_TRY(check_mx4_rows(ctx, "quantize mx4", x, dim, x_stride, x_dtype, scale_rule));
   if (rows == 0) return KRM_OK;
   KRM_REQUIRE(ctx, x && codes && scales, "quantize mx4: null buffer");
-  const size_t eb = dtype_bytes(x_dtype);
-  KRM_REQUIRE(ctx, x_stride >= dim && x_stride <= (1ull << 40) && x_stride * eb % 16 == 0,
-              "quantize mx4: x_stride %llu must be at least dim (%u) and keep rows 16-byte aligned",
-              (unsigned long long)x_stride, dim);
-  KRM_REQUIRE(ctx, aligned(x, 16) && aligned(codes, 16),
-              "quantize mx4: x and codes need 16-byte alignment");
+  KRM_REQUIRE(ctx, aligned(codes, 16), "quantize mx4: codes need 16-byte alignment");
   const uint32_t eighths = dim / 8;
   const dim3 grid((eighths + kThreads - 1) / kThreads, rows < 65535u ? rows : 65535u);
   const bool ceil = scale_rule == KRM_MX4_CEIL;
