@@ -23,19 +23,12 @@ int32_t check_product(krm_ctx* ctx, krm_buf w, krm_buf w_scales, krm_buf bias, k
   return KRM_OK;
 }
 
-Mx4Form mx4_form(uint32_t m, uint32_t n, uint32_t k) {
-  if (mx4_rows_fit(m, k)) return Mx4Form::kRows;
-  auto tiles = [&](uint32_t bm, uint32_t bn) { return (uint64_t)((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
-  if (tiles(256, 256) >= 256) return Mx4Form::kTiles256;
-  return tiles(128, 128) >= 256 ? Mx4Form::kTiles128 : Mx4Form::kTiles64;
-}
-
 Mx4Product product_of(krm_buf xq, krm_buf xs, krm_buf w, krm_buf w_scales, krm_buf bias, krm_buf residual, krm_buf out,
-                      uint32_t m, uint32_t n, uint32_t k, int32_t out_dtype, bool pairs, Mx4Form form) {
+                      uint32_t m, uint32_t n, uint32_t k, int32_t out_dtype, bool pairs, uint32_t at_once) {
   Mx4Product p{ptr<const uint8_t>(xq), ptr<const uint8_t>(xs), ptr<const uint8_t>(w), ptr<const uint8_t>(w_scales),
-               k / kMx4Block, {ptr<const float>(bias), ptr<const void>(residual), ptr<void>(out), m, n, false}};
-  const uint32_t at_once = form == Mx4Form::kRows ? 4 : 16;  // sums of a lane
-  p.out.wide = mx4_wide(pairs ? n / 2 : n, pairs ? at_once / 2 : at_once, out, residual, dtype_bytes(out_dtype));
+               k / kMx4Block, {ptr<const float>(bias), ptr<const void>(residual), ptr<void>(out), m, n, 0}};
+  // (at_once: sums of a lane)
+  p.out.pack = mx4_pack(pairs ? n / 2 : n, pairs ? at_once / 2 : at_once, out, residual, dtype_bytes(out_dtype));
   return p;
 }
 
@@ -43,9 +36,15 @@ int32_t launch_product(krm_ctx* ctx, krm_buf xq, krm_buf xs, krm_buf w, krm_buf 
                        krm_buf residual, krm_buf out, uint32_t m, uint32_t n, uint32_t k, int32_t out_dtype,
                        int32_t epilogue) {
   const bool pairs = epilogue == KRM_EPILOGUE_SILU_PAIRS, half = out_dtype == KRM_F16;
-  const Mx4Form form = mx4_form(m, n, k);
-  const Mx4Product p = product_of(xq, xs, w, w_scales, bias, residual, out, m, n, k, out_dtype, pairs, form);
-  return form == Mx4Form::kRows ? launch_mx4_rows(ctx, p, half, pairs) : launch_mx4_tiles(ctx, p, half, pairs, form);
+  // (parts of a tile are joined through the context's scratch, which ops share in launch order)
+  const bool serial = ctx->stream == ctx->main_stream;
+  const Mx4Form form = mx4_form(m, n, k, ctx->num_cus, serial ? 2 * kGemmPartialBytes * ctx->num_cus : 0,
+                                serial ? kTicketSlots : 0);
+  const bool tiles = form.kernel == Mx4Kernel::kTiles;
+  KRM_REQUIRE(ctx, !tiles || mx4_tile_count(form.rows, m, n) * form.parts <= 0x7ffffff0ull, "linear mx4: %u x %u is too large", m, n);
+  const Mx4Product p = product_of(xq, xs, w, w_scales, bias, residual, out, m, n, k, out_dtype, pairs, tiles ? 16 : 4);
+  if (form.kernel == Mx4Kernel::kRows) return launch_mx4_rows(ctx, p, half, pairs);
+  return tiles ? launch_mx4_tiles(ctx, p, half, pairs, form) : launch_mx4_batch(ctx, p, half, pairs);
 }
 
 }  // namespace
@@ -72,7 +71,7 @@ extern "C" int32_t krm_linear_mx4_fused(krm_ctx* ctx, krm_buf x, krm_buf xq, krm
   if (mx4_rows_fit(m, k)) {
     KRM_TRY(check_mx4_rows(ctx, "linear mx4 (fused)", x, k, x_stride, x_dtype, scale_rule));
     const bool pairs = epilogue == KRM_EPILOGUE_SILU_PAIRS;
-    const Mx4Product p = product_of(0, 0, w, w_scales, bias, residual, out, m, n, k, out_dtype, pairs, Mx4Form::kRows);
+    const Mx4Product p = product_of(0, 0, w, w_scales, bias, residual, out, m, n, k, out_dtype, pairs, 4);
     return launch_mx4_rows_of(ctx, p, x, x_stride, x_dtype, scale_rule == KRM_MX4_CEIL, out_dtype == KRM_F16, pairs);
   }
   KRM_REQUIRE(ctx, xq && xs, "linear mx4 (fused): this shape (m=%u, k=%u) takes two launches and needs the xq and xs "

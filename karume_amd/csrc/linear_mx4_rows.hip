@@ -23,10 +23,8 @@ struct Mx4Floats {
   bool ceil;
 };
 
-// x in LDS: rows of codes 16 bytes apart more than they are long (rows at one column spread over all banks), then their
-// scales in whole quarters of a run.
-__host__ __device__ inline uint32_t code_pitch(uint32_t blocks) { return blocks * 16u + 16u; }
-__host__ __device__ inline uint32_t scale_pitch(uint32_t blocks) { return (blocks + 15u) & ~15u; }
+// (x in LDS: rows of codes 16 bytes apart more than they are long, so that rows at one column spread over all banks, then
+// their scales in whole quarters of a run.)
 
 // A turn of a wave is U steps of 128 codes of 16 rows of w: codes, then scales (whole words of a row and step, or a
 // byte a lane), DEPTH of them in LDS.
@@ -35,6 +33,9 @@ constexpr uint32_t kTurn = U * 1024u + (ALIGNED ? 256u : U * 256u);
 constexpr uint32_t kSums = 2 * kStreams * 1024;
 template <int U, int DEPTH, bool ALIGNED>
 constexpr uint32_t kHeld = 160u * 1024u - kStreams * DEPTH * kTurn<U, ALIGNED> - kSums;  // bytes for x
+static_assert(kHeld<4, 2, false> >= kMx4HeldBytes && kHeld<4, 2, true> >= kMx4HeldBytes && kHeld<2, 3, false> >= kMx4HeldBytes &&
+                  kHeld<1, 3, false> >= kMx4HeldBytes,
+              "what mx4_rows_fit lets in");
 
 // One workgroup a CU walks pieces of 16 rows of w.  Eight waves share a piece's turns in a fixed order, each with a ring
 // of its own in LDS that memory fills without registers or barriers, over the ends of pieces too; another eight
@@ -51,7 +52,7 @@ __global__ __launch_bounds__(kThreads) void linear_mx4_rows_kernel(X x, const ui
   __shared__ __align__(16) uint8_t s_x[kHeld<U, DEPTH, ALIGNED>];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t r = lane & 15u, kb = lane >> 4;
-  const uint32_t rows = o.m, x_pitch = code_pitch(blocks), xs_pitch = scale_pitch(blocks);
+  const uint32_t rows = o.m, x_pitch = mx4_code_pitch(blocks), xs_pitch = mx4_scale_pitch(blocks);
   uint8_t* const s_scales = s_x + rows * x_pitch;
   auto met = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };  // (what streams goes on)
 
@@ -195,8 +196,124 @@ __global__ __launch_bounds__(kThreads) void linear_mx4_rows_kernel(X x, const ui
   }
 }
 
-// Bytes of x in LDS, and how a K and its scales are walked.
-uint64_t held_bytes(uint32_t m, uint32_t blocks) { return (uint64_t)m * (code_pitch(blocks) + scale_pitch(blocks)); }
+// 17 to 64 rows of x: the same walk, a step a turn, with the rows of x (MB times 16) streamed beside those of w, from the
+// L2 that they stay in.  Tiles that share their rows in LDS hold too few CUs here, and parts of K joined through memory
+// cost 4 to 5 us.
+// Bound by what a CU takes from its L2: x once for 16 rows of w.
+template <int MB, bool ALIGNED>
+constexpr uint32_t kBatchTurn = (1 + MB) * 1024u + (ALIGNED ? 512u : (1 + MB) * 256u);
+
+template <typename OT, bool PAIRS, int MB, int DEPTH, bool ALIGNED>
+__global__ __launch_bounds__(64 * kStreams) void linear_mx4_batch_kernel(const uint8_t* __restrict__ xq,
+                                                                         const uint8_t* __restrict__ xs,
+                                                                         const uint8_t* __restrict__ w,
+                                                                         const uint8_t* __restrict__ ws, uint32_t blocks,
+                                                                         Mx4Out o) {
+  constexpr uint32_t kLoads = 1 + MB + (ALIGNED ? 2 : 1 + MB);  // of a turn
+  constexpr uint32_t kBytes = kBatchTurn<MB, ALIGNED>, kScalesAt = (1 + MB) * 1024u;
+  __shared__ __align__(1024) uint8_t s_ring[kStreams][DEPTH][kBytes];
+  __shared__ v4f s_sum[kStreams / 2][MB][64];
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t r = lane & 15u, kb = lane >> 4;
+  const uint32_t steps = (blocks + 3u) / 4u, pieces = (o.n + 15u) / 16u, turns = (steps + kStreams - 1u) / kStreams;
+  const uint32_t my_pieces = (pieces - blockIdx.x + gridDim.x - 1u) / gridDim.x, total = my_pieces * turns;
+  auto met = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+  auto lds_address = [](const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
+  };
+  const uint32_t ring_lds = lds_address(&s_ring[wave][0][0]);
+  struct Place {
+    uint32_t piece, turn, slot;
+  };
+  auto advance = [&](Place& at) {
+    if (++at.slot == DEPTH) at.slot = 0;
+    if (++at.turn == turns) at.turn = 0, at.piece += gridDim.x;
+  };
+  auto step_of = [&](const Place& at) { return at.turn * kStreams + wave; };
+  const uint32_t chunk = (lane & 3u) ^ ((lane >> 3) & 3u);
+  uint32_t x_row[MB];
+#pragma unroll
+  for (uint32_t b = 0; b < MB; ++b) x_row[b] = least(b * 16u + lane / 4u, o.m - 1u) * blocks;
+  const uint32_t x_scale_row = least(least(lane, MB * 16u - 1u), o.m - 1u) * blocks;
+  auto request = [&](const Place& at) {
+    const uint32_t n0 = at.piece * 16u, n_last = least(o.n - 1u - n0, 15u), step = step_of(at);
+    const uint8_t* const w_piece = w + (size_t)n0 * blocks * 16u;
+    const uint8_t* const ws_piece = ws + (size_t)n0 * blocks;
+    const uint32_t lds = ring_lds + at.slot * kBytes, block = least(step * 4u + chunk, blocks - 1u);
+    stream_to_lds(lds, (least(lane / 4u, n_last) * blocks + block) * 16u, w_piece);
+#pragma unroll
+    for (uint32_t b = 0; b < MB; ++b) stream_to_lds(lds + (1u + b) * 1024u, (x_row[b] + block) * 16u, xq);
+    if constexpr (ALIGNED) {
+      const uint32_t word = least(step * 4u, blocks - 4u);
+      stream_word_to_lds(lds + kScalesAt, least(least(lane, 15u), n_last) * blocks + word, ws_piece, false);
+      stream_word_to_lds(lds + kScalesAt + 256u, x_scale_row + word, xs, false);
+    } else {
+      const uint32_t byte = least(step * 4u + kb, blocks - 1u);
+      stream_byte_to_lds(lds + kScalesAt, least(r, n_last) * blocks + byte, ws_piece);
+#pragma unroll
+      for (uint32_t b = 0; b < MB; ++b)
+        stream_byte_to_lds(lds + kScalesAt + (1u + b) * 256u, least(b * 16u + r, o.m - 1u) * blocks + byte, xs);
+    }
+  };
+
+  Place at{blockIdx.x, 0, 0}, ahead = at;
+  uint32_t asked = 0;
+  for (; asked < DEPTH && asked < total; ++asked) {
+    request(ahead);
+    advance(ahead);
+  }
+  const uint32_t code_at = r * 64u + ((kb ^ ((r >> 1) & 3u)) * 16u);
+  v4f sum[MB];
+#pragma unroll
+  for (uint32_t b = 0; b < MB; ++b) sum[b] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t t = 0; t < total; ++t) {
+    if (asked - t == DEPTH) wait_vm<(DEPTH - 1) * kLoads>(); else wait_vm<0>();
+    const uint8_t* const turn = s_ring[wave][at.slot];
+    const v4i wc = *reinterpret_cast<const v4i*>(turn + code_at);
+    const uint32_t w_word = *reinterpret_cast<const uint32_t*>(turn + kScalesAt + (ALIGNED ? r : lane) * 4u);
+    v4i xc[MB];
+    uint32_t x_word[MB];
+#pragma unroll
+    for (uint32_t b = 0; b < MB; ++b) {
+      xc[b] = *reinterpret_cast<const v4i*>(turn + (1u + b) * 1024u + code_at);
+      x_word[b] = *reinterpret_cast<const uint32_t*>(turn + kScalesAt + (ALIGNED ? 256u + (b * 16u + r) * 4u : (1u + b) * 256u + lane * 4u));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the turn's place is free
+    if (asked < total) {
+      request(ahead);
+      advance(ahead);
+      ++asked;
+    }
+    // past the end of K both scales are 2^-127: their product is below f32's range
+    const bool there = step_of(at) * 4u + (ALIGNED ? 0u : kb) < blocks;
+    const uint32_t shift = ALIGNED ? 8u * kb : 0u, w_scale = there ? w_word >> shift : 0u;
+#pragma unroll
+    for (uint32_t b = 0; b < MB; ++b) sum[b] = mx4_step(wc, w_scale, xc[b], there ? x_word[b] >> shift : 0u, sum[b]);
+    if (at.turn + 1u == turns) {
+      // the upper four waves' sums to the lower four, whose sums then make the rows of 16 of one wave each
+      if (wave >= kStreams / 2) {
+#pragma unroll
+        for (uint32_t b = 0; b < MB; ++b) s_sum[wave - kStreams / 2][b][lane] = sum[b];
+      }
+      met();
+      if (wave < kStreams / 2) {
+#pragma unroll
+        for (uint32_t b = 0; b < MB; ++b) s_sum[wave][b][lane] = sum[b] + s_sum[wave][b][lane];
+      }
+      met();
+      if (wave < MB) {
+        v4f whole[1] = {s_sum[0][wave][lane]};
+#pragma unroll
+        for (uint32_t v = 1; v < kStreams / 2; ++v) whole[0] += s_sum[v][wave][lane];
+        mx4_finish<OT, PAIRS, 1>(o, wave * 16u + r, at.piece * 16u + kb * 4u, whole);
+      }
+      met();  // (the sums' place is free)
+#pragma unroll
+      for (uint32_t b = 0; b < MB; ++b) sum[b] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    advance(at);
+  }
+}
 
 // Steps a turn: four, or as many as leave every wave a turn.
 uint32_t steps_a_turn(uint32_t blocks) {
@@ -209,7 +326,8 @@ void launch_rows_of(krm_ctx* ctx, const X& x, const Mx4Product& p, bool half, bo
   const bool words = p.blocks % 4 == 0 && aligned((krm_buf)(uintptr_t)p.ws, 4);
   const uint32_t pieces = (p.out.n + 15) / 16, grid = pieces < (uint32_t)ctx->num_cus ? pieces : ctx->num_cus;
   const uint32_t u = steps_a_turn(p.blocks);
-  const bool deep = held_bytes(p.out.m, p.blocks) <= (words ? kHeld<4, 3, true> : kHeld<4, 3, false>);
+  const uint64_t held = (uint64_t)p.out.m * (mx4_code_pitch(p.blocks) + mx4_scale_pitch(p.blocks));
+  const bool deep = held <= (words ? kHeld<4, 3, true> : kHeld<4, 3, false>);
   auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, ctx->stream>>>(x, p.w, p.ws, p.blocks, p.out); };
 #define KRM_MX4_ROWS_FORM(OT, PAIRS, U, DEPTH)                                                   \
   do {                                                                                           \
@@ -229,12 +347,28 @@ void launch_rows_of(krm_ctx* ctx, const X& x, const Mx4Product& p, bool half, bo
 #undef KRM_MX4_ROWS_FORM
 }
 
+template <int MB, int DEPTH>
+void launch_batch(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs) {
+  const bool words = p.blocks % 4 == 0 && aligned((krm_buf)(uintptr_t)p.xs | (krm_buf)(uintptr_t)p.ws, 4);
+  const uint32_t pieces = (p.out.n + 15) / 16, grid = pieces < (uint32_t)ctx->num_cus ? pieces : ctx->num_cus;
+  auto launch = [&](auto kernel) { kernel<<<grid, 64 * kStreams, 0, ctx->stream>>>(p.xq, p.xs, p.w, p.ws, p.blocks, p.out); };
+#define KRM_MX4_BATCH(OT, PAIRS)                                                    \
+  do {                                                                              \
+    if (words) launch(linear_mx4_batch_kernel<OT, PAIRS, MB, DEPTH, true>);         \
+    else launch(linear_mx4_batch_kernel<OT, PAIRS, MB, DEPTH == 3 ? 2 : DEPTH, false>);              \
+  } while (0)
+  if (half) { if (pairs) KRM_MX4_BATCH(__half, true); else KRM_MX4_BATCH(__half, false); }
+  else { if (pairs) KRM_MX4_BATCH(float, true); else KRM_MX4_BATCH(float, false); }
+#undef KRM_MX4_BATCH
+}
+
 }  // namespace
 
 namespace krm {
 
-bool mx4_rows_fit(uint32_t m, uint32_t k) {
-  return m <= 16 && k <= (1u << 24) && held_bytes(m, k / kMx4Block) <= kHeld<4, 2, false>;
+int32_t launch_mx4_batch(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs) {
+  if (p.out.m <= 32) launch_batch<2, 5>(ctx, p, half, pairs); else launch_batch<4, 3>(ctx, p, half, pairs);
+  return launched(ctx, "linear_mx4_batch_kernel");
 }
 
 int32_t launch_mx4_rows(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs) {

@@ -24,6 +24,11 @@ __device__ inline void mx4_step_in_place(v4i w, uint32_t w_scale, v4i x, uint32_
   else KRM_MX4_STEP("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
 #undef KRM_MX4_STEP
 }
+// 16 bytes to memory that every XCD sees, straight from a sum's registers (a vector instruction that wrote them next would
+// need a wait).
+__device__ inline void publish4(v4f* p, v4f& sum) {
+  asm volatile("global_store_dwordx4 %1, %0, off sc1\n\ts_nop 0" : "+a"(sum) : "v"(p) : "memory");
+}
 __device__ inline void operands_stand() { asm volatile("s_nop 1"); }
 template <bool WAIT>
 __device__ inline void settled(v4f& sum) {
@@ -32,20 +37,23 @@ __device__ inline void settled(v4f& sum) {
 
 // A workgroup of WM x WN waves has a tile of WM FM 16 rows of x by WN FN 16 rows of w; a wave FM x FN pieces of 16 x 16.
 //
-// A stage is 128 codes of every row (64 bytes), four stages in LDS.  At step t the waves meet, ask for stage t + 3 in
-// the place of stage t - 1, multiply stage t, its pieces of w read from LDS a little ahead of their products, and
-// read the pieces of x of stage t + 1 beside them.
-// Scales come in runs of 16 blocks (four steps), a quarter of a run to come asked for with every stage;
-// a lane picks the four bytes of its block out of a run's words, and the product instruction one of the four.
+// A stage is 128 codes of every row (64 bytes), four of them in LDS; a step multiplies a stage.  The operands of a step are
+// read from LDS during the step before it.  At step t the waves meet, stage t + 1 is there, and stage t + 4 is asked for in
+// the place of stage t.  (Eight places and a meeting every other step: 64 x 128 and 128 x 128 tiles up to 15 % slower, where
+// a CU holds fewer of them; no faster where it holds one anyway.)
+// Scales come in runs of 16 blocks (four steps), a quarter of a run to come asked for with every stage; a lane picks the
+// four bytes of its block out of a run's words, and the product instruction one of the four.
 // Scales that are no whole words in memory (ALIGNED false) come as the words that they lie in: a run's sixteen bytes
 // may end in the first word of the next run, so that runs are asked for one earlier.
 // Past the end of K both scales are set to 2^-127: their product is below f32's range, so that whatever codes lie there
 // add nothing.
 // Rows of w lie in LDS so that a lane's sums of four pieces are 16 neighbouring columns.
+// Several workgroups may share a tile, each some of its runs: all but the last to arrive leave their sums in memory, and the
+// last one joins them in the order of K.
 template <typename OT, bool PAIRS, int FM, int FN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
     const uint8_t* __restrict__ xq, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w,
-    const uint8_t* __restrict__ ws, uint32_t blocks, uint32_t m_tiles, uint32_t n_tiles, Mx4Out o) {
+    const uint8_t* __restrict__ ws, uint32_t blocks, uint32_t m_tiles, uint32_t n_tiles, Mx4Split split, Mx4Out o) {
   static_assert(FN % 4 == 0, "a lane's columns are made of four pieces");
   constexpr uint32_t kWaves = WM * WN, kThreads = 64 * kWaves;
   constexpr uint32_t BM = WM * FM * 16, BN = WN * FN * 16;
@@ -65,11 +73,14 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
 
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t r = lane & 15u, kb = lane >> 4;
-  uint32_t mt, nt;
-  if (!mx4_tile_of(blockIdx.x, m_tiles, n_tiles, mt, nt)) return;  // the whole workgroup leaves
+  uint32_t mt, nt, part_of;
+  if (!mx4_tile_of(blockIdx.x, m_tiles, n_tiles, split.parts, mt, nt, part_of)) return;  // the whole workgroup leaves
   const uint32_t m0 = mt * BM, n0 = nt * BN;
   const uint32_t wm = wave / WN, wn = wave % WN;
-  const uint32_t steps = (blocks + 3u) / 4u;
+  // this workgroup's runs of the tile
+  const uint32_t runs = (blocks + 15u) / 16u;
+  const uint32_t run0 = split.first_run(part_of), run_end = least(split.first_run(part_of + 1u), runs);
+  const uint32_t steps = least(run_end * 4u, (blocks + 3u) / 4u);
   const uint32_t m_last = o.m - 1u - m0, n_last = o.n - 1u - n0;  // rows past it: itself again, not stored
   const uint8_t* const x_tile = xq + (size_t)m0 * blocks * 16u;
   const uint8_t* const w_tile = w + (size_t)n0 * blocks * 16u;
@@ -134,90 +145,163 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
   const uint8_t* const x_piece = s_x + wm * FM * 1024u + code_at;
   auto read_w = [&](uint32_t place, int i) { return *reinterpret_cast<const v4i*>(w_piece + place * BN * 64u + i * 1024); };
   auto read_x = [&](uint32_t place, int j) { return *reinterpret_cast<const v4i*>(x_piece + place * BM * 64u + j * 1024); };
-  // byte kb of four words, one a step; `row`: of x, or BM + of w
+  // byte kb of four words, one a step
   const uint32_t pick = 0x0c0c0400u + kb * 0x0101u;
   const uint32_t x_low = (r & 3u) * blocks + xs_low, w_low = (r & 3u) * blocks + ws_low;  // where a row begins in its word
-  auto read_scales = [&](uint32_t run, uint32_t row, uint32_t low, uint32_t keep) {
-    const v4i v = *reinterpret_cast<const v4i*>(s_scales + run % kRuns * kRun + row * 16u);
-    uint32_t d[5] = {(uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3], 0u};
+  struct Scales {
+    v4i words;
+    uint32_t fifth;
+  };
+  auto read_scales = [&](uint32_t run, int f) {  // of piece f of w, or f - FN of x
+    const uint32_t row = f < FN ? BM + wn * FN * 16u + f * 16u + r : wm * FM * 16u + (f - FN) * 16u + r;
+    Scales d;
+    d.words = *reinterpret_cast<const v4i*>(s_scales + run % kRuns * kRun + row * 16u);
+    d.fifth = ALIGNED ? 0u : *reinterpret_cast<const uint32_t*>(s_scales + (run + 1u) % kRuns * kRun + row * 16u);
+    return d;
+  };
+  auto scale_word = [&](const Scales& s, int f, uint32_t keep) {
+    uint32_t d[5] = {(uint32_t)s.words[0], (uint32_t)s.words[1], (uint32_t)s.words[2], (uint32_t)s.words[3], s.fifth};
     if constexpr (!ALIGNED) {
-      d[4] = *reinterpret_cast<const uint32_t*>(s_scales + (run + 1u) % kRuns * kRun + row * 16u);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) d[s] = __builtin_amdgcn_alignbyte(d[s + 1], d[s], low);
+      for (int i = 0; i < 4; ++i) d[i] = __builtin_amdgcn_alignbyte(d[i + 1], d[i], f < FN ? w_low : x_low);
     }
     const uint32_t a = __builtin_amdgcn_perm(d[1], d[0], pick), b = __builtin_amdgcn_perm(d[3], d[2], pick);
     return __builtin_amdgcn_perm(b, a, 0x05040100u) & keep;
   };
-  uint32_t w_scale[FN], x_scale[FM];
-  auto read_run = [&](uint32_t run) {
-    // bytes of a lane's words that are there
+  auto kept = [&](uint32_t run) {  // bytes of a lane's words that are there
     const int32_t count = (int32_t)(blocks + 3u - kb - run * 16u) >> 2;
-    const uint32_t keep = (uint32_t)((1ull << (8u * (uint32_t)max(min(count, 4), 0))) - 1ull);
-#pragma unroll
-    for (uint32_t i = 0; i < FN; ++i) w_scale[i] = read_scales(run, BM + wn * FN * 16u + i * 16u + r, w_low, keep);
-#pragma unroll
-    for (uint32_t j = 0; j < FM; ++j) x_scale[j] = read_scales(run, wm * FM * 16u + j * 16u + r, x_low, keep);
+    return (uint32_t)((1ull << (8u * (uint32_t)max(min(count, 4), 0))) - 1ull);
   };
 
 #pragma unroll
-  for (uint32_t i = 0; i < kLead * 4 * kScaleLoads; ++i) request_scales(i / (4 * kScaleLoads), i % (4 * kScaleLoads));
+  for (uint32_t i = 0; i < kLead * 4 * kScaleLoads; ++i) request_scales(run0 + i / (4 * kScaleLoads), i % (4 * kScaleLoads));
 #pragma unroll
-  for (uint32_t s = 0; s < 3; ++s) {
+  for (uint32_t s = 0; s < kPlaces; ++s) {
 #pragma unroll
-    for (uint32_t i = 0; i < kLoads; i += pair(i)) request(code_part(s), s, i);
+    for (uint32_t i = 0; i < kLoads; i += pair(i)) request(code_part(run0 * 4u + s), s, i);
 #pragma unroll
-    for (uint32_t i = 0; i < kScaleLoads; ++i) request_scales(kLead, s * kScaleLoads + i);
+    for (uint32_t i = 0; i < kScaleLoads; ++i) request_scales(run0 + kLead, s * kScaleLoads + i);
   }
-  wait_vm<2 * kGroup>();
+  wait_vm<3 * kGroup>();
   __builtin_amdgcn_s_barrier();
-  // operands: all pieces of x of a step and of the one behind it, pieces of w as they come
-  constexpr int kRing = 4, kAhead = 2;
-  v4i x_held[2][FM], w_ring[kRing];
-  read_run(0);
+  // operands of a step and of the one behind it
+  v4i w_held[2][FN], x_held[2][FM];
+  uint32_t w_scale[FN], x_scale[FM];
+  {
+    const uint32_t keep = kept(run0);
 #pragma unroll
-  for (int j = 0; j < FM; ++j) x_held[0][j] = read_x(0, j);
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) w_ring[i] = read_w(0, i);
+    for (int f = 0; f < FN + FM; ++f) {
+      if (f < FN) w_scale[f] = scale_word(read_scales(run0, f), f, keep), w_held[0][f] = read_w(0, f);
+      else x_scale[f - FN] = scale_word(read_scales(run0, f), f, keep), x_held[0][f - FN] = read_x(0, f - FN);
+    }
+  }
   // (steps past the end: codes of the last stage, scales of nothing)
-  for (uint32_t run = 0; run * 4u < steps; ++run) {
+  for (uint32_t run = run0; run < run_end; ++run) {
+    uint32_t next_scale[FN + FM];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      wait_vm<kGroup>();                                  // stage t + 1 is there
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and stage t - 1 has been read
+      wait_vm<2 * kGroup>();                              // stage t + 1 is there
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and stage t has been read
       __builtin_amdgcn_s_barrier();
-      const uint32_t part = code_part(run * 4u + s + 3u);
+      const uint32_t part = code_part(run * 4u + s + kPlaces);
       if (s == 0) operands_stand();
-      // Between the products, one every few of them: the step's loads, its reads of pieces of w two rows of pieces
-      // ahead and of pieces of x a step ahead.
+      // Between the products, one every few of them: the step's loads, and what the next step takes from LDS, in the
+      // first three quarters, so that it is there when they meet.
       constexpr int kProducts = FN * FM, kReads = FN + FM, kAsks = kLoads + kScaleLoads;
+      constexpr int kEvery = kProducts * 3 / 4 / kReads > 0 ? kProducts * 3 / 4 / kReads : 1;
+      const uint32_t keep = kept(run + 1u);
+      Scales raw[3];
 #pragma unroll
       for (int p = 0; p < kProducts; ++p) {
         const int i = p / FM, j = p % FM;
-#pragma unroll
-        for (int q = p * kAsks / kProducts; q < (p + 1) * kAsks / kProducts; ++q) {
-          if (q >= (int)kLoads) request_scales(run + kLead + (s + 3) / 4, ((s + 3) & 3) * kScaleLoads + q - kLoads);
-          else if ((q < (int)kXLoads ? q : q - (int)kXLoads) % 2 == 0) request(part, (s + 3) & 3, q);
+        if (const int q = p * kAsks / kProducts; q != (p + 1) * kAsks / kProducts) {
+          if (q >= (int)kLoads) request_scales(run + 1u + kLead, s * kScaleLoads + q - kLoads);
+          else if ((q < (int)kXLoads ? q : q - (int)kXLoads) % 2 == 0) request(part, s, q);
         }
-#pragma unroll
-        for (int q = p * kReads / kProducts; q < (p + 1) * kReads / kProducts; ++q) {
-          // (in the order in which they are needed: w of this row + 2, then x)
-          const int row = q * FN / kReads;
-          const bool is_w = q == (row * kReads + FN - 1) / FN;
-          if (is_w) w_ring[(row + kAhead) % kRing] = row + kAhead < FN ? read_w(s, row + kAhead) : read_w((s + 1) & 3, row + kAhead - FN);
-          else x_held[(s + 1) & 1][q - row - 1] = read_x((s + 1) & 3, q - row - 1);
+        if (p % kEvery == 0 && p / kEvery < kReads) {
+          const int f = p / kEvery;
+          if (f < FM) x_held[(s + 1) & 1][f] = read_x((s + 1) & 3, f); else w_held[(s + 1) & 1][f - FM] = read_w((s + 1) & 3, f - FM);
+          if (s == 3) {
+            raw[f % 3] = read_scales(run + 1u, f);
+            if (f >= 2) next_scale[f - 2] = scale_word(raw[(f - 2) % 3], f - 2, keep);
+          }
         }
-        const v4i wi = w_ring[i % kRing];
-        const v4i xj = x_held[s & 1][j];
-        if (s == 0) mx4_step_in_place<0>(wi, w_scale[i], xj, x_scale[j], sum[i][j]);
-        if (s == 1) mx4_step_in_place<1>(wi, w_scale[i], xj, x_scale[j], sum[i][j]);
-        if (s == 2) mx4_step_in_place<2>(wi, w_scale[i], xj, x_scale[j], sum[i][j]);
-        if (s == 3) mx4_step_in_place<3>(wi, w_scale[i], xj, x_scale[j], sum[i][j]);
+        if (s == 0) mx4_step_in_place<0>(w_held[0][i], w_scale[i], x_held[0][j], x_scale[j], sum[i][j]);
+        if (s == 1) mx4_step_in_place<1>(w_held[1][i], w_scale[i], x_held[1][j], x_scale[j], sum[i][j]);
+        if (s == 2) mx4_step_in_place<2>(w_held[0][i], w_scale[i], x_held[0][j], x_scale[j], sum[i][j]);
+        if (s == 3) mx4_step_in_place<3>(w_held[1][i], w_scale[i], x_held[1][j], x_scale[j], sum[i][j]);
         __builtin_amdgcn_sched_barrier(0);
       }
+      static_assert((kProducts + kEvery - 1) / kEvery >= kReads && kAsks <= kProducts, "one a product at most, and all of them");
+      if (s == 3) {
+#pragma unroll
+        for (int f = kReads - 2; f < kReads; ++f) next_scale[f] = scale_word(raw[f % 3], f, keep);
+      }
     }
-    read_run(run + 1);
+#pragma unroll
+    for (int f = 0; f < FN + FM; ++f) {
+      if (f < FN) w_scale[f] = next_scale[f]; else x_scale[f - FN] = next_scale[f];
+    }
   }
   wait_vm<0>();  // (nothing may land in LDS that is another workgroup's)
+  if (split.parts > 1u) {
+    // pieces of a workgroup's sums: 16 bytes of thread t at [piece][t]
+    constexpr uint32_t kPieces = FN * FM;
+    v4f* const tile = reinterpret_cast<v4f*>(split.sums) + (size_t)(mt * n_tiles + nt) * split.parts * kPieces * kThreads + threadIdx.x;
+    uint32_t* const ticket = split.tickets + (size_t)(mt * n_tiles + nt) * kTicketStride;
+    __shared__ uint32_t s_arrived;
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j) {
+        if (i == 0 && j == 0) settled<true>(sum[0][0]);
+        publish4(tile + ((size_t)part_of * kPieces + i * FM + j) * kThreads, sum[i][j]);
+      }
+    wait_vm<0>();  // this thread's sums are in memory
+    __syncthreads();
+    if (threadIdx.x == 0) s_arrived = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (s_arrived + 1u != split.parts) return;
+    if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // sixteen neighbouring columns of some pieces of x from some parts at once: 128 registers of loads on their way, or 64
+    // (a CU holds two workgroups of 128 x 128 up to 256 registers a lane)
+    constexpr int kX = FM < 4 ? FM : 4, kAtOnce = FM == 4 ? 1 : 8 / kX;
+#pragma unroll
+    for (int j0 = 0; j0 < FM * (FN / 4); j0 += kX) {
+      const int g = j0 / FM;
+      v4f whole[kX][4];
+      for (uint32_t part = 0; part < split.parts; part += kAtOnce) {
+        uint64_t raw[kAtOnce][kX][4][2];
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a)
+#pragma unroll
+          for (int j = 0; j < kX; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint64_t* from = reinterpret_cast<const uint64_t*>(
+                  tile + ((size_t)least(part + a, split.parts - 1u) * kPieces + (4 * g + i) * FM + (j0 + j) % FM) * kThreads);
+              raw[a][j][i][0] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+              raw[a][j][i][1] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a) {
+          if (part + a >= split.parts) break;
+#pragma unroll
+          for (int j = 0; j < kX; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              struct Raw { uint64_t r[2]; } r = {{raw[a][j][i][0], raw[a][j][i][1]}};
+              const v4f add = __builtin_bit_cast(v4f, r);
+              whole[j][i] = part + a == 0 ? add : whole[j][i] + add;
+            }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kX; ++j)
+        mx4_finish<OT, PAIRS, 4>(o, m0 + wm * FM * 16u + (j0 + j) % FM * 16u + r, n0 + wn * FN * 16u + g * 64u + kb * 16u, whole[j]);
+    }
+    return;
+  }
 #pragma unroll
   for (int g = 0; g < FN / 4; ++g)
 #pragma unroll
@@ -234,18 +318,19 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
 }
 
 template <int FM, int FN, int WM, int WN>
-void launch_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs) {
+void launch_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, uint32_t parts) {
   constexpr uint32_t BM = WM * FM * 16, BN = WN * FN * 16;
-  const uint32_t m_tiles = (p.out.m + BM - 1) / BM, n_tiles = (p.out.n + BN - 1) / BN;
+  const uint32_t m_tiles = (p.out.m + BM - 1) / BM, n_tiles = (p.out.n + BN - 1) / BN, runs = (p.blocks + 15) / 16;
   const bool aligned = p.blocks % 4 == 0 && krm::aligned((krm_buf)(uintptr_t)p.xs | (krm_buf)(uintptr_t)p.ws, 4);
-  const dim3 grid(mx4_tile_grid(m_tiles, n_tiles));
+  const Mx4Split split{parts, runs / parts, runs % parts, ctx->gemm_partials, ctx->tickets};
+  const dim3 grid(mx4_tile_grid(m_tiles, n_tiles, parts));
   auto launch = [&](auto kernel) {
-    kernel<<<grid, 64 * WM * WN, 0, ctx->stream>>>(p.xq, p.xs, p.w, p.ws, p.blocks, m_tiles, n_tiles, p.out);
+    kernel<<<grid, 64 * WM * WN, 0, ctx->stream>>>(p.xq, p.xs, p.w, p.ws, p.blocks, m_tiles, n_tiles, split, p.out);
   };
-#define KRM_MX4_TILES(OT, PAIRS)                                                       \
-  do {                                                                                 \
-    if (aligned) launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, true>);   \
-    else launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, false>);          \
+#define KRM_MX4_TILES(OT, PAIRS)                                                                     \
+  do {                                                                                               \
+    if (aligned) launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, true>);       \
+    else launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, false>);              \
   } while (0)
   if (half) { if (pairs) KRM_MX4_TILES(__half, true); else KRM_MX4_TILES(__half, false); }
   else { if (pairs) KRM_MX4_TILES(float, true); else KRM_MX4_TILES(float, false); }
@@ -256,11 +341,11 @@ void launch_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs) {
 
 namespace krm {
 
-int32_t launch_mx4_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, Mx4Form form) {
-  switch (form) {
-    case Mx4Form::kTiles256: launch_tiles<8, 8, 2, 2>(ctx, p, half, pairs); break;
-    case Mx4Form::kTiles128: launch_tiles<4, 4, 2, 2>(ctx, p, half, pairs); break;
-    default: launch_tiles<2, 4, 2, 2>(ctx, p, half, pairs); break;
+int32_t launch_mx4_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, const Mx4Form& form) {
+  switch (form.rows) {
+    case 256: launch_tiles<8, 8, 2, 2>(ctx, p, half, pairs, form.parts); break;
+    case 128: launch_tiles<4, 4, 2, 2>(ctx, p, half, pairs, form.parts); break;
+    default: launch_tiles<2, 4, 2, 2>(ctx, p, half, pairs, form.parts); break;
   }
   return launched(ctx, "linear_mx4_tile_kernel");
 }

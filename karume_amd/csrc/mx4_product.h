@@ -3,6 +3,9 @@
 
 #include "mx4.h"
 
+#include <initializer_list>
+#include <type_traits>
+
 namespace krm {
 namespace {
 
@@ -26,7 +29,7 @@ struct Mx4Out {
   const void* residual;  // [m, n_out] or 0; may be out
   void* out;             // [m, n_out]
   uint32_t m, n;
-  bool wide;             // a lane's neighbouring results are stored as whole packs
+  uint32_t pack;         // bytes of a lane's neighbouring results that are stored at once: 16, 8, or one result's
 };
 
 // g / (1 + 2^(-g log2 e)) on the exponential and reciprocal of the hardware, off by a step each.  An f32 result takes the
@@ -70,11 +73,13 @@ __device__ inline void mx4_finish(const Mx4Out& o, uint32_t row, uint32_t col, c
   const size_t at = (size_t)row * width + first;
   OT* out = static_cast<OT*>(o.out) + at;
   const OT* residual = static_cast<const OT*>(o.residual) + at;
-  if (o.wide) {  // (the width is a multiple of kCount, rows are aligned to a pack)
-    constexpr int kPack = kCount * sizeof(OT) > 16 ? 16 / sizeof(OT) : kCount;
+  // packs of a row end where the row does (its bytes are a multiple of a pack's, and so is its address)
+  auto store = [&](auto bytes) {
+    constexpr int kPack = decltype(bytes)::value / (int)sizeof(OT) < kCount ? decltype(bytes)::value / (int)sizeof(OT) : kCount;
     struct alignas(kPack * sizeof(OT)) Pack { OT e[kPack]; };
 #pragma unroll
     for (int p = 0; p < kCount / kPack; ++p) {
+      if (first + p * kPack >= width) break;
       Pack pack;
       if (o.residual) {
         pack = reinterpret_cast<const Pack*>(residual)[p];
@@ -85,16 +90,18 @@ __device__ inline void mx4_finish(const Mx4Out& o, uint32_t row, uint32_t col, c
       for (int i = 0; i < kPack; ++i) mx4_store(&pack.e[i], v[p * kPack + i]);
       reinterpret_cast<Pack*>(out)[p] = pack;
     }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < kCount; ++i)
-    if (first + i < width) mx4_store(out + i, o.residual ? v[i] + mx4_load(residual + i) : v[i]);
+  };
+  if (o.pack == 16u) store(std::integral_constant<int, 16>());
+  else if (o.pack == 8u) store(std::integral_constant<int, 8>());
+  else store(std::integral_constant<int, (int)sizeof(OT)>());
 }
-// Whether rows of `width` results can be stored `count` (of eb bytes) at once.
-inline bool mx4_wide(uint32_t width, uint32_t count, krm_buf out, krm_buf residual, size_t eb) {
-  const size_t pack = count * eb < 16 ? count * eb : 16;
-  return width % count == 0 && aligned(out | residual, pack);
+// Bytes that rows of `width` results, `count` neighbours a lane, can be stored in at once.
+inline uint32_t mx4_pack(uint32_t width, uint32_t count, krm_buf out, krm_buf residual, size_t eb) {
+  for (size_t pack : {(size_t)16, (size_t)8}) {
+    const size_t mine = pack < count * eb ? pack : count * eb;
+    if ((uint64_t)width * eb % mine == 0 && aligned(out | residual, mine)) return (uint32_t)pack;
+  }
+  return (uint32_t)eb;
 }
 
 }  // namespace

@@ -1,6 +1,7 @@
-// Which workgroup of a product of mx4 rows has which tile, and what the launchers hand over.
+// Which workgroup of a product of mx4 rows has which tile and which part of K, and what the launchers hand over.
 #pragma once
 
+#include "mx4_plan.h"
 #include "mx4_product.h"
 
 namespace krm {
@@ -11,26 +12,33 @@ struct Mx4Product {
   Mx4Out out;
 };
 
-enum class Mx4Form { kRows, kTiles64, kTiles128, kTiles256 };
-
-// Up to 16 rows of x, in codes or quantised by every workgroup for itself, where they fit LDS.
 int32_t launch_mx4_rows(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs);
-bool mx4_rows_fit(uint32_t m, uint32_t k);
 int32_t launch_mx4_rows_of(krm_ctx* ctx, const Mx4Product& p, krm_buf x, uint64_t stride, int32_t x_dtype, bool ceil,
                            bool half, bool pairs);
-int32_t launch_mx4_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, Mx4Form form);
+int32_t launch_mx4_batch(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs);
+int32_t launch_mx4_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, const Mx4Form& form);
+
+// Runs of 512 codes dealt to the workgroups of a tile, and where those leave their sums.
+struct Mx4Split {
+  uint32_t parts, each, extra;  // the first `extra` parts have one run more
+  float* sums;
+  uint32_t* tickets;            // one a tile, kTicketStride words apart, zero at rest
+  __host__ __device__ uint32_t first_run(uint32_t part) const { return part * each + (part < extra ? part : extra); }
+};
 
 // Workgroups go to the eight XCDs in turn.  Each XCD has a run of the tiles' order, in which four tiles of x follow
-// one another for a tile of w: neighbours in time share both through its L2.
+// one another for a tile of w (neighbours in time share both through its L2) and the parts of a tile one another.
 constexpr uint32_t kMx4Xcds = 8, kMx4Band = 4;
-__host__ __device__ inline uint32_t mx4_tile_grid(uint32_t m_tiles, uint32_t n_tiles) {
-  return (m_tiles * n_tiles + kMx4Xcds - 1) / kMx4Xcds * kMx4Xcds;
+__host__ __device__ inline uint32_t mx4_tile_grid(uint32_t m_tiles, uint32_t n_tiles, uint32_t parts) {
+  return (m_tiles * n_tiles * parts + kMx4Xcds - 1) / kMx4Xcds * kMx4Xcds;
 }
-__host__ __device__ inline bool mx4_tile_of(uint32_t block, uint32_t m_tiles, uint32_t n_tiles, uint32_t& mt,
-                                            uint32_t& nt) {
-  const uint32_t tiles = m_tiles * n_tiles, run = (tiles + kMx4Xcds - 1) / kMx4Xcds;
-  const uint32_t at = block % kMx4Xcds * run + block / kMx4Xcds;
-  if (at >= tiles) return false;
+__host__ __device__ inline bool mx4_tile_of(uint32_t block, uint32_t m_tiles, uint32_t n_tiles, uint32_t parts,
+                                            uint32_t& mt, uint32_t& nt, uint32_t& part) {
+  const uint32_t count = m_tiles * n_tiles * parts, run = (count + kMx4Xcds - 1) / kMx4Xcds;
+  const uint32_t unit = block % kMx4Xcds * run + block / kMx4Xcds;
+  if (unit >= count) return false;
+  const uint32_t at = unit / parts;
+  part = unit - at * parts;
   const uint32_t band = at / (kMx4Band * n_tiles), in_band = at - band * kMx4Band * n_tiles;
   const uint32_t high = m_tiles - band * kMx4Band < kMx4Band ? m_tiles - band * kMx4Band : kMx4Band;
   nt = in_band / high;

@@ -164,7 +164,8 @@ def run_product(gpu, m, n, k, *, out="f32", io=None, pairs=False, bias=False, re
 PRODUCTS = [(1, 1, 32), (1, 16, 32), (1, 17, 64), (2, 2, 96), (1, 130, 128), (3, 33, 160), (16, 16, 512), (17, 48, 544),
             (15, 31, 4096), (1, 4096, 512), (8, 1000, 2048), (31, 257, 1056), (33, 64, 4128), (64, 200, 736),
             (65, 129, 288), (100, 514, 1024), (128, 256, 512), (129, 255, 480), (200, 130, 2080), (256, 512, 256),
-            (257, 513, 1184), (300, 1030, 320), (1, 64, 16416), (16, 40, 11008)]
+            (257, 513, 1184), (300, 1030, 320), (1, 64, 16416), (16, 40, 11008), (50, 130, 1024), (17, 300, 544), (9, 100, 1568),
+            (40, 5001, 2048)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
@@ -184,6 +185,28 @@ def test_products_of_floats_are_those_of_their_codes(gpu_ctx, m, n, k, io):
     got = run_product(gpu_ctx, m, n, k, io=io, x=x, stride=k + 8 * (m % 3), **kw)
     same = run_product(gpu_ctx, m, n, k, x=x, **kw)
     assert np.array_equal(got.view(np.uint8), same.view(np.uint8))
+
+
+# forms that only larger products take, and the same with scales that are no whole words (see test_mx4_plan.py)
+LARGE = [(65, 130, 4096), (70, 130, 4128), (1605, 530, 8192), (1605, 530, 8224), (65, 16530, 64), (65, 16530, 256),
+         (1670, 2330, 8192), (1670, 2330, 8224), (435, 16530, 64), (435, 16530, 256), (16, 500, 8192), (3, 200, 16384)]
+
+
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_large_products(gpu_ctx, m, n, k):
+    rng = np.random.default_rng(m + n)
+    w = (rng.integers(0, 256, (n, k // 2), dtype=np.uint8), rng.integers(112, 122, (n, k // 32), dtype=np.uint8))
+    kw = dict(w=w, bias=True, residual=True, out="f16" if k % 128 else "f32")
+    a = run_product(gpu_ctx, m, n, k, pairs=m % 2 == 1, **kw)
+    b = run_product(gpu_ctx, m, n, k, pairs=m % 2 == 1, io="f32", **kw)
+    assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+
+
+@pytest.mark.parametrize("m,k", [(1, 32), (1, 2048), (5, 4096), (16, 6144), (7, 544)])
+@pytest.mark.parametrize("io", ["f16", "f32"])
+def test_few_rows_do_without_work_buffers(gpu_ctx, m, k, io):
+    run_product(gpu_ctx, m, 333, k, io=io, given=False, stride=k + 64, bias=True)
+    run_product(gpu_ctx, m, 5000, k, io=io, given=False, pairs=True, out="f16")
 
 
 @pytest.mark.parametrize("m", [1, 5, 40, 300])
