@@ -39,7 +39,8 @@ static_assert(kHeld<4, 2, false> >= kMx4HeldBytes && kHeld<4, 2, true> >= kMx4He
 
 // One workgroup a CU walks pieces of 16 rows of w.  Eight waves share a piece's turns in a fixed order, each with a ring
 // of its own in LDS that memory fills without registers or barriers, over the ends of pieces too; another eight
-// bring x meanwhile and leave.  The first eight join their sums in LDS, one wave in turn stores a piece.  The order of a row's
+// bring x meanwhile and leave.  Those that bring x come first: asked for behind a CU's rows of w, x would arrive behind
+// them (1 x 4096 x 4096 4.8 us, so 4.1; 8 x 22016 x 4096 15.0 / 13.1; 1 x 4096 x 11008 8.8 / 7.5).  The streaming waves join their sums in LDS, one wave in turn stores a piece.  The order of a row's
 // sums depends on K alone, so that it does not matter where x came from.
 // Bound by w's bytes: what a CU has on its way (96 KiB) is what keeps memory busy.
 template <typename OT, bool PAIRS, typename X, int U, int DEPTH, bool ALIGNED>
@@ -50,26 +51,29 @@ __global__ __launch_bounds__(kThreads) void linear_mx4_rows_kernel(X x, const ui
   __shared__ __align__(1024) uint8_t s_ring[kStreams][DEPTH][kTurn<U, ALIGNED>];
   __shared__ v4f s_sum[2][kStreams][64];
   __shared__ __align__(16) uint8_t s_x[kHeld<U, DEPTH, ALIGNED>];
-  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t lane = threadIdx.x & 63u, any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t r = lane & 15u, kb = lane >> 4;
   const uint32_t rows = o.m, x_pitch = mx4_code_pitch(blocks), xs_pitch = mx4_scale_pitch(blocks);
   uint8_t* const s_scales = s_x + rows * x_pitch;
   auto met = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };  // (what streams goes on)
 
-  if (wave >= kStreams) {
+  if (any_wave < kBringers) {
     // blocks of codes or pieces of eight floats, one after the other over all rows, a few of a thread's at once
     constexpr bool kCopies = std::is_same<X, Mx4Codes>::value;
     constexpr uint32_t kBringing = kBringers * 64u, kAtOnce = 4;
     const uint32_t length = kCopies ? blocks : blocks * 4u, count = rows * length;
-    const uint32_t thread = threadIdx.x - kStreams * 64u;
+    const uint32_t thread = threadIdx.x;
     uint32_t row = thread / length, at = thread - row * length;
+    const uint32_t more_rows = kBringing / length, more = kBringing - more_rows * length;
     for (uint32_t first = thread; first < count; first += kBringing * kAtOnce) {
       uint32_t rows_of[kAtOnce], at_of[kAtOnce];
 #pragma unroll
       for (uint32_t i = 0; i < kAtOnce; ++i) {
         rows_of[i] = least(row, rows - 1u);
         at_of[i] = at;
-        for (at += kBringing; at >= length; at -= length) ++row;
+        row += more_rows;
+        at += more;
+        if (at >= length) at -= length, ++row;
       }
       auto there = [&](uint32_t i) { return first + i * kBringing < count; };
       if constexpr (kCopies) {
@@ -106,6 +110,7 @@ __global__ __launch_bounds__(kThreads) void linear_mx4_rows_kernel(X x, const ui
     return;  // (a barrier waits for the waves that are left)
   }
 
+  const uint32_t wave = any_wave - kBringers;
   const uint32_t steps = (blocks + 3u) / 4u, pieces = (o.n + 15u) / 16u;
   const uint32_t turns = ((steps + U - 1u) / U + kStreams - 1u) / kStreams;  // of a wave and piece
   const uint32_t my_pieces = (pieces - blockIdx.x + gridDim.x - 1u) / gridDim.x, total = my_pieces * turns;
