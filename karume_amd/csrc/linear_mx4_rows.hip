@@ -190,10 +190,10 @@ __global__ __launch_bounds__(kThreads) void linear_mx4_rows_kernel(X x, const ui
       sum = v4f{0.f, 0.f, 0.f, 0.f};
       met();
       if (wave == done % kStreams) {
-        v4f whole[1] = {s_sum[done & 1u][0][lane]};
+        v4f whole = s_sum[done & 1u][0][lane];
 #pragma unroll
-        for (uint32_t v = 1; v < kStreams; ++v) whole[0] += s_sum[done & 1u][v][lane];
-        mx4_finish<OT, PAIRS, 1>(o, r, at.piece * 16u + kb * 4u, whole);
+        for (uint32_t v = 1; v < kStreams; ++v) whole += s_sum[done & 1u][v][lane];
+        mx4_finish<OT, PAIRS>(o, r, at.piece * 16u + kb * 4u, whole);
       }
       ++done;
     }
@@ -201,26 +201,29 @@ __global__ __launch_bounds__(kThreads) void linear_mx4_rows_kernel(X x, const ui
   }
 }
 
-// 17 to 64 rows of x: the same walk, a step a turn, with the rows of x (MB times 16) streamed beside those of w, from the
-// L2 that they stay in.  Tiles that share their rows in LDS hold too few CUs here, and parts of K joined through memory
-// cost 4 to 5 us.
-// Bound by what a CU takes from its L2: x once for 16 rows of w.
+// 17 to 64 rows of x: the same walk by four waves, 256 codes a turn, with the rows of x (MB times 16) streamed beside those
+// of w, from the L2 that they stay in.  Tiles that share their rows in LDS hold too few CUs here, and parts of K joined
+// through memory cost 4 to 5 us.
+// Bound by what a CU takes from its L2: x once for 16 rows of w.  Eight waves with half lines of 64 bytes took 19.0 us for
+// 64 x 4096 x 11008 where this takes 15.0, and 13.4 for 32 rows (10.9); 64 x 4096 x 4096 6.9 and 6.5.
+constexpr uint32_t kBatchStreams = 4;
 template <int MB, bool ALIGNED>
-constexpr uint32_t kBatchTurn = (1 + MB) * 1024u + (ALIGNED ? 512u : (1 + MB) * 256u);
+constexpr uint32_t kBatchTurn = (1 + MB) * 2048u + (ALIGNED ? 256u + (MB * 32 + 63) / 64 * 256u : (1 + MB) * 512u);
 
 template <typename OT, bool PAIRS, int MB, int DEPTH, bool ALIGNED>
-__global__ __launch_bounds__(64 * kStreams) void linear_mx4_batch_kernel(const uint8_t* __restrict__ xq,
-                                                                         const uint8_t* __restrict__ xs,
-                                                                         const uint8_t* __restrict__ w,
-                                                                         const uint8_t* __restrict__ ws, uint32_t blocks,
-                                                                         Mx4Out o) {
-  constexpr uint32_t kLoads = 1 + MB + (ALIGNED ? 2 : 1 + MB);  // of a turn
-  constexpr uint32_t kBytes = kBatchTurn<MB, ALIGNED>, kScalesAt = (1 + MB) * 1024u;
-  __shared__ __align__(1024) uint8_t s_ring[kStreams][DEPTH][kBytes];
-  __shared__ v4f s_sum[kStreams / 2][MB][64];
+__global__ __launch_bounds__(64 * kBatchStreams) void linear_mx4_batch_kernel(const uint8_t* __restrict__ xq,
+                                                                              const uint8_t* __restrict__ xs,
+                                                                              const uint8_t* __restrict__ w,
+                                                                              const uint8_t* __restrict__ ws, uint32_t blocks,
+                                                                              Mx4Out o) {
+  constexpr uint32_t kXWords = (MB * 32 + 63) / 64;                             // loads of x's scales: two words a row
+  constexpr uint32_t kLoads = 2 * (1 + MB) + (ALIGNED ? 1 + kXWords : 2 * (1 + MB));  // of a turn
+  constexpr uint32_t kBytes = kBatchTurn<MB, ALIGNED>, kScalesAt = (1 + MB) * 2048u;
+  __shared__ __align__(1024) uint8_t s_ring[kBatchStreams][DEPTH][kBytes];
+  __shared__ v4f s_sum[kBatchStreams / 2][MB][64];
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t r = lane & 15u, kb = lane >> 4;
-  const uint32_t steps = (blocks + 3u) / 4u, pieces = (o.n + 15u) / 16u, turns = (steps + kStreams - 1u) / kStreams;
+  const uint32_t stages = (blocks + 7u) / 8u, pieces = (o.n + 15u) / 16u, turns = (stages + kBatchStreams - 1u) / kBatchStreams;
   const uint32_t my_pieces = (pieces - blockIdx.x + gridDim.x - 1u) / gridDim.x, total = my_pieces * turns;
   auto met = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   auto lds_address = [](const void* p) {
@@ -234,30 +237,38 @@ __global__ __launch_bounds__(64 * kStreams) void linear_mx4_batch_kernel(const u
     if (++at.slot == DEPTH) at.slot = 0;
     if (++at.turn == turns) at.turn = 0, at.piece += gridDim.x;
   };
-  auto step_of = [&](const Place& at) { return at.turn * kStreams + wave; };
-  const uint32_t chunk = (lane & 3u) ^ ((lane >> 3) & 3u);
-  uint32_t x_row[MB];
+  auto first_block = [&](const Place& at) { return (at.turn * kBatchStreams + wave) * 8u; };
+  // eight lanes bring 128 neighbouring bytes of a row, their pieces of 16 turned by the row's number
+  const uint32_t chunk = (lane & 7u) ^ (lane >> 3);
+  uint32_t x_row[2 * MB];
 #pragma unroll
-  for (uint32_t b = 0; b < MB; ++b) x_row[b] = least(b * 16u + lane / 4u, o.m - 1u) * blocks;
-  const uint32_t x_scale_row = least(least(lane, MB * 16u - 1u), o.m - 1u) * blocks;
+  for (uint32_t b = 0; b < 2 * MB; ++b) x_row[b] = least(b * 8u + lane / 8u, o.m - 1u) * blocks;
+  uint32_t x_scale_row[kXWords];
+#pragma unroll
+  for (uint32_t b = 0; b < kXWords; ++b) x_scale_row[b] = least(b * 32u + lane / 2u, o.m - 1u) * blocks;
   auto request = [&](const Place& at) {
-    const uint32_t n0 = at.piece * 16u, n_last = least(o.n - 1u - n0, 15u), step = step_of(at);
+    const uint32_t n0 = at.piece * 16u, n_last = least(o.n - 1u - n0, 15u), from = first_block(at);
     const uint8_t* const w_piece = w + (size_t)n0 * blocks * 16u;
     const uint8_t* const ws_piece = ws + (size_t)n0 * blocks;
-    const uint32_t lds = ring_lds + at.slot * kBytes, block = least(step * 4u + chunk, blocks - 1u);
-    stream_to_lds(lds, (least(lane / 4u, n_last) * blocks + block) * 16u, w_piece);
+    const uint32_t lds = ring_lds + at.slot * kBytes, block = least(from + chunk, blocks - 1u);
 #pragma unroll
-    for (uint32_t b = 0; b < MB; ++b) stream_to_lds(lds + (1u + b) * 1024u, (x_row[b] + block) * 16u, xq);
+    for (uint32_t b = 0; b < 2; ++b) stream_to_lds(lds + b * 1024u, (least(b * 8u + lane / 8u, n_last) * blocks + block) * 16u, w_piece);
+#pragma unroll
+    for (uint32_t b = 0; b < 2 * MB; ++b) stream_to_lds(lds + (2u + b) * 1024u, (x_row[b] + block) * 16u, xq);
     if constexpr (ALIGNED) {
-      const uint32_t word = least(step * 4u, blocks - 4u);
-      stream_word_to_lds(lds + kScalesAt, least(least(lane, 15u), n_last) * blocks + word, ws_piece, false);
-      stream_word_to_lds(lds + kScalesAt + 256u, x_scale_row + word, xs, false);
-    } else {
-      const uint32_t byte = least(step * 4u + kb, blocks - 1u);
-      stream_byte_to_lds(lds + kScalesAt, least(r, n_last) * blocks + byte, ws_piece);
+      const uint32_t word = least(from + (lane & 1u) * 4u, blocks - 4u);
+      stream_word_to_lds(lds + kScalesAt, least(least(lane / 2u, 15u), n_last) * blocks + word, ws_piece, false);
 #pragma unroll
-      for (uint32_t b = 0; b < MB; ++b)
-        stream_byte_to_lds(lds + kScalesAt + (1u + b) * 256u, least(b * 16u + r, o.m - 1u) * blocks + byte, xs);
+      for (uint32_t b = 0; b < kXWords; ++b) stream_word_to_lds(lds + kScalesAt + 256u + b * 256u, x_scale_row[b] + word, xs, false);
+    } else {
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t byte = least(from + h * 4u + kb, blocks - 1u);
+        stream_byte_to_lds(lds + kScalesAt + h * 256u, least(r, n_last) * blocks + byte, ws_piece);
+#pragma unroll
+        for (uint32_t b = 0; b < MB; ++b)
+          stream_byte_to_lds(lds + kScalesAt + ((1u + b) * 2u + h) * 256u, least(b * 16u + r, o.m - 1u) * blocks + byte, xs);
+      }
     }
   };
 
@@ -267,21 +278,25 @@ __global__ __launch_bounds__(64 * kStreams) void linear_mx4_batch_kernel(const u
     request(ahead);
     advance(ahead);
   }
-  const uint32_t code_at = r * 64u + ((kb ^ ((r >> 1) & 3u)) * 16u);
+  const uint32_t code_at = r * 128u + ((kb ^ (r & 7u)) * 16u);
   v4f sum[MB];
 #pragma unroll
   for (uint32_t b = 0; b < MB; ++b) sum[b] = v4f{0.f, 0.f, 0.f, 0.f};
   for (uint32_t t = 0; t < total; ++t) {
     if (asked - t == DEPTH) wait_vm<(DEPTH - 1) * kLoads>(); else wait_vm<0>();
     const uint8_t* const turn = s_ring[wave][at.slot];
-    const v4i wc = *reinterpret_cast<const v4i*>(turn + code_at);
-    const uint32_t w_word = *reinterpret_cast<const uint32_t*>(turn + kScalesAt + (ALIGNED ? r : lane) * 4u);
-    v4i xc[MB];
-    uint32_t x_word[MB];
+    v4i wc[2], xc[2][MB];
+    uint32_t w_word[2], x_word[2][MB];
 #pragma unroll
-    for (uint32_t b = 0; b < MB; ++b) {
-      xc[b] = *reinterpret_cast<const v4i*>(turn + (1u + b) * 1024u + code_at);
-      x_word[b] = *reinterpret_cast<const uint32_t*>(turn + kScalesAt + (ALIGNED ? 256u + (b * 16u + r) * 4u : (1u + b) * 256u + lane * 4u));
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t code = code_at ^ h * 64u;
+      wc[h] = *reinterpret_cast<const v4i*>(turn + code);
+      w_word[h] = *reinterpret_cast<const uint32_t*>(turn + kScalesAt + (ALIGNED ? r * 2u + h : h * 64u + lane) * 4u);
+#pragma unroll
+      for (uint32_t b = 0; b < MB; ++b) {
+        xc[h][b] = *reinterpret_cast<const v4i*>(turn + (1u + b) * 2048u + code);
+        x_word[h][b] = *reinterpret_cast<const uint32_t*>(turn + kScalesAt + (ALIGNED ? 256u + ((b * 16u + r) * 2u + h) * 4u : ((1u + b) * 2u + h) * 256u + lane * 4u));
+      }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the turn's place is free
     if (asked < total) {
@@ -289,28 +304,31 @@ __global__ __launch_bounds__(64 * kStreams) void linear_mx4_batch_kernel(const u
       advance(ahead);
       ++asked;
     }
-    // past the end of K both scales are 2^-127: their product is below f32's range
-    const bool there = step_of(at) * 4u + (ALIGNED ? 0u : kb) < blocks;
-    const uint32_t shift = ALIGNED ? 8u * kb : 0u, w_scale = there ? w_word >> shift : 0u;
 #pragma unroll
-    for (uint32_t b = 0; b < MB; ++b) sum[b] = mx4_step(wc, w_scale, xc[b], there ? x_word[b] >> shift : 0u, sum[b]);
+    for (uint32_t h = 0; h < 2; ++h) {
+      // past the end of K both scales are 2^-127: their product is below f32's range
+      const bool there = first_block(at) + h * 4u + (ALIGNED ? 0u : kb) < blocks;
+      const uint32_t shift = ALIGNED ? 8u * kb : 0u, w_scale = there ? w_word[h] >> shift : 0u;
+#pragma unroll
+      for (uint32_t b = 0; b < MB; ++b) sum[b] = mx4_step(wc[h], w_scale, xc[h][b], there ? x_word[h][b] >> shift : 0u, sum[b]);
+    }
     if (at.turn + 1u == turns) {
-      // the upper four waves' sums to the lower four, whose sums then make the rows of 16 of one wave each
-      if (wave >= kStreams / 2) {
+      // the upper waves' sums to the lower ones, whose sums then make the rows of 16 of one wave each
+      if (wave >= kBatchStreams / 2) {
 #pragma unroll
-        for (uint32_t b = 0; b < MB; ++b) s_sum[wave - kStreams / 2][b][lane] = sum[b];
+        for (uint32_t b = 0; b < MB; ++b) s_sum[wave - kBatchStreams / 2][b][lane] = sum[b];
       }
       met();
-      if (wave < kStreams / 2) {
+      if (wave < kBatchStreams / 2) {
 #pragma unroll
         for (uint32_t b = 0; b < MB; ++b) s_sum[wave][b][lane] = sum[b] + s_sum[wave][b][lane];
       }
       met();
       if (wave < MB) {
-        v4f whole[1] = {s_sum[0][wave][lane]};
+        v4f whole = s_sum[0][wave][lane];
 #pragma unroll
-        for (uint32_t v = 1; v < kStreams / 2; ++v) whole[0] += s_sum[v][wave][lane];
-        mx4_finish<OT, PAIRS, 1>(o, wave * 16u + r, at.piece * 16u + kb * 4u, whole);
+        for (uint32_t v = 1; v < kBatchStreams / 2; ++v) whole += s_sum[v][wave][lane];
+        mx4_finish<OT, PAIRS>(o, wave * 16u + r, at.piece * 16u + kb * 4u, whole);
       }
       met();  // (the sums' place is free)
 #pragma unroll
@@ -356,7 +374,7 @@ template <int MB, int DEPTH>
 void launch_batch(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs) {
   const bool words = p.blocks % 4 == 0 && aligned((krm_buf)(uintptr_t)p.xs | (krm_buf)(uintptr_t)p.ws, 4);
   const uint32_t pieces = (p.out.n + 15) / 16, grid = pieces < (uint32_t)ctx->num_cus ? pieces : ctx->num_cus;
-  auto launch = [&](auto kernel) { kernel<<<grid, 64 * kStreams, 0, ctx->stream>>>(p.xq, p.xs, p.w, p.ws, p.blocks, p.out); };
+  auto launch = [&](auto kernel) { kernel<<<grid, 64 * kBatchStreams, 0, ctx->stream>>>(p.xq, p.xs, p.w, p.ws, p.blocks, p.out); };
 #define KRM_MX4_BATCH(OT, PAIRS)                                                    \
   do {                                                                              \
     if (words) launch(linear_mx4_batch_kernel<OT, PAIRS, MB, DEPTH, true>);         \

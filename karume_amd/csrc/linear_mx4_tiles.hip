@@ -35,40 +35,88 @@ __device__ inline void settled(v4f& sum) {
   if constexpr (WAIT) asm volatile("s_nop 15" : "+a"(sum)); else asm volatile("" : "+a"(sum));
 }
 
+// Pieces of 16 columns whose sums make 16 bytes of results in a lane: that many pieces of w in LDS hold a lane's neighbours,
+// and the four lanes of a row 64 bytes.
+template <typename OT, bool PAIRS>
+constexpr uint32_t kMx4Beside = (PAIRS ? 2 : 1) * 4 / sizeof(OT);
+
+// The sums of 16 rows from row0 on (a lane's is r) and PIECES x 16 columns from col0 on.  Two neighbouring sets of 64 bytes
+// change places between rows eight apart, so that a store writes whole lines of 128 bytes, which go past the caches.  (Halves
+// of lines through the caches: 4096 x 22016 x 4096 249 us, past them 230, whole lines past them 220; halves of 32 bytes past
+// them no better than through them.)
+template <typename OT, bool PAIRS, int PIECES>
+__device__ inline void finish_rows(const Mx4Out& o, uint32_t row0, uint32_t col0, uint32_t r, uint32_t kb, const v4f (&sum)[PIECES]) {
+  constexpr uint32_t kBeside = kMx4Beside<OT, PAIRS>, kSets = PIECES / kBeside, kValues = 16 / sizeof(OT);
+  constexpr uint32_t kTogether = kSets > 1 ? 2 : 1;
+  const uint32_t width = PAIRS ? o.n / 2 : o.n;
+#pragma unroll
+  for (uint32_t set = 0; set < kSets; set += kTogether) {
+    float v[kTogether][4 * kBeside];
+#pragma unroll
+    for (uint32_t t = 0; t < kTogether; ++t)
+      mx4_values<OT, PAIRS, (int)kBeside>(o, col0 + ((set + t) * 4u + kb) * 4u * kBeside, &sum[(set + t) * kBeside], v[t]);
+    if constexpr (kTogether == 2) {
+#pragma unroll
+      for (uint32_t i = 0; i < kValues; ++i) {
+        const int a = __float_as_int(v[0][i]), b = __float_as_int(v[1][i]);
+        v[0][i] = __int_as_float(__builtin_amdgcn_update_dpp(a, b, 0x128, 0xf, 0xc, false));  // lanes 8 .. 15 from 0 .. 7
+        v[1][i] = __int_as_float(__builtin_amdgcn_update_dpp(b, a, 0x128, 0xf, 0x3, false));  // lanes 0 .. 7 from 8 .. 15
+      }
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < kTogether; ++t) {
+      const uint32_t row = row0 + (kTogether == 2 ? t * 8u + (r & 7u) : r);
+      const uint32_t at = set + (kTogether == 2 ? r >> 3 : 0u);
+      const uint32_t first = (PAIRS ? col0 / 2u : col0) + (at * 4u + kb) * kValues;
+      if (row < o.m && first < width) mx4_put<OT, (int)kValues, true>(o, row, first, width, v[t]);
+    }
+  }
+}
+
 // A workgroup of WM x WN waves has a tile of WM FM 16 rows of x by WN FN 16 rows of w; a wave FM x FN pieces of 16 x 16.
+// Three tiles: 256 x 256 (a wave's sums fill its accumulation registers: fewest reads from LDS), 128 x 128 and 64 x 128, of
+// which a CU holds two where there are enough.  us of fp16 results, weights from memory:
+//   m x n x k                256 x 256   128 x 128   64 x 128
+//   8192 x 8192 x 8192             255         358        475   (4.3 PFLOP/s)
+//   512 x 22016 x 4096, pairs       36          46         60
+//   1001 x 4100 x 11040            100          65         89
+//   509 x 2560 x 2048               21         9.5        7.6
+// Bound by power and by the matrix cores' waits for operands: at 8192 cubed the cores run at 1.8 GHz and are busy half of the
+// time; 232 us without the stores, 245 without the reads from LDS, 196 without reads and loads, 165 at the rate that
+// products of random codes reach from registers.
 //
-// A stage is 128 codes of every row (64 bytes), four of them in LDS; a step multiplies a stage.  The operands of a step are
-// read from LDS during the step before it.  At step t the waves meet, stage t + 1 is there, and stage t + 4 is asked for in
-// the place of stage t.  (Eight places and a meeting every other step: 64 x 128 and 128 x 128 tiles up to 15 % slower, where
-// a CU holds fewer of them; no faster where it holds one anyway.)
-// Scales come in runs of 16 blocks (four steps), a quarter of a run to come asked for with every stage; a lane picks the
+// A stage is 256 codes of every row: 128 bytes, a whole line (of half lines a CU gets half as many bytes a second of rows of
+// its own: 58 GB/s, so 107; 1001 x 4100 x 11040 in 128 x 128 tiles 84 us, so 65).  PLACES stages in LDS, two steps of 128
+// codes in each: two, or as many as fit where no CU has two workgroups (256 x 4096 x 4096 12.4 us with two, 10.5 with five;
+// 1024 x 4096 x 4096, two workgroups a CU, 17.8 and 21.2).  The operands of a step are read from LDS during the step before
+// it.  In front of a stage's second step the waves meet: the next stage is there, and the place of this one, all of which has
+// been read, is asked to be filled again.
+// Scales come in runs of 16 blocks (four steps), half of a run to come asked for with every stage; a lane picks the
 // four bytes of its block out of a run's words, and the product instruction one of the four.
 // Scales that are no whole words in memory (ALIGNED false) come as the words that they lie in: a run's sixteen bytes
 // may end in the first word of the next run, so that runs are asked for one earlier.
 // Past the end of K both scales are set to 2^-127: their product is below f32's range, so that whatever codes lie there
 // add nothing.
-// Rows of w lie in LDS so that a lane's sums of four pieces are 16 neighbouring columns.
 // Several workgroups may share a tile, each some of its runs: all but the last to arrive leave their sums in memory, and the
 // last one joins them in the order of K.
-template <typename OT, bool PAIRS, int FM, int FN, int WM, int WN, bool ALIGNED>
+template <typename OT, bool PAIRS, int FM, int FN, int WM, int WN, int PLACES, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
     const uint8_t* __restrict__ xq, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w,
     const uint8_t* __restrict__ ws, uint32_t blocks, uint32_t m_tiles, uint32_t n_tiles, Mx4Split split, Mx4Out o) {
-  static_assert(FN % 4 == 0, "a lane's columns are made of four pieces");
+  static_assert(FN % 4 == 0, "pieces come in fours");
   constexpr uint32_t kWaves = WM * WN, kThreads = 64 * kWaves;
   constexpr uint32_t BM = WM * FM * 16, BN = WN * FN * 16;
-  constexpr uint32_t kPlaces = 4;
-  constexpr uint32_t kXLoads = BM / 16 / kWaves, kWLoads = BN / 16 / kWaves;   // of a wave and stage
-  static_assert(kXLoads * kWaves * 16 == BM && kWLoads * kWaves * 16 == BN, "whole loads");
+  constexpr uint32_t kXLoads = BM / 8 / kWaves, kWLoads = BN / 8 / kWaves;     // of a wave and stage
+  static_assert(kXLoads * kWaves * 8 == BM && kWLoads * kWaves * 8 == BN, "whole loads");
   // words of scales: four a row and run, four threads a row
   constexpr uint32_t kXWords = BM * 4 / kThreads, kWWords = BN * 4 / kThreads, kWords = kXWords + kWWords;
   static_assert(kXWords * kThreads == BM * 4 && kWWords * kThreads == BN * 4, "whole loads");
-  constexpr uint32_t kScaleLoads = (kWords + 3) / 4;                           // of a wave and step
+  constexpr uint32_t kScaleLoads = (kWords + 1) / 2;                           // of a wave and stage
   constexpr uint32_t kRun = (BM + BN) * 16;                                    // bytes of a run in LDS
-  constexpr uint32_t kLead = ALIGNED ? 1 : 2, kRuns = kLead + 1;               // runs asked for ahead, runs in LDS
-  constexpr uint32_t kGroup = kXLoads + kWLoads + kScaleLoads;                 // loads of a step
-  __shared__ __align__(1024) uint8_t s_x[kPlaces * BM * 64];
-  __shared__ __align__(1024) uint8_t s_w[kPlaces * BN * 64];
+  constexpr uint32_t kLead = ALIGNED ? 1 : 2, kRuns = kLead + (PLACES + 1) / 2; // runs asked for ahead, runs in LDS
+  constexpr uint32_t kGroup = kXLoads + kWLoads + kScaleLoads;                 // loads of a stage
+  __shared__ __align__(1024) uint8_t s_x[PLACES * BM * 128];
+  __shared__ __align__(1024) uint8_t s_w[PLACES * BN * 128];
   __shared__ __align__(1024) uint8_t s_scales[kRuns * kRun];
 
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -80,7 +128,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
   // this workgroup's runs of the tile
   const uint32_t runs = (blocks + 15u) / 16u;
   const uint32_t run0 = split.first_run(part_of), run_end = least(split.first_run(part_of + 1u), runs);
-  const uint32_t steps = least(run_end * 4u, (blocks + 3u) / 4u);
+  const uint32_t stages = least(run_end * 2u, (blocks + 7u) / 8u);
   const uint32_t m_last = o.m - 1u - m0, n_last = o.n - 1u - n0;  // rows past it: itself again, not stored
   const uint8_t* const x_tile = xq + (size_t)m0 * blocks * 16u;
   const uint8_t* const w_tile = w + (size_t)n0 * blocks * 16u;
@@ -88,25 +136,29 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
   };
   const uint32_t x_lds = lds_address(s_x), w_lds = lds_address(s_w), scales_lds = lds_address(s_scales);
-  // the row of w at a row of LDS: piece i of four has rows 4 i .. 4 i + 3 of each 16
-  auto w_row_at = [](uint32_t at) { return (at & ~63u) + ((at >> 2) & 3u) * 16u + ((at >> 4) & 3u) * 4u + (at & 3u); };
+  // the row of w at a row of LDS (piece i of the kBeside has four rows of each 4 kBeside)
+  auto w_row_at = [](uint32_t at) {
+    constexpr uint32_t kBeside = kMx4Beside<OT, PAIRS>;
+    const uint32_t piece = at >> 4 & 3u;
+    return (at & ~63u) + ((piece / kBeside * 4u + (at >> 2 & 3u)) * kBeside + piece % kBeside) * 4u + (at & 3u);
+  };
 
-  // A load of a wave brings 16 rows of a stage; their four pieces are turned by the row's number, so that the rows
-  // that are read at once spread over all banks.  A wave's loads are neighbours in LDS, two to an instruction's base.
+  // A load of a wave brings eight rows of a stage; their pieces of 16 bytes are turned by the row's number, so that the
+  // rows that are read at once spread over all banks.  A wave's loads are neighbours in LDS, two to an instruction's base.
   constexpr uint32_t kLoads = kXLoads + kWLoads;
   uint32_t code_row[kLoads];
 #pragma unroll
   for (uint32_t i = 0; i < kLoads; ++i)
-    code_row[i] = (i < kXLoads ? least((wave * kXLoads + i) * 16u + lane / 4u, m_last)
-                               : least(w_row_at((wave * kWLoads + i - kXLoads) * 16u + lane / 4u), n_last)) * blocks * 16u;
-  const uint32_t piece = (lane & 3u) ^ ((lane >> 3) & 3u);
-  auto code_part = [&](uint32_t asked) { return least(least(asked, steps - 1u) * 4u + piece, blocks - 1u) * 16u; };
+    code_row[i] = (i < kXLoads ? least((wave * kXLoads + i) * 8u + lane / 8u, m_last)
+                               : least(w_row_at((wave * kWLoads + i - kXLoads) * 8u + lane / 8u), n_last)) * blocks * 16u;
+  const uint32_t piece = (lane & 7u) ^ (lane >> 3);
+  auto code_part = [&](uint32_t asked) { return least(least(asked, stages - 1u) * 8u + piece, blocks - 1u) * 16u; };
   // loads `first` and, where there is one of the same rows, the next: how many
   auto pair = [](uint32_t first) { return first + 1 < (first < kXLoads ? kXLoads : kLoads) ? 2u : 1u; };
   auto request = [&](uint32_t part, uint32_t place, uint32_t i) {
     const bool is_x = i < kXLoads;
-    const uint32_t lds = is_x ? x_lds + place * BM * 64u + (wave * kXLoads + i) * 1024u
-                              : w_lds + place * BN * 64u + (wave * kWLoads + i - kXLoads) * 1024u;
+    const uint32_t lds = is_x ? x_lds + place * BM * 128u + (wave * kXLoads + i) * 1024u
+                              : w_lds + place * BN * 128u + (wave * kWLoads + i - kXLoads) * 1024u;
     const uint8_t* const tile = is_x ? x_tile : w_tile;
     if (pair(i) == 2u) stream_two_to_lds(lds, code_row[i] + part, code_row[i + 1] + part, tile);
     else stream_to_lds(lds, code_row[i] + part, tile);
@@ -140,11 +192,12 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
 #pragma unroll
     for (int j = 0; j < FM; ++j) sum[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  const uint32_t code_at = r * 64u + ((kb ^ ((r >> 1) & 3u)) * 16u);
-  const uint8_t* const w_piece = s_w + wn * FN * 1024u + code_at;
-  const uint8_t* const x_piece = s_x + wm * FM * 1024u + code_at;
-  auto read_w = [&](uint32_t place, int i) { return *reinterpret_cast<const v4i*>(w_piece + place * BN * 64u + i * 1024); };
-  auto read_x = [&](uint32_t place, int j) { return *reinterpret_cast<const v4i*>(x_piece + place * BM * 64u + j * 1024); };
+  // a step's four pieces of a row's eight: the other step's are 64 bytes off in the turned order
+  const uint32_t code_at = r * 128u + ((kb ^ (r & 7u)) * 16u);
+  const uint8_t* const w_pieces[2] = {s_w + wn * FN * 2048u + code_at, s_w + wn * FN * 2048u + (code_at ^ 64u)};
+  const uint8_t* const x_pieces[2] = {s_x + wm * FM * 2048u + code_at, s_x + wm * FM * 2048u + (code_at ^ 64u)};
+  auto read_w = [&](uint32_t place, int step, int i) { return *reinterpret_cast<const v4i*>(w_pieces[step] + place * BN * 128u + i * 2048); };
+  auto read_x = [&](uint32_t place, int step, int j) { return *reinterpret_cast<const v4i*>(x_pieces[step] + place * BM * 128u + j * 2048); };
   // byte kb of four words, one a step
   const uint32_t pick = 0x0c0c0400u + kb * 0x0101u;
   const uint32_t x_low = (r & 3u) * blocks + xs_low, w_low = (r & 3u) * blocks + ws_low;  // where a row begins in its word
@@ -174,15 +227,15 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
   };
 
 #pragma unroll
-  for (uint32_t i = 0; i < kLead * 4 * kScaleLoads; ++i) request_scales(run0 + i / (4 * kScaleLoads), i % (4 * kScaleLoads));
+  for (uint32_t i = 0; i < kLead * 2 * kScaleLoads; ++i) request_scales(run0 + i / (2 * kScaleLoads), i % (2 * kScaleLoads));
 #pragma unroll
-  for (uint32_t s = 0; s < kPlaces; ++s) {
+  for (uint32_t d = 0; d < PLACES; ++d) {
 #pragma unroll
-    for (uint32_t i = 0; i < kLoads; i += pair(i)) request(code_part(run0 * 4u + s), s, i);
+    for (uint32_t i = 0; i < kLoads; i += pair(i)) request(code_part(run0 * 2u + d), d, i);
 #pragma unroll
-    for (uint32_t i = 0; i < kScaleLoads; ++i) request_scales(run0 + kLead, s * kScaleLoads + i);
+    for (uint32_t i = 0; i < kScaleLoads; ++i) request_scales(run0 + d / 2u + kLead, d % 2u * kScaleLoads + i);
   }
-  wait_vm<3 * kGroup>();
+  wait_vm<(PLACES - 1) * kGroup>();
   __builtin_amdgcn_s_barrier();
   // operands of a step and of the one behind it
   v4i w_held[2][FN], x_held[2][FM];
@@ -191,22 +244,26 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
     const uint32_t keep = kept(run0);
 #pragma unroll
     for (int f = 0; f < FN + FM; ++f) {
-      if (f < FN) w_scale[f] = scale_word(read_scales(run0, f), f, keep), w_held[0][f] = read_w(0, f);
-      else x_scale[f - FN] = scale_word(read_scales(run0, f), f, keep), x_held[0][f - FN] = read_x(0, f - FN);
+      if (f < FN) w_scale[f] = scale_word(read_scales(run0, f), f, keep), w_held[0][f] = read_w(0, 0, f);
+      else x_scale[f - FN] = scale_word(read_scales(run0, f), f, keep), x_held[0][f - FN] = read_x(0, 0, f - FN);
     }
   }
   // (steps past the end: codes of the last stage, scales of nothing)
+  uint32_t place = 0;
   for (uint32_t run = run0; run < run_end; ++run) {
     uint32_t next_scale[FN + FM];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      wait_vm<2 * kGroup>();                              // stage t + 1 is there
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and stage t has been read
-      __builtin_amdgcn_s_barrier();
-      const uint32_t part = code_part(run * 4u + s + kPlaces);
+      const uint32_t next_place = place + 1u == PLACES ? 0u : place + 1u;
+      if (s % 2 == 1) {
+        wait_vm<(PLACES - 2) * kGroup>();                   // the next stage is there
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and all of this one has been read
+        __builtin_amdgcn_s_barrier();
+      }
+      const uint32_t part = code_part(run * 2u + s / 2 + PLACES);
       if (s == 0) operands_stand();
-      // Between the products, one every few of them: the step's loads, and what the next step takes from LDS, in the
-      // first three quarters, so that it is there when they meet.
+      // Between the products, one every few of them: a stage's loads, and what the next step takes from LDS, in the first
+      // three quarters, so that it is there when the waves meet.
       constexpr int kProducts = FN * FM, kReads = FN + FM, kAsks = kLoads + kScaleLoads;
       constexpr int kEvery = kProducts * 3 / 4 / kReads > 0 ? kProducts * 3 / 4 / kReads : 1;
       const uint32_t keep = kept(run + 1u);
@@ -214,13 +271,16 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
 #pragma unroll
       for (int p = 0; p < kProducts; ++p) {
         const int i = p / FM, j = p % FM;
-        if (const int q = p * kAsks / kProducts; q != (p + 1) * kAsks / kProducts) {
-          if (q >= (int)kLoads) request_scales(run + 1u + kLead, s * kScaleLoads + q - kLoads);
-          else if ((q < (int)kXLoads ? q : q - (int)kXLoads) % 2 == 0) request(part, s, q);
+        if (s % 2 == 1) {
+          if (const int q = p * kAsks / kProducts; q < (p + 1) * kAsks / kProducts) {
+            if (q >= (int)kLoads) request_scales(run + (s / 2 + PLACES) / 2u + kLead, (s / 2 + PLACES) % 2u * kScaleLoads + q - kLoads);
+            else if ((q < (int)kXLoads ? q : q - (int)kXLoads) % 2 == 0) request(part, place, q);
+          }
         }
         if (p % kEvery == 0 && p / kEvery < kReads) {
           const int f = p / kEvery;
-          if (f < FM) x_held[(s + 1) & 1][f] = read_x((s + 1) & 3, f); else w_held[(s + 1) & 1][f - FM] = read_w((s + 1) & 3, f - FM);
+          const uint32_t from = s % 2 == 0 ? place : next_place;
+          if (f < FM) x_held[(s + 1) & 1][f] = read_x(from, (s + 1) & 1, f); else w_held[(s + 1) & 1][f - FM] = read_w(from, (s + 1) & 1, f - FM);
           if (s == 3) {
             raw[f % 3] = read_scales(run + 1u, f);
             if (f >= 2) next_scale[f - 2] = scale_word(raw[(f - 2) % 3], f - 2, keep);
@@ -233,6 +293,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
         __builtin_amdgcn_sched_barrier(0);
       }
       static_assert((kProducts + kEvery - 1) / kEvery >= kReads && kAsks <= kProducts, "one a product at most, and all of them");
+      if (s % 2 == 1) place = next_place;
       if (s == 3) {
 #pragma unroll
         for (int f = kReads - 2; f < kReads; ++f) next_scale[f] = scale_word(raw[f % 3], f, keep);
@@ -298,26 +359,24 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
       }
 #pragma unroll
       for (int j = 0; j < kX; ++j)
-        mx4_finish<OT, PAIRS, 4>(o, m0 + wm * FM * 16u + (j0 + j) % FM * 16u + r, n0 + wn * FN * 16u + g * 64u + kb * 16u, whole[j]);
+        finish_rows<OT, PAIRS, 4>(o, m0 + (wm * FM + (j0 + j) % FM) * 16u, n0 + wn * FN * 16u + g * 64u, r, kb, whole[j]);
     }
     return;
   }
 #pragma unroll
-  for (int g = 0; g < FN / 4; ++g)
+  for (int j = 0; j < FM; ++j) {
+    v4f row[FN];
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const uint32_t row = m0 + wm * FM * 16u + j * 16u + r, col = n0 + wn * FN * 16u + g * 64u + kb * 16u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (g == 0 && j == 0 && i == 0) settled<true>(sum[0][0]); else settled<false>(sum[4 * g + i][j]);
-      }
-      const v4f sums[4] = {sum[4 * g][j], sum[4 * g + 1][j], sum[4 * g + 2][j], sum[4 * g + 3][j]};
-      mx4_finish<OT, PAIRS, 4>(o, row, col, sums);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < FN; ++i) {
+      if (j == 0 && i == 0) settled<true>(sum[0][0]); else settled<false>(sum[i][j]);
+      row[i] = sum[i][j];
     }
+    finish_rows<OT, PAIRS, FN>(o, m0 + (wm * FM + j) * 16u, n0 + wn * FN * 16u, r, kb, row);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
-template <int FM, int FN, int WM, int WN>
+template <int FM, int FN, int WM, int WN, int PLACES>
 void launch_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, uint32_t parts) {
   constexpr uint32_t BM = WM * FM * 16, BN = WN * FN * 16;
   const uint32_t m_tiles = (p.out.m + BM - 1) / BM, n_tiles = (p.out.n + BN - 1) / BN, runs = (p.blocks + 15) / 16;
@@ -329,8 +388,8 @@ void launch_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, uint
   };
 #define KRM_MX4_TILES(OT, PAIRS)                                                                     \
   do {                                                                                               \
-    if (aligned) launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, true>);       \
-    else launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, false>);              \
+    if (aligned) launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, PLACES, true>);            \
+    else launch(linear_mx4_tile_kernel<OT, PAIRS, FM, FN, WM, WN, PLACES, false>);                   \
   } while (0)
   if (half) { if (pairs) KRM_MX4_TILES(__half, true); else KRM_MX4_TILES(__half, false); }
   else { if (pairs) KRM_MX4_TILES(float, true); else KRM_MX4_TILES(float, false); }
@@ -343,9 +402,15 @@ namespace krm {
 
 int32_t launch_mx4_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, const Mx4Form& form) {
   switch (form.rows) {
-    case 256: launch_tiles<8, 8, 2, 2>(ctx, p, half, pairs, form.parts); break;
-    case 128: launch_tiles<4, 4, 2, 2>(ctx, p, half, pairs, form.parts); break;
-    default: launch_tiles<2, 4, 2, 2>(ctx, p, half, pairs, form.parts); break;
+    case 256: launch_tiles<8, 8, 2, 2, 2>(ctx, p, half, pairs, form.parts); break;
+    case 128:
+      if (form.deep) launch_tiles<4, 4, 2, 2, 4>(ctx, p, half, pairs, form.parts);
+      else launch_tiles<4, 4, 2, 2, 2>(ctx, p, half, pairs, form.parts);
+      break;
+    default:
+      if (form.deep) launch_tiles<2, 4, 2, 2, 5>(ctx, p, half, pairs, form.parts);
+      else launch_tiles<2, 4, 2, 2, 2>(ctx, p, half, pairs, form.parts);
+      break;
   }
   return launched(ctx, "linear_mx4_tile_kernel");
 }

@@ -52,33 +52,34 @@ __device__ inline float mx4_load(const __half* p) { return __half2float(*p); }
 __device__ inline void mx4_store(float* p, float v) { *p = v; }
 __device__ inline void mx4_store(__half* p, float v) { *p = __float2half_rn(v); }
 
-// Four or sixteen neighbouring sums of row `row` from column col on (a multiple of as many): bias, silu(gate) * up where
-// the columns are such pairs, residual, one rounding to the stored type.
+// Neighbouring sums from column col on (a multiple of as many), with bias, and as silu(gate) * up where the columns are such
+// pairs.
 template <typename OT, bool PAIRS, int PIECES>
-__device__ inline void mx4_finish(const Mx4Out& o, uint32_t row, uint32_t col, const v4f (&sum)[PIECES]) {
-  if (row >= o.m || col >= o.n) return;
-  constexpr int kSums = 4 * PIECES, kCount = PAIRS ? kSums / 2 : kSums;
-  float v[kSums];
+__device__ inline void mx4_values(const Mx4Out& o, uint32_t col, const v4f* sum, float (&v)[4 * PIECES]) {
 #pragma unroll
-  for (int i = 0; i < kSums; ++i) v[i] = sum[i / 4][i % 4];
+  for (int i = 0; i < 4 * PIECES; ++i) v[i] = sum[i / 4][i % 4];
   if (o.bias) {
 #pragma unroll
-    for (int i = 0; i < kSums; ++i) v[i] += o.bias[least(col + i, o.n - 1)];
+    for (int i = 0; i < 4 * PIECES; ++i) v[i] += o.bias[least(col + i, o.n - 1)];
   }
   if constexpr (PAIRS) {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) v[i] = mx4_silu<OT>(v[2 * i]) * v[2 * i + 1];
+    for (int i = 0; i < 2 * PIECES; ++i) v[i] = mx4_silu<OT>(v[2 * i]) * v[2 * i + 1];
   }
-  const uint32_t width = PAIRS ? o.n / 2 : o.n, first = PAIRS ? col / 2 : col;
+}
+// COUNT neighbouring values of row `row` from column `first` of the result on: residual, one rounding to the stored type.
+// STREAM: past the caches.
+template <typename OT, int COUNT, bool STREAM>
+__device__ inline void mx4_put(const Mx4Out& o, uint32_t row, uint32_t first, uint32_t width, float* v) {
   const size_t at = (size_t)row * width + first;
   OT* out = static_cast<OT*>(o.out) + at;
   const OT* residual = static_cast<const OT*>(o.residual) + at;
   // packs of a row end where the row does (its bytes are a multiple of a pack's, and so is its address)
   auto store = [&](auto bytes) {
-    constexpr int kPack = decltype(bytes)::value / (int)sizeof(OT) < kCount ? decltype(bytes)::value / (int)sizeof(OT) : kCount;
+    constexpr int kPack = decltype(bytes)::value / (int)sizeof(OT) < COUNT ? decltype(bytes)::value / (int)sizeof(OT) : COUNT;
     struct alignas(kPack * sizeof(OT)) Pack { OT e[kPack]; };
 #pragma unroll
-    for (int p = 0; p < kCount / kPack; ++p) {
+    for (int p = 0; p < COUNT / kPack; ++p) {
       if (first + p * kPack >= width) break;
       Pack pack;
       if (o.residual) {
@@ -88,12 +89,21 @@ __device__ inline void mx4_finish(const Mx4Out& o, uint32_t row, uint32_t col, c
       }
 #pragma unroll
       for (int i = 0; i < kPack; ++i) mx4_store(&pack.e[i], v[p * kPack + i]);
-      reinterpret_cast<Pack*>(out)[p] = pack;
+      if constexpr (STREAM && sizeof(Pack) == 16) __builtin_nontemporal_store(__builtin_bit_cast(v4i, pack), reinterpret_cast<v4i*>(out) + p);
+      else reinterpret_cast<Pack*>(out)[p] = pack;
     }
   };
   if (o.pack == 16u) store(std::integral_constant<int, 16>());
   else if (o.pack == 8u) store(std::integral_constant<int, 8>());
   else store(std::integral_constant<int, (int)sizeof(OT)>());
+}
+// Four neighbouring sums of row `row` from column col on.
+template <typename OT, bool PAIRS>
+__device__ inline void mx4_finish(const Mx4Out& o, uint32_t row, uint32_t col, const v4f& sum) {
+  if (row >= o.m || col >= o.n) return;
+  float v[4];
+  mx4_values<OT, PAIRS, 1>(o, col, &sum, v);
+  mx4_put<OT, PAIRS ? 2 : 4, false>(o, row, PAIRS ? col / 2 : col, PAIRS ? o.n / 2 : o.n, v);
 }
 // Bytes that rows of `width` results, `count` neighbours a lane, can be stored in at once.
 inline uint32_t mx4_pack(uint32_t width, uint32_t count, krm_buf out, krm_buf residual, size_t eb) {

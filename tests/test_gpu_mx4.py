@@ -188,8 +188,9 @@ def test_products_of_floats_are_those_of_their_codes(gpu_ctx, m, n, k, io):
 
 
 # forms that only larger products take, and the same with scales that are no whole words (see test_mx4_plan.py)
-LARGE = [(65, 130, 4096), (70, 130, 4128), (1605, 530, 8192), (1605, 530, 8224), (65, 16530, 64), (65, 16530, 256),
-         (1670, 2330, 8192), (1670, 2330, 8224), (435, 16530, 64), (435, 16530, 256), (16, 500, 8192), (3, 200, 16384)]
+LARGE = [(65, 130, 8192), (70, 130, 8224), (67, 9430, 11008), (67, 9430, 11040), (197, 17830, 11008), (197, 17830, 11040),
+         (65, 16530, 64), (65, 16530, 256), (197, 12230, 64), (197, 12230, 256), (272, 20630, 64), (272, 20630, 256),
+         (517, 19230, 64), (517, 19230, 256), (16, 500, 8192), (3, 200, 16384), (64, 516, 11008), (31, 300, 11040)]
 
 
 @pytest.mark.parametrize("m,n,k", LARGE)

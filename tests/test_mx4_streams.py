@@ -76,7 +76,7 @@ def test_products_in_place(tmp_path):
                 assert not registers(operands[0]) & registers(code[at - 1][1][1]), (name, op, operands)
         assert products in (32, 64, 256), name
         checked += 1
-    assert checked == 3 * 2 * 2 * 2    # tiles, stored types, pairs, whole words
+    assert checked == 5 * 2 * 2 * 2    # tiles and depths, stored types, pairs, whole words
 
 
 def test_rings_are_filled_behind_their_reads(tmp_path):
