@@ -161,6 +161,7 @@ extern "C" int32_t krm_block_norm(krm_ctx* ctx, krm_buf y, krm_buf post_weight, 
                        aligned(norm_out, nb) && aligned(post_weight, 4) && aligned(pre_weight, 4),
               "block_norm: misaligned buffer");
   KRM_REQUIRE(ctx, sum_out != norm_out, "block_norm: sum_out and norm_out are one buffer");
+  KRM_REQUIRE(ctx, !gate || (gate != sum_out && gate != norm_out), "block_norm: a result is the gate's buffer");
   KRM_REQUIRE(ctx, nb == eb || (!norm_out || (norm_out != y && norm_out != residual)),
               "block_norm: norm_out may be y or residual only if their types are the same");
   NormArgs a{ptr<const void>(y),        ptr<const float>(post_weight), ptr<const void>(gate),

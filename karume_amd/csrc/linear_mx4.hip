@@ -10,12 +10,14 @@ using namespace krm;
 namespace {
 
 int32_t check_product(krm_ctx* ctx, krm_buf w, krm_buf w_scales, krm_buf bias, krm_buf residual, krm_buf out,
-                      uint32_t n, uint32_t k, int32_t out_dtype, int32_t epilogue) {
+                      uint32_t m, uint32_t n, uint32_t k, int32_t out_dtype, int32_t epilogue) {
   KRM_REQUIRE(ctx, valid_dtype(out_dtype), "linear mx4: unknown dtype %d", out_dtype);
   KRM_REQUIRE(ctx, epilogue == KRM_EPILOGUE_NONE || epilogue == KRM_EPILOGUE_SILU_PAIRS,
               "linear mx4: unknown epilogue %d", epilogue);
   KRM_REQUIRE(ctx, epilogue == KRM_EPILOGUE_NONE || n % 2 == 0, "linear mx4: pairs need an even n (%u)", n);
   KRM_REQUIRE(ctx, k <= (1u << 24), "linear mx4: k %u is above 2^24", k);
+  // (a launch has fewer than 2^32 threads: 256 a tile, of 64 x 128 at least)
+  KRM_REQUIRE(ctx, ((m + 63ull) / 64) * ((n + 127ull) / 128) < (1u << 24) - 8u, "linear mx4: %u x %u is too large", m, n);
   KRM_REQUIRE(ctx, k > 0 && k % kMx4Block == 0, "linear mx4: k must be a positive multiple of 32 (%u)", k);
   const size_t eb = dtype_bytes(out_dtype);
   KRM_REQUIRE(ctx, aligned(w, 16) && aligned(out, eb) && aligned(residual, eb) && aligned(bias, 4),
@@ -41,7 +43,6 @@ int32_t launch_product(krm_ctx* ctx, krm_buf xq, krm_buf xs, krm_buf w, krm_buf 
   const Mx4Form form = mx4_form(m, n, k, ctx->num_cus, serial ? 2 * kGemmPartialBytes * ctx->num_cus : 0,
                                 serial ? kTicketSlots : 0);
   const bool tiles = form.kernel == Mx4Kernel::kTiles;
-  KRM_REQUIRE(ctx, !tiles || mx4_tile_count(form.rows, m, n) * form.parts <= 0x7ffffff0ull, "linear mx4: %u x %u is too large", m, n);
   const Mx4Product p = product_of(xq, xs, w, w_scales, bias, residual, out, m, n, k, out_dtype, pairs, tiles ? 16 : 4);
   if (form.kernel == Mx4Kernel::kRows) return launch_mx4_rows(ctx, p, half, pairs);
   return tiles ? launch_mx4_tiles(ctx, p, half, pairs, form) : launch_mx4_batch(ctx, p, half, pairs);
@@ -53,7 +54,7 @@ extern "C" int32_t krm_linear_mx4(krm_ctx* ctx, krm_buf xq, krm_buf xs, krm_buf 
                                   krm_buf residual, krm_buf out, uint32_t m, uint32_t n, uint32_t k,
                                   int32_t out_dtype, int32_t epilogue) {
   KRM_TRY(enter(ctx));
-  KRM_TRY(check_product(ctx, w, w_scales, bias, residual, out, n, k, out_dtype, epilogue));
+  KRM_TRY(check_product(ctx, w, w_scales, bias, residual, out, m, n, k, out_dtype, epilogue));
   KRM_REQUIRE(ctx, aligned(xq, 16), "linear mx4: misaligned buffer (codes need 16 bytes)");
   if (m == 0 || n == 0) return KRM_OK;
   KRM_REQUIRE(ctx, xq && xs && w && w_scales && out, "linear mx4: null buffer");
@@ -65,7 +66,7 @@ extern "C" int32_t krm_linear_mx4_fused(krm_ctx* ctx, krm_buf x, krm_buf xq, krm
                                         uint32_t n, uint32_t k, uint64_t x_stride, int32_t x_dtype,
                                         int32_t out_dtype, int32_t scale_rule, int32_t epilogue) {
   KRM_TRY(enter(ctx));
-  KRM_TRY(check_product(ctx, w, w_scales, bias, residual, out, n, k, out_dtype, epilogue));
+  KRM_TRY(check_product(ctx, w, w_scales, bias, residual, out, m, n, k, out_dtype, epilogue));
   if (m == 0 || n == 0) return KRM_OK;
   KRM_REQUIRE(ctx, x && w && w_scales && out, "linear mx4: null buffer");
   if (mx4_rows_fit(m, k)) {

@@ -40,8 +40,9 @@ static_assert(kHeld<4, 2, false> >= kMx4HeldBytes && kHeld<4, 2, true> >= kMx4He
 // One workgroup a CU walks pieces of 16 rows of w.  Eight waves share a piece's turns in a fixed order, each with a ring
 // of its own in LDS that memory fills without registers or barriers, over the ends of pieces too; another eight
 // bring x meanwhile and leave.  Those that bring x come first: asked for behind a CU's rows of w, x would arrive behind
-// them (1 x 4096 x 4096 4.8 us, so 4.1; 8 x 22016 x 4096 15.0 / 13.1; 1 x 4096 x 11008 8.8 / 7.5).  The streaming waves join their sums in LDS, one wave in turn stores a piece.  The order of a row's
-// sums depends on K alone, so that it does not matter where x came from.
+// them (1 x 4096 x 4096 4.8 us, so 4.1; 8 x 22016 x 4096 15.0 / 13.1; 1 x 4096 x 11008 8.8 / 7.5).  The streaming waves join
+// their sums in LDS, one wave in turn stores a piece.  The order of a row's sums depends on K alone, so that it does not
+// matter where x came from.
 // Bound by w's bytes: what a CU has on its way (96 KiB) is what keeps memory busy.
 template <typename OT, bool PAIRS, typename X, int U, int DEPTH, bool ALIGNED>
 __global__ __launch_bounds__(kThreads) void linear_mx4_rows_kernel(X x, const uint8_t* __restrict__ w,

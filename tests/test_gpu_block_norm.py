@@ -117,7 +117,8 @@ def test_refusals(gpu_ctx):
                dict(gate_kind=2), dict(norm_out=None), dict(pre_weight=None), dict(sum_out=None, norm_out=None, pre_weight=None),
                dict(sum_out=at + 12289), dict(residual=at + 2), dict(pre_weight=at + 2), dict(post_weight=at + 1),
                dict(gate=at + 3), dict(norm_out=at + 12288), dict(norm_dtype=ka.F16, norm_out=at),
-               dict(norm_dtype=ka.F16, norm_out=at + 4096), dict(norm_out=at + 16385)):
+               dict(norm_dtype=ka.F16, norm_out=at + 4096), dict(norm_out=at + 16385), dict(gate=at + 12288),
+               dict(gate=at + 16384, gate_span=1)):
         with pytest.raises(ka.GpuValidationError):
             gpu_ctx.block_norm(at, **{**good, **kw})
     with pytest.raises(ka.GpuValidationError):

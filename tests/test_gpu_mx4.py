@@ -346,6 +346,9 @@ def test_refusals(gpu_ctx):
     for m, n, k, kw in ((2, 4, 0, {}), (2, 4, 48, {}), (2, 3, 64, dict(epilogue=1)), (2, 4, 64, dict(epilogue=2)),
                         (2, 4, 64, dict(out_dtype=5)), (2, 4, 64, dict(bias=at + 2)), (2, 4, 64, dict(residual=at + 2))):
         refused(p, at, at, at, at, at, m, n, k, **kw)
+    for m, n, k in ((2, 4, (1 << 24) + 32), (1 << 31, 4, 64), ((1 << 32) - 1, 4, 64), (2, (1 << 32) - 1, 64), (17, 1 << 31, 64),
+                    (1 << 30, 16, 64), (1 << 20, 1 << 17, 64)):
+        refused(p, at, at, at, at, at, m, n, k)
     for i in range(5):
         args = [at] * 5
         args[i] = 0
