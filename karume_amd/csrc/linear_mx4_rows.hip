@@ -43,7 +43,9 @@ static_assert(kHeld<4, 2, false> >= kMx4HeldBytes && kHeld<4, 2, true> >= kMx4He
 // them (1 x 4096 x 4096 4.8 us, so 4.1; 8 x 22016 x 4096 15.0 / 13.1; 1 x 4096 x 11008 8.8 / 7.5).  The streaming waves join
 // their sums in LDS, one wave in turn stores a piece.  The order of a row's sums depends on K alone, so that it does not
 // matter where x came from.
-// Bound by w's bytes: what a CU has on its way (96 KiB) is what keeps memory busy.
+// Bound by w's bytes: what a CU has on its way (96 KiB) is what keeps memory busy.  1 x 65536 x 4096 26 us, 5.5 TB/s;
+// 16 x 32000 x 2048 11.0 us, 3.3 TB/s, eight pieces of two turns a wave each; 1 x 4096 x 4096 3.9 us, of which 2 are a launch.
+// (Lines of 128 bytes a load as in the batch's kernel: no difference past 1 %.)
 template <typename OT, bool PAIRS, typename X, int U, int DEPTH, bool ALIGNED>
 __global__ __launch_bounds__(kThreads) void linear_mx4_rows_kernel(X x, const uint8_t* __restrict__ w,
                                                                    const uint8_t* __restrict__ ws, uint32_t blocks,
@@ -253,14 +255,16 @@ __global__ __launch_bounds__(64 * kBatchStreams) void linear_mx4_batch_kernel(co
     const uint8_t* const ws_piece = ws + (size_t)n0 * blocks;
     const uint32_t lds = ring_lds + at.slot * kBytes, block = least(from + chunk, blocks - 1u);
 #pragma unroll
-    for (uint32_t b = 0; b < 2; ++b) stream_to_lds(lds + b * 1024u, (least(b * 8u + lane / 8u, n_last) * blocks + block) * 16u, w_piece);
+    for (uint32_t b = 0; b < 2; ++b)
+      stream_to_lds(lds + b * 1024u, (least(b * 8u + lane / 8u, n_last) * blocks + block) * 16u, w_piece);
 #pragma unroll
     for (uint32_t b = 0; b < 2 * MB; ++b) stream_to_lds(lds + (2u + b) * 1024u, (x_row[b] + block) * 16u, xq);
     if constexpr (ALIGNED) {
       const uint32_t word = least(from + (lane & 1u) * 4u, blocks - 4u);
       stream_word_to_lds(lds + kScalesAt, least(least(lane / 2u, 15u), n_last) * blocks + word, ws_piece, false);
 #pragma unroll
-      for (uint32_t b = 0; b < kXWords; ++b) stream_word_to_lds(lds + kScalesAt + 256u + b * 256u, x_scale_row[b] + word, xs, false);
+      for (uint32_t b = 0; b < kXWords; ++b)
+        stream_word_to_lds(lds + kScalesAt + 256u + b * 256u, x_scale_row[b] + word, xs, false);
     } else {
 #pragma unroll
       for (uint32_t h = 0; h < 2; ++h) {
@@ -296,7 +300,8 @@ __global__ __launch_bounds__(64 * kBatchStreams) void linear_mx4_batch_kernel(co
 #pragma unroll
       for (uint32_t b = 0; b < MB; ++b) {
         xc[h][b] = *reinterpret_cast<const v4i*>(turn + (1u + b) * 2048u + code);
-        x_word[h][b] = *reinterpret_cast<const uint32_t*>(turn + kScalesAt + (ALIGNED ? 256u + ((b * 16u + r) * 2u + h) * 4u : ((1u + b) * 2u + h) * 256u + lane * 4u));
+        const uint32_t word = ALIGNED ? 256u + ((b * 16u + r) * 2u + h) * 4u : ((1u + b) * 2u + h) * 256u + lane * 4u;
+        x_word[h][b] = *reinterpret_cast<const uint32_t*>(turn + kScalesAt + word);
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the turn's place is free
@@ -376,10 +381,10 @@ void launch_batch(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs) {
   const bool words = p.blocks % 4 == 0 && aligned((krm_buf)(uintptr_t)p.xs | (krm_buf)(uintptr_t)p.ws, 4);
   const uint32_t pieces = (p.out.n + 15) / 16, grid = pieces < (uint32_t)ctx->num_cus ? pieces : ctx->num_cus;
   auto launch = [&](auto kernel) { kernel<<<grid, 64 * kBatchStreams, 0, ctx->stream>>>(p.xq, p.xs, p.w, p.ws, p.blocks, p.out); };
-#define KRM_MX4_BATCH(OT, PAIRS)                                                    \
-  do {                                                                              \
-    if (words) launch(linear_mx4_batch_kernel<OT, PAIRS, MB, DEPTH, true>);         \
-    else launch(linear_mx4_batch_kernel<OT, PAIRS, MB, DEPTH == 3 ? 2 : DEPTH, false>);              \
+#define KRM_MX4_BATCH(OT, PAIRS)                                                         \
+  do {                                                                                   \
+    if (words) launch(linear_mx4_batch_kernel<OT, PAIRS, MB, DEPTH, true>);              \
+    else launch(linear_mx4_batch_kernel<OT, PAIRS, MB, DEPTH == 3 ? 2 : DEPTH, false>); \
   } while (0)
   if (half) { if (pairs) KRM_MX4_BATCH(__half, true); else KRM_MX4_BATCH(__half, false); }
   else { if (pairs) KRM_MX4_BATCH(float, true); else KRM_MX4_BATCH(float, false); }

@@ -45,7 +45,8 @@ constexpr uint32_t kMx4Beside = (PAIRS ? 2 : 1) * 4 / sizeof(OT);
 // of lines through the caches: 4096 x 22016 x 4096 249 us, past them 230, whole lines past them 220; halves of 32 bytes past
 // them no better than through them.)
 template <typename OT, bool PAIRS, int PIECES>
-__device__ inline void finish_rows(const Mx4Out& o, uint32_t row0, uint32_t col0, uint32_t r, uint32_t kb, const v4f (&sum)[PIECES]) {
+__device__ inline void finish_rows(const Mx4Out& o, uint32_t row0, uint32_t col0, uint32_t r, uint32_t kb,
+                                   const v4f (&sum)[PIECES]) {
   constexpr uint32_t kBeside = kMx4Beside<OT, PAIRS>, kSets = PIECES / kBeside, kValues = 16 / sizeof(OT);
   constexpr uint32_t kTogether = kSets > 1 ? 2 : 1;
   const uint32_t width = PAIRS ? o.n / 2 : o.n;
@@ -196,8 +197,12 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
   const uint32_t code_at = r * 128u + ((kb ^ (r & 7u)) * 16u);
   const uint8_t* const w_pieces[2] = {s_w + wn * FN * 2048u + code_at, s_w + wn * FN * 2048u + (code_at ^ 64u)};
   const uint8_t* const x_pieces[2] = {s_x + wm * FM * 2048u + code_at, s_x + wm * FM * 2048u + (code_at ^ 64u)};
-  auto read_w = [&](uint32_t place, int step, int i) { return *reinterpret_cast<const v4i*>(w_pieces[step] + place * BN * 128u + i * 2048); };
-  auto read_x = [&](uint32_t place, int step, int j) { return *reinterpret_cast<const v4i*>(x_pieces[step] + place * BM * 128u + j * 2048); };
+  auto read_w = [&](uint32_t place, int step, int i) {
+    return *reinterpret_cast<const v4i*>(w_pieces[step] + place * BN * 128u + i * 2048);
+  };
+  auto read_x = [&](uint32_t place, int step, int j) {
+    return *reinterpret_cast<const v4i*>(x_pieces[step] + place * BM * 128u + j * 2048);
+  };
   // byte kb of four words, one a step
   const uint32_t pick = 0x0c0c0400u + kb * 0x0101u;
   const uint32_t x_low = (r & 3u) * blocks + xs_low, w_low = (r & 3u) * blocks + ws_low;  // where a row begins in its word
@@ -280,7 +285,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
         if (p % kEvery == 0 && p / kEvery < kReads) {
           const int f = p / kEvery;
           const uint32_t from = s % 2 == 0 ? place : next_place;
-          if (f < FM) x_held[(s + 1) & 1][f] = read_x(from, (s + 1) & 1, f); else w_held[(s + 1) & 1][f - FM] = read_w(from, (s + 1) & 1, f - FM);
+          constexpr int kNext[4] = {1, 0, 1, 0};
+          if (f < FM) x_held[kNext[s]][f] = read_x(from, kNext[s], f);
+          else w_held[kNext[s]][f - FM] = read_w(from, kNext[s], f - FM);
           if (s == 3) {
             raw[f % 3] = read_scales(run + 1u, f);
             if (f >= 2) next_scale[f - 2] = scale_word(raw[(f - 2) % 3], f - 2, keep);

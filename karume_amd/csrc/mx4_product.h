@@ -89,8 +89,9 @@ __device__ inline void mx4_put(const Mx4Out& o, uint32_t row, uint32_t first, ui
       }
 #pragma unroll
       for (int i = 0; i < kPack; ++i) mx4_store(&pack.e[i], v[p * kPack + i]);
-      if constexpr (STREAM && sizeof(Pack) == 16) __builtin_nontemporal_store(__builtin_bit_cast(v4i, pack), reinterpret_cast<v4i*>(out) + p);
-      else reinterpret_cast<Pack*>(out)[p] = pack;
+      Pack* const to = reinterpret_cast<Pack*>(out) + p;
+      if constexpr (STREAM && sizeof(Pack) == 16) __builtin_nontemporal_store(__builtin_bit_cast(v4i, pack), reinterpret_cast<v4i*>(to));
+      else *to = pack;
     }
   };
   if (o.pack == 16u) store(std::integral_constant<int, 16>());

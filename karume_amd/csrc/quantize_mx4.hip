@@ -10,7 +10,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A thread has eight elements, four threads a block.  Bound by bytes: 2 or 4 in and 17/32 out an element.
+// A thread has eight elements, four threads a block (they exchange its largest magnitude in registers): whole pieces of 16
+// bytes in, a word of codes out.  Bound by bytes, 2 or 4 in and 17/32 out an element: 4099 rows of 11008 f32 36.9 us,
+// 5.5 TB/s, of fp16 18.5, 6.2 (two or four rows a thread: within 3 %, and few rows slower); 16 rows of 4096 a launch.
 template <typename XT>
 __global__ __launch_bounds__(kThreads) void quantize_mx4_kernel(const XT* __restrict__ x,
                                                                 uint32_t* __restrict__ codes,
@@ -36,6 +38,7 @@ __device__ inline float mx4_value(uint32_t code, uint32_t byte) {
   return code & 8u ? -v : v;
 }
 
+// Bound by what it writes: the same rows back as f32 33.6 us, 6.1 TB/s.
 template <typename OT>
 __global__ __launch_bounds__(kThreads) void dequant_mx4_kernel(const uint32_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales,
