@@ -80,14 +80,14 @@ __device__ inline void finish_rows(const Mx4Out& o, uint32_t row0, uint32_t col0
 //   m x n x k                256 x 256   128 x 128   64 x 128
 //   8192 x 8192 x 8192             255         358        475   (4.3 PFLOP/s)
 //   512 x 22016 x 4096, pairs       36          46         60
-//   1001 x 4100 x 11040            100          65         89
+//   1001 x 4100 x 11040            100          53         89
 //   509 x 2560 x 2048               21         9.5        7.6
 // Bound by power and by the matrix cores' waits for operands: at 8192 cubed the cores run at 1.8 GHz and are busy half of the
 // time; 232 us without the stores, 245 without the reads from LDS, 196 without reads and loads, 165 at the rate that
 // products of random codes reach from registers.
 //
 // A stage is 256 codes of every row: 128 bytes, a whole line (of half lines a CU gets half as many bytes a second of rows of
-// its own: 58 GB/s, so 107; 1001 x 4100 x 11040 in 128 x 128 tiles 84 us, so 65).  PLACES stages in LDS, two steps of 128
+// its own: 58 GB/s, so 107; 1001 x 4100 x 11040 in 128 x 128 tiles 84 us, so 65, no tile shared).  PLACES stages in LDS, two steps of 128
 // codes in each: two, or as many as fit where no CU has two workgroups (256 x 4096 x 4096 12.4 us with two, 10.5 with five;
 // 1024 x 4096 x 4096, two workgroups a CU, 17.8 and 21.2).  The operands of a step are read from LDS during the step before
 // it.  In front of a stage's second step the waves meet: the next stage is there, and the place of this one, all of which has
@@ -122,13 +122,15 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
 
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t r = lane & 15u, kb = lane >> 4;
-  uint32_t mt, nt, part_of;
-  if (!mx4_tile_of(blockIdx.x, m_tiles, n_tiles, split.parts, mt, nt, part_of)) return;  // the whole workgroup leaves
-  const uint32_t m0 = mt * BM, n0 = nt * BN;
+  Mx4Tile tile_at;
+  if (!mx4_tile_of(blockIdx.x, m_tiles, n_tiles, split.whole, split.parts, tile_at)) return;  // the whole workgroup leaves
+  const uint32_t m0 = tile_at.mt * BM, n0 = tile_at.nt * BN;
   const uint32_t wm = wave / WN, wn = wave % WN;
   // this workgroup's runs of the tile
   const uint32_t runs = (blocks + 15u) / 16u;
-  const uint32_t run0 = split.first_run(part_of), run_end = least(split.first_run(part_of + 1u), runs);
+  const uint32_t part_of = tile_at.part, parts = tile_at.parts;
+  const uint32_t run0 = parts > 1u ? split.first_run(part_of) : 0u;
+  const uint32_t run_end = parts > 1u ? least(split.first_run(part_of + 1u), runs) : runs;
   const uint32_t stages = least(run_end * 2u, (blocks + 7u) / 8u);
   const uint32_t m_last = o.m - 1u - m0, n_last = o.n - 1u - n0;  // rows past it: itself again, not stored
   const uint8_t* const x_tile = xq + (size_t)m0 * blocks * 16u;
@@ -312,11 +314,11 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
     }
   }
   wait_vm<0>();  // (nothing may land in LDS that is another workgroup's)
-  if (split.parts > 1u) {
+  if (parts > 1u) {
     // pieces of a workgroup's sums: 16 bytes of thread t at [piece][t]
     constexpr uint32_t kPieces = FN * FM;
-    v4f* const tile = reinterpret_cast<v4f*>(split.sums) + (size_t)(mt * n_tiles + nt) * split.parts * kPieces * kThreads + threadIdx.x;
-    uint32_t* const ticket = split.tickets + (size_t)(mt * n_tiles + nt) * kTicketStride;
+    v4f* const tile = reinterpret_cast<v4f*>(split.sums) + (size_t)tile_at.shared * parts * kPieces * kThreads + threadIdx.x;
+    uint32_t* const ticket = split.tickets + (size_t)tile_at.shared * kTicketStride;
     __shared__ uint32_t s_arrived;
 #pragma unroll
     for (int i = 0; i < FN; ++i)
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
     __syncthreads();
     if (threadIdx.x == 0) s_arrived = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (s_arrived + 1u != split.parts) return;
+    if (s_arrived + 1u != parts) return;
     if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // sixteen neighbouring columns of some pieces of x from some parts at once: 128 registers of loads on their way, or 64
     // (a CU holds two workgroups of 128 x 128 up to 256 registers a lane)
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
     for (int j0 = 0; j0 < FM * (FN / 4); j0 += kX) {
       const int g = j0 / FM;
       v4f whole[kX][4];
-      for (uint32_t part = 0; part < split.parts; part += kAtOnce) {
+      for (uint32_t part = 0; part < parts; part += kAtOnce) {
         uint64_t raw[kAtOnce][kX][4][2];
 #pragma unroll
         for (int a = 0; a < kAtOnce; ++a)
@@ -347,13 +349,13 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint64_t* from = reinterpret_cast<const uint64_t*>(
-                  tile + ((size_t)least(part + a, split.parts - 1u) * kPieces + (4 * g + i) * FM + (j0 + j) % FM) * kThreads);
+                  tile + ((size_t)least(part + a, parts - 1u) * kPieces + (4 * g + i) * FM + (j0 + j) % FM) * kThreads);
               raw[a][j][i][0] = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
               raw[a][j][i][1] = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
 #pragma unroll
         for (int a = 0; a < kAtOnce; ++a) {
-          if (part + a >= split.parts) break;
+          if (part + a >= parts) break;
 #pragma unroll
           for (int j = 0; j < kX; ++j)
 #pragma unroll
@@ -384,12 +386,12 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_mx4_tile_kernel(
 }
 
 template <int FM, int FN, int WM, int WN, int PLACES>
-void launch_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, uint32_t parts) {
+void launch_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, const Mx4Form& form) {
   constexpr uint32_t BM = WM * FM * 16, BN = WN * FN * 16;
   const uint32_t m_tiles = (p.out.m + BM - 1) / BM, n_tiles = (p.out.n + BN - 1) / BN, runs = (p.blocks + 15) / 16;
   const bool aligned = p.blocks % 4 == 0 && krm::aligned((krm_buf)(uintptr_t)p.xs | (krm_buf)(uintptr_t)p.ws, 4);
-  const Mx4Split split{parts, runs / parts, runs % parts, ctx->gemm_partials, ctx->tickets};
-  const dim3 grid(mx4_tile_grid(m_tiles, n_tiles, parts));
+  const Mx4Split split{form.whole, form.parts, runs / form.parts, runs % form.parts, ctx->gemm_partials, ctx->tickets};
+  const dim3 grid(mx4_tile_grid(m_tiles * n_tiles, form.whole, form.parts));
   auto launch = [&](auto kernel) {
     kernel<<<grid, 64 * WM * WN, 0, ctx->stream>>>(p.xq, p.xs, p.w, p.ws, p.blocks, m_tiles, n_tiles, split, p.out);
   };
@@ -409,14 +411,14 @@ namespace krm {
 
 int32_t launch_mx4_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, const Mx4Form& form) {
   switch (form.rows) {
-    case 256: launch_tiles<8, 8, 2, 2, 2>(ctx, p, half, pairs, form.parts); break;
+    case 256: launch_tiles<8, 8, 2, 2, 2>(ctx, p, half, pairs, form); break;
     case 128:
-      if (form.deep) launch_tiles<4, 4, 2, 2, 4>(ctx, p, half, pairs, form.parts);
-      else launch_tiles<4, 4, 2, 2, 2>(ctx, p, half, pairs, form.parts);
+      if (form.deep) launch_tiles<4, 4, 2, 2, 4>(ctx, p, half, pairs, form);
+      else launch_tiles<4, 4, 2, 2, 2>(ctx, p, half, pairs, form);
       break;
     default:
-      if (form.deep) launch_tiles<2, 4, 2, 2, 5>(ctx, p, half, pairs, form.parts);
-      else launch_tiles<2, 4, 2, 2, 2>(ctx, p, half, pairs, form.parts);
+      if (form.deep) launch_tiles<2, 4, 2, 2, 5>(ctx, p, half, pairs, form);
+      else launch_tiles<2, 4, 2, 2, 2>(ctx, p, half, pairs, form);
       break;
   }
   return launched(ctx, "linear_mx4_tile_kernel");

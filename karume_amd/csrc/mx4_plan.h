@@ -7,13 +7,14 @@
 namespace krm {
 
 // kRows: up to 16 rows of x that fit LDS, floats too.  kBatch: up to 64 rows of codes.  kTiles: tiles of `rows` rows of x
-// (256: by 256 rows of w, else by 128), each shared by `parts` workgroups that have some of K each.  `deep`: with a CU's whole
-// LDS to a workgroup, where no CU has two.
+// (256: by 256 rows of w, else by 128), those behind the first `whole` ones shared by `parts` workgroups that have some of K each.
+// `deep`: with a CU's whole LDS to a workgroup, where no CU has two.
 enum class Mx4Kernel : uint32_t { kRows, kBatch, kTiles };
 struct Mx4Form {
   Mx4Kernel kernel;
   uint32_t rows, parts;
   bool deep;
+  uint32_t whole;
 };
 
 constexpr uint32_t kMx4HeldBytes = 64u * 1024u;  // of x in LDS beside two turns of every wave (linear_mx4_rows.hip)
@@ -56,8 +57,8 @@ inline bool mx4_deep(uint32_t rows, uint64_t workgroups, uint32_t cus) { return 
 
 // `scratch`: bytes for the sums of parts, `counters` of tiles that are shared; 0 where a tile must not be shared.
 inline Mx4Form mx4_form(uint32_t m, uint32_t n, uint32_t k, uint32_t cus, uint64_t scratch, uint32_t counters) {
-  if (mx4_rows_fit(m, k)) return {Mx4Kernel::kRows, 16, 1, false};
-  Mx4Form best{Mx4Kernel::kBatch, 64, 1, false};
+  if (mx4_rows_fit(m, k)) return {Mx4Kernel::kRows, 16, 1, false, 0};
+  Mx4Form best{Mx4Kernel::kBatch, 64, 1, false, 0};
   float us = m <= 64 ? mx4_batch_us(m, n, k, cus) : 3.4e38f;
   for (uint32_t rows : {64u, 128u, 256u}) {
     const uint64_t tiles = mx4_tile_count(rows, m, n);
@@ -65,8 +66,19 @@ inline Mx4Form mx4_form(uint32_t m, uint32_t n, uint32_t k, uint32_t cus, uint64
       const uint64_t bytes = tiles * parts * rows * (rows == 256 ? 256u : 128u) * 4u;
       if (parts > 1 && (parts > (k + 511) / 512 || bytes > scratch || tiles > counters)) break;
       const float estimate = mx4_tiles_us(rows, parts, tiles, k, cus);
-      if (estimate < us) us = estimate, best = {Mx4Kernel::kTiles, rows, parts, mx4_deep(rows, tiles * parts, cus)};
+      if (estimate < us) us = estimate, best = {Mx4Kernel::kTiles, rows, parts, mx4_deep(rows, tiles * parts, cus), parts > 1 ? 0u : (uint32_t)tiles};
     }
+  }
+  // A last round of few tiles of 128 rows is shared: its CUs would hold one workgroup more than the others.  1.05 to 1.29
+  // times as fast where K is above 6144 (1001 x 4100 x 11040, 264 tiles, 65.2 us, so 52.5; 1200 x 4096 x 8192, 320 tiles, 40.6 /
+  // 36.4); the join takes it away again below (1100 x 4096 x 4096 21.2 / 22.6), and so does a last round past 7/16 of the CUs
+  // (K of 11744 and 357 tiles 76.8 / 68.0, of 11296 and 396 tiles 70.3 / 89.0).  (Tiles of 64 rows are not picked where there
+  // are two rounds of them and such a K.)
+  const uint32_t runs = (k + 511) / 512;
+  if (best.kernel == Mx4Kernel::kTiles && best.rows == 128 && best.parts == 1 && best.whole > cus && runs > 12) {
+    const uint32_t last = best.whole % cus, parts = last * 3 <= cus ? 3 : 2;
+    if (last > 0 && last * 16 <= cus * 7 && (uint64_t)last * parts * 128u * 128u * 4u <= scratch && last <= counters)
+      best.parts = parts, best.whole -= last;
   }
   return best;
 }

@@ -18,9 +18,10 @@ int32_t launch_mx4_rows_of(krm_ctx* ctx, const Mx4Product& p, krm_buf x, uint64_
 int32_t launch_mx4_batch(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs);
 int32_t launch_mx4_tiles(krm_ctx* ctx, const Mx4Product& p, bool half, bool pairs, const Mx4Form& form);
 
-// Runs of 512 codes dealt to the workgroups of a tile, and where those leave their sums.
+// Tiles from `whole` on (in the order below) are shared by `parts` workgroups: runs of 512 codes dealt to them, and where
+// they leave their sums.
 struct Mx4Split {
-  uint32_t parts, each, extra;  // the first `extra` parts have one run more
+  uint32_t whole, parts, each, extra;  // the first `extra` parts have one run more
   float* sums;
   uint32_t* tickets;            // one a tile, kTicketStride words apart, zero at rest
   __host__ __device__ uint32_t first_run(uint32_t part) const { return part * each + (part < extra ? part : extra); }
@@ -29,20 +30,29 @@ struct Mx4Split {
 // Workgroups go to the eight XCDs in turn.  Each XCD has a run of the tiles' order, in which four tiles of x follow
 // one another for a tile of w (neighbours in time share both through its L2) and the parts of a tile one another.
 constexpr uint32_t kMx4Xcds = 8, kMx4Band = 4;
-__host__ __device__ inline uint32_t mx4_tile_grid(uint32_t m_tiles, uint32_t n_tiles, uint32_t parts) {
-  return (m_tiles * n_tiles * parts + kMx4Xcds - 1) / kMx4Xcds * kMx4Xcds;
+__host__ __device__ inline uint32_t mx4_tile_grid(uint32_t tiles, uint32_t whole, uint32_t parts) {
+  return ((whole + kMx4Xcds - 1) / kMx4Xcds + ((tiles - whole) * parts + kMx4Xcds - 1) / kMx4Xcds) * kMx4Xcds;
 }
-__host__ __device__ inline bool mx4_tile_of(uint32_t block, uint32_t m_tiles, uint32_t n_tiles, uint32_t parts,
-                                            uint32_t& mt, uint32_t& nt, uint32_t& part) {
-  const uint32_t count = m_tiles * n_tiles * parts, run = (count + kMx4Xcds - 1) / kMx4Xcds;
-  const uint32_t unit = block % kMx4Xcds * run + block / kMx4Xcds;
+struct Mx4Tile {
+  uint32_t mt, nt;
+  uint32_t shared, part, parts;  // which of the shared tiles; one part: of none
+};
+__host__ __device__ inline bool mx4_tile_of(uint32_t block, uint32_t m_tiles, uint32_t n_tiles, uint32_t whole, uint32_t parts,
+                                            Mx4Tile& t) {
+  const uint32_t alone = (whole + kMx4Xcds - 1) / kMx4Xcds * kMx4Xcds;
+  const bool shares = block >= alone;
+  const uint32_t count = shares ? (m_tiles * n_tiles - whole) * parts : whole;
+  const uint32_t in_order = shares ? block - alone : block, run = (count + kMx4Xcds - 1) / kMx4Xcds;
+  const uint32_t unit = in_order % kMx4Xcds * run + in_order / kMx4Xcds;
   if (unit >= count) return false;
-  const uint32_t at = unit / parts;
-  part = unit - at * parts;
+  t.parts = shares ? parts : 1u;
+  t.shared = unit / t.parts;
+  t.part = unit - t.shared * t.parts;
+  const uint32_t at = shares ? whole + t.shared : unit;
   const uint32_t band = at / (kMx4Band * n_tiles), in_band = at - band * kMx4Band * n_tiles;
   const uint32_t high = m_tiles - band * kMx4Band < kMx4Band ? m_tiles - band * kMx4Band : kMx4Band;
-  nt = in_band / high;
-  mt = band * kMx4Band + in_band % high;
+  t.nt = in_band / high;
+  t.mt = band * kMx4Band + in_band % high;
   return true;
 }
 

@@ -190,7 +190,8 @@ def test_products_of_floats_are_those_of_their_codes(gpu_ctx, m, n, k, io):
 # forms that only larger products take, and the same with scales that are no whole words (see test_mx4_plan.py)
 LARGE = [(65, 130, 8192), (70, 130, 8224), (67, 9430, 11008), (67, 9430, 11040), (197, 17830, 11008), (197, 17830, 11040),
          (65, 16530, 64), (65, 16530, 256), (197, 12230, 64), (197, 12230, 256), (272, 20630, 64), (272, 20630, 256),
-         (517, 19230, 64), (517, 19230, 256), (16, 500, 8192), (3, 200, 16384), (64, 516, 11008), (31, 300, 11040)]
+         (517, 19230, 64), (517, 19230, 256), (16, 500, 8192), (3, 200, 16384), (64, 516, 11008), (31, 300, 11040),
+         (131, 22030, 6656), (197, 16430, 6656), (197, 16430, 6688)]
 
 
 @pytest.mark.parametrize("m,n,k", LARGE)

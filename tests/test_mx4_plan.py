@@ -13,7 +13,7 @@ SHIM = """
 #include "mx4_plan.h"
 extern "C" void form(uint32_t m, uint32_t n, uint32_t k, uint64_t scratch, uint32_t counters, uint32_t* out) {
   const krm::Mx4Form f = krm::mx4_form(m, n, k, 256, scratch, counters);
-  out[0] = (uint32_t)f.kernel; out[1] = f.rows; out[2] = f.parts; out[3] = f.deep;
+  out[0] = (uint32_t)f.kernel; out[1] = f.rows; out[2] = f.parts; out[3] = f.deep; out[4] = f.whole;
 }
 extern "C" uint32_t fits(uint32_t m, uint32_t k) { return krm::mx4_rows_fit(m, k); }
 """
@@ -34,7 +34,7 @@ def plan(tmp_path_factory):
 
 
 def form(plan, m, n, k, scratch=SCRATCH, counters=COUNTERS):
-    out = (C.c_uint32 * 4)()
+    out = (C.c_uint32 * 5)()
     plan.form(m, n, k, C.c_uint64(scratch), counters, out)
     return tuple(out)
 
@@ -42,7 +42,7 @@ def form(plan, m, n, k, scratch=SCRATCH, counters=COUNTERS):
 def test_every_form_has_a_product_that_the_gpu_tests_run(plan):
     seen = set()
     for m, n, k in test_gpu_mx4.PRODUCTS + test_gpu_mx4.LARGE:
-        kernel, rows, parts, deep = form(plan, m, n, k)
+        kernel, rows, parts, deep, whole = form(plan, m, n, k)
         words = k % 128 == 0
         if kernel == ROWS:
             steps = (k + 127) // 128
@@ -51,12 +51,16 @@ def test_every_form_has_a_product_that_the_gpu_tests_run(plan):
             seen.add((kernel, 32 if m <= 32 else 64, words))
         else:
             seen.add((kernel, rows, deep, parts > 1, words))
+            if parts > 1 and whole:
+                seen.add(("last round", rows, parts, words))
     for words in (True, False):
         assert {(ROWS, u, words) for u in (1, 2, 4)} <= seen
         assert {(BATCH, rows, words) for rows in (32, 64)} <= seen
         assert {(TILES, rows, True, shared, words) for rows in (64, 128) for shared in (True, False)} <= seen
         assert {(TILES, rows, False, False, words) for rows in (64, 128, 256)} <= seen
         assert (TILES, 256, False, True, words) in seen
+    assert {("last round", 128, 3, words) for words in (True, False)} <= seen
+    assert ("last round", 128, 2, True) in seen
 
 
 def test_few_rows_fit_lds(plan):
@@ -75,11 +79,14 @@ def test_parts_have_a_run_and_a_place_each(plan):
     for m in (17, 65, 300, 900, 1700, 5000):
         for n in (16, 130, 2330, 16530, 40000):
             for k in (32, 512, 544, 4096, 8224, 100000):
-                kernel, rows, parts, deep = form(plan, m, n, k)
+                kernel, rows, parts, deep, whole = form(plan, m, n, k)
                 columns = 256 if rows == 256 else 128
                 tiles = -(-m // rows) * -(-n // columns)
                 assert deep == (kernel == TILES and rows < 256 and tiles * parts <= 256)
+                if kernel == TILES:
+                    assert whole == tiles if parts == 1 else whole % 256 == 0 and whole < tiles
                 if parts > 1:
-                    assert kernel == TILES and parts <= -(-k // 512) and tiles <= COUNTERS
-                    assert tiles * parts * rows * columns * 4 <= SCRATCH
+                    shared = tiles - whole
+                    assert kernel == TILES and parts <= -(-k // 512) and shared <= COUNTERS
+                    assert shared * parts * rows * columns * 4 <= SCRATCH
                 assert form(plan, m, n, k, 0, 0)[2] == 1   # without scratch nothing is shared
