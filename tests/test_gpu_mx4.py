@@ -366,3 +366,47 @@ def test_refusals(gpu_ctx):
     refused(f, at + 8, at, at, at, 40, 4, 64, xq=at, xs=at)
     refused(f, 0, at, at, at, 40, 4, 64, xq=at, xs=at)
     assert not buf.download(np.uint8, (1 << 16,)).any()
+
+
+def test_shared_tiles_on_two_streams_and_in_two_graphs(gpu_ctx):
+    """Products whose tiles several workgroups share, in two contexts at once (own streams, own scratch) and in two graphs of one
+    context that use the same scratch: the bits of a product alone."""
+    m, n, k = 65, 130, 8192
+    rng = np.random.default_rng(7)
+    other = ka.acquire_gpu(0)
+    try:
+        held = []
+        for gpu in (gpu_ctx, other):
+            w, ws = weights(rng, n, k)
+            xq, xs = ref.quantised(activations(rng, m, k, np.float64), False)
+            args = [gpu.upload(a) for a in (xq, xs, w, ws)]
+            alone, outs = gpu.zeros(m * n * 4), [gpu.zeros(m * n * 4) for _ in range(12)]
+            gpu.linear_mx4(*args, alone, m, n, k)
+            gpu.sync()
+            held.append((gpu, args, alone.download(np.float32, (m, n)), outs))
+        for i in range(12):
+            for gpu, args, _, outs in held:
+                gpu.linear_mx4(*args, outs[i], m, n, k)
+        for gpu, _, want, outs in held:
+            gpu.sync()
+            assert np.abs(want).max() > 0
+            for out in outs:
+                assert np.array_equal(out.download(np.float32, (m, n)).view(np.uint32), want.view(np.uint32))
+        gpu, args, want, outs = held[0]
+        graphs = []
+        for i in range(2):
+            outs[i].zero()
+            with gpu.record() as rec:
+                gpu.linear_mx4(*args, outs[i], m, n, k)
+            graphs.append(rec.graph)
+        for turn in range(3):
+            for graph in graphs:
+                graph.launch()
+            gpu.linear_mx4(*args, outs[2], m, n, k)
+            gpu.sync()
+            for out in outs[:3]:
+                assert np.array_equal(out.download(np.float32, (m, n)).view(np.uint32), want.view(np.uint32)), turn
+        for graph in graphs:
+            graph.destroy()
+    finally:
+        other.destroy()
