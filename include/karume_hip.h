@@ -663,6 +663,8 @@ int32_t krm_dequant_mx4(krm_ctx* ctx, krm_buf codes, krm_buf scales, krm_buf out
  *   s[m, n] = sum_k x[m, k] * w[n, k] + bias[n]      products exact, sums f32
  *   out     = s + residual, or with KRM_EPILOGUE_SILU_PAIRS (rows (2i, 2i+1) of w = (gate_i, up_i), n even,
  *             n_out = n / 2) silu(gate) * up + residual, rounded to out_dtype once
+ *   silu(g) = g / (1 + e^-g): 0 for gates below -174 (fp16 results: from -87.4 down, where its size is below
+ *             2^-119), the gate itself where it is large, NaN at minus infinity
  *   xq, xs  [m, k] codes and scales        w, w_scales  [n, k]
  *   bias    [n] f32 or 0                   residual  [m, n_out] out_dtype or 0; may be out
  * A sum whose terms (with both scales) stay in f32's normal range is of f32 class; terms below it may be

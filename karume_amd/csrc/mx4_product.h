@@ -32,20 +32,30 @@ struct Mx4Out {
   uint32_t pack;         // bytes of a lane's neighbouring results that are stored at once: 16, 8, or one result's
 };
 
-// g / (1 + 2^(-g log2 e)) on the exponential and reciprocal of the hardware, off by a step each.  An f32 result takes the
-// low part of the exponent's product and a Newton step of the reciprocal with it: four steps at most.  Without them
-// the exponential is off by |g| 2^-23, 2^-18 where an fp16 result is not zero, which moves one rounding in a hundred.
+// silu(g) * up, g times its logistic 1 / (1 + e^-g), on the exponential and reciprocal of the hardware, off by a step each.
+// fp16 results: as written; 1 + e^-g is infinite or its reciprocal flushed from g = -87.4 down, where silu is zero then
+// (2^-119: an fp16 result would need an up past 2^94).  The exponent's rounding makes the exponential off by |g| 2^-23, 2^-18
+// where a result of such an up as models have is not zero, which moves one rounding in a hundred.
+// f32 results, with e^-|g| = h h1, neither of which ends before |g| = 174: h = 2^y with y about half of the exponent, h1 = h with
+// what y's roundings have lost.  1 / (1 + h h1) is silu over g, times h h1 where g < 0: h1 before up and h behind
+// it, so that no product is infinite or subnormal before the result is.  Seven steps at most, and two roundings of a
+// subnormal result; gates past 174 are -0 or themselves.  (From 1000 on the gate is held there, so that nothing is infinite
+// but g itself; it comes in again as a factor, as does NaN.)
 template <typename OT>
-__device__ inline float mx4_silu(float g) {
-  constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147182f;
-  const float y = -g * kLog2e;
-  float t = __builtin_amdgcn_exp2f(y);
-  if constexpr (sizeof(OT) == 2) return g * __builtin_amdgcn_rcpf(1.0f + t);
-  const float low = fmaf(-g, kLog2eLow, fmaf(-g, kLog2e, -y)) * kLn2;
-  t = fminf(t, 0x1p126f);  // (past it the result is below f32's range, and infinities make no sum)
-  const float d = 1.0f + fmaf(t, low, t);
-  const float r = __builtin_amdgcn_rcpf(d);
-  return g * fmaf(fmaf(-d, r, 1.0f), r, r);
+__device__ inline float mx4_silu_times(float g, float up) {
+  if constexpr (sizeof(OT) == 2) {
+    constexpr float kLog2e = 1.44269502f;
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g * kLog2e)) * up;
+  } else {
+    constexpr float kHalfLog2e = 0.721347511f, kLn4 = 1.38629436f, kLn4Low = -3.80930843e-9f;
+    const float size = fabsf(__builtin_amdgcn_fmed3f(g, -1000.f, 1000.f));
+    const float y = -kHalfLog2e * size;
+    const float h = __builtin_amdgcn_exp2f(y);
+    const float lost = fmaf(y, -kLn4Low, fmaf(y, -kLn4, -size));  // -size - 2 y ln 2
+    const float h1 = fmaf(h, lost, h), r = __builtin_amdgcn_rcpf(fmaf(h, h1, 1.0f));
+    const bool below = g < 0.f;
+    return g * (below ? h1 : 1.0f) * r * up * (below ? h : 1.0f);
+  }
 }
 __device__ inline float mx4_load(const float* p) { return *p; }
 __device__ inline float mx4_load(const __half* p) { return __half2float(*p); }
@@ -64,7 +74,7 @@ __device__ inline void mx4_values(const Mx4Out& o, uint32_t col, const v4f* sum,
   }
   if constexpr (PAIRS) {
 #pragma unroll
-    for (int i = 0; i < 2 * PIECES; ++i) v[i] = mx4_silu<OT>(v[2 * i]) * v[2 * i + 1];
+    for (int i = 0; i < 2 * PIECES; ++i) v[i] = mx4_silu_times<OT>(v[2 * i], v[2 * i + 1]);
   }
 }
 // COUNT neighbouring values of row `row` from column `first` of the result on: residual, one rounding to the stored type.
