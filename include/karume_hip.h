@@ -672,10 +672,10 @@ int32_t krm_dequant_mx4(krm_ctx* ctx, krm_buf codes, krm_buf scales, krm_buf out
  * branch of a graph, which takes the forms that need no scratch.  k is at most 2^24, and
  * ceil(m / 64) * ceil(n / 128) less than 2^24 - 8; out overlaps nothing but residual.
  * krm_linear_mx4_fused: krm_quantize_mx4 of x [m, k] (f32 or fp16, rows x_stride elements apart, 16-byte
- * aligned) and the product behind one call, the same result bit for bit.  Few rows (up to
- * 16, whose codes and scales take 64 KiB at most: 16 of k = 7680, one of 122880) are quantised inside the
- * product's launch; every other shape goes through xq [m, k/2] and xs [m, k/32], which must then be given
- * (a call without them is refused where it needs them). */
+ * aligned) and the product behind one call, the same result bit for bit.  Few rows (up to 16, which take
+ * 64 KiB at most at k/2 + 16 bytes of codes and k/32, rounded up to 16, of scales a row: 16 of k = 7680, one of 123328)
+ * are quantised inside the product's launch; every other shape goes through xq [m, k/2] and xs [m, k/32], which must
+ * then be given (a call without them is refused where it needs them). */
 int32_t krm_linear_mx4(krm_ctx* ctx, krm_buf xq, krm_buf xs, krm_buf w, krm_buf w_scales,
                        krm_buf bias_f32, krm_buf residual, krm_buf out, uint32_t m, uint32_t n,
                        uint32_t k, int32_t out_dtype, int32_t epilogue);

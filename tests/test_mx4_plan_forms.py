@@ -1,4 +1,8 @@
-"""The shapes of test_gpu_mx4_forms.py take every form that a product of mx4 rows has; no GPU."""
+"""The shapes of test_gpu_mx4_forms.py take every form that a product of mx4 rows has, and the limits that the header states are the
+plan's; no GPU."""
+import os
+import re
+
 import test_gpu_mx4_forms as forms
 from test_mx4_plan import BATCH, ROWS, TILES, form, plan  # noqa: F401  (plan: a fixture)
 
@@ -40,3 +44,11 @@ def test_tiles_have_every_size_depth_and_share(plan):  # noqa: F811
         want |= {(rows, rows < 256, "all", "runs", words) for rows in (64, 128, 256)}
         want |= {(128, False, f"last of {parts}", "runs", words) for parts in (2, 3)}
         assert want <= {s for s in seen if s[-1] == words}, want - seen
+
+
+def test_the_published_limits_of_few_rows(plan):  # noqa: F811
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = open(os.path.join(root, "include", "karume_hip.h")).read()
+    sixteen, one = map(int, re.search(r"16 of k = (\d+), one of (\d+)\)", text).groups())
+    assert plan.fits(16, sixteen) and not plan.fits(16, sixteen + 32) and not plan.fits(17, 32)
+    assert plan.fits(1, one) and not plan.fits(1, one + 32)
