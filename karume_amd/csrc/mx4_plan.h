@@ -71,9 +71,9 @@ inline Mx4Form mx4_form(uint32_t m, uint32_t n, uint32_t k, uint32_t cus, uint64
   }
   // A last round of few tiles of 128 rows is shared: its CUs would hold one workgroup more than the others.  1.05 to 1.29
   // times as fast where K is above 6144 (1001 x 4100 x 11040, 264 tiles, 65.2 us, so 52.5; 1200 x 4096 x 8192, 320 tiles, 40.6 /
-  // 36.4); the join takes it away again below (1100 x 4096 x 4096 21.2 / 22.6), and so does a last round past 7/16 of the CUs
-  // (K of 11744 and 357 tiles 76.8 / 68.0, of 11296 and 396 tiles 70.3 / 89.0).  (Tiles of 64 rows are not picked where there
-  // are two rounds of them and such a K.)
+  // 36.4); the join takes it away again below (1100 x 4096 x 4096 21.2 / 22.6).  A last round of up to 7/16 of the CUs: 101
+  // tiles for 256 CUs still gain (357 tiles, K of 11744, 76.8 / 68.0), 140 lose (396 tiles, K of 11296, 70.3 / 89.0).  (Tiles
+  // of 64 rows are not picked where there are two rounds of them and such a K.)
   const uint32_t runs = (k + 511) / 512;
   if (best.kernel == Mx4Kernel::kTiles && best.rows == 128 && best.parts == 1 && best.whole > cus && runs > 12) {
     const uint32_t last = best.whole % cus, parts = last * 3 <= cus ? 3 : 2;
