@@ -11,8 +11,10 @@ namespace {
 constexpr int kThreads = 256;
 
 // A thread has eight elements, four threads a block (they exchange its largest magnitude in registers): whole pieces of 16
-// bytes in, a word of codes out.  Bound by bytes, 2 or 4 in and 17/32 out an element: 4099 rows of 11008 f32 36.9 us,
-// 5.5 TB/s, of fp16 18.5, 6.2 (two or four rows a thread: within 3 %, and few rows slower); 16 rows of 4096 a launch.
+// bytes in, a word of codes out.  Bound by bytes, 2 or 4 in and 17/32 out an element: 4099 rows of 11008 that come from
+// memory, f32 38.8 us, 5.3 TB/s, fp16 23.1, 4.9 (a copy of them 5.6); from the last-level cache 29.6 and 18.1; f32 rows behind a
+// kernel whose 180 MB of results are still on their way to memory 47.5.  (Two or four rows a thread: within 3 %, and few
+// rows slower.)  16 rows of 4096 a launch.
 template <typename XT>
 __global__ __launch_bounds__(kThreads) void quantize_mx4_kernel(const XT* __restrict__ x,
                                                                 uint32_t* __restrict__ codes,
@@ -38,7 +40,8 @@ __device__ inline float mx4_value(uint32_t code, uint32_t byte) {
   return code & 8u ? -v : v;
 }
 
-// Bound by what it writes: the same rows back as f32 33.6 us, 6.1 TB/s.
+// Bound by what it writes: the same rows back as f32 48.6 us, 4.2 TB/s, as fp16 30.4, 3.8; as f32 behind each
+// quantisation 33.6, where the next quantisation is what waits for the results' way to memory.
 template <typename OT>
 __global__ __launch_bounds__(kThreads) void dequant_mx4_kernel(const uint32_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales,
