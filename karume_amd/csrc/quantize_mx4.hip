@@ -75,6 +75,7 @@ extern "C" int32_t krm_quantize_mx4(krm_ctx* ctx, krm_buf x, krm_buf codes, krm_
                                     int32_t scale_rule) {
   KRM_TRY(enter(ctx));
   KRM_TRY(check_mx4_rows(ctx, "quantize mx4", x, dim, x_stride, x_dtype, scale_rule));
+  KRM_REQUIRE(ctx, rows <= 0x7fffffffu, "quantize mx4: %u rows", rows);  // (a row's number and the step to the next fit 32 bits)
   if (rows == 0) return KRM_OK;
   KRM_REQUIRE(ctx, x && codes && scales, "quantize mx4: null buffer");
   KRM_REQUIRE(ctx, aligned(codes, 16), "quantize mx4: codes need 16-byte alignment");
@@ -96,6 +97,7 @@ extern "C" int32_t krm_dequant_mx4(krm_ctx* ctx, krm_buf codes, krm_buf scales, 
   KRM_REQUIRE(ctx, valid_dtype(out_dtype), "dequant mx4: unknown dtype %d", out_dtype);
   KRM_REQUIRE(ctx, dim > 0 && dim % kMx4Block == 0,
               "dequant mx4: dim must be a positive multiple of 32 (%u)", dim);
+  KRM_REQUIRE(ctx, rows <= 0x7fffffffu, "dequant mx4: %u rows", rows);
   if (rows == 0) return KRM_OK;
   KRM_REQUIRE(ctx, codes && scales && out, "dequant mx4: null buffer");
   KRM_REQUIRE(ctx, aligned(codes, 16) && aligned(out, 16),
