@@ -652,7 +652,7 @@ int32_t krm_kv4_attention(krm_ctx* ctx, krm_buf q, krm_buf cache, krm_buf page_t
  * fp16, 16-byte aligned) are x_stride elements apart.
  * krm_dequant_mx4: the values back, f32 exact or rounded to fp16 once (past either type's range:
  * infinite); NaN where E = 255.
- * Either takes up to 2^31 - 1 rows. */
+ * Either takes up to 2^31 - 1 rows; what it writes overlaps nothing that it reads or writes besides. */
 #define KRM_MX4_FLOOR 0
 #define KRM_MX4_CEIL 1
 int32_t krm_quantize_mx4(krm_ctx* ctx, krm_buf x, krm_buf codes, krm_buf scales, uint32_t rows,

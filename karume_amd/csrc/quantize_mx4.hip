@@ -79,6 +79,7 @@ extern "C" int32_t krm_quantize_mx4(krm_ctx* ctx, krm_buf x, krm_buf codes, krm_
   if (rows == 0) return KRM_OK;
   KRM_REQUIRE(ctx, x && codes && scales, "quantize mx4: null buffer");
   KRM_REQUIRE(ctx, aligned(codes, 16), "quantize mx4: codes need 16-byte alignment");
+  KRM_REQUIRE(ctx, x != codes && x != scales && codes != scales, "quantize mx4: two of x, codes and scales are one buffer");
   const uint32_t eighths = dim / 8;
   const dim3 grid((eighths + kThreads - 1) / kThreads, rows < 65535u ? rows : 65535u);
   const bool ceil = scale_rule == KRM_MX4_CEIL;
@@ -102,6 +103,7 @@ extern "C" int32_t krm_dequant_mx4(krm_ctx* ctx, krm_buf codes, krm_buf scales, 
   KRM_REQUIRE(ctx, codes && scales && out, "dequant mx4: null buffer");
   KRM_REQUIRE(ctx, aligned(codes, 16) && aligned(out, 16),
               "dequant mx4: codes and out need 16-byte alignment");
+  KRM_REQUIRE(ctx, out != codes && out != scales, "dequant mx4: out is the codes' or the scales' buffer");
   const uint64_t eighths = (uint64_t)rows * (dim / 8);
   const uint64_t blocks = (eighths + kThreads - 1) / kThreads;
   const dim3 grid((uint32_t)(blocks < 65536 ? blocks : 65536));
